@@ -190,6 +190,73 @@ TENZO_HIP_API int tenzo_hip_attn_paged_int8_decode(const float* q, const float* 
                                                    int layer, const float* rope_cs, int Hq,
                                                    int Hkv, int pos, float* out, void* stream);
 
+/* ---- paged cache in 4 bits: append, read, attention ---------------------- */
+
+/* No counterpart in the reference. A cache row of 128 values is four groups of
+ * 32, each 32 E2M1 codes (0 .5 1 1.5 2 3 4 6, bit 3 the sign) times 2^(s - 127)
+ * with a scale byte s of its own (E8M0): pools of 16-token pages as
+ * tenzo_hip_attn_paged_int8_decode has them, codes pk / pv
+ * [n_blocks][n_layers][Hkv][16][64] (byte i: dim 2i low, dim 2i + 1 high) and
+ * scales pks / pvs [n_blocks][n_layers][Hkv][16][4]; code pools 16-byte
+ * aligned, scale pools 4-byte.
+ *
+ * A call takes T rows of B sequences. Sequence b has block table row
+ * block_tables + b * table_stride (table_width entries; entry p holds the page
+ * of positions 16p .. 16p + 15) and ctx_lens[b] tokens, the call's own
+ * included. Its rows are cu_q[b] .. cu_q[b + 1] - 1 (cu_q: B + 1 non-decreasing
+ * row numbers; null: row b is sequence b's only one, T == B) and stand at its
+ * last positions: row i of n at ctx_lens[b] - n + i. rope_cs: n_pos rows of
+ * cos[64], sin[64], row p for position p (null: no rotation).
+ * ctx_lens, cu_q and the tables are read on the device, so what is wrong there
+ * is left out, not reported: a length of 0 or less or above
+ * min(16 * table_width, n_pos) stands for a padding slot (no tokens), rows at
+ * negative positions for none, a table entry outside 0 .. n_blocks - 1 for a
+ * page of absent tokens. Rows from cu_q[B] on are neither read nor written.
+ * dtype of k, v, q, out: 0 = fp32, 1 = fp16; strides in elements. */
+
+/* Rotates k ([T] rows of Hkv heads of 128, k_stride apart), rounds k and v to
+ * the cache's values and writes them at their positions. The rotation is
+ * computed in 64 bits and every element rounded once: group scale = the
+ * smallest power of two with max |x| <= 7 * 2^(s - 127) (s >= 1), code = the
+ * nearest value, the even code where two are as near. NaN counts as 0,
+ * magnitudes above 1.75 * 2^127 as that. Two rows of a call at the same place
+ * (one page in two tables) race. */
+TENZO_HIP_API int tenzo_hip_kv4_append(const void* k, const void* v, int dtype, int64_t k_stride,
+                                       int64_t v_stride, uint8_t* pk, uint8_t* pv, uint8_t* pks,
+                                       uint8_t* pvs, int64_t n_blocks, int n_layers, int layer,
+                                       int Hkv, const int32_t* block_tables,
+                                       int64_t table_stride, int table_width,
+                                       const int32_t* ctx_lens, const int32_t* cu_q, int B,
+                                       int64_t T, const float* rope_cs, int n_pos, void* stream);
+/* The cached values at the positions of the T rows (what append wrote for
+ * them): k_out / v_out [T][Hkv][128] of dtype, zeros for rows that stand
+ * nowhere. */
+TENZO_HIP_API int tenzo_hip_kv4_read(const uint8_t* pk, const uint8_t* pv, const uint8_t* pks,
+                                     const uint8_t* pvs, int64_t n_blocks, int n_layers,
+                                     int layer, int Hkv, const int32_t* block_tables,
+                                     int64_t table_stride, int table_width,
+                                     const int32_t* ctx_lens, const int32_t* cu_q, int B,
+                                     int64_t T, void* k_out, void* v_out, int dtype,
+                                     void* stream);
+/* Attention of the T rows over the cache: q [T] rows of Hq heads, q_stride
+ * apart, rotated at their positions; row r's head h attends with scale
+ * 1/sqrt(128) to kv head h / (Hq/Hkv) at positions 0 .. its own (the cache has
+ * to hold them: append first), out likewise out_stride apart. A row that sees
+ * no token is zero. Hq / Hkv 1 to 16. out must not overlap q. ws: a workspace
+ * of tenzo_hip_attn_kv4_ws_bytes(...) bytes, 16-byte aligned, of this call
+ * alone until it has run (null where that is 0). */
+TENZO_HIP_API size_t tenzo_hip_attn_kv4_ws_bytes(int64_t T, int B, int Hq, int Hkv,
+                                                 int table_width);
+TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,
+                                     const uint8_t* pk, const uint8_t* pv, const uint8_t* pks,
+                                     const uint8_t* pvs, int64_t n_blocks, int n_layers,
+                                     int layer, int Hq, int Hkv, const int32_t* block_tables,
+                                     int64_t table_stride, int table_width,
+                                     const int32_t* ctx_lens, const int32_t* cu_q, int B,
+                                     int64_t T, const float* rope_cs, int n_pos, void* out,
+                                     int64_t out_stride, void* ws, size_t ws_bytes,
+                                     void* stream);
+
 /* HOST function: fills cs[pos - pos0][0..127] = cos/sin table rows for
  * positions pos0 .. pos0+n_pos-1 with the reference's RoPE angles
  * (TenzoEngine.cpp:465-469; theta is 10000 there and a parameter here). */
@@ -282,6 +349,38 @@ TENZO_HIP_API int tenzo_hip_quant_rows_i8(const float* E, int64_t V, int64_t H, 
 TENZO_HIP_API int tenzo_hip_sample_top_k_top_p(const float* logits, int64_t V, int top_k,
                                                float top_p, float temperature, float r,
                                                int32_t* out_token, void* stream);
+/* Beam search, no counterpart in the reference: the best k continuations of
+ * each of B requests with W beams. Candidate (w, t) of a request has the score
+ * scores[b][w] + log_softmax(logits[b][w])[t] (row b * W + w of the logits at
+ * row_stride elements); the k largest, in order, go to out_scores, out_beams
+ * (w) and out_tokens (t), each [B][k]. Scores are compared in 64 bits; among
+ * equal ones the lower beam comes first, then the larger logit, then the lower
+ * token. A logit or a score that is not below +inf (NaN too) counts as -inf;
+ * -inf candidates come last. W and k up to 64, k <= W * V. ws: as above,
+ * tenzo_hip_beam_select_ws_bytes(...) bytes. */
+TENZO_HIP_API size_t tenzo_hip_beam_select_ws_bytes(int B, int W, int64_t V, int k);
+TENZO_HIP_API int tenzo_hip_beam_select(const float* logits, int64_t row_stride,
+                                        const float* scores, int B, int W, int64_t V, int k,
+                                        float* out_scores, int32_t* out_beams,
+                                        int32_t* out_tokens, void* ws, size_t ws_bytes,
+                                        void* stream);
+/* Reorders the paged caches of B requests with W beams (table rows b * W + i),
+ * in place: slot i of request b goes on from slot parents[b][i] (parent_stride
+ * apart; outside 0 .. W - 1: from itself). With c = ctx_lens[b * W], the length
+ * of all of a request's beams: the table's entries of full pages (p < c / 16)
+ * are the parent's afterwards, the c % 16 rows of the page in progress are
+ * copied, in every layer and head, from the parent's page c / 16 into the
+ * slot's own, and the entries from c / 16 on stay. So a slot's pages from
+ * c / 16 on have to be its own, and full pages are shared, never written
+ * again. Pools of 4-bit rows (row_bytes 64) or of the int8 paged cache (128:
+ * its fp32 scale is a row's 4 scale bytes). Lengths and table entries out of
+ * range: nothing is moved there. */
+TENZO_HIP_API int tenzo_hip_beam_reorder_paged(const int32_t* parents, int64_t parent_stride,
+                                               int32_t* block_tables, int64_t table_stride,
+                                               int table_width, const int32_t* ctx_lens, int B,
+                                               int W, void* pk, void* pv, void* pks, void* pvs,
+                                               int64_t n_blocks, int n_layers, int Hkv,
+                                               int row_bytes, void* stream);
 /* embedding_lookup, int8 branch (TenzoEngine.cpp:1294-1316), reading the
  * table in the LM-head device layout: x = float(E[token]) * scales[token].
  * token is read from device memory (token_dev). */

@@ -40,6 +40,17 @@ SIGNATURES = {
     "tenzo_hip_attn_paged_int8_decode": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P, _I,
                                               _I, _I, _P, _P]),
     "tenzo_hip_engine_block_table": (_I, [_P, _P, _I]),
+    "tenzo_hip_kv4_append": (_I, [_P, _P, _I, _I64, _I64, _P, _P, _P, _P, _I64, _I, _I, _I, _P,
+                                  _I64, _I, _P, _P, _I, _I64, _P, _I, _P]),
+    "tenzo_hip_kv4_read": (_I, [_P, _P, _P, _P, _I64, _I, _I, _I, _P, _I64, _I, _P, _P, _I, _I64,
+                                _P, _P, _I, _P]),
+    "tenzo_hip_attn_kv4_ws_bytes": (_SZ, [_I64, _I, _I, _I, _I]),
+    "tenzo_hip_attn_kv4": (_I, [_P, _I, _I64, _P, _P, _P, _P, _I64, _I, _I, _I, _I, _P, _I64, _I,
+                                _P, _P, _I, _I64, _P, _I, _P, _I64, _P, _SZ, _P]),
+    "tenzo_hip_beam_select_ws_bytes": (_SZ, [_I, _I, _I64, _I]),
+    "tenzo_hip_beam_select": (_I, [_P, _I64, _P, _I, _I, _I64, _I, _P, _P, _P, _P, _SZ, _P]),
+    "tenzo_hip_beam_reorder_paged": (_I, [_P, _I64, _P, _I64, _I, _P, _I, _I, _P, _P, _P, _P,
+                                          _I64, _I, _I, _I, _P]),
     "tenzo_hip_rope_table": (None, [_F, _I, _I, _I, _P]),
     "tenzo_hip_gemv_q4_0": (_I, [_P, _I, _P, _P, _I, _I, _I, _P]),
     "tenzo_hip_gemv_q8_0": (_I, [_P, _I, _P, _P, _I, _I, _I, _P]),

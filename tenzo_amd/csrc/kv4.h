@@ -1,0 +1,113 @@
+// The paged cache held in 4 bits: its layout, the sequences of a call and the conversions that
+// its kernels share (kv4_cache.hip, attention_kv4.hip).
+//
+// A row of 128 values is four groups of 32, each E2M1 codes (0 .5 1 1.5 2 3 4 6 and their
+// negatives) times a power of two of its own (E8M0: 2^(s - 127)): 64 + 4 bytes in place of the
+// 128 + 4 of an int8 row. Every value is exact in bf16, and the codes are what gfx950 converts
+// two at a time with the scale applied, so a row costs 64 conversions and no multiplication.
+// Byte i of a row holds dim 2i in its low nibble and dim 2i + 1 in its high one. Pools as the
+// int8 paged cache has them: codes [blocks][n_layers][Hkv][16][64], scales
+// [blocks][n_layers][Hkv][16][4].
+#pragma once
+
+#include "common.h"
+
+namespace tz {
+
+constexpr int kKv4Dim = 128;
+constexpr int kKv4Page = 16;
+constexpr int kKv4Row = 64;    // code bytes of a row
+constexpr int kKv4Scales = 4;  // scale bytes of a row
+
+// The sequences of a call. Row r of the T rows belongs to sequence s with cu[s] <= r < cu[s + 1]
+// (cu null: row r is sequence r's only one) and stands at position ctx[s] - n + (r - cu[s]), n
+// the sequence's rows. What the device finds in these arrays is checked before it is used: a
+// length above `limit` (the table's width, the rotation's rows) counts as 0, a page outside the
+// pool as absent.
+struct Kv4Seqs {
+    const int32_t* tables;
+    const int32_t* ctx;
+    const int32_t* cu;
+    int64_t table_stride;
+    int64_t n_blocks;
+    int B, limit;
+    int n_layers, layer, Hkv;
+
+    __device__ __forceinline__ int length(int s) const {
+        const int c = ctx[s];
+        return c > 0 && c <= limit ? c : 0;
+    }
+    // Row (of 16-token pages) of head 0 in logical page `p` of sequence s, or -1.
+    __device__ __forceinline__ int64_t page_base(int s, int p) const {
+        const int64_t blk = tables[(int64_t)s * table_stride + p];
+        return blk >= 0 && blk < n_blocks ? (blk * n_layers + layer) * Hkv * kKv4Page : -1;
+    }
+};
+
+// The sequence of row r: how many of cu[1 .. B] are <= r, counted by the 16 lanes of a DPP row
+// (all of them active and with the same r). B or a sequence whose range does not hold r: none.
+__device__ __forceinline__ int kv4_seq_of_row(const Kv4Seqs& q, int r, int lane16) {
+    int n = 0;
+    for (int b = lane16; b < q.B; b += 16) n += q.cu[b + 1] <= r ? 1 : 0;
+    n += dpp_i<kDppXor1>(n);
+    n += dpp_i<kDppXor2>(n);
+    n += dpp_i<kDppHalfMirror>(n);
+    n += dpp_i<kDppMirror>(n);
+    return n;
+}
+
+// Position of row r and its sequence; false where it stands nowhere (padding).
+__device__ __forceinline__ bool kv4_place(const Kv4Seqs& q, int r, int lane16, int& seq,
+                                          int& pos) {
+    int n = 1, i = 0;
+    seq = r;
+    if (q.cu) {
+        seq = kv4_seq_of_row(q, r, lane16);
+        if (seq >= q.B) return false;
+        const int first = q.cu[seq];
+        n = q.cu[seq + 1] - first;
+        i = r - first;
+    }
+    const int c = q.length(seq);
+    pos = c - n + i;
+    return i >= 0 && i < n && pos >= 0 && pos < c;
+}
+
+// 2^(s - 127) as fp32 (s = 255, which no append writes, is NaN as the format says).
+__device__ __forceinline__ float e8m0_to_float(uint32_t s) {
+    return __uint_as_float(s == 0 ? 0x00400000u : s == 255 ? 0x7fc00000u : s << 23);
+}
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// The eight values of a word of codes, in order.
+__device__ __forceinline__ void fp4_to_float8(uint32_t w, float scale, float (&v)[8]) {
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 0);
+    const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 1);
+    const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 2);
+    const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 3);
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+    v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
+}
+
+template <bool HALF>
+__device__ __forceinline__ float ld_act(const void* p, int64_t i) {
+    return HALF ? __half2float(reinterpret_cast<const __half*>(p)[i])
+                : reinterpret_cast<const float*>(p)[i];
+}
+template <bool HALF>
+__device__ __forceinline__ void st_act(void* p, int64_t i, float v) {
+    if (HALF)
+        reinterpret_cast<uint16_t*>(p)[i] = float_to_half_bits(v);
+    else
+        reinterpret_cast<float*>(p)[i] = v;
+}
+
+// Argument checks that the entry points share. Fills `q`.
+int kv4_check(const char* what, const void* pk, const void* pv, const void* pks, const void* pvs,
+              int64_t n_blocks, int n_layers, int layer, int Hkv, const int32_t* block_tables,
+              int64_t table_stride, int table_width, const int32_t* ctx_lens,
+              const int32_t* cu_q, int B, int64_t T, const float* rope_cs, int n_pos, Kv4Seqs& q);
+
+}  // namespace tz

@@ -1,0 +1,252 @@
+// Writing to and reading from the paged cache held in 4 bits (layout: kv4.h).
+#include "kv4.h"
+
+namespace tz {
+namespace {
+
+struct Kv4Append {
+    const void* k;
+    const void* v;
+    int64_t k_stride, v_stride;
+    uint8_t* pk;
+    uint8_t* pv;
+    uint8_t* pks;
+    uint8_t* pvs;
+    const float* rope;
+    int64_t items;  // T * Hkv * 2
+};
+
+constexpr float kKv4Max = 0x1.cp127f;  // the largest magnitude whose codes stay finite: 7 * 2^125
+
+// r rounded to fp32 so that it never meets the border of two codes unless it lies on it: towards
+// zero, with the last bit set when anything was cut off. The borders are fp32 numbers of a few
+// bits, so a code taken from this value is the one that r itself rounds to.
+__device__ __forceinline__ float round_sticky(double r) {
+    const float t = (float)r;
+    const double back = (double)t;
+    uint32_t b = __float_as_uint(t);
+    if (fabs(back) > fabs(r)) b -= 1;
+    if (back != r) b |= 1;
+    return __uint_as_float(b);
+}
+
+__device__ __forceinline__ float tame(float x) {  // NaN counts as 0, what is beyond is held there
+    return x == x ? fminf(fmaxf(x, -kKv4Max), kKv4Max) : 0.0f;
+}
+
+// The scale byte of a group: the smallest e with amax <= 7 * 2^(e - 127) (codes up to 7 go to 6,
+// the last one), at least 1. In the bits: the exponent field less 2, one more above 1.75.
+__device__ __forceinline__ int group_scale(float amax) {
+    return max((int)((__float_as_uint(amax) + 0x1FFFFFu) >> 23) - 2, 1);
+}
+
+// Four values of one group as codes, the first in the low nibble.
+__device__ __forceinline__ uint32_t codes4(const float (&x)[4], int e) {
+    const float s = __uint_as_float((uint32_t)e << 23);
+    uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x[0], x[1], s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
+    return w & 0xffffu;
+}
+
+__device__ __forceinline__ float max8(float m) {  // over the 8 lanes of a half DPP row
+    m = fmaxf(m, dpp_f<kDppXor1>(m));
+    m = fmaxf(m, dpp_f<kDppXor2>(m));
+    return fmaxf(m, dpp_f<kDppHalfMirror>(m));
+}
+
+// 16 lanes to a row of 128: lane l has dims 4l .. 4l + 3 and 64 + 4l .. 64 + 4l + 3, so that a
+// dim and its partner of the rotation meet in one lane and a group of 32 lies in 8 lanes.
+template <bool HALF>
+__global__ void __launch_bounds__(256) kv4_append_kernel(Kv4Append a, Kv4Seqs sq) {
+    const int l = threadIdx.x & 15;
+    const int64_t item = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (item >= a.items) return;
+    const int per_row = sq.Hkv * 2;
+    const int row = (int)(item / per_row);
+    const int rest = (int)(item - (int64_t)row * per_row);
+    const bool is_v = rest >= sq.Hkv;
+    const int h = is_v ? rest - sq.Hkv : rest;
+    int seq, pos;
+    if (!kv4_place(sq, row, l, seq, pos)) return;
+    const int64_t base = sq.page_base(seq, pos / kKv4Page);
+    if (base < 0) return;
+    const int64_t dst = base + h * kKv4Page + pos % kKv4Page;
+    const void* src = is_v ? a.v : a.k;
+    const int64_t at = row * (is_v ? a.v_stride : a.k_stride) + h * kKv4Dim + 4 * l;
+    float lo[4], hi[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        lo[j] = ld_act<HALF>(src, at + j);
+        hi[j] = ld_act<HALF>(src, at + 64 + j);
+    }
+    if (!is_v && a.rope) {
+        // in 64 bits, where both products are exact: a key is rounded once, to its code
+        const float* cs = a.rope + (int64_t)pos * kKv4Dim + 4 * l;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const double c = cs[j], s = cs[64 + j], x0 = lo[j], x1 = hi[j];
+            lo[j] = round_sticky(__builtin_fma(-x1, s, x0 * c));
+            hi[j] = round_sticky(__builtin_fma(x1, c, x0 * s));
+        }
+    }
+    float ml = 0.0f, mh = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        lo[j] = tame(lo[j]);
+        hi[j] = tame(hi[j]);
+        ml = fmaxf(ml, fabsf(lo[j]));
+        mh = fmaxf(mh, fabsf(hi[j]));
+    }
+    const int el = group_scale(max8(ml)), eh = group_scale(max8(mh));
+    uint8_t* codes = (is_v ? a.pv : a.pk) + dst * kKv4Row;
+    reinterpret_cast<uint16_t*>(codes)[l] = (uint16_t)codes4(lo, el);
+    reinterpret_cast<uint16_t*>(codes)[16 + l] = (uint16_t)codes4(hi, eh);
+    if ((l & 7) == 0) {
+        uint8_t* sc = (is_v ? a.pvs : a.pks) + dst * kKv4Scales;
+        sc[l >> 3] = (uint8_t)el;
+        sc[2 + (l >> 3)] = (uint8_t)eh;
+    }
+}
+
+struct Kv4Read {
+    const uint8_t* pk;
+    const uint8_t* pv;
+    const uint8_t* pks;
+    const uint8_t* pvs;
+    void* k;
+    void* v;
+    int64_t items;
+};
+
+// 16 lanes to a row: lane l has dims 8l .. 8l + 7.
+template <bool HALF>
+__global__ void __launch_bounds__(256) kv4_read_kernel(Kv4Read a, Kv4Seqs sq) {
+    const int l = threadIdx.x & 15;
+    const int64_t item = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (item >= a.items) return;
+    const int per_row = sq.Hkv * 2;
+    const int row = (int)(item / per_row);
+    const int rest = (int)(item - (int64_t)row * per_row);
+    const bool is_v = rest >= sq.Hkv;
+    const int h = is_v ? rest - sq.Hkv : rest;
+    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    int seq, pos;
+    if (kv4_place(sq, row, l, seq, pos)) {
+        const int64_t base = sq.page_base(seq, pos / kKv4Page);
+        if (base >= 0) {
+            const int64_t src = base + h * kKv4Page + pos % kKv4Page;
+            const uint32_t w =
+                reinterpret_cast<const uint32_t*>((is_v ? a.pv : a.pk) + src * kKv4Row)[l];
+            fp4_to_float8(w, e8m0_to_float((is_v ? a.pvs : a.pks)[src * kKv4Scales + (l >> 2)]),
+                          v);
+        }
+    }
+    void* out = is_v ? a.v : a.k;
+    const int64_t at = ((int64_t)row * sq.Hkv + h) * kKv4Dim + 8 * l;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) st_act<HALF>(out, at + j, v[j]);
+}
+
+}  // namespace
+
+int kv4_check(const char* what, const void* pk, const void* pv, const void* pks, const void* pvs,
+              int64_t n_blocks, int n_layers, int layer, int Hkv, const int32_t* block_tables,
+              int64_t table_stride, int table_width, const int32_t* ctx_lens,
+              const int32_t* cu_q, int B, int64_t T, const float* rope_cs, int n_pos,
+              Kv4Seqs& q) {
+    TZ_CHECK(B >= 0 && T >= 0 && T <= INT32_MAX, "%s: B=%d T=%lld", what, B, (long long)T);
+    TZ_CHECK(Hkv > 0 && Hkv <= 65535, "%s: bad head count (Hkv=%d)", what, Hkv);
+    TZ_CHECK(n_layers > 0 && layer >= 0 && layer < n_layers, "%s: layer %d of %d", what, layer,
+             n_layers);
+    TZ_CHECK(n_blocks >= 0 && n_blocks <= INT32_MAX, "%s: %lld blocks", what,
+             (long long)n_blocks);
+    TZ_CHECK(table_width >= 0 && table_width <= INT32_MAX / kKv4Page &&
+                 (table_stride >= table_width || B <= 1),
+             "%s: block tables of %d pages, %lld apart", what, table_width,
+             (long long)table_stride);
+    TZ_CHECK(cu_q || T == B, "%s: %lld rows for %d sequences of one token", what, (long long)T, B);
+    TZ_CHECK(!rope_cs || n_pos >= 0, "%s: %d rotation rows", what, n_pos);
+    q.tables = block_tables;
+    q.ctx = ctx_lens;
+    q.cu = cu_q;
+    q.table_stride = table_stride;
+    q.n_blocks = n_blocks;
+    q.B = B;
+    q.limit = table_width * kKv4Page;
+    if (rope_cs && n_pos < q.limit) q.limit = n_pos;
+    q.n_layers = n_layers;
+    q.layer = layer;
+    q.Hkv = Hkv;
+    if (T == 0 || B == 0) return TENZO_SUCCESS;
+    TZ_CHECK(ctx_lens, "%s: null pointer", what);
+    TZ_CHECK((pk && pv && pks && pvs) || n_blocks == 0, "%s: null pointer", what);
+    TZ_CHECK(block_tables || table_width == 0, "%s: null pointer", what);
+    TZ_CHECK((((uintptr_t)pk | (uintptr_t)pv) & 15) == 0 &&
+                 (((uintptr_t)pks | (uintptr_t)pvs) & 3) == 0,
+             "%s: code pools must be 16-byte aligned, scale pools 4-byte", what);
+    return TENZO_SUCCESS;
+}
+
+}  // namespace tz
+
+using namespace tz;
+
+extern "C" {
+
+TENZO_HIP_API int tenzo_hip_kv4_append(const void* k, const void* v, int dtype, int64_t k_stride,
+                                       int64_t v_stride, uint8_t* pk, uint8_t* pv, uint8_t* pks,
+                                       uint8_t* pvs, int64_t n_blocks, int n_layers, int layer,
+                                       int Hkv, const int32_t* block_tables,
+                                       int64_t table_stride, int table_width,
+                                       const int32_t* ctx_lens, const int32_t* cu_q, int B,
+                                       int64_t T, const float* rope_cs, int n_pos, void* stream) {
+    Kv4Seqs q{};
+    const int rc = kv4_check("kv4_append", pk, pv, pks, pvs, n_blocks, n_layers, layer, Hkv,
+                             block_tables, table_stride, table_width, ctx_lens, cu_q, B, T,
+                             rope_cs, n_pos, q);
+    if (rc) return rc;
+    TZ_CHECK(dtype == 0 || dtype == 1, "kv4_append: dtype %d", dtype);
+    if (T == 0 || B == 0) return TENZO_SUCCESS;
+    TZ_CHECK(k && v, "kv4_append: null pointer");
+    TZ_CHECK(T == 1 || (k_stride >= (int64_t)Hkv * kKv4Dim && v_stride >= (int64_t)Hkv * kKv4Dim),
+             "kv4_append: row strides %lld, %lld below %d heads", (long long)k_stride,
+             (long long)v_stride, Hkv);
+    Kv4Append a{k, v, k_stride, v_stride, pk, pv, pks, pvs, rope_cs, T * Hkv * 2};
+    const int64_t blocks = ceil_div(a.items, 16);
+    TZ_CHECK(blocks <= INT32_MAX, "kv4_append: %lld rows of %d heads", (long long)T, Hkv);
+    const dim3 grid((unsigned)blocks);
+    if (dtype)
+        hipLaunchKernelGGL(kv4_append_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, a, q);
+    else
+        hipLaunchKernelGGL(kv4_append_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, a,
+                           q);
+    return launch_status("kv4_append_kernel");
+}
+
+TENZO_HIP_API int tenzo_hip_kv4_read(const uint8_t* pk, const uint8_t* pv, const uint8_t* pks,
+                                     const uint8_t* pvs, int64_t n_blocks, int n_layers,
+                                     int layer, int Hkv, const int32_t* block_tables,
+                                     int64_t table_stride, int table_width,
+                                     const int32_t* ctx_lens, const int32_t* cu_q, int B,
+                                     int64_t T, void* k_out, void* v_out, int dtype,
+                                     void* stream) {
+    Kv4Seqs q{};
+    const int rc = kv4_check("kv4_read", pk, pv, pks, pvs, n_blocks, n_layers, layer, Hkv,
+                             block_tables, table_stride, table_width, ctx_lens, cu_q, B, T,
+                             nullptr, 0, q);
+    if (rc) return rc;
+    TZ_CHECK(dtype == 0 || dtype == 1, "kv4_read: dtype %d", dtype);
+    if (T == 0) return TENZO_SUCCESS;
+    TZ_CHECK(k_out && v_out, "kv4_read: null pointer");
+    Kv4Read a{pk, pv, pks, pvs, k_out, v_out, T * Hkv * 2};
+    const int64_t blocks = ceil_div(a.items, 16);
+    TZ_CHECK(blocks <= INT32_MAX, "kv4_read: %lld rows of %d heads", (long long)T, Hkv);
+    const dim3 grid((unsigned)blocks);
+    if (dtype)
+        hipLaunchKernelGGL(kv4_read_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, a, q);
+    else
+        hipLaunchKernelGGL(kv4_read_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, a, q);
+    return launch_status("kv4_read_kernel");
+}
+
+}  // extern "C"

@@ -5,12 +5,14 @@ Mirrors the reference operator surface - ``ROCmRuntime::executeBitLinearTL1``
 free GEMV functions ``compute_linear_gguf_q4_0`` / ``_gptq`` / ``_awq``
 (``TenzoEngine.cpp:1022-1175``), ``FusedKVCache::forward_attention_raw``
 (``TenzoEngine.cpp:447-919``) and ``compute_logits`` (``:1634-1720``) - with
-the same argument meaning. Every call goes through libtenzo_hip.so on the
-current torch stream; tensors must live on the GPU.
+the same argument meaning; and, without a counterpart there, the operators of
+batched beam decoding over a paged cache in 4 bits. Every call goes through
+libtenzo_hip.so on the current torch stream; tensors must live on the GPU.
 """
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -232,6 +234,160 @@ def attn_paged_int8_decode(q, k_new, v_new, pk, pv, pks, pvs, block_table, layer
     return out
 
 
+# ------------------------------------------------- paged cache in 4 bits ----
+
+KV4_PAGE = 16
+
+
+def _dev() -> int:
+    return torch._C._cuda_getDevice()
+
+
+def _on(t: torch.Tensor, dev: int, dtype: torch.dtype, name: str) -> int:
+    """The address of a tensor of the current device (the kernels run on its stream)."""
+    if t.get_device() != dev:
+        raise ValueError(f"{name}: on {t.device}, the current device is cuda:{dev}")
+    if t.dtype != dtype:
+        raise ValueError(f"{name}: {t.dtype}, not {dtype}")
+    return t.data_ptr()
+
+
+def _whole(t: torch.Tensor, dev: int, dtype: torch.dtype, name: str) -> int:
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: not contiguous")
+    return _on(t, dev, dtype, name)
+
+
+def _row_stride(t: torch.Tensor, cols: int, name: str) -> int:
+    """Elements between the rows of t, [rows][cols] or more dims that fold to it."""
+    if t.dim() == 2 and t.shape[1] == cols and (cols == 0 or t.stride(1) == 1):
+        return t.stride(0) if t.shape[0] > 1 else max(cols, t.stride(0))
+    if t.dim() > 2 and math.prod(t.shape[1:]) == cols and (not t.numel() or
+                                                           t[0].is_contiguous()):
+        return t.stride(0) if t.shape[0] > 1 else cols
+    raise ValueError(f"{name}: {tuple(t.shape)} with strides {t.stride()}, not rows of {cols}")
+
+
+def kv4_pool(n_blocks: int, n_layers: int, n_kv_heads: int, device="cuda"):
+    """Empty pools (pk, pv, pks, pvs) of n_blocks 16-token pages of a cache in 4 bits: codes
+    [blocks][layers][kv heads][16][64] and scales [blocks][layers][kv heads][16][4], uint8."""
+    shape = (n_blocks, n_layers, n_kv_heads, KV4_PAGE)
+    return tuple(torch.zeros((*shape, w), dtype=torch.uint8, device=device)
+                 for w in (64, 64, 4, 4))
+
+
+def _kv4_cache(pk, pv, pks, pvs, block_tables, ctx_lens, cu_q, layer, rows, dev):
+    """The arguments that the calls on a cache share, checked: (pool addresses), (n_blocks,
+    n_layers, layer, Hkv), (tables, stride, width, lengths, cu_q, B, rows)."""
+    if pk.dim() != 5 or pk.shape[3:] != (KV4_PAGE, 64) or pv.shape != pk.shape:
+        raise ValueError(f"pk, pv: {tuple(pk.shape)}, {tuple(pv.shape)}, not "
+                         "[blocks][layers][kv heads][16][64]")
+    nb, n_layers, Hkv = pk.shape[:3]
+    want = (nb, n_layers, Hkv, KV4_PAGE, 4)
+    if pks.shape != want or pvs.shape != want:
+        raise ValueError(f"pks, pvs: {tuple(pks.shape)}, {tuple(pvs.shape)}, not {want}")
+    if block_tables.dim() != 2 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+        raise ValueError("block_tables: a row of page numbers per sequence")
+    B, width = block_tables.shape
+    if ctx_lens.shape != (B,):
+        raise ValueError(f"ctx_lens: {tuple(ctx_lens.shape)}, not a length for each of {B} "
+                         "sequences")
+    if cu_q is None:
+        if rows != B:
+            raise ValueError(f"{rows} rows for {B} sequences of one token: pass cu_q")
+    elif cu_q.shape != (B + 1,):
+        raise ValueError(f"cu_q: {tuple(cu_q.shape)}, not ({B + 1},)")
+    u8, i32 = torch.uint8, torch.int32
+    pools = (_whole(pk, dev, u8, "pk"), _whole(pv, dev, u8, "pv"), _whole(pks, dev, u8, "pks"),
+             _whole(pvs, dev, u8, "pvs"))
+    return pools, (nb, n_layers, layer, Hkv), (
+        _on(block_tables, dev, i32, "block_tables"),
+        block_tables.stride(0) if B > 1 else width, width, _whole(ctx_lens, dev, i32, "ctx_lens"),
+        None if cu_q is None else _whole(cu_q, dev, i32, "cu_q"), B, rows)
+
+
+def _rope_rows(rope_cs, dev):
+    if rope_cs is None:
+        return None, 0
+    if rope_cs.dim() != 2 or rope_cs.shape[1] != 128:
+        raise ValueError(f"rope_cs: {tuple(rope_cs.shape)}, not [positions][128]")
+    return _whole(rope_cs, dev, torch.float32, "rope_cs"), rope_cs.shape[0]
+
+
+def kv4_append(k, v, pk, pv, pks, pvs, block_tables, ctx_lens, layer: int, rope_cs=None,
+               cu_q=None) -> None:
+    """Rotates the keys of new tokens, rounds keys and values to 4 bits and writes them into
+    the paged cache (pools of kv4_pool, updated in place).
+
+    k, v [T][Hkv*128] (or [T][Hkv][128]) fp32 or fp16, rows any stride apart (slices of a
+    fused q | k | v do); block_tables int32 [B][pages], ctx_lens int32 [B], the new tokens
+    included. cu_q int32 [B+1]: sequence b's rows are cu_q[b] .. cu_q[b+1]-1, at its last
+    positions; None: row b is sequence b's one new token. rope_cs: rows cos | sin of
+    positions 0, 1, ... (rope_table; None: no rotation). Lengths of 0 or less, or above what
+    the tables or rope_cs hold, are padding slots; pages outside the pool are skipped."""
+    dev = _dev()
+    T = k.shape[0]
+    pools, where, seqs = _kv4_cache(pk, pv, pks, pvs, block_tables, ctx_lens, cu_q, layer, T, dev)
+    dt = _dtype_code(k)
+    cols = where[3] * 128
+    ks, vs = _row_stride(k, cols, "k"), _row_stride(v, cols, "v")
+    if v.shape[0] != T:
+        raise ValueError(f"{T} rows of k, {v.shape[0]} of v")
+    _lib.check(_lib.load().tenzo_hip_kv4_append(
+        _on(k, dev, k.dtype, "k"), _on(v, dev, k.dtype, "v"), dt, ks, vs, *pools, *where, *seqs,
+        *_rope_rows(rope_cs, dev), _stream()), "kv4_append")
+
+
+def kv4_read(pk, pv, pks, pvs, block_tables, ctx_lens, layer: int, rows: int | None = None,
+             cu_q=None, dtype=torch.float32):
+    """The cached keys (rotated) and values at the positions of a call's rows, as kv4_append
+    places them: (k, v) [rows][Hkv][128]. rows: as many as the call has (with cu_q; without,
+    one a sequence). Rows that stand nowhere are zeros."""
+    dev = _dev()
+    if rows is None:
+        if cu_q is not None:
+            raise ValueError("kv4_read: rows is needed with cu_q")
+        rows = block_tables.shape[0]
+    pools, where, seqs = _kv4_cache(pk, pv, pks, pvs, block_tables, ctx_lens, cu_q, layer, rows,
+                                    dev)
+    k = torch.empty((rows, where[3], 128), dtype=dtype, device=pk.device)
+    v = torch.empty_like(k)
+    _lib.check(_lib.load().tenzo_hip_kv4_read(*pools, *where, *seqs, k.data_ptr(), v.data_ptr(),
+                                              _dtype_code(k), _stream()), "kv4_read")
+    return k, v
+
+
+def attn_kv4(q, pk, pv, pks, pvs, block_tables, ctx_lens, layer: int, rope_cs=None, cu_q=None,
+             out=None):
+    """Attention over a paged cache in 4 bits: q [T][Hq*128] (or [T][Hq][128]) fp32 or fp16,
+    rotated at its rows' positions (rope_cs, None: not), each row attending to the positions
+    up to its own; the other arguments as kv4_append, which comes first. Returns out like q
+    (into `out` when given: rows behind the last sequence stay as they are; they are not
+    initialised otherwise). Rows that see no token are zeros."""
+    dev = _dev()
+    T = q.shape[0]
+    pools, where, seqs = _kv4_cache(pk, pv, pks, pvs, block_tables, ctx_lens, cu_q, layer, T, dev)
+    cols = math.prod(q.shape[1:])
+    Hkv = where[3]
+    if cols % 128 or (cols // 128) % Hkv:
+        raise ValueError(f"q: {tuple(q.shape)}, not rows of heads of 128 over {Hkv} kv heads")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError(f"out: {tuple(out.shape)}, q: {tuple(q.shape)}")
+    if not T:
+        return out
+    L, Hq = _lib.load(), cols // 128
+    dt, qs, os = _dtype_code(q), _row_stride(q, cols, "q"), _row_stride(out, cols, "out")
+    nbytes = L.tenzo_hip_attn_kv4_ws_bytes(T, seqs[5], Hq, Hkv, seqs[2])
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device).data_ptr() if nbytes else None
+    _lib.check(L.tenzo_hip_attn_kv4(
+        _on(q, dev, q.dtype, "q"), dt, qs, *pools, *where[:3], Hq, Hkv, *seqs,
+        *_rope_rows(rope_cs, dev), _on(out, dev, q.dtype, "out"), os, ws, nbytes, _stream()),
+        "attn_kv4")
+    return out
+
+
 # -------------------------------------------------------- quantized GEMV ---
 
 def gemv_q4_0(act: torch.Tensor, w: torch.Tensor, K: int, N: int) -> torch.Tensor:
@@ -340,6 +496,73 @@ def sample_top_k_top_p(logits: torch.Tensor, top_k: int, top_p: float, temperatu
         _ptr(logits), logits.numel(), int(top_k), float(top_p), float(temperature), float(r),
         _ptr(out), _stream()), "sample_top_k_top_p")
     return int(out.item())
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int):
+    """The best k continuations of each request: logits [B][W][V] fp32 (beams any stride
+    apart), scores [B][W] fp32, the beams' running log-probabilities. Returns (scores [B][k]
+    fp32, beams [B][k] int32, tokens [B][k] int32) of the candidates scores + log_softmax(
+    logits), compared in 64 bits, in falling order; among equal ones the lower beam, then the
+    larger logit, then the lower token comes first. NaN and +inf count as -inf, which comes
+    last."""
+    dev = _dev()
+    if logits.dim() != 3 or scores.shape != logits.shape[:2]:
+        raise ValueError(f"logits [B][W][V] and scores [B][W]: {tuple(logits.shape)}, "
+                         f"{tuple(scores.shape)}")
+    B, W, V = logits.shape
+    ld = logits.stride(1) if W > 1 else logits.stride(0) if B > 1 else V
+    if (V > 1 and logits.stride(2) != 1) or (B > 1 and logits.stride(0) != W * ld):
+        raise ValueError(f"logits: strides {logits.stride()}")
+    lp = _on(logits, dev, torch.float32, "logits")
+    sp = _whole(scores, dev, torch.float32, "scores")
+    L = _lib.load()
+    nbytes = L.tenzo_hip_beam_select_ws_bytes(B, W, V, k)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+    out = torch.empty((B, k), dtype=torch.float32, device=logits.device)
+    beams = torch.empty((B, k), dtype=torch.int32, device=logits.device)
+    tokens = torch.empty_like(beams)
+    _lib.check(L.tenzo_hip_beam_select(lp, ld, sp, B, W, V, k, out.data_ptr(), beams.data_ptr(),
+                                       tokens.data_ptr(), ws.data_ptr(), nbytes, _stream()),
+               "beam_select")
+    return out, beams, tokens
+
+
+def beam_reorder_paged(parents, block_tables, ctx_lens, pk, pv, pks, pvs) -> None:
+    """Reorders the paged caches of B requests with W beams in place: slot i of request b goes
+    on from slot parents[b][i] (int32 [B][W], for instance beams[:, :W] of beam_select).
+
+    block_tables int32 [B*W][pages] and ctx_lens int32 [B*W] (the beams of a request have one
+    length c): table entries of full pages (below c // 16) are taken from the parent, the c %
+    16 rows of the page in progress are copied into the slot's own page c // 16, in all layers
+    and heads. A slot's pages from c // 16 on have to be its own. Pools of kv4_pool or of the
+    int8 paged cache (codes [blocks][layers][kv heads][16][128] int8, scales [..][16] fp32)."""
+    dev = _dev()
+    if parents.dim() != 2 or (parents.shape[1] > 1 and parents.stride(1) != 1):
+        raise ValueError("parents: a row of W slots per request")
+    B, W = parents.shape
+    if block_tables.dim() != 2 or block_tables.shape[0] != B * W or (
+            block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+        raise ValueError(f"block_tables: {tuple(block_tables.shape)}, not a row of page numbers "
+                         f"for each of {B} x {W} beams")
+    if ctx_lens.shape != (B * W,):
+        raise ValueError(f"ctx_lens: {tuple(ctx_lens.shape)}, not ({B * W},)")
+    shape = tuple(pk.shape)
+    kv4 = pk.dtype == torch.uint8
+    code, scale = (torch.uint8, torch.uint8) if kv4 else (torch.int8, torch.float32)
+    if len(shape) != 5 or shape[3:] != (KV4_PAGE, 64 if kv4 else 128) or pv.shape != shape:
+        raise ValueError(f"pk, pv: {shape}, {tuple(pv.shape)}")
+    want = shape[:4] + ((4,) if kv4 else ())
+    if pks.shape != want or pvs.shape != want:
+        raise ValueError(f"pks, pvs: {tuple(pks.shape)}, {tuple(pvs.shape)}, not {want}")
+    width = block_tables.shape[1]
+    _lib.check(_lib.load().tenzo_hip_beam_reorder_paged(
+        _on(parents, dev, torch.int32, "parents"), parents.stride(0) if B > 1 else W,
+        _on(block_tables, dev, torch.int32, "block_tables"),
+        block_tables.stride(0) if B * W > 1 else width, width,
+        _whole(ctx_lens, dev, torch.int32, "ctx_lens"), B, W, _whole(pk, dev, code, "pk"),
+        _whole(pv, dev, code, "pv"), _whole(pks, dev, scale, "pks"),
+        _whole(pvs, dev, scale, "pvs"), shape[0], shape[1], shape[2], 64 if kv4 else 128,
+        _stream()), "beam_reorder_paged")
 
 
 def embed_i8(w_packed, scales, token: torch.Tensor, V: int, H: int) -> torch.Tensor:
