@@ -194,7 +194,8 @@ TENZO_HIP_API int tenzo_hip_attn_paged_int8_decode(const float* q, const float* 
 
 /* No counterpart in the reference. A cache row of 128 values is four groups of
  * 32, each 32 E2M1 codes (0 .5 1 1.5 2 3 4 6, bit 3 the sign) times 2^(s - 127)
- * with a scale byte s of its own (E8M0): pools of 16-token pages as
+ * with a scale byte s of its own (E8M0; bytes above 252, which append never
+ * writes, count as 0): pools of 16-token pages as
  * tenzo_hip_attn_paged_int8_decode has them, codes pk / pv
  * [n_blocks][n_layers][Hkv][16][64] (byte i: dim 2i low, dim 2i + 1 high) and
  * scales pks / pvs [n_blocks][n_layers][Hkv][16][4]; code pools 16-byte
@@ -246,7 +247,7 @@ TENZO_HIP_API int tenzo_hip_kv4_read(const uint8_t* pk, const uint8_t* pv, const
  * of tenzo_hip_attn_kv4_ws_bytes(...) bytes, 16-byte aligned, of this call
  * alone until it has run (null where that is 0). */
 TENZO_HIP_API size_t tenzo_hip_attn_kv4_ws_bytes(int64_t T, int B, int Hq, int Hkv,
-                                                 int table_width);
+                                                 int table_width, int has_cu, int dtype);
 TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,
                                      const uint8_t* pk, const uint8_t* pv, const uint8_t* pks,
                                      const uint8_t* pvs, int64_t n_blocks, int n_layers,

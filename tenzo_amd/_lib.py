@@ -44,7 +44,7 @@ SIGNATURES = {
                                   _I64, _I, _P, _P, _I, _I64, _P, _I, _P]),
     "tenzo_hip_kv4_read": (_I, [_P, _P, _P, _P, _I64, _I, _I, _I, _P, _I64, _I, _P, _P, _I, _I64,
                                 _P, _P, _I, _P]),
-    "tenzo_hip_attn_kv4_ws_bytes": (_SZ, [_I64, _I, _I, _I, _I]),
+    "tenzo_hip_attn_kv4_ws_bytes": (_SZ, [_I64, _I, _I, _I, _I, _I, _I]),
     "tenzo_hip_attn_kv4": (_I, [_P, _I, _I64, _P, _P, _P, _P, _I64, _I, _I, _I, _I, _P, _I64, _I,
                                 _P, _P, _I, _I64, _P, _I, _P, _I64, _P, _SZ, _P]),
     "tenzo_hip_beam_select_ws_bytes": (_SZ, [_I, _I, _I64, _I]),

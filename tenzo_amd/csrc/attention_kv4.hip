@@ -8,6 +8,11 @@ namespace {
 
 constexpr float kQkScale = 0.08838834764831845f;  // 1/sqrt(128)
 
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kTile = 64;           // tokens of a wave's step
+constexpr int kMaxPages = 1024;     // pages of a workgroup's part of the context
+constexpr int kVStride = 144;       // bf16 of a value row in LDS: 288 bytes, 8 rows over all banks
+
 struct Kv4Attn {
     const void* q;
     void* out;
@@ -17,77 +22,544 @@ struct Kv4Attn {
     const uint8_t* pks;
     const uint8_t* pvs;
     const float* rope;
-    int G;
+    float* part_o;   // [T * Hq][splits][128]
+    float2* part_ml; // [T * Hq][splits]: maximum (base 2) and sum
+    int G, Hq, T;
+    int chunk, splits;  // tokens of a split
+    int vec;            // q, out and rope allow 16-byte accesses
 };
 
-// The plain form: a workgroup per (row, query head), a token to a thread, 256 at a time with the
-// running maximum and sum of the softmax.
-template <bool HALF>
-__global__ void __launch_bounds__(256) kv4_attn_plain_kernel(Kv4Attn a, Kv4Seqs sq) {
-    __shared__ float qs[kKv4Dim], ps[256], red[4];
-    __shared__ int64_t rows[256];
-    const int tid = threadIdx.x, row = blockIdx.x, qh = blockIdx.y, h = qh / a.G;
-    int seq, pos;
-    const bool there = kv4_place(sq, row, tid & 15, seq, pos);
-    if (!there) {
-        if (seq < sq.B && (!sq.cu || row >= sq.cu[0]) && tid < kKv4Dim)
-            st_act<HALF>(a.out, row * a.out_stride + (int64_t)qh * kKv4Dim + tid, 0.0f);
-        return;
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+union Frag {
+    uint32_t w[4];
+    bf16x8 v;
+};
+
+template <int CTRL>
+__device__ __forceinline__ float ror16(float v) {  // rotation within 16 lanes
+    return dpp_f<CTRL>(v);
+}
+constexpr int kDppRor4 = 0x124, kDppRor8 = 0x128;
+
+// Both halves' (quarters') values of x in every lane: {x of lane l % 32, x of that + 32}, and
+// {x of the lower, x of the upper lane of the pair l, l ^ 16}.
+__device__ __forceinline__ void halves(float x, float& lo, float& hi) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                    false);
+    lo = __uint_as_float(r[0]);
+    hi = __uint_as_float(r[1]);
+}
+__device__ __forceinline__ void quarters(float x, float& lo, float& hi) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                    false);
+    lo = __uint_as_float(r[0]);
+    hi = __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float max_quarters(float x) {
+    float a, b;
+    halves(x, a, b);
+    quarters(fmaxf(a, b), a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float sum_quarters(float x) {
+    float a, b;
+    halves(x, a, b);
+    quarters(a + b, a, b);
+    return a + b;
+}
+
+// The upper halves of two floats (bf16 towards zero), a in the low half.
+__device__ __forceinline__ uint32_t pack_hi(float a, float b) {
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+__device__ __forceinline__ float masked(float v, uint32_t m) {
+    return __uint_as_float(__float_as_uint(v) & m);
+}
+
+// Sequence and row tile of a work unit: the unit-th tile when every sequence has
+// ceil(rows * G / RT) of them. False past the last.
+__device__ __forceinline__ bool find_unit(const Kv4Seqs& sq, int unit, int G, int RT, int& seq,
+                                          int& tile) {
+    if (!sq.cu) {
+        const int per = (G + RT - 1) / RT;
+        seq = unit / per;
+        tile = unit - seq * per;
+        return seq < sq.B;
     }
-    if (tid < 64) {
-        const int64_t at = row * a.q_stride + (int64_t)qh * kKv4Dim + tid;
-        float x0 = ld_act<HALF>(a.q, at), x1 = ld_act<HALF>(a.q, at + 64);
-        if (a.rope) {
-            const float* cs = a.rope + (int64_t)pos * kKv4Dim + tid;
-            const float c = cs[0], s = cs[64], y0 = x0;
-            x0 = __builtin_fmaf(x0, c, -__fmul_rn(x1, s));
-            x1 = __builtin_fmaf(y0, s, __fmul_rn(x1, c));
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < sq.B; base += 64) {
+        const int b = base + lane;
+        int n = 0;
+        if (b < sq.B) n = max(0, sq.cu[b + 1] - sq.cu[b]);
+        const int nt = (int)(((int64_t)n * G + RT - 1) / RT);
+        int incl = nt;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(incl, d);
+            if (lane >= d) incl += o;
         }
-        qs[tid] = __fmul_rn(x0, kQkScale);
-        qs[tid + 64] = __fmul_rn(x1, kQkScale);
+        const uint64_t past = __ballot(incl > unit);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            seq = base + l;
+            tile = unit - __builtin_amdgcn_readlane(incl - nt, l);
+            return true;
+        }
+        unit -= __builtin_amdgcn_readlane(incl, 63);
     }
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (int t0 = 0; t0 <= pos; t0 += 256) {
-        const int t = t0 + tid;
-        float s = -INFINITY;
-        int64_t r = -1;
-        if (t <= pos) {
-            const int64_t base = sq.page_base(seq, t / kKv4Page);
-            if (base >= 0) {
-                r = base + h * kKv4Page + t % kKv4Page;
-                s = 0.0f;
-                for (int w = 0; w < 16; ++w) {
-                    float v[8];
-                    fp4_to_float8(reinterpret_cast<const uint32_t*>(a.pk + r * kKv4Row)[w],
-                                  e8m0_to_float(a.pks[r * kKv4Scales + w / 4]), v);
-                    for (int j = 0; j < 8; ++j) s = __builtin_fmaf(qs[8 * w + j], v[j], s);
+    return false;
+}
+
+// One workgroup: RT = ROWS * RW rows (token, query head of one kv head) of a sequence against a
+// part of its tokens. Wave w has the rows group w % RW and every (4 / RW)-th step of 64 tokens.
+//
+// Scores come transposed, S^T = K Q^T, so that a lane keeps one row: K is the A operand (16
+// tokens x 32 dims: the lane's 16 code bytes are a token's group of 32 dims, one scale, four
+// steps of 8 dims), Q the B operand. In S^T's layout a lane holds 4 tokens of its row per 16,
+// which is what the B operand of O^T = V^T P^T wants when the value rows are taken in the same
+// order: no weight changes lanes. V^T comes from value rows in LDS (bf16, private to the wave)
+// by transposing reads. Codes times scale are exact in bf16; queries and weights are split into
+// NP parts of 8 bits (fp32: 3, every bit; fp16: 2). With ROWS < 16 the parts stand in columns
+// side by side (column = part * ROWS + row) and one MFMA serves all of them.
+template <int ROWS, int NP, int RW, bool HALF>
+__global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
+    constexpr int SLOTS = 16 / ROWS, NM = SLOTS == 1 ? NP : 1, TW = 4 / RW, RT = ROWS * RW;
+    static_assert(SLOTS == 1 || SLOTS >= NP, "a column for each part");
+    __shared__ __align__(16) uint16_t vbuf[4][32 * kVStride];
+    __shared__ float2 ml[4][16];
+    __shared__ int pg[kMaxPages];
+    static_assert(sizeof(vbuf[0]) >= 16 * kKv4Dim * 4, "the rows' sums fit a wave's part");
+
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, j = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rw = wave % RW, tw = wave / RW;
+    const int per_unit = sq.Hkv * a.splits;
+    const int unit = blockIdx.x / per_unit, rest = blockIdx.x - unit * per_unit;
+    const int split = rest / sq.Hkv, h = rest - split * sq.Hkv;
+    int seq, tile;
+    if (!find_unit(sq, unit, a.G, RT, seq, tile)) return;
+    int n = 1, first = seq;
+    if (sq.cu) {
+        first = sq.cu[seq];
+        n = sq.cu[seq + 1] - first;
+    }
+    const int c = sq.length(seq);
+    const int row0 = tile * RT;                       // of the sequence's n * G
+    const int last_i = min(n - 1, (row0 + RT - 1) / a.G);
+    const int t0 = split * a.chunk;
+    const int t1 = min(min(t0 + a.chunk, c - n + last_i + 1), c);  // tokens that some row sees
+    if (split > 0 && t0 >= t1) return;
+
+    // the lane's row
+    const int slot = col / ROWS, r = row0 + rw * ROWS + col % ROWS;
+    const int qi = r / a.G, head = h * a.G + (r - qi * a.G);
+    const bool row_ok = qi < n && first >= 0 && first + qi < a.T;
+    const int pos = row_ok && c > 0 ? c - n + qi : -1;
+    const int64_t grow = (int64_t)first + qi;
+
+    const int npg = t1 > t0 ? (t1 - t0 + kKv4Page - 1) / kKv4Page : 0;
+    for (int p = tid; p < npg; p += 256) {
+        const int blk = sq.tables[(int64_t)seq * sq.table_stride + t0 / kKv4Page + p];
+        pg[p] = blk >= 0 && blk < sq.n_blocks ? blk : -1;
+    }
+
+    // Q: the lane's 32 dims 32j .. 32j + 31, rotated with those 64 away (lane ^ 32)
+    Frag qf[NM][4];
+    {
+        float x[32];
+        const int64_t at = grow * a.q_stride + (int64_t)head * kKv4Dim + 32 * j;
+        if (pos < 0) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = 0.0f;
+        } else if (!HALF && a.vec) {
+            const float4* p = reinterpret_cast<const float4*>((const float*)a.q + at);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float4 v = p[e];
+                x[4 * e] = v.x, x[4 * e + 1] = v.y, x[4 * e + 2] = v.z, x[4 * e + 3] = v.w;
+            }
+        } else if (HALF && a.vec) {
+            const uint4* p = reinterpret_cast<const uint4*>((const uint16_t*)a.q + at);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint4 v = p[e];
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    x[8 * e + 2 * k] = half_bits_to_float((uint16_t)w[k]);
+                    x[8 * e + 2 * k + 1] = half_bits_to_float((uint16_t)(w[k] >> 16));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = ld_act<HALF>(a.q, at + e);
+        }
+        if (a.rope) {
+            const float* cs = a.rope + (int64_t)max(pos, 0) * kKv4Dim + 32 * (j & 1);
+            const bool upper = lane >= 32;
+            if (pos < 0) cs = a.rope;  // (zeros stay zeros; row 0 may not exist: not read)
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+                float cv[4] = {1.0f, 1.0f, 1.0f, 1.0f}, sv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (pos >= 0) {
+                    if (a.vec) {
+                        const float4 u = *reinterpret_cast<const float4*>(cs + e);
+                        const float4 w = *reinterpret_cast<const float4*>(cs + 64 + e);
+                        cv[0] = u.x, cv[1] = u.y, cv[2] = u.z, cv[3] = u.w;
+                        sv[0] = w.x, sv[1] = w.y, sv[2] = w.z, sv[3] = w.w;
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) cv[k] = cs[e + k], sv[k] = cs[64 + e + k];
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float x0, x1;
+                    halves(x[e + k], x0, x1);
+                    // lower dims x0 c - x1 s, upper ones x0 s + x1 c
+                    const float u = upper ? sv[k] : cv[k], w = upper ? cv[k] : -sv[k];
+                    x[e + k] = __builtin_fmaf(x0, u, __fmul_rn(x1, w));
                 }
             }
         }
-        const float mc = fmaxf(m, block256_max(s, red));
-        const float scale = m == -INFINITY ? 0.0f : expf(m - mc);
-        ps[tid] = r < 0 ? 0.0f : expf(s - mc);
-        rows[tid] = r;
-        m = mc;
-        __syncthreads();
-        l *= scale;
-        o *= scale;
-        for (int i = 0; i < 256; ++i) {
-            if (rows[i] < 0) continue;
-            l += ps[i];
-            if (tid < kKv4Dim) {
-                const uint32_t c = (a.pv[rows[i] * kKv4Row + tid / 2] >> (4 * (tid & 1))) & 15;
-                const f32x2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(
-                    c, e8m0_to_float(a.pvs[rows[i] * kKv4Scales + tid / 32]), 0);
-                o = __builtin_fmaf(ps[i], v.x, o);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = __fmul_rn(x[e], kQkScale * kLog2e);
+        // part p of a value: what its parts before leave, cut to 8 bits
+        if (SLOTS > 1) {
+            const uint32_t m1 = slot >= 1 ? 0xffff0000u : 0, m2 = slot >= 2 ? 0xffff0000u : 0;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+                x[e] -= masked(x[e], m1);
+                if (NP == 3) x[e] -= masked(x[e], m2);
+                if (slot >= NP) x[e] = 0.0f;
             }
         }
-        __syncthreads();
+#pragma unroll
+        for (int p = 0; p < NM; ++p)
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+                qf[p][e >> 3].w[(e >> 1) & 3] = pack_hi(x[e], x[e + 1]);
+                x[e] -= masked(x[e], 0xffff0000u);
+                x[e + 1] -= masked(x[e + 1], 0xffff0000u);
+            }
     }
-    if (tid < kKv4Dim)
-        st_act<HALF>(a.out, row * a.out_stride + (int64_t)qh * kKv4Dim + tid,
-                     l > 0.0f || l != l ? o / l : 0.0f);
+    __syncthreads();
+
+    f32x4 acc[8];
+#pragma unroll
+    for (int d = 0; d < 8; ++d) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+
+    uint4 kr[4], vr[4];
+    uint32_t ksc[4], vsc[4];
+    int ids[4];
+    const uint32_t lane_code = (uint32_t)(col * kKv4Row + j * 16);
+    const uint32_t lane_scale = (uint32_t)(col * kKv4Scales + j);
+    auto page_row = [&](int t, int tt) -> int64_t {
+        const int p = min(((t - t0) >> 4) + tt, npg - 1);
+        const int id = __builtin_amdgcn_readfirstlane(pg[p]);
+        ids[tt] = id;
+        return (((int64_t)max(id, 0) * sq.n_layers + sq.layer) * sq.Hkv + h) * kKv4Page;
+    };
+    auto load_k = [&](int t) {
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+            const int64_t row = page_row(t, tt);
+            kr[tt] = *reinterpret_cast<const uint4*>(a.pk + row * kKv4Row + lane_code);
+            ksc[tt] = (a.pks + row * kKv4Scales)[lane_scale];
+        }
+    };
+    auto load_v = [&](int t) {
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+            const int64_t row = page_row(t, tt);
+            vr[tt] = *reinterpret_cast<const uint4*>(a.pv + row * kKv4Row + lane_code);
+            vsc[tt] = (a.pvs + row * kKv4Scales)[lane_scale];
+        }
+    };
+    uint16_t* vb = vbuf[wave];
+    const uint32_t vw = (uint32_t)(col * kVStride + j * 32);
+    const uint32_t vrd = (uint32_t)((4 * j + (col >> 2)) * kVStride + (col & 3) * 4);
+
+    int t = t0 + kTile * tw;
+    const bool any = sq.n_blocks > 0;
+    if (t < t1 && any) {
+        load_k(t);
+        load_v(t);
+    }
+    for (; t < t1 && any; t += kTile * TW) {
+        const int next = t + kTile * TW;
+        f32x4 s[4];
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+            const float sc = e8m0_to_float(ksc[tt]);
+            const uint32_t w[4] = {kr[tt].x, kr[tt].y, kr[tt].z, kr[tt].w};
+            s[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int st = 0; st < 4; ++st) {
+                union {
+                    bf16x2 p[4];
+                    bf16x8 v;
+                } kf;
+                kf.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 0);
+                kf.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 1);
+                kf.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 2);
+                kf.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 3);
+#pragma unroll
+                for (int p = 0; p < NM; ++p)
+                    s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf.v, qf[p][st].v, s[tt], 0, 0,
+                                                                    0);
+            }
+        }
+        bool bad = false;
+        int id_now[4];
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+            const int p = ((t - t0) >> 4) + tt;
+            id_now[tt] = p < npg ? __builtin_amdgcn_readfirstlane(pg[p]) : -1;
+            bad = bad || id_now[tt] < 0;
+        }
+        if (next < t1) load_k(next);
+        float top = -INFINITY;
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v = s[tt][i];
+                if (ROWS == 4) v += ror16<kDppRor8>(v);
+                if (ROWS == 4) v += ror16<kDppRor4>(v);
+                if (ROWS == 8) v += ror16<kDppRor8>(v);
+                s[tt][i] = v;
+            }
+        // a step that a row may not see whole: past its position, or absent pages
+        if (bad || t + kTile - 1 > c - n + row0 / a.G) {
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (id_now[tt] < 0 || t + 16 * tt + 4 * j + i > pos) s[tt][i] = -INFINITY;
+        }
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[tt][i]);
+        const float mn = fmaxf(m, max_quarters(top));
+        const float base = mn == -INFINITY ? 0.0f : mn;
+        const float alpha = __builtin_amdgcn_exp2f(m - base);
+        m = mn;
+        if (__ballot(alpha != 1.0f)) {
+#pragma unroll
+            for (int d = 0; d < 8; ++d) acc[d] *= alpha;
+            l *= alpha;
+        }
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[tt][i] = __builtin_amdgcn_exp2f(s[tt][i] - base);
+                l += s[tt][i];
+            }
+        const uint32_t m1 = slot >= 1 ? 0xffff0000u : 0, m2 = slot >= 2 ? 0xffff0000u : 0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            // 32 value rows, by two 16-token pages
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int tt = 2 * u + k;
+                const float sc = e8m0_to_float(vsc[tt]);
+                const uint32_t w[4] = {vr[tt].x, vr[tt].y, vr[tt].z, vr[tt].w};
+#pragma unroll
+                for (int st = 0; st < 4; ++st) {
+                    union {
+                        bf16x2 p[4];
+                        uint4 v;
+                    } f;
+                    f.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 0);
+                    f.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 1);
+                    f.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 2);
+                    f.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 3);
+                    *reinterpret_cast<uint4*>(vb + vw + k * 16 * kVStride + st * 8) = f.v;
+                }
+            }
+            if (u == 1 && next < t1) load_v(next);
+            Frag pf[NM];
+            float p8[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                p8[e] = s[2 * u + (e >> 2)][e & 3];
+                if (SLOTS > 1) {
+                    p8[e] -= masked(p8[e], m1);
+                    if (NP == 3) p8[e] -= masked(p8[e], m2);
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < NM; ++p)
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    pf[p].w[e >> 1] = pack_hi(p8[e], p8[e + 1]);
+                    p8[e] -= masked(p8[e], 0xffff0000u);
+                    p8[e + 1] -= masked(p8[e + 1], 0xffff0000u);
+                }
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+                typedef __attribute__((address_space(3))) s16x4* lds4;
+                union {
+                    s16x4 h[2];
+                    bf16x8 v;
+                } vf;
+                vf.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vb + vrd + d * 16));
+                vf.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds4)(vb + vrd + 16 * kVStride + d * 16));
+#pragma unroll
+                for (int p = 0; p < NM; ++p)
+                    acc[d] =
+                        __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.v, pf[p].v, acc[d], 0, 0, 0);
+            }
+        }
+    }
+
+    l = sum_quarters(l);
+    if (SLOTS > 1) {
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v = slot < NP ? acc[d][i] : 0.0f;
+                v += ror16<kDppRor8>(v);
+                if (ROWS == 4) v += ror16<kDppRor4>(v);
+                acc[d][i] = v;
+            }
+    }
+    if (TW > 1) {
+        // the waves' sums meet: every wave's rows in its own part of the value buffer
+        float* o = reinterpret_cast<float*>(vb);
+        if (slot == 0) {
+#pragma unroll
+            for (int d = 0; d < 8; ++d)
+                *reinterpret_cast<f32x4*>(o + col * kKv4Dim + 16 * d + 4 * j) = acc[d];
+            if (j == 0) ml[wave][col] = make_float2(m, l);
+        }
+        __syncthreads();
+        for (int it = tid; it < RT * 32; it += 256) {
+            const int rr = it >> 5, d4 = it & 31, grp = rr / ROWS, cc = rr % ROWS;
+            const int r2 = row0 + rr, i2 = r2 / a.G;
+            if (i2 >= n || first < 0 || first + i2 >= a.T) continue;
+            float M = -INFINITY, L = 0.0f;
+            f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < TW; ++w) M = fmaxf(M, ml[w * RW + grp][cc].x);
+            const float base = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+            for (int w = 0; w < TW; ++w) {
+                const float2 e = ml[w * RW + grp][cc];
+                const float f = __builtin_amdgcn_exp2f(e.x - base);
+                L += e.y * f;
+                v += f * *reinterpret_cast<const f32x4*>(
+                             reinterpret_cast<const float*>(vbuf[w * RW + grp]) + cc * kKv4Dim +
+                             4 * d4);
+            }
+            const int p2 = c > 0 ? c - n + i2 : -1;
+            const int64_t g2 = (int64_t)first + i2, hd = h * a.G + (r2 - i2 * a.G);
+            if (p2 < a.chunk || a.splits == 1) {
+                if (split == 0)
+                    for (int k = 0; k < 4; ++k)
+                        st_act<HALF>(a.out, g2 * a.out_stride + hd * kKv4Dim + 4 * d4 + k,
+                                     L != 0.0f ? v[k] / L : 0.0f);
+            } else {
+                const int64_t at = (g2 * a.Hq + hd) * a.splits + split;
+                *reinterpret_cast<f32x4*>(a.part_o + at * kKv4Dim + 4 * d4) = v;
+                if (d4 == 0) a.part_ml[at] = make_float2(M, L);
+            }
+        }
+    } else if (row_ok && slot == 0) {
+        if (pos < a.chunk || a.splits == 1) {
+            if (split == 0)
+#pragma unroll
+                for (int d = 0; d < 8; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        st_act<HALF>(a.out,
+                                     grow * a.out_stride + (int64_t)head * kKv4Dim + 16 * d +
+                                         4 * j + i,
+                                     l != 0.0f ? acc[d][i] / l : 0.0f);
+        } else {
+            const int64_t at = (grow * a.Hq + head) * a.splits + split;
+#pragma unroll
+            for (int d = 0; d < 8; ++d)
+                *reinterpret_cast<f32x4*>(a.part_o + at * kKv4Dim + 16 * d + 4 * j) = acc[d];
+            if (j == 0) a.part_ml[at] = make_float2(m, l);
+        }
+    }
+}
+
+// Joins the splits of a row and head: 32 lanes x 4 dims, 16 groups of splits.
+template <bool HALF>
+__global__ void __launch_bounds__(512) kv4_join_kernel(Kv4Attn a, Kv4Seqs sq) {
+    __shared__ f32x4 ov[16][32];
+    __shared__ float lv[16];
+    const int row = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
+    int seq, pos;
+    if (!kv4_place(sq, row, tid & 15, seq, pos) || pos < a.chunk) return;
+    const int ns = pos / a.chunk + 1;
+    const int64_t at = ((int64_t)row * a.Hq + head) * a.splits;
+    const float2* ml = a.part_ml + at;
+    float M = -INFINITY;
+    for (int s = 0; s < ns; ++s) M = fmaxf(M, ml[s].x);
+    const float base = M == -INFINITY ? 0.0f : M;
+    const int d4 = tid & 31, g = tid >> 5;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    float L = 0.0f;
+    for (int s = g; s < ns; s += 16) {
+        const float2 e = ml[s];
+        const float f = __builtin_amdgcn_exp2f(e.x - base);
+        L += e.y * f;
+        v += f * *reinterpret_cast<const f32x4*>(a.part_o + (at + s) * kKv4Dim + 4 * d4);
+    }
+    ov[g][d4] = v;
+    if (d4 == 0) lv[g] = L;
+    __syncthreads();
+    if (g == 0) {
+        for (int k = 1; k < 16; ++k) v += ov[k][d4], L += lv[k];
+        for (int k = 0; k < 4; ++k)
+            st_act<HALF>(a.out, row * a.out_stride + (int64_t)head * kKv4Dim + 4 * d4 + k,
+                         L != 0.0f ? v[k] / L : 0.0f);
+    }
+}
+
+// Rows of a workgroup, tokens of a split and how many splits, from what the host knows.
+struct Kv4Plan {
+    int rows, rw, splits, chunk;
+    int64_t units;
+};
+Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, bool half) {
+    Kv4Plan p{};
+    const int64_t per = cu ? ceil_div(T * G, B) : G;  // rows of an average sequence
+    const int packed = half ? 8 : 4;
+    p.rows = per <= packed ? packed : 16;
+    p.rw = per <= 16 ? 1 : per <= 32 ? 2 : 4;
+    const int rt = p.rows * p.rw;
+    p.units = cu ? T * G / rt + B : (int64_t)B * ceil_div(G, rt);
+    const int64_t ctx = (int64_t)table_width * kKv4Page;
+    const int64_t step = kTile * (4 / p.rw);
+    // enough workgroups for every CU to have two, each wave a step of tokens at least
+    int64_t s = ceil_div(512, p.units * Hkv);
+    s = s < ceil_div(ctx, step) ? s : ceil_div(ctx, step);
+    if (s < 1) s = 1;
+    int64_t chunk = ceil_div(ceil_div(ctx, s), step) * step;
+    if (chunk > kMaxPages * kKv4Page) chunk = kMaxPages * kKv4Page;
+    if (chunk < step) chunk = step;
+    p.chunk = (int)chunk;
+    p.splits = ctx > 0 ? (int)ceil_div(ctx, chunk) : 1;
+    return p;
+}
+
+template <int ROWS, int NP, int RW, bool HALF>
+void launch_kv4(const Kv4Attn& a, const Kv4Seqs& s, dim3 grid, hipStream_t st) {
+    hipLaunchKernelGGL((kv4_attn_kernel<ROWS, NP, RW, HALF>), grid, dim3(256), 0, st, a, s);
 }
 
 }  // namespace
@@ -98,8 +570,10 @@ using namespace tz;
 extern "C" {
 
 TENZO_HIP_API size_t tenzo_hip_attn_kv4_ws_bytes(int64_t T, int B, int Hq, int Hkv,
-                                                 int table_width) {
-    return 0;
+                                                 int table_width, int has_cu, int dtype) {
+    if (T <= 0 || B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || table_width < 0) return 0;
+    const Kv4Plan p = kv4_plan(T, B, Hq / Hkv, Hkv, table_width, has_cu != 0, dtype != 0);
+    return p.splits > 1 ? (size_t)T * Hq * p.splits * (kKv4Dim * 4 + 8) : 0;
 }
 
 TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,
@@ -124,18 +598,64 @@ TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,
     TZ_CHECK(T == 1 || (q_stride >= (int64_t)Hq * kKv4Dim && out_stride >= (int64_t)Hq * kKv4Dim),
              "attn_kv4: row strides %lld, %lld below %d heads", (long long)q_stride,
              (long long)out_stride, Hq);
-    const size_t need = tenzo_hip_attn_kv4_ws_bytes(T, B, Hq, Hkv, table_width);
-    TZ_CHECK(need == 0 || (ws && ws_bytes >= need), "attn_kv4: %zu bytes of workspace needed, %zu given",
-             need, ws ? ws_bytes : 0);
-    Kv4Attn a{q, out, q_stride, out_stride, pk, pv, pks, pvs, rope_cs, Hq / Hkv};
-    const dim3 grid((unsigned)T, (unsigned)Hq);
+    const size_t need = tenzo_hip_attn_kv4_ws_bytes(T, B, Hq, Hkv, table_width, cu_q != nullptr,
+                                                    dtype);
+    TZ_CHECK(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0),
+             "attn_kv4: %zu bytes of workspace needed, 16-byte aligned, %zu given", need,
+             ws ? ws_bytes : 0);
+    const int G = Hq / Hkv;
+    const Kv4Plan p = kv4_plan(T, B, G, Hkv, table_width, cu_q != nullptr, dtype != 0);
+    const int64_t wgs = p.units * p.splits * Hkv;
+    TZ_CHECK(wgs <= 0xffffff && T <= 0x7fffff && Hq <= 65535, "attn_kv4: %lld rows of %d heads",
+             (long long)T, Hq);
+    Kv4Attn a{};
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.pk = pk;
+    a.pv = pv;
+    a.pks = pks;
+    a.pvs = pvs;
+    a.rope = rope_cs;
+    a.part_o = (float*)ws;
+    a.part_ml = (float2*)((char*)ws + (size_t)T * Hq * p.splits * kKv4Dim * 4);
+    a.G = G;
+    a.Hq = Hq;
+    a.T = (int)T;
+    a.chunk = p.chunk;
+    a.splits = p.splits;
+    const int64_t esize = dtype ? 2 : 4;
+    a.vec = (((uintptr_t)q | (uintptr_t)rope_cs | (uintptr_t)(q_stride * esize)) & 15) == 0;
+    hipStream_t st = (hipStream_t)stream;
+    const dim3 grid((unsigned)wgs);
+    if (dtype) {
+        if (p.rows == 8)
+            launch_kv4<8, 2, 1, true>(a, s, grid, st);
+        else if (p.rw == 1)
+            launch_kv4<16, 2, 1, true>(a, s, grid, st);
+        else if (p.rw == 2)
+            launch_kv4<16, 2, 2, true>(a, s, grid, st);
+        else
+            launch_kv4<16, 2, 4, true>(a, s, grid, st);
+    } else {
+        if (p.rows == 4)
+            launch_kv4<4, 3, 1, false>(a, s, grid, st);
+        else if (p.rw == 1)
+            launch_kv4<16, 3, 1, false>(a, s, grid, st);
+        else if (p.rw == 2)
+            launch_kv4<16, 3, 2, false>(a, s, grid, st);
+        else
+            launch_kv4<16, 3, 4, false>(a, s, grid, st);
+    }
+    const int rc2 = launch_status("kv4_attn_kernel");
+    if (rc2 || p.splits == 1) return rc2;
+    const dim3 jgrid((unsigned)T, (unsigned)Hq);
     if (dtype)
-        hipLaunchKernelGGL(kv4_attn_plain_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream,
-                           a, s);
+        hipLaunchKernelGGL(kv4_join_kernel<true>, jgrid, dim3(512), 0, st, a, s);
     else
-        hipLaunchKernelGGL(kv4_attn_plain_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream,
-                           a, s);
-    return launch_status("kv4_attn_plain_kernel");
+        hipLaunchKernelGGL(kv4_join_kernel<false>, jgrid, dim3(512), 0, st, a, s);
+    return launch_status("kv4_join_kernel");
 }
 
 }  // extern "C"

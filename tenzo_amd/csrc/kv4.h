@@ -73,9 +73,10 @@ __device__ __forceinline__ bool kv4_place(const Kv4Seqs& q, int r, int lane16, i
     return i >= 0 && i < n && pos >= 0 && pos < c;
 }
 
-// 2^(s - 127) as fp32 (s = 255, which no append writes, is NaN as the format says).
+// 2^(s - 127) as fp32. Bytes above 252, which no append writes, count as 0: whatever a pool holds
+// is finite, so that a token with weight 0 adds nothing.
 __device__ __forceinline__ float e8m0_to_float(uint32_t s) {
-    return __uint_as_float(s == 0 ? 0x00400000u : s == 255 ? 0x7fc00000u : s << 23);
+    return __uint_as_float(s == 0 || s > 252 ? 0x00400000u : s << 23);
 }
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));

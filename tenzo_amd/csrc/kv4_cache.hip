@@ -213,7 +213,7 @@ TENZO_HIP_API int tenzo_hip_kv4_append(const void* k, const void* v, int dtype, 
              (long long)v_stride, Hkv);
     Kv4Append a{k, v, k_stride, v_stride, pk, pv, pks, pvs, rope_cs, T * Hkv * 2};
     const int64_t blocks = ceil_div(a.items, 16);
-    TZ_CHECK(blocks <= INT32_MAX, "kv4_append: %lld rows of %d heads", (long long)T, Hkv);
+    TZ_CHECK(blocks <= 0xffffff, "kv4_append: %lld rows of %d heads", (long long)T, Hkv);
     const dim3 grid((unsigned)blocks);
     if (dtype)
         hipLaunchKernelGGL(kv4_append_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, a, q);
@@ -240,7 +240,7 @@ TENZO_HIP_API int tenzo_hip_kv4_read(const uint8_t* pk, const uint8_t* pv, const
     TZ_CHECK(k_out && v_out, "kv4_read: null pointer");
     Kv4Read a{pk, pv, pks, pvs, k_out, v_out, T * Hkv * 2};
     const int64_t blocks = ceil_div(a.items, 16);
-    TZ_CHECK(blocks <= INT32_MAX, "kv4_read: %lld rows of %d heads", (long long)T, Hkv);
+    TZ_CHECK(blocks <= 0xffffff, "kv4_read: %lld rows of %d heads", (long long)T, Hkv);
     const dim3 grid((unsigned)blocks);
     if (dtype)
         hipLaunchKernelGGL(kv4_read_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, a, q);

@@ -379,7 +379,7 @@ def attn_kv4(q, pk, pv, pks, pvs, block_tables, ctx_lens, layer: int, rope_cs=No
         return out
     L, Hq = _lib.load(), cols // 128
     dt, qs, os = _dtype_code(q), _row_stride(q, cols, "q"), _row_stride(out, cols, "out")
-    nbytes = L.tenzo_hip_attn_kv4_ws_bytes(T, seqs[5], Hq, Hkv, seqs[2])
+    nbytes = L.tenzo_hip_attn_kv4_ws_bytes(T, seqs[5], Hq, Hkv, seqs[2], cu_q is not None, dt)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device).data_ptr() if nbytes else None
     _lib.check(L.tenzo_hip_attn_kv4(
         _on(q, dev, q.dtype, "q"), dt, qs, *pools, *where[:3], Hq, Hkv, *seqs,

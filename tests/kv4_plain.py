@@ -24,7 +24,7 @@ def quantize(x):
 def values(codes, scales):
     c = np.stack([codes & 15, codes >> 4], -1).reshape(*codes.shape[:-1], 4, 32)
     v = np.where(c & 8, -1.0, 1.0) * LEVELS[c & 7]
-    s = np.where(scales == 255, np.nan, np.ldexp(1.0, scales.astype(int) - 127))
+    s = np.ldexp(1.0, np.where(scales > 252, 0, scales.astype(int)) - 127)
     return (v * s[..., None]).reshape(*codes.shape[:-1], D)
 
 

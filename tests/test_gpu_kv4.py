@@ -27,7 +27,8 @@ def ops(torch_dev):
 
 
 class Setup:
-    """Sequences of (rows, length) over a pool whose slots that no sequence holds are NaN."""
+    """Sequences of (rows, length) over a pool whose slots that no sequence holds have scales of
+    2^125 and of no meaning."""
 
     def __init__(self, seqs, Hq, Hkv, layers=2, seed=0, extra=3, width=None, cu=True, rope=True,
                  dtype=np.float32, tail=0, fill=True):
@@ -48,7 +49,7 @@ class Setup:
         self.T = sum(n for n, _ in seqs) + tail
         shape = (self.nb, layers, Hkv, PAGE)
         codes = [rng.integers(0, 256, shape + (64,), dtype=np.uint8) for _ in range(2)]
-        scales = [np.full(shape + (4,), 255, np.uint8) for _ in range(2)]
+        scales = [rng.choice(np.array([252, 252, 255], np.uint8), shape + (4,)) for _ in range(2)]
         if fill:
             for b, (_, c) in enumerate(seqs):
                 for t0 in range(0, min(max(c, 0), width * PAGE), PAGE):
