@@ -45,30 +45,16 @@ __device__ __forceinline__ float ror16(float v) {  // rotation within 16 lanes
 }
 constexpr int kDppRor4 = 0x124, kDppRor8 = 0x128;
 
-// Both halves' (quarters') values of x in every lane: {x of lane l % 32, x of that + 32}, and
-// {x of the lower, x of the upper lane of the pair l, l ^ 16}.
-__device__ __forceinline__ void halves(float x, float& lo, float& hi) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
-                                                    false);
-    lo = __uint_as_float(r[0]);
-    hi = __uint_as_float(r[1]);
-}
-__device__ __forceinline__ void quarters(float x, float& lo, float& hi) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
-                                                    false);
-    lo = __uint_as_float(r[0]);
-    hi = __uint_as_float(r[1]);
-}
 __device__ __forceinline__ float max_quarters(float x) {
     float a, b;
-    halves(x, a, b);
-    quarters(fmaxf(a, b), a, b);
+    lane_halves(x, a, b);
+    lane_pairs16(fmaxf(a, b), a, b);
     return fmaxf(a, b);
 }
 __device__ __forceinline__ float sum_quarters(float x) {
     float a, b;
-    halves(x, a, b);
-    quarters(a + b, a, b);
+    lane_halves(x, a, b);
+    lane_pairs16(a + b, a, b);
     return a + b;
 }
 
@@ -219,7 +205,7 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     float x0, x1;
-                    halves(x[e + k], x0, x1);
+                    lane_halves(x[e + k], x0, x1);
                     // lower dims x0 c - x1 s, upper ones x0 s + x1 c
                     const float u = upper ? sv[k] : cv[k], w = upper ? cv[k] : -sv[k];
                     x[e + k] = __builtin_fmaf(x0, u, __fmul_rn(x1, w));

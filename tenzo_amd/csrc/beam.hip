@@ -12,104 +12,341 @@
 namespace tz {
 namespace {
 
-constexpr int kBeamMax = 64;  // beams and candidates, upper bounds
+constexpr int kBeamMax = 64;      // beams and candidates, upper bounds
+constexpr int kSliceCand = 1024;  // a slice's candidates in LDS
+constexpr int kPickCand = 512;    // the candidates that the last step ranks
 
 struct BeamSelect {
     const float* logits;
     const float* scores;
     int64_t stride;
-    int W, k;
-    int V;
-    double* lse;   // [B * W]
-    float2* cand;  // [B * W][k] value, index
+    int W, k, V;
+    int ns;         // slices of a row
+    double2* sums;  // [B * W][ns]: a slice's maximum and its sum of exponentials below it
+    float2* cand;   // [B * W][ns][k]: its best logits, in order: value, token (INT_MAX: none)
     float* out_scores;
     int32_t* out_beams;
     int32_t* out_tokens;
 };
 
-__device__ __forceinline__ float beam_logit(float x) { return x < INFINITY ? x : -INFINITY; }
+// NaN and +inf count as -inf; -0 as 0.
+__device__ __forceinline__ float beam_logit(float x) { return (x < INFINITY ? x : -INFINITY) + 0.0f; }
 
-// Order "a before b" of (value, index).
-__device__ __forceinline__ bool before(double a, int ia, double b, int ib) {
-    return a > b || (a == b && ia < ib);
+// Bits in the order of the values.
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float from_ordered(uint32_t o) {
+    return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
 }
 
-// The first of a workgroup's (value, index) pairs, in every thread.
-__device__ __forceinline__ void block_first(double& v, int& i, double* rv, int* ri) {
-    for (int d = 32; d > 0; d >>= 1) {
-        const double ov = __shfl_xor(v, d);
-        const int oi = __shfl_xor(i, d);
-        if (before(ov, oi, v, i)) v = ov, i = oi;
+// The value of lane l ^ M.
+template <int M>
+__device__ __forceinline__ float lane_xor(float v) {
+    if constexpr (M >= 32) {
+        float lo, hi;
+        lane_halves(lane_xor<M - 32>(v), lo, hi);
+        return threadIdx.x & 32 ? lo : hi;
+    } else if constexpr (M >= 16) {
+        float lo, hi;
+        lane_pairs16(lane_xor<M - 16>(v), lo, hi);
+        return threadIdx.x & 16 ? lo : hi;
+    } else if constexpr (M == 15) {
+        return dpp_f<kDppMirror>(v);
+    } else if constexpr (M == 8) {
+        return dpp_f<0x128>(v);  // row_ror:8
+    } else if constexpr (M == 7) {
+        return dpp_f<kDppHalfMirror>(v);
+    } else if constexpr (M == 4) {
+        return dpp_f<0x1B>(dpp_f<kDppHalfMirror>(v));
+    } else if constexpr (M == 3) {
+        return dpp_f<0x1B>(v);  // quad_perm [3,2,1,0]
+    } else if constexpr (M == 2) {
+        return dpp_f<kDppXor2>(v);
+    } else if constexpr (M == 1) {
+        return dpp_f<kDppXor1>(v);
+    } else {
+        static_assert(M == 0, "no such exchange");
+        return v;
     }
-    if ((threadIdx.x & 63) == 0) rv[threadIdx.x >> 6] = v, ri[threadIdx.x >> 6] = i;
-    __syncthreads();
-    for (int w = 0; w < 4; ++w)
-        if (before(rv[w], ri[w], v, i)) v = rv[w], i = ri[w];
-    __syncthreads();
 }
 
-// The plain form: a workgroup per beam, one pass for the sum of exponentials and k for the best
-// k logits, each the first after the one before.
-__global__ void __launch_bounds__(256) beam_rows_kernel(BeamSelect a) {
-    __shared__ double rv[4];
-    __shared__ int ri[4];
-    const int row = blockIdx.x, tid = threadIdx.x;
+// One step of a descending bitonic sort over the 64 lanes: lane l and l ^ M, the one without
+// the mask's top bit keeps the larger.
+template <int M>
+__device__ __forceinline__ float sort_step(float v) {
+    constexpr int top = M >= 32 ? 32 : M >= 16 ? 16 : M >= 8 ? 8 : M >= 4 ? 4 : M >= 2 ? 2 : 1;
+    const float o = lane_xor<M>(v);
+    return threadIdx.x & top ? fminf(v, o) : fmaxf(v, o);
+}
+__device__ __forceinline__ float sort64_desc(float v) {
+    v = sort_step<1>(v);
+    v = sort_step<1>(sort_step<3>(v));
+    v = sort_step<1>(sort_step<2>(sort_step<7>(v)));
+    v = sort_step<1>(sort_step<2>(sort_step<4>(sort_step<15>(v))));
+    v = sort_step<1>(sort_step<2>(sort_step<4>(sort_step<8>(sort_step<31>(v)))));
+    return sort_step<1>(
+        sort_step<2>(sort_step<4>(sort_step<8>(sort_step<16>(sort_step<63>(v))))));
+}
+
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// Stage 1, a workgroup per slice of 256 * E logits of a row, held in registers: the slice's
+// maximum and sum of exponentials, and its k best logits in order. The k-th largest of a wave's
+// 64 lane maxima is a bound that at least k of the slice reach, and the largest of the four
+// waves' bounds keeps the list of those that do short (about 2k of 8192 ordinary logits); the
+// list is put in order by counting. Where too many reach it (equal logits, masked vocabularies:
+// -inf is no bound) the k-th largest is found bit by bit instead, and among its equals the
+// lowest tokens.
+template <int E>
+__global__ void __launch_bounds__(256) beam_slice_kernel(BeamSelect a) {
+    __shared__ uint64_t list[kSliceCand];
+    __shared__ float bound[4], tops[4];
+    __shared__ double part[4];
+    __shared__ int cnt, red[4];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int row = blockIdx.x / a.ns, slice = blockIdx.x - row * a.ns;
+    const int base = slice * (256 * E) + tid * 4;  // element i, c: token base + 1024 i + c
     const float* x = a.logits + row * a.stride;
-    double last = INFINITY;
-    int last_i = -1;
-    double m = 0.0, sum = 0.0;
-    for (int j = 0; j < a.k; ++j) {
-        double v = -INFINITY;
-        int i = INT_MAX;
-        for (int t = tid; t < a.V; t += 256) {
-            const double xv = beam_logit(x[t]);
-            if (before(last, last_i, xv, t) && before(xv, t, v, i)) v = xv, i = t;
+    float v[E];
+    if (slice * (256 * E) + 256 * E <= a.V) {
+#pragma unroll
+        for (int i = 0; i < E / 4; ++i) {
+            const f32x4u q = __builtin_nontemporal_load(
+                reinterpret_cast<const f32x4u*>(x + base + 1024 * i));
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[4 * i + c] = q[c];
         }
-        block_first(v, i, rv, ri);
-        last = v;
-        last_i = i;
-        if (tid == 0) a.cand[(int64_t)row * a.k + j] = make_float2((float)v, __int_as_float(i));
-        if (j == 0) {
-            m = v == -INFINITY ? 0.0 : v;
-            for (int t = tid; t < a.V; t += 256) sum += exp((double)beam_logit(x[t]) - m);
-            for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-            if ((tid & 63) == 0) rv[tid >> 6] = sum;
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int t = base + 1024 * (i / 4) + i % 4;
+            v[i] = t < a.V ? x[t] : -INFINITY;
+        }
+    }
+    if (tid == 0) cnt = 0;
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        v[i] = beam_logit(v[i]);
+        top = fmaxf(top, v[i]);
+    }
+    const float sorted = sort64_desc(top);
+    const float bw = lane_f(sorted, a.k - 1);
+    if (lane == 0) bound[wave] = bw, tops[wave] = sorted;
+    __syncthreads();
+    const float M = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const float tau = fmaxf(fmaxf(bound[0], bound[1]), fmaxf(bound[2], bound[3]));
+    const float ref = M == -INFINITY ? 0.0f : M;
+
+    // few terms are added in 32 bits, their sums in 64
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < E; i += 8) {
+        float e[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            e[c] = __builtin_amdgcn_exp2f((v[i + c] - ref) * 1.4426950408889634f);
+        sum += (double)(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])));
+    }
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+    if (lane == 0) part[wave] = sum;
+
+    const auto token = [&](int i) { return base + 1024 * (i / 4) + i % 4; };
+    const auto key = [&](int i) {
+        return (uint64_t)ordered(v[i]) << 32 | (uint32_t)(INT_MAX - token(i));
+    };
+    if (tau > -INFINITY && top >= tau) {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (v[i] >= tau) {
+                const int at = atomicAdd(&cnt, 1);
+                if (at < kSliceCand) list[at] = key(i);
+            }
+    }
+    __syncthreads();
+    int n = cnt;
+    if (tau == -INFINITY || n > kSliceCand) {
+        // sum of a count over the workgroup
+        const auto total = [&](int c) {
+            c = wave_sum_i32(c);
             __syncthreads();
-            if (tid == 0) a.lse[row] = m + log((rv[0] + rv[1]) + (rv[2] + rv[3]));
+            if (lane == 0) red[wave] = c;
             __syncthreads();
+            return (red[0] + red[1]) + (red[2] + red[3]);
+        };
+        int mine = 0, real = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            mine += token(i) < a.V ? 1 : 0;
+            real += v[i] > -INFINITY ? 1 : 0;
+        }
+        const int want = min(a.k, total(mine));
+        uint32_t bar = ordered(-INFINITY);
+        if (total(real) >= want) {  // the want-th largest value, from its highest bit on
+            bar = 0;
+            for (int bit = 31; bit >= 0; --bit) {
+                const uint32_t up = bar | 1u << bit;
+                int c = 0;
+#pragma unroll
+                for (int i = 0; i < E; ++i) c += ordered(v[i]) >= up && token(i) < a.V ? 1 : 0;
+                if (total(c) >= want) bar = up;
+            }
+        }
+        const float least = from_ordered(bar);
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) c += v[i] > least ? 1 : 0;
+        const int need = want - total(c);
+        // its equals below token `until` are the ones needed
+        const int from = slice * (256 * E);
+        int below = 0;
+        for (int step = 256 * E; step > 0; step >>= 1) {
+            c = 0;
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                c += v[i] == least && token(i) < a.V && token(i) < from + below + step ? 1 : 0;
+            if (total(c) < need) below += step;
+        }
+        const int until = from + below + 1;
+        __syncthreads();
+        if (tid == 0) cnt = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (v[i] > least || (v[i] == least && token(i) < a.V && token(i) < until))
+                list[atomicAdd(&cnt, 1) & (kSliceCand - 1)] = key(i);
+        __syncthreads();
+        n = cnt;
+    }
+    const int64_t at = (int64_t)row * a.ns + slice;
+    if (tid == 0) a.sums[at] = make_double2(M, (part[0] + part[1]) + (part[2] + part[3]));
+    for (int i = tid; i < n; i += 256) {
+        const uint64_t me = list[i];
+        int rank = 0;
+        for (int o = 0; o < n; ++o) rank += list[o] > me ? 1 : 0;
+        if (rank < a.k)
+            a.cand[at * a.k + rank] = make_float2(
+                from_ordered((uint32_t)(me >> 32)), __int_as_float(INT_MAX - (int)(uint32_t)me));
+    }
+    if (tid >= n && tid < a.k) a.cand[at * a.k + tid] = make_float2(-INFINITY, __int_as_float(INT_MAX));
+}
+
+struct BeamCand {
+    double s;
+    float x;
+    int w, t;
+};
+__device__ __forceinline__ bool before(const BeamCand& a, const BeamCand& b) {
+    if (a.s != b.s) return a.s > b.s;
+    if (a.w != b.w) return a.w < b.w;
+    if (a.x != b.x) return a.x > b.x;
+    return a.t < b.t;
+}
+
+// Stage 2, a workgroup per request: the rows' log-sums, then the best k of the slices' lists.
+// As in stage 1 the heads of the lists give a bound that k candidates reach (in fp32, rounded
+// down: it keeps too many rather than too few), and those that do are ranked by counting; where
+// they are many (equal scores, masked beams) the k best are taken one after the other.
+__global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
+    __shared__ double lse[kBeamMax], own[kBeamMax];
+    __shared__ double ls[kPickCand];
+    __shared__ float lx[kPickCand], bound[16];
+    __shared__ int lw[kPickCand], lt[kPickCand], cnt;
+    __shared__ BeamCand best[16];
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    for (int w = wave; w < a.W; w += 16) {
+        const double2* sums = a.sums + ((int64_t)b * a.W + w) * a.ns;
+        double m = -INFINITY;
+        for (int i = lane; i < a.ns; i += 64) m = fmax(m, sums[i].x);
+        for (int d = 32; d > 0; d >>= 1) m = fmax(m, __shfl_xor(m, d));
+        double s = 0.0;
+        for (int i = lane; i < a.ns; i += 64)
+            if (sums[i].x > -INFINITY) s += sums[i].y * exp(sums[i].x - m);
+        for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
+        if (lane == 0) {
+            lse[w] = m > -INFINITY ? m + log(s) : 0.0;
+            own[w] = beam_logit(a.scores[b * a.W + w]);
+        }
+    }
+    if (tid == 0) cnt = 0;
+    __syncthreads();
+    const int per = a.ns * a.k, lists = a.W * a.ns;
+    const float2* cand = a.cand + (int64_t)b * a.W * per;
+    const auto get = [&](int c) {
+        const float2 e = cand[c];
+        BeamCand r;
+        r.w = c / per;
+        r.x = e.x;
+        r.t = __float_as_int(e.y);
+        r.s = e.x > -INFINITY ? ((double)e.x - lse[r.w]) + own[r.w] : -INFINITY;
+        return r;
+    };
+    float top = -INFINITY;
+    for (int i = tid; i < lists; i += 1024) top = fmaxf(top, __double2float_rd(get(i * a.k).s));
+    const float kth = lane_f(sort64_desc(top), a.k - 1);
+    if (lane == 0) bound[wave] = kth;
+    __syncthreads();
+    float tau = bound[0];
+#pragma unroll
+    for (int w = 1; w < 16; ++w) tau = fmaxf(tau, bound[w]);
+    for (int i = tid; i < lists; i += 1024)
+        for (int j = 0; j < a.k; ++j) {
+            const BeamCand c = get(i * a.k + j);
+            if (c.t == INT_MAX || __double2float_rd(c.s) < tau) break;
+            const int at = atomicAdd(&cnt, 1);
+            if (at >= kPickCand) break;
+            ls[at] = c.s, lx[at] = c.x, lw[at] = c.w, lt[at] = c.t;
+        }
+    __syncthreads();
+    const int n = cnt;
+    if (n <= kPickCand) {
+        for (int i = tid; i < n; i += 1024) {
+            const BeamCand me{ls[i], lx[i], lw[i], lt[i]};
+            int rank = 0;
+            for (int o = 0; o < n; ++o)
+                rank += before(BeamCand{ls[o], lx[o], lw[o], lt[o]}, me) ? 1 : 0;
+            if (rank < a.k) {
+                a.out_scores[b * a.k + rank] = (float)me.s;
+                a.out_beams[b * a.k + rank] = me.w;
+                a.out_tokens[b * a.k + rank] = me.t;
+            }
+        }
+        return;
+    }
+    BeamCand last{INFINITY, INFINITY, -1, -1};
+    const BeamCand none{-INFINITY, -INFINITY, INT_MAX, INT_MAX};
+    for (int j = 0; j < a.k; ++j) {
+        BeamCand m = none;
+        for (int c = tid; c < a.W * per; c += 1024) {
+            const BeamCand e = get(c);
+            if (e.t != INT_MAX && before(last, e) && before(e, m)) m = e;
+        }
+        for (int d = 32; d > 0; d >>= 1) {
+            const BeamCand o{__shfl_xor(m.s, d), __shfl_xor(m.x, d), __shfl_xor(m.w, d),
+                             __shfl_xor(m.t, d)};
+            if (before(o, m)) m = o;
+        }
+        if (lane == 0) best[wave] = m;
+        __syncthreads();
+        m = best[0];
+        for (int w = 1; w < 16; ++w)
+            if (before(best[w], m)) m = best[w];
+        __syncthreads();
+        last = m;
+        if (tid == 0) {
+            a.out_scores[b * a.k + j] = (float)m.s;
+            a.out_beams[b * a.k + j] = m.w;
+            a.out_tokens[b * a.k + j] = m.t;
         }
     }
 }
 
-__global__ void __launch_bounds__(256) beam_pick_kernel(BeamSelect a) {
-    __shared__ double rv[4];
-    __shared__ int ri[4];
-    const int b = blockIdx.x, tid = threadIdx.x, n = a.W * a.k;
-    double last = INFINITY;
-    int last_i = -1;
-    for (int j = 0; j < a.k; ++j) {
-        double v = -INFINITY;
-        int i = INT_MAX;
-        for (int c = tid; c < n; c += 256) {
-            const int w = c / a.k;
-            const float2 e = a.cand[(int64_t)b * n + c];
-            const int t = __float_as_int(e.y);
-            if (t == INT_MAX) continue;  // a vocabulary smaller than k
-            const double lse = a.lse[b * a.W + w], s = beam_logit(a.scores[b * a.W + w]);
-            double xv = -INFINITY;
-            if (e.x > -INFINITY) xv = s + ((double)e.x - lse);
-            if (before(last, last_i, xv, c) && before(xv, c, v, i)) v = xv, i = c;
-        }
-        block_first(v, i, rv, ri);
-        last = v;
-        last_i = i;
-        if (tid == 0) {
-            a.out_scores[b * a.k + j] = (float)v;
-            a.out_beams[b * a.k + j] = i / a.k;
-            a.out_tokens[b * a.k + j] = __float_as_int(a.cand[(int64_t)b * n + i].y);
-        }
-    }
-}
+// Logits a thread of stage 1 holds: 32 where that fills the GPU, 8 for few rows.
+int beam_elems(int64_t rows, int64_t V) { return rows * ceil_div(V, 256 * 32) >= 512 ? 32 : 8; }
 
 // ------------------------------------------------------------- reordering --
 
@@ -125,6 +362,36 @@ struct BeamReorder {
 };
 
 constexpr int kPageTokens = 16;
+
+// One piece of the page in progress, for all slots of a request.
+template <int WMAX, typename P>
+__device__ __forceinline__ void move_piece(const BeamReorder& a, const int32_t* table,
+                                           const int32_t* parents, uint8_t* pool, int64_t plane,
+                                           int page_bytes, int off, int full) {
+    P v[WMAX];
+    bool moved[WMAX];
+#pragma unroll
+    for (int i = 0; i < WMAX; ++i) {
+        v[i] = P{};
+        moved[i] = false;
+        if (i < a.W) {
+            const int par = parents[i];
+            const bool other = par >= 0 && par < a.W && par != i;
+            const int64_t from = table[(other ? par : i) * a.table_stride + full];
+            const int64_t to = table[i * a.table_stride + full];
+            moved[i] = other && from >= 0 && from < a.n_blocks && to >= 0 && to < a.n_blocks;
+            if (moved[i])
+                v[i] = *reinterpret_cast<const P*>(pool + (from * a.planes + plane) * page_bytes +
+                                                   off);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < WMAX; ++i)
+        if (moved[i]) {
+            const int64_t to = table[i * a.table_stride + full];
+            *reinterpret_cast<P*>(pool + (to * a.planes + plane) * page_bytes + off) = v[i];
+        }
+}
 
 // In place: slot i of a request takes the cached tokens of slot parents[i]. The pages that are
 // full change hands through the table; the rows of the page in progress are copied into the
@@ -171,42 +438,20 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(BeamReorder a) {
         off = (p - which * a.row_bytes) * 16;
         token = off / a.row_bytes;
         page_bytes = a.row_bytes * kPageTokens;
-        pool = a.codes[which];
+        pool = which ? a.codes[1] : a.codes[0];
     } else {
         p -= 2 * a.row_bytes;
         which = p >= kPageTokens;
         token = p - which * kPageTokens;
         off = token * 4;
         page_bytes = 4 * kPageTokens;
-        pool = a.scales[which];
+        pool = which ? a.scales[1] : a.scales[0];
     }
     if (token >= fill) return;
-    uint4 v[WMAX];
-    int64_t dst[WMAX];
-#pragma unroll
-    for (int i = 0; i < WMAX; ++i) {
-        dst[i] = -1;
-        if (i >= a.W) continue;
-        const int par = parents[i];
-        if (par < 0 || par >= a.W || par == i) continue;
-        const int64_t from = table[par * a.table_stride + full];
-        const int64_t to = table[i * a.table_stride + full];
-        if (from < 0 || from >= a.n_blocks || to < 0 || to >= a.n_blocks) continue;
-        const uint8_t* src = pool + (from * a.planes + plane) * page_bytes + off;
-        dst[i] = (to * a.planes + plane) * page_bytes + off;
-        if (code)
-            v[i] = *reinterpret_cast<const uint4*>(src);
-        else
-            v[i].x = *reinterpret_cast<const uint32_t*>(src);
-    }
-#pragma unroll
-    for (int i = 0; i < WMAX; ++i) {
-        if (i >= a.W || dst[i] < 0) continue;
-        if (code)
-            *reinterpret_cast<uint4*>(pool + dst[i]) = v[i];
-        else
-            *reinterpret_cast<uint32_t*>(pool + dst[i]) = v[i].x;
-    }
+    if (code)
+        move_piece<WMAX, uint4>(a, table, parents, pool, plane, page_bytes, off, full);
+    else
+        move_piece<WMAX, uint32_t>(a, table, parents, pool, plane, page_bytes, off, full);
 }
 
 }  // namespace
@@ -217,9 +462,9 @@ using namespace tz;
 extern "C" {
 
 TENZO_HIP_API size_t tenzo_hip_beam_select_ws_bytes(int B, int W, int64_t V, int k) {
-    (void)V;
-    if (B <= 0 || W <= 0 || k <= 0) return 0;
-    return (size_t)B * W * (8 + (size_t)k * 8);
+    if (B <= 0 || W <= 0 || k <= 0 || V <= 0) return 0;
+    const int64_t rows = (int64_t)B * W;
+    return (size_t)(rows * ceil_div(V, 256 * beam_elems(rows, V))) * (16 + (size_t)k * 8);
 }
 
 TENZO_HIP_API int tenzo_hip_beam_select(const float* logits, int64_t row_stride,
@@ -229,16 +474,19 @@ TENZO_HIP_API int tenzo_hip_beam_select(const float* logits, int64_t row_stride,
                                         void* stream) {
     TZ_CHECK(B >= 0 && W > 0 && W <= kBeamMax && k > 0 && k <= kBeamMax,
              "beam_select: B=%d, 1 to %d beams (%d) and candidates (%d)", B, kBeamMax, W, k);
-    TZ_CHECK(V > 0 && V * W < INT32_MAX && k <= V * W,
+    TZ_CHECK(V > 0 && V <= (1 << 30) && V * W < INT32_MAX && k <= V * W,
              "beam_select: %d of %lld candidates (V=%lld)", k, (long long)(V * W), (long long)V);
-    TZ_CHECK((int64_t)B * W <= INT32_MAX / kBeamMax, "beam_select: %d x %d beams", B, W);
+    const int64_t rows = (int64_t)B * W;
+    const int elems = beam_elems(rows, V);
+    const int64_t ns = ceil_div(V, 256 * elems);
+    TZ_CHECK(rows * ns <= 0xffffff && B <= 0x3fffff, "beam_select: %d x %d beams", B, W);
     if (B == 0) return TENZO_SUCCESS;
     TZ_CHECK(logits && scores && out_scores && out_beams && out_tokens,
              "beam_select: null pointer");
     TZ_CHECK(row_stride >= V || B * W == 1, "beam_select: rows %lld apart, V=%lld",
              (long long)row_stride, (long long)V);
     const size_t need = tenzo_hip_beam_select_ws_bytes(B, W, V, k);
-    TZ_CHECK(ws && ws_bytes >= need && ((uintptr_t)ws & 7) == 0,
+    TZ_CHECK(ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0,
              "beam_select: %zu bytes of workspace needed, %zu given", need, ws ? ws_bytes : 0);
     BeamSelect a{};
     a.logits = logits;
@@ -247,16 +495,20 @@ TENZO_HIP_API int tenzo_hip_beam_select(const float* logits, int64_t row_stride,
     a.W = W;
     a.k = k;
     a.V = (int)V;
-    a.lse = (double*)ws;
-    a.cand = (float2*)((char*)ws + (size_t)B * W * 8);
+    a.ns = (int)ns;
+    a.sums = (double2*)ws;
+    a.cand = (float2*)((char*)ws + (size_t)(rows * ns) * 16);
     a.out_scores = out_scores;
     a.out_beams = out_beams;
     a.out_tokens = out_tokens;
-    hipLaunchKernelGGL(beam_rows_kernel, dim3((unsigned)(B * W)), dim3(256), 0,
-                       (hipStream_t)stream, a);
-    const int rc = launch_status("beam_rows_kernel");
+    const dim3 grid((unsigned)(rows * ns));
+    if (elems == 32)
+        hipLaunchKernelGGL(beam_slice_kernel<32>, grid, dim3(256), 0, (hipStream_t)stream, a);
+    else
+        hipLaunchKernelGGL(beam_slice_kernel<8>, grid, dim3(256), 0, (hipStream_t)stream, a);
+    const int rc = launch_status("beam_slice_kernel");
     if (rc) return rc;
-    hipLaunchKernelGGL(beam_pick_kernel, dim3((unsigned)B), dim3(256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(beam_pick_kernel, dim3((unsigned)B), dim3(1024), 0, (hipStream_t)stream, a);
     return launch_status("beam_pick_kernel");
 }
 

@@ -114,6 +114,21 @@ __device__ __forceinline__ float wave_max(float v) {
     return fmaxf(fmaxf(lane_f(v, 0), lane_f(v, 16)), fmaxf(lane_f(v, 32), lane_f(v, 48)));
 }
 
+// Both 32-lane halves' values of x in every lane ({x of lane l % 32, x of that + 32}), and both
+// of the pair l, l ^ 16 ({the lower lane's, the upper one's}).
+__device__ __forceinline__ void lane_halves(float x, float& lo, float& hi) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                    false);
+    lo = __uint_as_float(r[0]);
+    hi = __uint_as_float(r[1]);
+}
+__device__ __forceinline__ void lane_pairs16(float x, float& lo, float& hi) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                    false);
+    lo = __uint_as_float(r[0]);
+    hi = __uint_as_float(r[1]);
+}
+
 // Block-wide max / integer sum for 256 threads (order-independent).
 __device__ __forceinline__ float block256_max(float v, float* red) {
     v = wave_max(v);
