@@ -9,8 +9,10 @@ namespace {
 constexpr float kQkScale = 0.08838834764831845f;  // 1/sqrt(128)
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kTile = 64;           // tokens of a wave's step
+constexpr int kSub = 4;             // 16-token pages of a wave's step
+constexpr int kTile = 16 * kSub;    // tokens of a wave's step
 constexpr int kMaxPages = 1024;     // pages of a workgroup's part of the context
+constexpr int kQStride = 132;       // floats of a query in LDS
 constexpr int kVStride = 144;       // bf16 of a value row in LDS: 288 bytes, 8 rows over all banks
 
 struct Kv4Attn {
@@ -26,7 +28,7 @@ struct Kv4Attn {
     float2* part_ml; // [T * Hq][splits]: maximum (base 2) and sum
     int G, Hq, T;
     int chunk, splits;  // tokens of a split
-    int vec;            // q, out and rope allow 16-byte accesses
+    int vec_out;        // out allows accesses of 4 elements
 };
 
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -64,6 +66,25 @@ __device__ __forceinline__ uint32_t pack_hi(float a, float b) {
 }
 __device__ __forceinline__ float masked(float v, uint32_t m) {
     return __uint_as_float(__float_as_uint(v) & m);
+}
+
+// Four outputs, the weighted sum over the sum of weights (0 where no token was seen).
+template <bool HALF>
+__device__ __forceinline__ void store4(const Kv4Attn& a, int64_t at, f32x4 v, float l) {
+    float o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = l != 0.0f ? v[k] / l : 0.0f;
+    if (!a.vec_out) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) st_act<HALF>(a.out, at + k, o[k]);
+    } else if (HALF) {
+        uint2 w;
+        w.x = float_to_half_bits(o[0]) | (uint32_t)float_to_half_bits(o[1]) << 16;
+        w.y = float_to_half_bits(o[2]) | (uint32_t)float_to_half_bits(o[3]) << 16;
+        *reinterpret_cast<uint2*>((uint16_t*)a.out + at) = w;
+    } else {
+        *reinterpret_cast<float4*>((float*)a.out + at) = make_float4(o[0], o[1], o[2], o[3]);
+    }
 }
 
 // Sequence and row tile of a work unit: the unit-th tile when every sequence has
@@ -111,14 +132,15 @@ __device__ __forceinline__ bool find_unit(const Kv4Seqs& sq, int unit, int G, in
 // by transposing reads. Codes times scale are exact in bf16; queries and weights are split into
 // NP parts of 8 bits (fp32: 3, every bit; fp16: 2). With ROWS < 16 the parts stand in columns
 // side by side (column = part * ROWS + row) and one MFMA serves all of them.
-template <int ROWS, int NP, int RW, bool HALF>
-__global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
-    constexpr int SLOTS = 16 / ROWS, NM = SLOTS == 1 ? NP : 1, TW = 4 / RW, RT = ROWS * RW;
+template <int ROWS, int NP, int RW, int NW, bool HALF>
+__global__ void __launch_bounds__(64 * NW, NW == 4 ? 3 : 2) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
+    constexpr int SLOTS = 16 / ROWS, NM = SLOTS == 1 ? NP : 1, TW = NW / RW, RT = ROWS * RW;
     static_assert(SLOTS == 1 || SLOTS >= NP, "a column for each part");
-    __shared__ __align__(16) uint16_t vbuf[4][32 * kVStride];
-    __shared__ float2 ml[4][16];
+    __shared__ __align__(16) uint16_t vbuf[NW][32 * kVStride];
+    __shared__ float2 ml[NW][16];
     __shared__ int pg[kMaxPages];
     static_assert(sizeof(vbuf[0]) >= 16 * kKv4Dim * 4, "the rows' sums fit a wave's part");
+    static_assert(sizeof(vbuf) >= RT * kQStride * 4, "the queries fit the value buffer");
 
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -148,90 +170,31 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
     const int64_t grow = (int64_t)first + qi;
 
     const int npg = t1 > t0 ? (t1 - t0 + kKv4Page - 1) / kKv4Page : 0;
-    for (int p = tid; p < npg; p += 256) {
+    for (int p = tid; p < npg; p += 64 * NW) {
         const int blk = sq.tables[(int64_t)seq * sq.table_stride + t0 / kKv4Page + p];
         pg[p] = blk >= 0 && blk < sq.n_blocks ? blk : -1;
     }
 
-    // Q: the lane's 32 dims 32j .. 32j + 31, rotated with those 64 away (lane ^ 32)
-    Frag qf[NM][4];
-    {
-        float x[32];
-        const int64_t at = grow * a.q_stride + (int64_t)head * kKv4Dim + 32 * j;
-        if (pos < 0) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = 0.0f;
-        } else if (!HALF && a.vec) {
-            const float4* p = reinterpret_cast<const float4*>((const float*)a.q + at);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float4 v = p[e];
-                x[4 * e] = v.x, x[4 * e + 1] = v.y, x[4 * e + 2] = v.z, x[4 * e + 3] = v.w;
-            }
-        } else if (HALF && a.vec) {
-            const uint4* p = reinterpret_cast<const uint4*>((const uint16_t*)a.q + at);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint4 v = p[e];
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    x[8 * e + 2 * k] = half_bits_to_float((uint16_t)w[k]);
-                    x[8 * e + 2 * k + 1] = half_bits_to_float((uint16_t)(w[k] >> 16));
-                }
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = ld_act<HALF>(a.q, at + e);
-        }
-        if (a.rope) {
-            const float* cs = a.rope + (int64_t)max(pos, 0) * kKv4Dim + 32 * (j & 1);
-            const bool upper = lane >= 32;
-            if (pos < 0) cs = a.rope;  // (zeros stay zeros; row 0 may not exist: not read)
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-                float cv[4] = {1.0f, 1.0f, 1.0f, 1.0f}, sv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                if (pos >= 0) {
-                    if (a.vec) {
-                        const float4 u = *reinterpret_cast<const float4*>(cs + e);
-                        const float4 w = *reinterpret_cast<const float4*>(cs + 64 + e);
-                        cv[0] = u.x, cv[1] = u.y, cv[2] = u.z, cv[3] = u.w;
-                        sv[0] = w.x, sv[1] = w.y, sv[2] = w.z, sv[3] = w.w;
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) cv[k] = cs[e + k], sv[k] = cs[64 + e + k];
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    float x0, x1;
-                    lane_halves(x[e + k], x0, x1);
-                    // lower dims x0 c - x1 s, upper ones x0 s + x1 c
-                    const float u = upper ? sv[k] : cv[k], w = upper ? cv[k] : -sv[k];
-                    x[e + k] = __builtin_fmaf(x0, u, __fmul_rn(x1, w));
-                }
+    // the rows' queries, rotated and scaled, by way of LDS (each wave needs all of a row)
+    float* qs = reinterpret_cast<float*>(vbuf);
+    for (int it = tid; it < RT * 64; it += 64 * NW) {
+        const int rr = it >> 6, d = it & 63, r2 = row0 + rr, i2 = r2 / a.G;
+        const int p2 = i2 < n && first >= 0 && first + i2 < a.T && c > 0 ? c - n + i2 : -1;
+        float x0 = 0.0f, x1 = 0.0f;
+        if (p2 >= 0) {
+            const int64_t at = ((int64_t)first + i2) * a.q_stride +
+                               (int64_t)(h * a.G + (r2 - i2 * a.G)) * kKv4Dim + d;
+            x0 = ld_act<HALF>(a.q, at);
+            x1 = ld_act<HALF>(a.q, at + 64);
+            if (a.rope) {
+                const float* cs = a.rope + (int64_t)p2 * kKv4Dim + d;
+                const float cv = cs[0], sv = cs[64], y0 = x0;
+                x0 = __builtin_fmaf(x0, cv, -__fmul_rn(x1, sv));
+                x1 = __builtin_fmaf(y0, sv, __fmul_rn(x1, cv));
             }
         }
-#pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = __fmul_rn(x[e], kQkScale * kLog2e);
-        // part p of a value: what its parts before leave, cut to 8 bits
-        if (SLOTS > 1) {
-            const uint32_t m1 = slot >= 1 ? 0xffff0000u : 0, m2 = slot >= 2 ? 0xffff0000u : 0;
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-                x[e] -= masked(x[e], m1);
-                if (NP == 3) x[e] -= masked(x[e], m2);
-                if (slot >= NP) x[e] = 0.0f;
-            }
-        }
-#pragma unroll
-        for (int p = 0; p < NM; ++p)
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-                qf[p][e >> 3].w[(e >> 1) & 3] = pack_hi(x[e], x[e + 1]);
-                x[e] -= masked(x[e], 0xffff0000u);
-                x[e + 1] -= masked(x[e + 1], 0xffff0000u);
-            }
+        qs[rr * kQStride + d] = __fmul_rn(x0, kQkScale * kLog2e);
+        qs[rr * kQStride + d + 64] = __fmul_rn(x1, kQkScale * kLog2e);
     }
     __syncthreads();
 
@@ -240,20 +203,18 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
     for (int d = 0; d < 8; ++d) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
 
-    uint4 kr[4], vr[4];
-    uint32_t ksc[4], vsc[4];
-    int ids[4];
+    uint4 kr[kSub], vr[kSub];
+    uint32_t ksc[kSub], vsc[kSub];
     const uint32_t lane_code = (uint32_t)(col * kKv4Row + j * 16);
     const uint32_t lane_scale = (uint32_t)(col * kKv4Scales + j);
     auto page_row = [&](int t, int tt) -> int64_t {
         const int p = min(((t - t0) >> 4) + tt, npg - 1);
         const int id = __builtin_amdgcn_readfirstlane(pg[p]);
-        ids[tt] = id;
         return (((int64_t)max(id, 0) * sq.n_layers + sq.layer) * sq.Hkv + h) * kKv4Page;
     };
     auto load_k = [&](int t) {
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
+        for (int tt = 0; tt < kSub; ++tt) {
             const int64_t row = page_row(t, tt);
             kr[tt] = *reinterpret_cast<const uint4*>(a.pk + row * kKv4Row + lane_code);
             ksc[tt] = (a.pks + row * kKv4Scales)[lane_scale];
@@ -261,7 +222,7 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
     };
     auto load_v = [&](int t) {
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
+        for (int tt = 0; tt < kSub; ++tt) {
             const int64_t row = page_row(t, tt);
             vr[tt] = *reinterpret_cast<const uint4*>(a.pv + row * kKv4Row + lane_code);
             vsc[tt] = (a.pvs + row * kKv4Scales)[lane_scale];
@@ -277,11 +238,37 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
         load_k(t);
         load_v(t);
     }
+    // Q as B operands: the lane's 32 dims 32j .. 32j + 31 of its row, in parts (part p of a value:
+    // what its parts before leave, cut to 8 bits)
+    Frag qf[NM][4];
+    {
+        const uint32_t m1 = slot >= 1 ? 0xffff0000u : 0, m2 = slot >= 2 ? 0xffff0000u : 0;
+        const float* src = qs + (rw * ROWS + col % ROWS) * kQStride + 32 * j;
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+            f32x4 x = *reinterpret_cast<const f32x4*>(src + e);
+            if (SLOTS > 1)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    x[k] -= masked(x[k], m1);
+                    if (NP == 3) x[k] -= masked(x[k], m2);
+                    if (SLOTS > NP && slot >= NP) x[k] = 0.0f;
+                }
+#pragma unroll
+            for (int p = 0; p < NM; ++p) {
+                qf[p][e >> 3].w[(e >> 1) & 3] = pack_hi(x[0], x[1]);
+                qf[p][e >> 3].w[((e >> 1) & 3) + 1] = pack_hi(x[2], x[3]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] -= masked(x[k], 0xffff0000u);
+            }
+        }
+    }
+    __syncthreads();
     for (; t < t1 && any; t += kTile * TW) {
         const int next = t + kTile * TW;
-        f32x4 s[4];
+        f32x4 s[kSub];
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
+        for (int tt = 0; tt < kSub; ++tt) {
             const float sc = e8m0_to_float(ksc[tt]);
             const uint32_t w[4] = {kr[tt].x, kr[tt].y, kr[tt].z, kr[tt].w};
             s[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -302,9 +289,9 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
             }
         }
         bool bad = false;
-        int id_now[4];
+        int id_now[kSub];
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
+        for (int tt = 0; tt < kSub; ++tt) {
             const int p = ((t - t0) >> 4) + tt;
             id_now[tt] = p < npg ? __builtin_amdgcn_readfirstlane(pg[p]) : -1;
             bad = bad || id_now[tt] < 0;
@@ -312,7 +299,7 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
         if (next < t1) load_k(next);
         float top = -INFINITY;
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt)
+        for (int tt = 0; tt < kSub; ++tt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float v = s[tt][i];
@@ -324,13 +311,13 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
         // a step that a row may not see whole: past its position, or absent pages
         if (bad || t + kTile - 1 > c - n + row0 / a.G) {
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt)
+            for (int tt = 0; tt < kSub; ++tt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (id_now[tt] < 0 || t + 16 * tt + 4 * j + i > pos) s[tt][i] = -INFINITY;
         }
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt)
+        for (int tt = 0; tt < kSub; ++tt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, s[tt][i]);
         const float mn = fmaxf(m, max_quarters(top));
@@ -343,7 +330,7 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
             l *= alpha;
         }
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt)
+        for (int tt = 0; tt < kSub; ++tt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 s[tt][i] = __builtin_amdgcn_exp2f(s[tt][i] - base);
@@ -351,7 +338,7 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
             }
         const uint32_t m1 = slot >= 1 ? 0xffff0000u : 0, m2 = slot >= 2 ? 0xffff0000u : 0;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < kSub / 2; ++u) {
             // 32 value rows, by two 16-token pages
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -371,7 +358,7 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
                     *reinterpret_cast<uint4*>(vb + vw + k * 16 * kVStride + st * 8) = f.v;
                 }
             }
-            if (u == 1 && next < t1) load_v(next);
+            if (u == kSub / 2 - 1 && next < t1) load_v(next);
             Frag pf[NM];
             float p8[8];
 #pragma unroll
@@ -430,7 +417,7 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
             if (j == 0) ml[wave][col] = make_float2(m, l);
         }
         __syncthreads();
-        for (int it = tid; it < RT * 32; it += 256) {
+        for (int it = tid; it < RT * 32; it += 64 * NW) {
             const int rr = it >> 5, d4 = it & 31, grp = rr / ROWS, cc = rr % ROWS;
             const int r2 = row0 + rr, i2 = r2 / a.G;
             if (i2 >= n || first < 0 || first + i2 >= a.T) continue;
@@ -452,9 +439,7 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
             const int64_t g2 = (int64_t)first + i2, hd = h * a.G + (r2 - i2 * a.G);
             if (p2 < a.chunk || a.splits == 1) {
                 if (split == 0)
-                    for (int k = 0; k < 4; ++k)
-                        st_act<HALF>(a.out, g2 * a.out_stride + hd * kKv4Dim + 4 * d4 + k,
-                                     L != 0.0f ? v[k] / L : 0.0f);
+                    store4<HALF>(a, g2 * a.out_stride + hd * kKv4Dim + 4 * d4, v, L);
             } else {
                 const int64_t at = (g2 * a.Hq + hd) * a.splits + split;
                 *reinterpret_cast<f32x4*>(a.part_o + at * kKv4Dim + 4 * d4) = v;
@@ -466,12 +451,8 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
             if (split == 0)
 #pragma unroll
                 for (int d = 0; d < 8; ++d)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        st_act<HALF>(a.out,
-                                     grow * a.out_stride + (int64_t)head * kKv4Dim + 16 * d +
-                                         4 * j + i,
-                                     l != 0.0f ? acc[d][i] / l : 0.0f);
+                    store4<HALF>(a, grow * a.out_stride + (int64_t)head * kKv4Dim + 16 * d + 4 * j,
+                                 acc[d], l);
         } else {
             const int64_t at = (grow * a.Hq + head) * a.splits + split;
 #pragma unroll
@@ -494,11 +475,13 @@ __global__ void __launch_bounds__(512) kv4_join_kernel(Kv4Attn a, Kv4Seqs sq) {
     const int64_t at = ((int64_t)row * a.Hq + head) * a.splits;
     const float2* ml = a.part_ml + at;
     float M = -INFINITY;
-    for (int s = 0; s < ns; ++s) M = fmaxf(M, ml[s].x);
+    for (int s = tid & 63; s < ns; s += 64) M = fmaxf(M, ml[s].x);
+    M = wave_max(M);
     const float base = M == -INFINITY ? 0.0f : M;
     const int d4 = tid & 31, g = tid >> 5;
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     float L = 0.0f;
+#pragma unroll 4
     for (int s = g; s < ns; s += 16) {
         const float2 e = ml[s];
         const float f = __builtin_amdgcn_exp2f(e.x - base);
@@ -510,15 +493,13 @@ __global__ void __launch_bounds__(512) kv4_join_kernel(Kv4Attn a, Kv4Seqs sq) {
     __syncthreads();
     if (g == 0) {
         for (int k = 1; k < 16; ++k) v += ov[k][d4], L += lv[k];
-        for (int k = 0; k < 4; ++k)
-            st_act<HALF>(a.out, row * a.out_stride + (int64_t)head * kKv4Dim + 4 * d4 + k,
-                         L != 0.0f ? v[k] / L : 0.0f);
+        store4<HALF>(a, row * a.out_stride + (int64_t)head * kKv4Dim + 4 * d4, v, L);
     }
 }
 
-// Rows of a workgroup, tokens of a split and how many splits, from what the host knows.
+// Rows and waves of a workgroup, tokens of a split and how many splits, from what the host knows.
 struct Kv4Plan {
-    int rows, rw, splits, chunk;
+    int rows, rw, nw, splits, chunk;
     int64_t units;
 };
 Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, bool half) {
@@ -530,9 +511,12 @@ Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, boo
     const int rt = p.rows * p.rw;
     p.units = cu ? T * G / rt + B : (int64_t)B * ceil_div(G, rt);
     const int64_t ctx = (int64_t)table_width * kKv4Page;
-    const int64_t step = kTile * (4 / p.rw);
-    // enough workgroups for every CU to have two, each wave a step of tokens at least
-    int64_t s = ceil_div(512, p.units * Hkv);
+    const int64_t wgs = p.units * Hkv;
+    // few sequences that three steps of 8 waves get through: the second launch costs more
+    p.nw = p.rw == 1 && wgs <= 256 && ctx <= 3 * 8 * kTile ? 8 : 4;
+    const int64_t step = kTile * (p.nw / p.rw);
+    // else enough workgroups for every CU to have four, each wave a step of tokens at least
+    int64_t s = p.nw == 8 ? 1 : ceil_div(1024, wgs);
     s = s < ceil_div(ctx, step) ? s : ceil_div(ctx, step);
     if (s < 1) s = 1;
     int64_t chunk = ceil_div(ceil_div(ctx, s), step) * step;
@@ -543,9 +527,26 @@ Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, boo
     return p;
 }
 
-template <int ROWS, int NP, int RW, bool HALF>
-void launch_kv4(const Kv4Attn& a, const Kv4Seqs& s, dim3 grid, hipStream_t st) {
-    hipLaunchKernelGGL((kv4_attn_kernel<ROWS, NP, RW, HALF>), grid, dim3(256), 0, st, a, s);
+template <int ROWS, int NP, int RW, int NW, bool HALF>
+void launch_kv4(const Kv4Attn& a, const Kv4Seqs& s, unsigned wgs, hipStream_t st) {
+    hipLaunchKernelGGL((kv4_attn_kernel<ROWS, NP, RW, NW, HALF>), dim3(wgs), dim3(64 * NW), 0, st,
+                       a, s);
+}
+template <int PACKED, int NP, bool HALF>
+void launch_kv4_plan(const Kv4Plan& p, const Kv4Attn& a, const Kv4Seqs& s, unsigned wgs,
+                     hipStream_t st) {
+    if (p.rows == PACKED && p.nw == 8)
+        launch_kv4<PACKED, NP, 1, 8, HALF>(a, s, wgs, st);
+    else if (p.rows == PACKED)
+        launch_kv4<PACKED, NP, 1, 4, HALF>(a, s, wgs, st);
+    else if (p.nw == 8)
+        launch_kv4<16, NP, 1, 8, HALF>(a, s, wgs, st);
+    else if (p.rw == 1)
+        launch_kv4<16, NP, 1, 4, HALF>(a, s, wgs, st);
+    else if (p.rw == 2)
+        launch_kv4<16, NP, 2, 4, HALF>(a, s, wgs, st);
+    else
+        launch_kv4<16, NP, 4, 4, HALF>(a, s, wgs, st);
 }
 
 }  // namespace
@@ -611,29 +612,12 @@ TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,
     a.T = (int)T;
     a.chunk = p.chunk;
     a.splits = p.splits;
-    const int64_t esize = dtype ? 2 : 4;
-    a.vec = (((uintptr_t)q | (uintptr_t)rope_cs | (uintptr_t)(q_stride * esize)) & 15) == 0;
+    a.vec_out = (((uintptr_t)out | (uintptr_t)(out_stride * (dtype ? 2 : 4))) & 15) == 0;
     hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)wgs);
-    if (dtype) {
-        if (p.rows == 8)
-            launch_kv4<8, 2, 1, true>(a, s, grid, st);
-        else if (p.rw == 1)
-            launch_kv4<16, 2, 1, true>(a, s, grid, st);
-        else if (p.rw == 2)
-            launch_kv4<16, 2, 2, true>(a, s, grid, st);
-        else
-            launch_kv4<16, 2, 4, true>(a, s, grid, st);
-    } else {
-        if (p.rows == 4)
-            launch_kv4<4, 3, 1, false>(a, s, grid, st);
-        else if (p.rw == 1)
-            launch_kv4<16, 3, 1, false>(a, s, grid, st);
-        else if (p.rw == 2)
-            launch_kv4<16, 3, 2, false>(a, s, grid, st);
-        else
-            launch_kv4<16, 3, 4, false>(a, s, grid, st);
-    }
+    if (dtype)
+        launch_kv4_plan<8, 2, true>(p, a, s, (unsigned)wgs, st);
+    else
+        launch_kv4_plan<4, 3, false>(p, a, s, (unsigned)wgs, st);
     const int rc2 = launch_status("kv4_attn_kernel");
     if (rc2 || p.splits == 1) return rc2;
     const dim3 jgrid((unsigned)T, (unsigned)Hq);
