@@ -13,7 +13,6 @@ constexpr int kSub = 4;             // 16-token pages of a wave's step
 constexpr int kTile = 16 * kSub;    // tokens of a wave's step
 constexpr int kMaxPages = 1024;     // pages of a workgroup's part of the context
 constexpr int kQStride = 132;       // floats of a query in LDS
-constexpr int kVStride = 144;       // bf16 of a value row in LDS: 288 bytes, 8 rows over all banks
 
 struct Kv4Attn {
     const void* q;
@@ -24,10 +23,11 @@ struct Kv4Attn {
     const uint8_t* pks;
     const uint8_t* pvs;
     const float* rope;
-    float* part_o;   // [T * Hq][splits][128]
-    float2* part_ml; // [T * Hq][splits]: maximum (base 2) and sum
+    float* part_o;    // records of rows' unfinished sums: 128 sums,
+    float2* part_ml;  // maximum (base 2) and sum of weights
     int G, Hq, T;
     int chunk, splits;  // tokens of a split
+    int wgs;            // workgroups of a call whose steps are dealt evenly
     int vec_out;        // out allows accesses of 4 elements
 };
 
@@ -121,6 +121,69 @@ __device__ __forceinline__ bool find_unit(const Kv4Seqs& sq, int unit, int G, in
     return false;
 }
 
+// Work of a sequence where steps are dealt evenly: each of its (kv head, row tile) units takes
+// ceil(length / 256) steps, whatever of them a row sees, and counts one more for what a unit costs
+// besides (its queries, the first tokens' way, the sums' meeting: about 4 us, a step 3 to 5).
+constexpr int kStep = 4 * kTile;
+struct SeqWork {
+    int first, n, c, steps, tiles;
+    __device__ __forceinline__ SeqWork(const Kv4Seqs& sq, int b, int G, int RT) {
+        first = sq.cu ? sq.cu[b] : b;
+        n = sq.cu ? max(0, sq.cu[b + 1] - first) : 1;
+        c = sq.length(b);
+        steps = (c + kStep - 1) / kStep;
+        tiles = (n * G + RT - 1) / RT;
+    }
+    __device__ __forceinline__ int slots() const { return steps + 1; }  // of a unit
+    __device__ __forceinline__ int total(int Hkv) const {
+        return c > 0 ? slots() * tiles * Hkv : 0;
+    }
+};
+
+// Sum of v over the threads before this one, and over all of them (64 * NW threads).
+template <int NW>
+__device__ __forceinline__ int block_scan(int v, int* wsum, int& all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int incl = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(incl, d);
+        if (lane >= d) incl += o;
+    }
+    if (lane == 63) wsum[wave] = incl;
+    __syncthreads();
+    int before = incl - v;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        before += w < wave ? wsum[w] : 0;
+        all += wsum[w];
+    }
+    return before;
+}
+
+// A value that all lanes of the wave hold, for scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Workgroup w of N has the slots [w q + min(w, r), + q + (w < r)), q and r of total / N.
+__device__ __forceinline__ int wg_start(int w, int total, int N) {
+    const int q = total / N, r = total - q * N;
+    return w * q + min(w, r);
+}
+__device__ __forceinline__ int wg_of(int g, int total, int N) {
+    const int q = total / N, r = total - q * N;
+    return g < r * (q + 1) ? g / (q + 1) : r + (g - r * (q + 1)) / q;
+}
+
+// A piece of work: the rows of a tile against the tokens [t0, t0 + len) of their sequence.
+struct Segment {
+    int seq, first, n, c, tile, h;
+    int t0, len;
+    bool whole;   // no other piece has these rows (steps dealt evenly)
+    int64_t rec;  // else the record of the first row
+    int split;    // (a grid of splits)
+};
+
 // One workgroup: RT = ROWS * RW rows (token, query head of one kv head) of a sequence against a
 // part of its tokens. Wave w has the rows group w % RW and every (4 / RW)-th step of 64 tokens.
 //
@@ -132,35 +195,35 @@ __device__ __forceinline__ bool find_unit(const Kv4Seqs& sq, int unit, int G, in
 // by transposing reads. Codes times scale are exact in bf16; queries and weights are split into
 // NP parts of 8 bits (fp32: 3, every bit; fp16: 2). With ROWS < 16 the parts stand in columns
 // side by side (column = part * ROWS + row) and one MFMA serves all of them.
-template <int ROWS, int NP, int RW, int NW, bool HALF>
-__global__ void __launch_bounds__(64 * NW, NW == 4 ? 3 : 2) kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
-    constexpr int SLOTS = 16 / ROWS, NM = SLOTS == 1 ? NP : 1, TW = NW / RW, RT = ROWS * RW;
-    static_assert(SLOTS == 1 || SLOTS >= NP, "a column for each part");
-    __shared__ __align__(16) uint16_t vbuf[NW][32 * kVStride];
-    __shared__ float2 ml[NW][16];
-    __shared__ int pg[kMaxPages];
-    static_assert(sizeof(vbuf[0]) >= 16 * kKv4Dim * 4, "the rows' sums fit a wave's part");
-    static_assert(sizeof(vbuf) >= RT * kQStride * 4, "the queries fit the value buffer");
+template <int ROWS, int NP, int RW, bool HALF>
+struct Kv4Smem {
+    static constexpr int RT = ROWS * RW;
+    // the queries first, then 32 value rows (bf16) a wave, at last the rows' sums
+    static constexpr int kMain =
+        4 * 32 * kKv4Dim > 2 * RT * kQStride ? 4 * 32 * kKv4Dim : 2 * RT * kQStride;
+    __align__(16) uint16_t main[kMain];
+    float2 ml[4][16];
+    int pg[kMaxPages];
+};
 
-    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, j = lane >> 4;
+template <int ROWS, int NP, int RW, bool HALF, bool EVEN>
+__device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq, const Segment& g,
+                                            Kv4Smem<ROWS, NP, RW, HALF>& sm) {
+    constexpr int SLOTS = 16 / ROWS, NM = SLOTS == 1 ? NP : 1, TW = 4 / RW, RT = ROWS * RW;
+    static_assert(SLOTS == 1 || SLOTS >= NP, "a column for each part");
+    static_assert(32 * kKv4Dim * 2 >= 16 * kKv4Dim * 4, "the rows' sums fit a wave's values");
+    uint16_t* smem = sm.main;
+    int* pg = sm.pg;
+    int tid = threadIdx.x;
+    // (opaque, so that what follows from it is not kept in registers from piece to piece)
+    if (EVEN) asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, col = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rw = wave % RW, tw = wave / RW;
-    const int per_unit = sq.Hkv * a.splits;
-    const int unit = blockIdx.x / per_unit, rest = blockIdx.x - unit * per_unit;
-    const int split = rest / sq.Hkv, h = rest - split * sq.Hkv;
-    int seq, tile;
-    if (!find_unit(sq, unit, a.G, RT, seq, tile)) return;
-    int n = 1, first = seq;
-    if (sq.cu) {
-        first = sq.cu[seq];
-        n = sq.cu[seq + 1] - first;
-    }
-    const int c = sq.length(seq);
-    const int row0 = tile * RT;                       // of the sequence's n * G
+    const int n = g.n, first = g.first, c = g.c, h = g.h, t0 = g.t0;
+    const int row0 = g.tile * RT;  // of the sequence's n * G
     const int last_i = min(n - 1, (row0 + RT - 1) / a.G);
-    const int t0 = split * a.chunk;
-    const int t1 = min(min(t0 + a.chunk, c - n + last_i + 1), c);  // tokens that some row sees
-    if (split > 0 && t0 >= t1) return;
+    const int t1 = min(min(t0 + g.len, c - n + last_i + 1), c);  // tokens that some row sees
 
     // the lane's row
     const int slot = col / ROWS, r = row0 + rw * ROWS + col % ROWS;
@@ -169,74 +232,94 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 3 : 2) kv4_attn_kernel(Kv4A
     const int pos = row_ok && c > 0 ? c - n + qi : -1;
     const int64_t grow = (int64_t)first + qi;
 
-    const int npg = t1 > t0 ? (t1 - t0 + kKv4Page - 1) / kKv4Page : 0;
-    for (int p = tid; p < npg; p += 64 * NW) {
-        const int blk = sq.tables[(int64_t)seq * sq.table_stride + t0 / kKv4Page + p];
-        pg[p] = blk >= 0 && blk < sq.n_blocks ? blk : -1;
-    }
-
-    // the rows' queries, rotated and scaled, by way of LDS (each wave needs all of a row)
-    float* qs = reinterpret_cast<float*>(vbuf);
-    for (int it = tid; it < RT * 64; it += 64 * NW) {
-        const int rr = it >> 6, d = it & 63, r2 = row0 + rr, i2 = r2 / a.G;
-        const int p2 = i2 < n && first >= 0 && first + i2 < a.T && c > 0 ? c - n + i2 : -1;
-        float x0 = 0.0f, x1 = 0.0f;
-        if (p2 >= 0) {
-            const int64_t at = ((int64_t)first + i2) * a.q_stride +
-                               (int64_t)(h * a.G + (r2 - i2 * a.G)) * kKv4Dim + d;
-            x0 = ld_act<HALF>(a.q, at);
-            x1 = ld_act<HALF>(a.q, at + 64);
-            if (a.rope) {
-                const float* cs = a.rope + (int64_t)p2 * kKv4Dim + d;
-                const float cv = cs[0], sv = cs[64], y0 = x0;
-                x0 = __builtin_fmaf(x0, cv, -__fmul_rn(x1, sv));
-                x1 = __builtin_fmaf(y0, sv, __fmul_rn(x1, cv));
-            }
+    // the page numbers of the first kMaxPages pages and the rows' queries, rotated and scaled, by
+    // way of LDS (each wave needs all of a row)
+    const int32_t* table = sq.tables + (int64_t)g.seq * sq.table_stride + t0 / kKv4Page;
+    const int pages = t1 > t0 ? (t1 - t0 + kKv4Page - 1) / kKv4Page : 0;
+    auto stage_pages = [&](int from) {
+        for (int p = from + tid; p < min(pages, from + kMaxPages); p += 256) {
+            const int id = table[p];
+            pg[p - from] = id >= 0 && id < sq.n_blocks ? id : -1;
         }
-        qs[rr * kQStride + d] = __fmul_rn(x0, kQkScale * kLog2e);
-        qs[rr * kQStride + d + 64] = __fmul_rn(x1, kQkScale * kLog2e);
+    };
+    float* qs = reinterpret_cast<float*>(smem);
+    constexpr int QT = RT / 4;
+    float x0[QT], x1[QT];
+#pragma unroll
+    for (int k = 0; k < QT; ++k) {
+        const int r2 = row0 + wave + 4 * k, i2 = r2 / a.G, p2 = c - n + i2;
+        x0[k] = x1[k] = 0.0f;
+        if (i2 < n && first >= 0 && first + i2 < a.T && p2 >= 0) {
+            const int64_t at = ((int64_t)first + i2) * a.q_stride +
+                               (int64_t)(h * a.G + (r2 - i2 * a.G)) * kKv4Dim + lane;
+            x0[k] = ld_act<HALF>(a.q, at);
+            x1[k] = ld_act<HALF>(a.q, at + 64);
+        }
+    }
+    stage_pages(0);
+#pragma unroll
+    for (int k = 0; k < QT; ++k) {
+        const int rr = wave + 4 * k, p2 = c - n + (row0 + rr) / a.G;
+        if (a.rope && p2 >= 0 && p2 < c) {
+            const float* cs = a.rope + (int64_t)p2 * kKv4Dim + lane;
+            const float cv = cs[0], sv = cs[64], y0 = x0[k];
+            x0[k] = __builtin_fmaf(y0, cv, -__fmul_rn(x1[k], sv));
+            x1[k] = __builtin_fmaf(y0, sv, __fmul_rn(x1[k], cv));
+        }
+        qs[rr * kQStride + lane] = __fmul_rn(x0[k], kQkScale * kLog2e);
+        qs[rr * kQStride + lane + 64] = __fmul_rn(x1[k], kQkScale * kLog2e);
     }
     __syncthreads();
+
+    uint4 kr[kSub], vr[kSub];
+    uint32_t ksc[kSub], vsc[kSub];
+    const uint32_t lane_code = (uint32_t)(col * kKv4Row + j * 16);
+    const uint32_t lane_scale = (uint32_t)(col * kKv4Scales + j);
+    // (a page that the pool does not hold: another one is read in its place and masked)
+    auto page_row = [&](int id) -> int64_t {
+        return (((int64_t)max(id, 0) * sq.n_layers + sq.layer) * sq.Hkv + h) * kKv4Page;
+    };
+    auto load_k = [&](int tt, int id) {
+        const int64_t row = page_row(id);
+        kr[tt] = *reinterpret_cast<const uint4*>(a.pk + row * kKv4Row + lane_code);
+        ksc[tt] = (a.pks + row * kKv4Scales)[lane_scale];
+    };
+    auto load_v = [&](int tt, int id) {
+        const int64_t row = page_row(id);
+        vr[tt] = *reinterpret_cast<const uint4*>(a.pv + row * kKv4Row + lane_code);
+        vsc[tt] = (a.pvs + row * kKv4Scales)[lane_scale];
+    };
+    int id_next[kSub];
+    // page numbers of the step at t out of the kMaxPages from token w0 on
+    auto next_ids = [&](int t, int w0) {
+#pragma unroll
+        for (int tt = 0; tt < kSub; ++tt) {
+            const int p = min(((t - w0) >> 4) + tt, pages - 1 - ((w0 - t0) >> 4));
+            id_next[tt] = __builtin_amdgcn_readfirstlane(pg[p]);
+        }
+    };
 
     f32x4 acc[8];
 #pragma unroll
     for (int d = 0; d < 8; ++d) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
 
-    uint4 kr[kSub], vr[kSub];
-    uint32_t ksc[kSub], vsc[kSub];
-    const uint32_t lane_code = (uint32_t)(col * kKv4Row + j * 16);
-    const uint32_t lane_scale = (uint32_t)(col * kKv4Scales + j);
-    auto page_row = [&](int t, int tt) -> int64_t {
-        const int p = min(((t - t0) >> 4) + tt, npg - 1);
-        const int id = __builtin_amdgcn_readfirstlane(pg[p]);
-        return (((int64_t)max(id, 0) * sq.n_layers + sq.layer) * sq.Hkv + h) * kKv4Page;
+    uint16_t* vb = smem + wave * (32 * kKv4Dim);
+    // value rows in LDS, 256 bytes each, their 16-byte pieces in an order of the row's own: eight
+    // lanes' writes (8 rows, one piece) and 16 lanes' transposing reads (4 rows, two pieces) both
+    // meet all banks once
+    auto piece = [](int row, int p) {
+        return row * kKv4Dim + ((p ^ (2 * (row & 3) + (row >> 2 & 1))) << 3);
     };
-    auto load_k = [&](int t) {
-#pragma unroll
-        for (int tt = 0; tt < kSub; ++tt) {
-            const int64_t row = page_row(t, tt);
-            kr[tt] = *reinterpret_cast<const uint4*>(a.pk + row * kKv4Row + lane_code);
-            ksc[tt] = (a.pks + row * kKv4Scales)[lane_scale];
-        }
-    };
-    auto load_v = [&](int t) {
-#pragma unroll
-        for (int tt = 0; tt < kSub; ++tt) {
-            const int64_t row = page_row(t, tt);
-            vr[tt] = *reinterpret_cast<const uint4*>(a.pv + row * kKv4Row + lane_code);
-            vsc[tt] = (a.pvs + row * kKv4Scales)[lane_scale];
-        }
-    };
-    uint16_t* vb = vbuf[wave];
-    const uint32_t vw = (uint32_t)(col * kVStride + j * 32);
-    const uint32_t vrd = (uint32_t)((4 * j + (col >> 2)) * kVStride + (col & 3) * 4);
 
     int t = t0 + kTile * tw;
     const bool any = sq.n_blocks > 0;
     if (t < t1 && any) {
-        load_k(t);
-        load_v(t);
+        next_ids(t, t0);
+#pragma unroll
+        for (int tt = 0; tt < kSub; ++tt) load_k(tt, id_next[tt]);
+#pragma unroll
+        for (int tt = 0; tt < kSub; ++tt) load_v(tt, id_next[tt]);
     }
     // Q as B operands: the lane's 32 dims 32j .. 32j + 31 of its row, in parts (part p of a value:
     // what its parts before leave, cut to 8 bits)
@@ -264,7 +347,10 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 3 : 2) kv4_attn_kernel(Kv4A
         }
     }
     __syncthreads();
-    for (; t < t1 && any; t += kTile * TW) {
+    // (kMaxPages pages at a time: page numbers in LDS)
+    for (int w0 = t0;;) {
+    const int w1 = min(t1, w0 + kMaxPages * kKv4Page);
+    for (; t < w1 && any; t += kTile * TW) {
         const int next = t + kTile * TW;
         f32x4 s[kSub];
 #pragma unroll
@@ -292,11 +378,14 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 3 : 2) kv4_attn_kernel(Kv4A
         int id_now[kSub];
 #pragma unroll
         for (int tt = 0; tt < kSub; ++tt) {
-            const int p = ((t - t0) >> 4) + tt;
-            id_now[tt] = p < npg ? __builtin_amdgcn_readfirstlane(pg[p]) : -1;
+            id_now[tt] = ((t - t0) >> 4) + tt < pages ? id_next[tt] : -1;
             bad = bad || id_now[tt] < 0;
         }
-        if (next < t1) load_k(next);
+        if (next < w1) {
+            next_ids(next, w0);
+#pragma unroll
+            for (int tt = 0; tt < kSub; ++tt) load_k(tt, id_next[tt]);
+        }
         float top = -INFINITY;
 #pragma unroll
         for (int tt = 0; tt < kSub; ++tt)
@@ -355,10 +444,12 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 3 : 2) kv4_attn_kernel(Kv4A
                     f.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 1);
                     f.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 2);
                     f.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 3);
-                    *reinterpret_cast<uint4*>(vb + vw + k * 16 * kVStride + st * 8) = f.v;
+                    *reinterpret_cast<uint4*>(vb + piece(k * 16 + col, 4 * j + st)) = f.v;
                 }
             }
-            if (u == kSub / 2 - 1 && next < t1) load_v(next);
+            if (u == kSub / 2 - 1 && next < w1)
+#pragma unroll
+                for (int tt = 0; tt < kSub; ++tt) load_v(tt, id_next[tt]);
             Frag pf[NM];
             float p8[8];
 #pragma unroll
@@ -384,15 +475,29 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 3 : 2) kv4_attn_kernel(Kv4A
                     s16x4 h[2];
                     bf16x8 v;
                 } vf;
-                vf.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vb + vrd + d * 16));
-                vf.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (lds4)(vb + vrd + 16 * kVStride + d * 16));
+                // (lane 4r + i of 16: half a piece of row r, in return for column 4r + i)
+                const int at = piece(4 * j + (col >> 2), 2 * d + (col >> 1 & 1)) + (col & 1) * 4;
+                vf.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vb + at));
+                vf.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vb + at + 16 * kKv4Dim));
 #pragma unroll
                 for (int p = 0; p < NM; ++p)
                     acc[d] =
                         __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.v, pf[p].v, acc[d], 0, 0, 0);
             }
         }
+    }
+    w0 += kMaxPages * kKv4Page;
+    if (w0 >= t1 || !any) break;
+    __syncthreads();
+    stage_pages((w0 - t0) / kKv4Page);
+    __syncthreads();
+    if (t < t1) {
+        next_ids(t, w0);
+#pragma unroll
+        for (int tt = 0; tt < kSub; ++tt) load_k(tt, id_next[tt]);
+#pragma unroll
+        for (int tt = 0; tt < kSub; ++tt) load_v(tt, id_next[tt]);
+    }
     }
 
     l = sum_quarters(l);
@@ -407,6 +512,11 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 3 : 2) kv4_attn_kernel(Kv4A
                 acc[d][i] = v;
             }
     }
+    // a row's sums: to `out` where no other piece has any of its tokens, else a record
+    auto direct = [&](int p) { return EVEN ? g.whole : p < a.chunk || a.splits == 1; };
+    auto record = [&](int rr, int64_t gr, int64_t hd) {
+        return EVEN ? g.rec + rr : (gr * a.Hq + hd) * a.splits + g.split;
+    };
     if (TW > 1) {
         // the waves' sums meet: every wave's rows in its own part of the value buffer
         float* o = reinterpret_cast<float*>(vb);
@@ -414,47 +524,47 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 3 : 2) kv4_attn_kernel(Kv4A
 #pragma unroll
             for (int d = 0; d < 8; ++d)
                 *reinterpret_cast<f32x4*>(o + col * kKv4Dim + 16 * d + 4 * j) = acc[d];
-            if (j == 0) ml[wave][col] = make_float2(m, l);
+            if (j == 0) sm.ml[wave][col] = make_float2(m, l);
         }
         __syncthreads();
-        for (int it = tid; it < RT * 32; it += 64 * NW) {
+        for (int it = tid; it < RT * 32; it += 256) {
             const int rr = it >> 5, d4 = it & 31, grp = rr / ROWS, cc = rr % ROWS;
             const int r2 = row0 + rr, i2 = r2 / a.G;
             if (i2 >= n || first < 0 || first + i2 >= a.T) continue;
             float M = -INFINITY, L = 0.0f;
             f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int w = 0; w < TW; ++w) M = fmaxf(M, ml[w * RW + grp][cc].x);
+            for (int w = 0; w < TW; ++w) M = fmaxf(M, sm.ml[w * RW + grp][cc].x);
             const float base = M == -INFINITY ? 0.0f : M;
 #pragma unroll
             for (int w = 0; w < TW; ++w) {
-                const float2 e = ml[w * RW + grp][cc];
+                const float2 e = sm.ml[w * RW + grp][cc];
                 const float f = __builtin_amdgcn_exp2f(e.x - base);
                 L += e.y * f;
                 v += f * *reinterpret_cast<const f32x4*>(
-                             reinterpret_cast<const float*>(vbuf[w * RW + grp]) + cc * kKv4Dim +
-                             4 * d4);
+                             reinterpret_cast<const float*>(smem + (w * RW + grp) * (32 * kKv4Dim)) +
+                             cc * kKv4Dim + 4 * d4);
             }
-            const int p2 = c > 0 ? c - n + i2 : -1;
             const int64_t g2 = (int64_t)first + i2, hd = h * a.G + (r2 - i2 * a.G);
-            if (p2 < a.chunk || a.splits == 1) {
-                if (split == 0)
+            if (direct(c - n + i2)) {
+                if (EVEN || g.split == 0)
                     store4<HALF>(a, g2 * a.out_stride + hd * kKv4Dim + 4 * d4, v, L);
             } else {
-                const int64_t at = (g2 * a.Hq + hd) * a.splits + split;
+                const int64_t at = record(rr, g2, hd);
                 *reinterpret_cast<f32x4*>(a.part_o + at * kKv4Dim + 4 * d4) = v;
                 if (d4 == 0) a.part_ml[at] = make_float2(M, L);
             }
         }
+        if (EVEN) __syncthreads();
     } else if (row_ok && slot == 0) {
-        if (pos < a.chunk || a.splits == 1) {
-            if (split == 0)
+        if (direct(pos)) {
+            if (g.split == 0)
 #pragma unroll
                 for (int d = 0; d < 8; ++d)
                     store4<HALF>(a, grow * a.out_stride + (int64_t)head * kKv4Dim + 16 * d + 4 * j,
                                  acc[d], l);
         } else {
-            const int64_t at = (grow * a.Hq + head) * a.splits + split;
+            const int64_t at = record(0, grow, head);
 #pragma unroll
             for (int d = 0; d < 8; ++d)
                 *reinterpret_cast<f32x4*>(a.part_o + at * kKv4Dim + 16 * d + 4 * j) = acc[d];
@@ -463,7 +573,153 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 3 : 2) kv4_attn_kernel(Kv4A
     }
 }
 
-// Joins the splits of a row and head: 32 lanes x 4 dims, 16 groups of splits.
+// A grid of (unit, split, kv head): every workgroup one piece.
+template <int ROWS, int NP, int RW, bool HALF>
+__global__ void __launch_bounds__(256, ROWS == 16 && NP == 3 ? 2 : 3)
+kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
+    __shared__ Kv4Smem<ROWS, NP, RW, HALF> sm;
+    const int per_unit = sq.Hkv * a.splits;
+    // (from the last unit on: the latest rows of a prompt see the most tokens)
+    const int back = blockIdx.x / per_unit, rest = blockIdx.x - back * per_unit;
+    const int unit = a.wgs / per_unit - 1 - back;
+    Segment g;
+    g.split = rest / sq.Hkv;
+    g.h = rest - g.split * sq.Hkv;
+    if (!find_unit(sq, unit, a.G, ROWS * RW, g.seq, g.tile)) return;
+    g.first = sq.cu ? sq.cu[g.seq] : g.seq;
+    g.n = sq.cu ? sq.cu[g.seq + 1] - g.first : 1;
+    g.c = sq.length(g.seq);
+    g.t0 = g.split * a.chunk;
+    g.len = a.chunk;
+    const int last_i = min(g.n - 1, (g.tile * ROWS * RW + ROWS * RW - 1) / a.G);
+    if (g.split > 0 && g.t0 >= min(g.c - g.n + last_i + 1, g.c)) return;
+    kv4_segment<ROWS, NP, RW, HALF, false>(a, sq, g, sm);
+}
+
+// Several sequences of a few rows: all their steps in a row (sequence by sequence, unit by unit)
+// and an equal share of them to each of as many workgroups as the GPU holds at once, so that
+// lengths, which only the device knows, need not be alike. A share holds the end of a unit that
+// an earlier workgroup began, whole units and the beginning of one: two records at most.
+template <int ROWS, int NP, bool HALF>
+__global__ void __launch_bounds__(256, ROWS == 16 && NP == 3 ? 2 : 3)
+kv4_attn_even_kernel(Kv4Attn a, Kv4Seqs sq) {
+    __shared__ Kv4Smem<ROWS, NP, 1, HALF> sm;
+    __shared__ int wsum[4], at_base, at_seq;
+    const int per = (sq.B + 255) / 256, b0 = threadIdx.x * per;
+    int mine = 0, total;
+    for (int b = b0; b < min(sq.B, b0 + per); ++b)
+        mine += SeqWork(sq, b, a.G, ROWS).total(sq.Hkv);
+    int base = block_scan<4>(mine, wsum, total);
+    total = uniform(total);
+    const int begin = wg_start(blockIdx.x, total, a.wgs);
+    const int end = wg_start(blockIdx.x + 1, total, a.wgs);
+    if (begin >= end) return;
+    if (begin >= base && begin < base + mine) {
+        int b = b0;
+        for (;; ++b) {
+            const int w = SeqWork(sq, b, a.G, ROWS).total(sq.Hkv);
+            if (begin < base + w) break;
+            base += w;
+        }
+        at_seq = b;
+        at_base = base;
+    }
+    __syncthreads();
+    int b = uniform(at_seq);
+    base = uniform(at_base);
+    for (int at = begin; at < end;) {
+        const SeqWork w(sq, b, a.G, ROWS);
+        const int past = at - base;
+        if (past >= w.total(sq.Hkv)) {
+            base += w.total(sq.Hkv);
+            ++b;
+            continue;
+        }
+        const int unit = past / w.slots(), s0 = past - unit * w.slots();
+        const int len = min(w.slots() - s0, end - at);
+        at += len;
+        // (slot 0 is the one without tokens)
+        const int from = max(s0 - 1, 0), to = s0 + len - 1;
+        if (to == from) continue;
+        Segment g;
+        g.seq = b;
+        g.first = w.first;
+        g.n = w.n;
+        g.c = w.c;
+        g.h = unit / w.tiles;
+        g.tile = unit - g.h * w.tiles;
+        g.t0 = from * kStep;
+        g.len = (to - from) * kStep;
+        g.whole = to - from == w.steps;
+        g.rec = ((int64_t)blockIdx.x * 2 + (from == 0 ? 1 : 0)) * ROWS;
+        g.split = 0;
+        kv4_segment<ROWS, NP, 1, HALF, true>(a, sq, g, sm);
+    }
+}
+
+// The records of a row's head, GROUPS lanes groups of 32 x 4 dims sharing them: record k of ns
+// is first + k * step, of k >= 1 `skip` less.
+struct Records {
+    int64_t first, step, skip;
+    int ns;
+    __device__ __forceinline__ int64_t at(int k) const {
+        return first + k * step - (k > 0 ? skip : 0);
+    }
+};
+template <bool HALF, int GROUPS>
+__device__ __forceinline__ void kv4_join(const Kv4Attn& a, const Records& rc, int64_t out_at, int g,
+                                         f32x4 (*ov)[32], float* lv) {
+    const int lane = threadIdx.x & 63, d4 = threadIdx.x & 31;
+    constexpr int kAhead = 4;  // a group's first sums on their way while the maximum is found
+    f32x4 pv[kAhead];
+    float2 pe[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+        const int s = g + GROUPS * k;
+        pv[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        pe[k] = make_float2(-INFINITY, 0.0f);
+        if (s < rc.ns) {
+            pv[k] = *reinterpret_cast<const f32x4*>(a.part_o + rc.at(s) * kKv4Dim + 4 * d4);
+            pe[k] = a.part_ml[rc.at(s)];
+        }
+    }
+    float M = -INFINITY;
+    if (GROUPS > 1) {
+        for (int s = lane; s < rc.ns; s += 64) M = fmaxf(M, a.part_ml[rc.at(s)].x);
+        M = wave_max(M);
+    } else {
+        for (int s = 0; s < rc.ns; ++s)
+            M = fmaxf(M, s < kAhead ? pe[0].x : a.part_ml[rc.at(s)].x);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) M = fmaxf(M, pe[k].x);
+    }
+    const float base = M == -INFINITY ? 0.0f : M;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    float L = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+        const float f = __builtin_amdgcn_exp2f(pe[k].x - base);
+        L += pe[k].y * f;
+        v += f * pv[k];
+    }
+#pragma unroll 4
+    for (int s = g + GROUPS * kAhead; s < rc.ns; s += GROUPS) {
+        const float2 e = a.part_ml[rc.at(s)];
+        const float f = __builtin_amdgcn_exp2f(e.x - base);
+        L += e.y * f;
+        v += f * *reinterpret_cast<const f32x4*>(a.part_o + rc.at(s) * kKv4Dim + 4 * d4);
+    }
+    if (GROUPS > 1) {
+        ov[g][d4] = v;
+        if (d4 == 0) lv[g] = L;
+        __syncthreads();
+        if (g > 0) return;
+        for (int k = 1; k < GROUPS; ++k) v += ov[k][d4], L += lv[k];
+    }
+    store4<HALF>(a, out_at + 4 * d4, v, L);
+}
+
+// Joins the splits of a grid: a workgroup per row and head.
 template <bool HALF>
 __global__ void __launch_bounds__(512) kv4_join_kernel(Kv4Attn a, Kv4Seqs sq) {
     __shared__ f32x4 ov[16][32];
@@ -471,36 +727,57 @@ __global__ void __launch_bounds__(512) kv4_join_kernel(Kv4Attn a, Kv4Seqs sq) {
     const int row = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
     int seq, pos;
     if (!kv4_place(sq, row, tid & 15, seq, pos) || pos < a.chunk) return;
-    const int ns = pos / a.chunk + 1;
-    const int64_t at = ((int64_t)row * a.Hq + head) * a.splits;
-    const float2* ml = a.part_ml + at;
-    float M = -INFINITY;
-    for (int s = tid & 63; s < ns; s += 64) M = fmaxf(M, ml[s].x);
-    M = wave_max(M);
-    const float base = M == -INFINITY ? 0.0f : M;
-    const int d4 = tid & 31, g = tid >> 5;
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    float L = 0.0f;
-#pragma unroll 4
-    for (int s = g; s < ns; s += 16) {
-        const float2 e = ml[s];
-        const float f = __builtin_amdgcn_exp2f(e.x - base);
-        L += e.y * f;
-        v += f * *reinterpret_cast<const f32x4*>(a.part_o + (at + s) * kKv4Dim + 4 * d4);
-    }
-    ov[g][d4] = v;
-    if (d4 == 0) lv[g] = L;
-    __syncthreads();
-    if (g == 0) {
-        for (int k = 1; k < 16; ++k) v += ov[k][d4], L += lv[k];
-        store4<HALF>(a, row * a.out_stride + (int64_t)head * kKv4Dim + 4 * d4, v, L);
-    }
+    const Records rc{((int64_t)row * a.Hq + head) * a.splits, 1, 0, pos / a.chunk + 1};
+    kv4_join<HALF, 16>(a, rc, row * a.out_stride + (int64_t)head * kKv4Dim, tid >> 5, ov, lv);
 }
 
-// Rows and waves of a workgroup, tokens of a split and how many splits, from what the host knows.
+// Joins the shares of steps dealt evenly: a workgroup has a row's head (WIDE: few rows, many
+// records a head, shared by 8 groups of lanes) or 8 of its heads. Rows of sequences without tokens,
+// which no workgroup has had, are written as zeros.
+template <int ROWS, bool HALF, bool WIDE>
+__global__ void __launch_bounds__(256) kv4_join_even_kernel(Kv4Attn a, Kv4Seqs sq) {
+    __shared__ f32x4 ov[WIDE ? 8 : 1][32];
+    __shared__ float lv[8];
+    __shared__ int wsum[4], at_base, at_seq;
+    const int row = blockIdx.x, tid = threadIdx.x, grp = tid >> 5;
+    const int per = (sq.B + 255) / 256, b0 = tid * per;
+    int mine = 0, total;
+    if (tid == 0) at_seq = -1;
+    for (int b = b0; b < min(sq.B, b0 + per); ++b)
+        mine += SeqWork(sq, b, a.G, ROWS).total(sq.Hkv);
+    int base = block_scan<4>(mine, wsum, total);
+    for (int b = b0; b < min(sq.B, b0 + per); ++b) {
+        const SeqWork w(sq, b, a.G, ROWS);
+        if (w.first >= 0 && row >= w.first && row < w.first + w.n) at_seq = b, at_base = base;
+        base += w.total(sq.Hkv);
+    }
+    __syncthreads();
+    const int seq = uniform(at_seq), head = WIDE ? (int)blockIdx.y : (int)blockIdx.y * 8 + grp;
+    if (seq < 0 || head >= a.Hq) return;
+    base = uniform(at_base);
+    total = uniform(total);
+    const SeqWork w(sq, seq, a.G, ROWS);
+    const int64_t out_at = row * a.out_stride + (int64_t)head * kKv4Dim;
+    if (w.c == 0) {
+        if (!WIDE || grp == 0)
+            store4<HALF>(a, out_at + 4 * (tid & 31), f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0.0f);
+        return;
+    }
+    const int h = head / a.G, r = (row - w.first) * a.G + head - h * a.G;
+    const int start = base + (h * w.tiles + r / ROWS) * w.slots() + 1;
+    const int w0 = wg_of(start, total, a.wgs), w1 = wg_of(start + w.steps - 1, total, a.wgs);
+    if (w0 == w1) return;
+    // workgroup w0 has the unit's beginning (its second record), those after it continue it
+    const Records rc{((int64_t)w0 * 2 + 1) * ROWS + r % ROWS, 2 * ROWS, ROWS, w1 - w0 + 1};
+    kv4_join<HALF, WIDE ? 8 : 1>(a, rc, out_at, WIDE ? grp : 0, ov, lv);
+}
+
+// Rows of a workgroup and how the tokens are dealt out, from what the host knows.
 struct Kv4Plan {
-    int rows, rw, nw, splits, chunk;
-    int64_t units;
+    int rows, rw, splits, chunk;
+    bool even;
+    int64_t wgs;
+    size_t records;
 };
 Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, bool half) {
     Kv4Plan p{};
@@ -509,44 +786,68 @@ Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, boo
     p.rows = per <= packed ? packed : 16;
     p.rw = per <= 16 ? 1 : per <= 32 ? 2 : 4;
     const int rt = p.rows * p.rw;
-    p.units = cu ? T * G / rt + B : (int64_t)B * ceil_div(G, rt);
+    const int64_t units = cu ? T * G / rt + B : (int64_t)B * ceil_div(G, rt);
     const int64_t ctx = (int64_t)table_width * kKv4Page;
-    const int64_t wgs = p.units * Hkv;
-    // few sequences that three steps of 8 waves get through: the second launch costs more
-    p.nw = p.rw == 1 && wgs <= 256 && ctx <= 3 * 8 * kTile ? 8 : 4;
-    const int64_t step = kTile * (p.nw / p.rw);
-    // else enough workgroups for every CU to have four, each wave a step of tokens at least
-    int64_t s = p.nw == 8 ? 1 : ceil_div(1024, wgs);
-    s = s < ceil_div(ctx, step) ? s : ceil_div(ctx, step);
-    if (s < 1) s = 1;
-    int64_t chunk = ceil_div(ceil_div(ctx, s), step) * step;
-    if (chunk > kMaxPages * kKv4Page) chunk = kMaxPages * kKv4Page;
-    if (chunk < step) chunk = step;
-    p.chunk = (int)chunk;
-    p.splits = ctx > 0 ? (int)ceil_div(ctx, chunk) : 1;
+    const int64_t step = kTile * (4 / p.rw);
+    const int64_t steps = ctx > 0 ? ceil_div(ctx, step) : 1;
+    const int room = 768;  // workgroups that the GPU holds at once, three a CU
+    const int64_t most = units * Hkv * (steps + 1);
+    // Units that fill the GPU twice over are balanced by its own scheduling, and where every
+    // workgroup has a step at most there is nothing to balance. Between: 48 sequences of up to 8190
+    // tokens, 32 / 8 heads, 59 us (a grid of splits 69).
+    p.even = p.rw == 1 && B > 1 && units * Hkv < 2 * room && units * Hkv * steps > room &&
+             most <= INT32_MAX;
+    if (p.even) {
+        p.wgs = most < room ? most : room;
+        p.splits = 1;
+        p.records = (size_t)p.wgs * 2 * p.rows;
+        return p;
+    }
+    int64_t s = room / (units * Hkv);
+    s = s < 1 ? 1 : s > steps ? steps : s;
+    const int64_t chunk = ceil_div(steps, s) * step;
+    p.chunk = (int)(chunk < INT32_MAX / 2 ? chunk : INT32_MAX / 2 / step * step);
+    p.splits = ctx > 0 ? (int)ceil_div(ctx, p.chunk) : 1;
+    p.wgs = units * p.splits * Hkv;
+    p.records = p.splits > 1 ? (size_t)T * G * Hkv * p.splits : 0;
     return p;
 }
 
-template <int ROWS, int NP, int RW, int NW, bool HALF>
-void launch_kv4(const Kv4Attn& a, const Kv4Seqs& s, unsigned wgs, hipStream_t st) {
-    hipLaunchKernelGGL((kv4_attn_kernel<ROWS, NP, RW, NW, HALF>), dim3(wgs), dim3(64 * NW), 0, st,
-                       a, s);
+template <int ROWS, int NP, int RW, bool HALF>
+void launch_kv4(const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
+    hipLaunchKernelGGL((kv4_attn_kernel<ROWS, NP, RW, HALF>), dim3(a.wgs), dim3(256), 0, st, a, s);
+}
+template <int ROWS, int NP, bool HALF>
+int launch_kv4_even(const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
+    hipLaunchKernelGGL((kv4_attn_even_kernel<ROWS, NP, HALF>), dim3(a.wgs), dim3(256), 0, st, a, s);
+    const int rc = launch_status("kv4_attn_even_kernel");
+    if (rc) return rc;
+    // few rows: a head to a workgroup, its records to 8 groups of lanes
+    if ((int64_t)a.T * a.Hq <= 1024)
+        hipLaunchKernelGGL((kv4_join_even_kernel<ROWS, HALF, true>), dim3(a.T, a.Hq), dim3(256), 0,
+                           st, a, s);
+    else
+        hipLaunchKernelGGL((kv4_join_even_kernel<ROWS, HALF, false>),
+                           dim3(a.T, (a.Hq + 7) / 8), dim3(256), 0, st, a, s);
+    return launch_status("kv4_join_even_kernel");
 }
 template <int PACKED, int NP, bool HALF>
-void launch_kv4_plan(const Kv4Plan& p, const Kv4Attn& a, const Kv4Seqs& s, unsigned wgs,
-                     hipStream_t st) {
-    if (p.rows == PACKED && p.nw == 8)
-        launch_kv4<PACKED, NP, 1, 8, HALF>(a, s, wgs, st);
-    else if (p.rows == PACKED)
-        launch_kv4<PACKED, NP, 1, 4, HALF>(a, s, wgs, st);
-    else if (p.nw == 8)
-        launch_kv4<16, NP, 1, 8, HALF>(a, s, wgs, st);
+int launch_kv4_plan(const Kv4Plan& p, const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
+    if (p.even)
+        return p.rows == PACKED ? launch_kv4_even<PACKED, NP, HALF>(a, s, st)
+                                : launch_kv4_even<16, NP, HALF>(a, s, st);
+    if (p.rows == PACKED)
+        launch_kv4<PACKED, NP, 1, HALF>(a, s, st);
     else if (p.rw == 1)
-        launch_kv4<16, NP, 1, 4, HALF>(a, s, wgs, st);
+        launch_kv4<16, NP, 1, HALF>(a, s, st);
     else if (p.rw == 2)
-        launch_kv4<16, NP, 2, 4, HALF>(a, s, wgs, st);
+        launch_kv4<16, NP, 2, HALF>(a, s, st);
     else
-        launch_kv4<16, NP, 4, 4, HALF>(a, s, wgs, st);
+        launch_kv4<16, NP, 4, HALF>(a, s, st);
+    const int rc = launch_status("kv4_attn_kernel");
+    if (rc || p.splits == 1) return rc;
+    hipLaunchKernelGGL(kv4_join_kernel<HALF>, dim3(a.T, a.Hq), dim3(512), 0, st, a, s);
+    return launch_status("kv4_join_kernel");
 }
 
 }  // namespace
@@ -560,7 +861,7 @@ TENZO_HIP_API size_t tenzo_hip_attn_kv4_ws_bytes(int64_t T, int B, int Hq, int H
                                                  int table_width, int has_cu, int dtype) {
     if (T <= 0 || B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || table_width < 0) return 0;
     const Kv4Plan p = kv4_plan(T, B, Hq / Hkv, Hkv, table_width, has_cu != 0, dtype != 0);
-    return p.splits > 1 ? (size_t)T * Hq * p.splits * (kKv4Dim * 4 + 8) : 0;
+    return p.records * (kKv4Dim * 4 + 8);
 }
 
 TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,
@@ -592,8 +893,7 @@ TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,
              ws ? ws_bytes : 0);
     const int G = Hq / Hkv;
     const Kv4Plan p = kv4_plan(T, B, G, Hkv, table_width, cu_q != nullptr, dtype != 0);
-    const int64_t wgs = p.units * p.splits * Hkv;
-    TZ_CHECK(wgs <= 0xffffff && T <= 0x7fffff && Hq <= 65535, "attn_kv4: %lld rows of %d heads",
+    TZ_CHECK(p.wgs <= 0xffffff && T <= 0x7fffff && Hq <= 65535, "attn_kv4: %lld rows of %d heads",
              (long long)T, Hq);
     Kv4Attn a{};
     a.q = q;
@@ -606,26 +906,16 @@ TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,
     a.pvs = pvs;
     a.rope = rope_cs;
     a.part_o = (float*)ws;
-    a.part_ml = (float2*)((char*)ws + (size_t)T * Hq * p.splits * kKv4Dim * 4);
+    a.part_ml = (float2*)((char*)ws + p.records * kKv4Dim * 4);
+    a.wgs = (int)p.wgs;
     a.G = G;
     a.Hq = Hq;
     a.T = (int)T;
     a.chunk = p.chunk;
     a.splits = p.splits;
     a.vec_out = (((uintptr_t)out | (uintptr_t)(out_stride * (dtype ? 2 : 4))) & 15) == 0;
-    hipStream_t st = (hipStream_t)stream;
-    if (dtype)
-        launch_kv4_plan<8, 2, true>(p, a, s, (unsigned)wgs, st);
-    else
-        launch_kv4_plan<4, 3, false>(p, a, s, (unsigned)wgs, st);
-    const int rc2 = launch_status("kv4_attn_kernel");
-    if (rc2 || p.splits == 1) return rc2;
-    const dim3 jgrid((unsigned)T, (unsigned)Hq);
-    if (dtype)
-        hipLaunchKernelGGL(kv4_join_kernel<true>, jgrid, dim3(512), 0, st, a, s);
-    else
-        hipLaunchKernelGGL(kv4_join_kernel<false>, jgrid, dim3(512), 0, st, a, s);
-    return launch_status("kv4_join_kernel");
+    return dtype ? launch_kv4_plan<8, 2, true>(p, a, s, (hipStream_t)stream)
+                 : launch_kv4_plan<4, 3, false>(p, a, s, (hipStream_t)stream);
 }
 
 }  // extern "C"

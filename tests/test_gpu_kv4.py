@@ -229,6 +229,36 @@ def test_attention_long(torch_dev, ops, ctx, Hq, Hkv, dtype):
     s.check_attention(ops.attn_kv4(s.d["q"], *s.args(), **s.opts()).cpu().numpy())
 
 
+@pytest.mark.parametrize("Hq,Hkv,dtype", [(4, 1, np.float32), (8, 1, np.float16),
+                                          (12, 1, np.float32), (8, 2, np.float16)])
+def test_attention_ragged_batch(torch_dev, ops, Hq, Hkv, dtype):
+    """Lengths from 0 to 9000 side by side: workgroups that end a sequence, take others whole
+    and begin the next; several rows a sequence, more of them than their length holds."""
+    rng = np.random.default_rng(Hq)
+    lens = [9000, 0, 256, 257, 1, 512, 0, 700, 5000, 255, 3000, 0] + list(rng.integers(1, 400, 20))
+    s = Setup([(1, int(c)) for c in lens], Hq, Hkv, layers=1, cu=False, dtype=dtype,
+              seed=Hq).dev(torch_dev)
+    print("attn ragged", Hq, Hkv, flush=True)
+    s.check_attention(ops.attn_kv4(s.d["q"], *s.args(), **s.opts()).cpu().numpy())
+    rows = [int(n) for n in rng.integers(0, 4, len(lens))]
+    s = Setup(list(zip(rows, map(int, lens))), Hq, Hkv, layers=1, dtype=dtype, seed=Hq + 1,
+              tail=2).dev(torch_dev)
+    start = np.full((s.T, Hq, D), 7.0, dtype)
+    out = torch_dev.from_numpy(start).cuda()
+    ops.attn_kv4(s.d["q"], *s.args(), **s.opts(), out=out)
+    s.check_attention(out.cpu().numpy(), start)
+
+
+def test_attention_many_pages(torch_dev, ops):
+    """More page numbers than a workgroup keeps at a time: one sequence of 17000 tokens among
+    slots that are empty but fill the GPU."""
+    lens = [0] * 450
+    lens[77], lens[300] = 17000, 16500
+    s = Setup([(1, c) for c in lens], 16, 4, layers=1, cu=False, seed=5).dev(torch_dev)
+    print("attn many pages", flush=True)
+    s.check_attention(ops.attn_kv4(s.d["q"], *s.args(), **s.opts()).cpu().numpy())
+
+
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])
 @pytest.mark.parametrize("Hq,Hkv,seqs", [
     (4, 1, [(2, 2), (3, 40), (1, 65)]), (8, 1, [(7, 100), (5, 5), (0, 30), (9, 2)]),
