@@ -100,7 +100,7 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 // -inf is no bound) the k-th largest is found bit by bit instead, and among its equals the
 // lowest tokens.
 template <int E>
-__global__ void __launch_bounds__(256) beam_slice_kernel(BeamSelect a) {
+__global__ void __launch_bounds__(256, 8) beam_slice_kernel(BeamSelect a) {
     __shared__ uint64_t list[kSliceCand];
     __shared__ float bound[4], tops[4];
     __shared__ double part[4];
@@ -253,11 +253,20 @@ __device__ __forceinline__ bool before(const BeamCand& a, const BeamCand& b) {
 __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
     __shared__ double lse[kBeamMax], own[kBeamMax];
     __shared__ double ls[kPickCand];
-    __shared__ float lx[kPickCand], bound[16];
+    __shared__ float lx[kPickCand], bound[16], tops[64];
     __shared__ int lw[kPickCand], lt[kPickCand], cnt;
     __shared__ BeamCand best[16];
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int per = a.ns * a.k, total = a.W * per, lists = a.W * a.ns;
+    const float2* cand = a.cand + (int64_t)b * total;
+    const float2 head = tid < lists ? cand[tid * a.k] : make_float2(-INFINITY, 0.0f);
+    constexpr int kOwn = 4;  // a thread's first candidates, on their way during the log-sums
+    float2 mine[kOwn];
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i)
+        mine[i] = tid + 1024 * i < total ? cand[tid + 1024 * i]
+                                         : make_float2(-INFINITY, __int_as_float(INT_MAX));
     for (int w = wave; w < a.W; w += 16) {
         const double2* sums = a.sums + ((int64_t)b * a.W + w) * a.ns;
         double m = -INFINITY;
@@ -274,10 +283,7 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
     }
     if (tid == 0) cnt = 0;
     __syncthreads();
-    const int per = a.ns * a.k, lists = a.W * a.ns;
-    const float2* cand = a.cand + (int64_t)b * a.W * per;
-    const auto get = [&](int c) {
-        const float2 e = cand[c];
+    const auto get = [&](int c, float2 e) {
         BeamCand r;
         r.w = c / per;
         r.x = e.x;
@@ -286,33 +292,48 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
         return r;
     };
     float top = -INFINITY;
-    for (int i = tid; i < lists; i += 1024) top = fmaxf(top, __double2float_rd(get(i * a.k).s));
-    const float kth = lane_f(sort64_desc(top), a.k - 1);
-    if (lane == 0) bound[wave] = kth;
+    if (tid < lists) top = __double2float_rd(get(tid * a.k, head).s);
+    for (int i = tid + 1024; i < lists; i += 1024)
+        top = fmaxf(top, __double2float_rd(get(i * a.k, cand[i * a.k]).s));
+    // two such bounds, the larger one holds: the k-th of a wave's 64 lanes, and the k-th of the
+    // 4 best lanes of every wave
+    const float sorted = sort64_desc(top);
+    if (lane < 4) tops[wave * 4 + lane] = sorted;
+    if (lane == 0) bound[wave] = lane_f(sorted, a.k - 1);
     __syncthreads();
-    float tau = bound[0];
+    float tau = lane_f(sort64_desc(tops[lane]), a.k - 1);
 #pragma unroll
-    for (int w = 1; w < 16; ++w) tau = fmaxf(tau, bound[w]);
-    for (int i = tid; i < lists; i += 1024)
-        for (int j = 0; j < a.k; ++j) {
-            const BeamCand c = get(i * a.k + j);
-            if (c.t == INT_MAX || __double2float_rd(c.s) < tau) break;
-            const int at = atomicAdd(&cnt, 1);
-            if (at >= kPickCand) break;
-            ls[at] = c.s, lx[at] = c.x, lw[at] = c.w, lt[at] = c.t;
-        }
+    for (int w = 0; w < 16; ++w) tau = fmaxf(tau, bound[w]);
+    const auto keep = [&](const BeamCand& c) {
+        if (c.t == INT_MAX || __double2float_rd(c.s) < tau) return;
+        const int at = atomicAdd(&cnt, 1);
+        if (at < kPickCand) ls[at] = c.s, lx[at] = c.x, lw[at] = c.w, lt[at] = c.t;
+    };
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i)
+        if (tid + 1024 * i < total) keep(get(tid + 1024 * i, mine[i]));
+    for (int c = tid + 1024 * kOwn; c < total; c += 1024) keep(get(c, cand[c]));
     __syncthreads();
     const int n = cnt;
     if (n <= kPickCand) {
-        for (int i = tid; i < n; i += 1024) {
-            const BeamCand me{ls[i], lx[i], lw[i], lt[i]};
+        // four lanes to a candidate; equal scores are rare and looked at in full
+        const int q = tid & 3;
+        for (int i0 = 0; i0 < n; i0 += 256) {
+            const int i = i0 + (tid >> 2);
+            const double me = ls[min(i, n - 1)];
             int rank = 0;
-            for (int o = 0; o < n; ++o)
-                rank += before(BeamCand{ls[o], lx[o], lw[o], lt[o]}, me) ? 1 : 0;
-            if (rank < a.k) {
-                a.out_scores[b * a.k + rank] = (float)me.s;
-                a.out_beams[b * a.k + rank] = me.w;
-                a.out_tokens[b * a.k + rank] = me.t;
+            for (int o = q; o < n; o += 4) {
+                rank += ls[o] > me ? 1 : 0;
+                if (ls[o] == me && i < n &&
+                    before(BeamCand{me, lx[o], lw[o], lt[o]}, BeamCand{me, lx[i], lw[i], lt[i]}))
+                    ++rank;
+            }
+            rank += dpp_i<kDppXor1>(rank);
+            rank += dpp_i<kDppXor2>(rank);
+            if (i < n && q == 0 && rank < a.k) {
+                a.out_scores[b * a.k + rank] = (float)me;
+                a.out_beams[b * a.k + rank] = lw[i];
+                a.out_tokens[b * a.k + rank] = lt[i];
             }
         }
         return;
@@ -321,8 +342,8 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
     const BeamCand none{-INFINITY, -INFINITY, INT_MAX, INT_MAX};
     for (int j = 0; j < a.k; ++j) {
         BeamCand m = none;
-        for (int c = tid; c < a.W * per; c += 1024) {
-            const BeamCand e = get(c);
+        for (int c = tid; c < total; c += 1024) {
+            const BeamCand e = get(c, cand[c]);
             if (e.t != INT_MAX && before(last, e) && before(e, m)) m = e;
         }
         for (int d = 32; d > 0; d >>= 1) {
@@ -345,8 +366,8 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
     }
 }
 
-// Logits a thread of stage 1 holds: 32 where that fills the GPU, 8 for few rows.
-int beam_elems(int64_t rows, int64_t V) { return rows * ceil_div(V, 256 * 32) >= 512 ? 32 : 8; }
+// Logits a thread of stage 1 holds: 16 where that fills the GPU, 8 for few rows.
+int beam_elems(int64_t rows, int64_t V) { return rows * ceil_div(V, 256 * 16) >= 256 ? 16 : 8; }
 
 // ------------------------------------------------------------- reordering --
 
@@ -358,46 +379,41 @@ struct BeamReorder {
     uint8_t* codes[2];
     uint8_t* scales[2];
     int B, W, width, row_bytes;
-    int piece_blocks;
+    int copiers;  // workgroups that copy a request's pieces
 };
 
 constexpr int kPageTokens = 16;
 
-// One piece of the page in progress, for all slots of a request.
+// What slot i of a request takes: from which page to which (in progress), or nothing.
+template <int WMAX>
+struct Moves {
+    int64_t from[WMAX], to[WMAX];  // first row of the pages' planes, -1: stays
+};
+
+// One piece of the page in progress (bytes `at` of pages of `size`), for all slots of a request:
+// every parent's is read before the first is written, so no slot's is lost whatever the
+// permutation, and no two threads touch the same piece.
 template <int WMAX, typename P>
-__device__ __forceinline__ void move_piece(const BeamReorder& a, const int32_t* table,
-                                           const int32_t* parents, uint8_t* pool, int64_t plane,
-                                           int page_bytes, int off, int full) {
+__device__ __forceinline__ void move_piece(const Moves<WMAX>& m, uint8_t* pool, int64_t size,
+                                           int64_t at) {
     P v[WMAX];
-    bool moved[WMAX];
 #pragma unroll
     for (int i = 0; i < WMAX; ++i) {
         v[i] = P{};
-        moved[i] = false;
-        if (i < a.W) {
-            const int par = parents[i];
-            const bool other = par >= 0 && par < a.W && par != i;
-            const int64_t from = table[(other ? par : i) * a.table_stride + full];
-            const int64_t to = table[i * a.table_stride + full];
-            moved[i] = other && from >= 0 && from < a.n_blocks && to >= 0 && to < a.n_blocks;
-            if (moved[i])
-                v[i] = *reinterpret_cast<const P*>(pool + (from * a.planes + plane) * page_bytes +
-                                                   off);
-        }
+        if (m.from[i] >= 0) v[i] = *reinterpret_cast<const P*>(pool + m.from[i] * size + at);
     }
 #pragma unroll
     for (int i = 0; i < WMAX; ++i)
-        if (moved[i]) {
-            const int64_t to = table[i * a.table_stride + full];
-            *reinterpret_cast<P*>(pool + (to * a.planes + plane) * page_bytes + off) = v[i];
-        }
+        if (m.from[i] >= 0) *reinterpret_cast<P*>(pool + m.to[i] * size + at) = v[i];
 }
 
 // In place: slot i of a request takes the cached tokens of slot parents[i]. The pages that are
-// full change hands through the table; the rows of the page in progress are copied into the
-// slot's own page. One thread moves one piece (16 bytes of codes, a row's scale or a column of
-// the table) for all W slots: it has read every parent's piece before it writes the first, so
-// no slot's piece is lost whatever the permutation, and no two threads touch the same piece.
+// full change hands through the table (a thread a column, all slots read before one is written);
+// the rows of the page in progress are copied into the slot's own page, in pieces of 16 bytes of
+// codes and 4 of scales. A page's planes lie side by side, so a request's moves are a few long
+// copies; each of its a.copiers workgroups takes pieces in turn (the page numbers, a chain of
+// three loads, are found once for all of them). 48 x 8 beams, 150 planes, 14 rows: 46 us, 4.4 TB/s
+// read and written (a workgroup for every 256 pieces, each finding its pages: 86).
 template <int WMAX>
 __global__ void __launch_bounds__(256) beam_reorder_kernel(BeamReorder a) {
     const int b = blockIdx.y;
@@ -406,8 +422,8 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(BeamReorder a) {
     const int full = c / kPageTokens, fill = c % kPageTokens;
     const int32_t* parents = a.parents + b * a.parent_stride;
     int32_t* table = a.tables + (int64_t)b * a.W * a.table_stride;
-    if ((int)blockIdx.x >= a.piece_blocks) {
-        const int col = ((int)blockIdx.x - a.piece_blocks) * 256 + threadIdx.x;
+    if ((int)blockIdx.x >= a.copiers) {
+        const int col = ((int)blockIdx.x - a.copiers) * 256 + threadIdx.x;
         if (col >= full) return;
         int32_t v[WMAX];
 #pragma unroll
@@ -425,33 +441,37 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(BeamReorder a) {
         return;
     }
     if (fill == 0) return;
-    const int per_plane = 2 * a.row_bytes + 2 * kPageTokens;
-    const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t plane = item / per_plane;
-    int p = (int)(item - plane * per_plane);
-    if (plane >= a.planes) return;
-    const bool code = p < 2 * a.row_bytes;
-    int which, token, off, page_bytes;
-    uint8_t* pool;
-    if (code) {
-        which = p >= a.row_bytes;
-        off = (p - which * a.row_bytes) * 16;
-        token = off / a.row_bytes;
-        page_bytes = a.row_bytes * kPageTokens;
-        pool = which ? a.codes[1] : a.codes[0];
-    } else {
-        p -= 2 * a.row_bytes;
-        which = p >= kPageTokens;
-        token = p - which * kPageTokens;
-        off = token * 4;
-        page_bytes = 4 * kPageTokens;
-        pool = which ? a.scales[1] : a.scales[0];
+    Moves<WMAX> m;
+#pragma unroll
+    for (int i = 0; i < WMAX; ++i) {
+        m.from[i] = m.to[i] = -1;
+        if (i < a.W) {
+            const int par = parents[i];
+            const bool other = par >= 0 && par < a.W && par != i;
+            const int64_t from = table[(other ? par : i) * a.table_stride + full];
+            const int64_t to = table[i * a.table_stride + full];
+            if (other && from >= 0 && from < a.n_blocks && to >= 0 && to < a.n_blocks) {
+                m.from[i] = from * a.planes;
+                m.to[i] = to * a.planes;
+            }
+        }
     }
-    if (token >= fill) return;
-    if (code)
-        move_piece<WMAX, uint4>(a, table, parents, pool, plane, page_bytes, off, full);
-    else
-        move_piece<WMAX, uint32_t>(a, table, parents, pool, plane, page_bytes, off, full);
+    const int step = a.copiers * 256, first = blockIdx.x * 256 + threadIdx.x;
+    // codes: row_bytes pieces a plane, token by token
+    const int pieces = (int)a.planes * a.row_bytes, shift = a.row_bytes == 64 ? 6 : 7;
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+        for (int p = first; p < pieces; p += step)
+            if ((p & (a.row_bytes - 1)) >> (shift - 4) < fill)
+                move_piece<WMAX, uint4>(m, w ? a.codes[1] : a.codes[0], a.row_bytes * kPageTokens,
+                                        (int64_t)p * 16);
+    const int rows = (int)a.planes * kPageTokens;
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+        for (int p = first; p < rows; p += step)
+            if ((p & (kPageTokens - 1)) < fill)
+                move_piece<WMAX, uint32_t>(m, w ? a.scales[1] : a.scales[0], 4 * kPageTokens,
+                                           (int64_t)p * 4);
 }
 
 }  // namespace
@@ -502,8 +522,8 @@ TENZO_HIP_API int tenzo_hip_beam_select(const float* logits, int64_t row_stride,
     a.out_beams = out_beams;
     a.out_tokens = out_tokens;
     const dim3 grid((unsigned)(rows * ns));
-    if (elems == 32)
-        hipLaunchKernelGGL(beam_slice_kernel<32>, grid, dim3(256), 0, (hipStream_t)stream, a);
+    if (elems == 16)
+        hipLaunchKernelGGL(beam_slice_kernel<16>, grid, dim3(256), 0, (hipStream_t)stream, a);
     else
         hipLaunchKernelGGL(beam_slice_kernel<8>, grid, dim3(256), 0, (hipStream_t)stream, a);
     const int rc = launch_status("beam_slice_kernel");
@@ -553,8 +573,9 @@ TENZO_HIP_API int tenzo_hip_beam_reorder_paged(const int32_t* parents, int64_t p
     a.W = W;
     a.width = table_width;
     a.row_bytes = row_bytes;
-    a.piece_blocks = (int)ceil_div(a.planes * (2 * row_bytes + 2 * kPageTokens), 256);
-    const dim3 grid((unsigned)(a.piece_blocks + ceil_div(table_width, 256)), (unsigned)B);
+    const int64_t most = ceil_div(a.planes * row_bytes, 256), share = ceil_div(2048, B);
+    a.copiers = (int)(most < share ? most : share);
+    const dim3 grid((unsigned)(a.copiers + ceil_div(table_width, 256)), (unsigned)B);
     if (W <= 8)
         hipLaunchKernelGGL(beam_reorder_kernel<8>, grid, dim3(256), 0, (hipStream_t)stream, a);
     else if (W <= 16)
