@@ -230,8 +230,8 @@ TENZO_HIP_API int tenzo_hip_kv4_append(const void* k, const void* v, int dtype, 
                                        const int32_t* ctx_lens, const int32_t* cu_q, int B,
                                        int64_t T, const float* rope_cs, int n_pos, void* stream);
 /* The cached values at the positions of the T rows (what append wrote for
- * them): k_out / v_out [T][Hkv][128] of dtype, zeros for rows that stand
- * nowhere. */
+ * them): k_out / v_out [T][Hkv][128] of dtype, 16-byte aligned, zeros for rows
+ * that stand nowhere. */
 TENZO_HIP_API int tenzo_hip_kv4_read(const uint8_t* pk, const uint8_t* pv, const uint8_t* pks,
                                      const uint8_t* pvs, int64_t n_blocks, int n_layers,
                                      int layer, int Hkv, const int32_t* block_tables,

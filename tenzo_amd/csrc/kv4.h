@@ -97,6 +97,23 @@ __device__ __forceinline__ float ld_act(const void* p, int64_t i) {
     return HALF ? __half2float(reinterpret_cast<const __half*>(p)[i])
                 : reinterpret_cast<const float*>(p)[i];
 }
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef _Float16 f16x4_any __attribute__((ext_vector_type(4), aligned(2)));
+// Four values in a row, at any element's address (one load: the GPU takes unaligned ones).
+template <bool HALF>
+__device__ __forceinline__ void ld_act4(const void* p, int64_t i, float (&v)[4]) {
+    if (HALF) {
+        const f16x4_any x =
+            *reinterpret_cast<const f16x4_any*>(reinterpret_cast<const uint16_t*>(p) + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = (float)x[k];
+    } else {
+        const f32x4_any x =
+            *reinterpret_cast<const f32x4_any*>(reinterpret_cast<const float*>(p) + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = x[k];
+    }
+}
 template <bool HALF>
 __device__ __forceinline__ void st_act(void* p, int64_t i, float v) {
     if (HALF)

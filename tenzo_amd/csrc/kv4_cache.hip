@@ -13,7 +13,7 @@ struct Kv4Append {
     uint8_t* pks;
     uint8_t* pvs;
     const float* rope;
-    int64_t items;  // T * Hkv * 2
+    int items;  // T * Hkv
 };
 
 constexpr float kKv4Max = 0x1.cp127f;  // the largest magnitude whose codes stay finite: 7 * 2^125
@@ -54,41 +54,9 @@ __device__ __forceinline__ float max8(float m) {  // over the 8 lanes of a half 
     return fmaxf(m, dpp_f<kDppHalfMirror>(m));
 }
 
-// 16 lanes to a row of 128: lane l has dims 4l .. 4l + 3 and 64 + 4l .. 64 + 4l + 3, so that a
-// dim and its partner of the rotation meet in one lane and a group of 32 lies in 8 lanes.
-template <bool HALF>
-__global__ void __launch_bounds__(256) kv4_append_kernel(Kv4Append a, Kv4Seqs sq) {
-    const int l = threadIdx.x & 15;
-    const int64_t item = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (item >= a.items) return;
-    const int per_row = sq.Hkv * 2;
-    const int row = (int)(item / per_row);
-    const int rest = (int)(item - (int64_t)row * per_row);
-    const bool is_v = rest >= sq.Hkv;
-    const int h = is_v ? rest - sq.Hkv : rest;
-    int seq, pos;
-    if (!kv4_place(sq, row, l, seq, pos)) return;
-    const int64_t base = sq.page_base(seq, pos / kKv4Page);
-    if (base < 0) return;
-    const int64_t dst = base + h * kKv4Page + pos % kKv4Page;
-    const void* src = is_v ? a.v : a.k;
-    const int64_t at = row * (is_v ? a.v_stride : a.k_stride) + h * kKv4Dim + 4 * l;
-    float lo[4], hi[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        lo[j] = ld_act<HALF>(src, at + j);
-        hi[j] = ld_act<HALF>(src, at + 64 + j);
-    }
-    if (!is_v && a.rope) {
-        // in 64 bits, where both products are exact: a key is rounded once, to its code
-        const float* cs = a.rope + (int64_t)pos * kKv4Dim + 4 * l;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const double c = cs[j], s = cs[64 + j], x0 = lo[j], x1 = hi[j];
-            lo[j] = round_sticky(__builtin_fma(-x1, s, x0 * c));
-            hi[j] = round_sticky(__builtin_fma(x1, c, x0 * s));
-        }
-    }
+// A row's codes and scales to its place: lane l of 16 has dims 4l .. 4l + 3 and 64 + 4l .. + 3.
+__device__ __forceinline__ void write_row(float (&lo)[4], float (&hi)[4], int l, uint8_t* codes,
+                                          uint8_t* scales) {
     float ml = 0.0f, mh = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -98,14 +66,49 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4Append a, Kv4Seqs sq
         mh = fmaxf(mh, fabsf(hi[j]));
     }
     const int el = group_scale(max8(ml)), eh = group_scale(max8(mh));
-    uint8_t* codes = (is_v ? a.pv : a.pk) + dst * kKv4Row;
     reinterpret_cast<uint16_t*>(codes)[l] = (uint16_t)codes4(lo, el);
     reinterpret_cast<uint16_t*>(codes)[16 + l] = (uint16_t)codes4(hi, eh);
     if ((l & 7) == 0) {
-        uint8_t* sc = (is_v ? a.pvs : a.pks) + dst * kKv4Scales;
-        sc[l >> 3] = (uint8_t)el;
-        sc[2 + (l >> 3)] = (uint8_t)eh;
+        scales[l >> 3] = (uint8_t)el;
+        scales[2 + (l >> 3)] = (uint8_t)eh;
     }
+}
+
+// 16 lanes to a head of a row, its key and its value: lane l has dims 4l .. 4l + 3 and 64 + 4l
+// .. 64 + 4l + 3, so that a dim and its partner of the rotation meet in one lane and a group of
+// 32 lies in 8 lanes. Bound by the bytes read (@APPEND@).
+template <bool HALF>
+__global__ void __launch_bounds__(256) kv4_append_kernel(Kv4Append a, Kv4Seqs sq) {
+    const int l = threadIdx.x & 15;
+    const int item = (int)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (item >= a.items) return;
+    const int row = item / sq.Hkv, h = item - row * sq.Hkv;
+    float klo[4], khi[4], vlo[4], vhi[4];
+    const int64_t ka = row * a.k_stride + h * kKv4Dim + 4 * l;
+    const int64_t va = row * a.v_stride + h * kKv4Dim + 4 * l;
+    ld_act4<HALF>(a.k, ka, klo);
+    ld_act4<HALF>(a.k, ka + 64, khi);
+    ld_act4<HALF>(a.v, va, vlo);
+    ld_act4<HALF>(a.v, va + 64, vhi);
+    int seq, pos;
+    if (!kv4_place(sq, row, l, seq, pos)) return;
+    const int64_t base = sq.page_base(seq, pos / kKv4Page);
+    if (base < 0) return;
+    const int64_t dst = base + h * kKv4Page + pos % kKv4Page;
+    write_row(vlo, vhi, l, a.pv + dst * kKv4Row, a.pvs + dst * kKv4Scales);
+    if (a.rope) {
+        // in 64 bits, where both products are exact: a key is rounded once, to its code
+        float c4[4], s4[4];
+        ld_act4<false>(a.rope, (int64_t)pos * kKv4Dim + 4 * l, c4);
+        ld_act4<false>(a.rope, (int64_t)pos * kKv4Dim + 64 + 4 * l, s4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const double c = c4[j], s = s4[j], x0 = klo[j], x1 = khi[j];
+            klo[j] = round_sticky(__builtin_fma(-x1, s, x0 * c));
+            khi[j] = round_sticky(__builtin_fma(x1, c, x0 * s));
+        }
+    }
+    write_row(klo, khi, l, a.pk + dst * kKv4Row, a.pks + dst * kKv4Scales);
 }
 
 struct Kv4Read {
@@ -115,36 +118,47 @@ struct Kv4Read {
     const uint8_t* pvs;
     void* k;
     void* v;
-    int64_t items;
+    int items;
 };
 
-// 16 lanes to a row: lane l has dims 8l .. 8l + 7.
+// 16 lanes to a head of a row, its key and its value: lane l has dims 8l .. 8l + 7.
 template <bool HALF>
 __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4Read a, Kv4Seqs sq) {
     const int l = threadIdx.x & 15;
-    const int64_t item = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int item = (int)blockIdx.x * 16 + (threadIdx.x >> 4);
     if (item >= a.items) return;
-    const int per_row = sq.Hkv * 2;
-    const int row = (int)(item / per_row);
-    const int rest = (int)(item - (int64_t)row * per_row);
-    const bool is_v = rest >= sq.Hkv;
-    const int h = is_v ? rest - sq.Hkv : rest;
-    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    const int row = item / sq.Hkv, h = item - row * sq.Hkv;
+    float v[2][8] = {};
     int seq, pos;
     if (kv4_place(sq, row, l, seq, pos)) {
         const int64_t base = sq.page_base(seq, pos / kKv4Page);
         if (base >= 0) {
             const int64_t src = base + h * kKv4Page + pos % kKv4Page;
-            const uint32_t w =
-                reinterpret_cast<const uint32_t*>((is_v ? a.pv : a.pk) + src * kKv4Row)[l];
-            fp4_to_float8(w, e8m0_to_float((is_v ? a.pvs : a.pks)[src * kKv4Scales + (l >> 2)]),
-                          v);
+            const uint32_t wk = reinterpret_cast<const uint32_t*>(a.pk + src * kKv4Row)[l];
+            const uint32_t wv = reinterpret_cast<const uint32_t*>(a.pv + src * kKv4Row)[l];
+            const uint32_t sk = a.pks[src * kKv4Scales + (l >> 2)];
+            const uint32_t sv = a.pvs[src * kKv4Scales + (l >> 2)];
+            fp4_to_float8(wk, e8m0_to_float(sk), v[0]);
+            fp4_to_float8(wv, e8m0_to_float(sv), v[1]);
         }
     }
-    void* out = is_v ? a.v : a.k;
-    const int64_t at = ((int64_t)row * sq.Hkv + h) * kKv4Dim + 8 * l;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) st_act<HALF>(out, at + j, v[j]);
+    for (int w = 0; w < 2; ++w) {
+        void* out = w ? a.v : a.k;
+        const int64_t at = (int64_t)item * kKv4Dim + 8 * l;
+        if (HALF) {
+            uint32_t p[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                p[k] = float_to_half_bits(v[w][2 * k]) |
+                       (uint32_t)float_to_half_bits(v[w][2 * k + 1]) << 16;
+            *reinterpret_cast<uint4*>((uint16_t*)out + at) = uint4{p[0], p[1], p[2], p[3]};
+        } else {
+            float4* o = reinterpret_cast<float4*>((float*)out + at);
+            o[0] = make_float4(v[w][0], v[w][1], v[w][2], v[w][3]);
+            o[1] = make_float4(v[w][4], v[w][5], v[w][6], v[w][7]);
+        }
+    }
 }
 
 }  // namespace
@@ -211,9 +225,10 @@ TENZO_HIP_API int tenzo_hip_kv4_append(const void* k, const void* v, int dtype, 
     TZ_CHECK(T == 1 || (k_stride >= (int64_t)Hkv * kKv4Dim && v_stride >= (int64_t)Hkv * kKv4Dim),
              "kv4_append: row strides %lld, %lld below %d heads", (long long)k_stride,
              (long long)v_stride, Hkv);
-    Kv4Append a{k, v, k_stride, v_stride, pk, pv, pks, pvs, rope_cs, T * Hkv * 2};
-    const int64_t blocks = ceil_div(a.items, 16);
+    Kv4Append a{k, v, k_stride, v_stride, pk, pv, pks, pvs, rope_cs, 0};
+    const int64_t blocks = ceil_div(T * Hkv, 16);
     TZ_CHECK(blocks <= 0xffffff, "kv4_append: %lld rows of %d heads", (long long)T, Hkv);
+    a.items = (int)(T * Hkv);
     const dim3 grid((unsigned)blocks);
     if (dtype)
         hipLaunchKernelGGL(kv4_append_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, a, q);
@@ -238,9 +253,12 @@ TENZO_HIP_API int tenzo_hip_kv4_read(const uint8_t* pk, const uint8_t* pv, const
     TZ_CHECK(dtype == 0 || dtype == 1, "kv4_read: dtype %d", dtype);
     if (T == 0) return TENZO_SUCCESS;
     TZ_CHECK(k_out && v_out, "kv4_read: null pointer");
-    Kv4Read a{pk, pv, pks, pvs, k_out, v_out, T * Hkv * 2};
-    const int64_t blocks = ceil_div(a.items, 16);
+    TZ_CHECK((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0,
+             "kv4_read: outputs must be 16-byte aligned");
+    Kv4Read a{pk, pv, pks, pvs, k_out, v_out, 0};
+    const int64_t blocks = ceil_div(T * Hkv, 16);
     TZ_CHECK(blocks <= 0xffffff, "kv4_read: %lld rows of %d heads", (long long)T, Hkv);
+    a.items = (int)(T * Hkv);
     const dim3 grid((unsigned)blocks);
     if (dtype)
         hipLaunchKernelGGL(kv4_read_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, a, q);

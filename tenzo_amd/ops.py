@@ -369,7 +369,8 @@ def kv4_read(pk, pv, pks, pvs, block_tables, ctx_lens, layer: int, rows: int | N
         rows = block_tables.shape[0]
     pools, where, seqs = _kv4_cache(pk, pv, pks, pvs, block_tables, ctx_lens, cu_q, layer, rows,
                                     dev)
-    k, v = torch.empty((2, rows, where[3], 128), dtype=dtype, device=pk.device).unbind()
+    k = pk.new_empty((rows, where[3], 128), dtype=dtype)
+    v = torch.empty_like(k)
     _lib.check(_lib.load().tenzo_hip_kv4_read(*pools, *where, *seqs, k.data_ptr(), v.data_ptr(),
                                               _dtype_code(k), _stream()), "kv4_read")
     return k, v

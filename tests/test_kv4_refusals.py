@@ -35,7 +35,7 @@ CACHE_BAD = [dict(pk=None), dict(pvs=None), dict(pk=A + 4), dict(pks=A + 2), dic
              dict(T=4), dict(B=-1), dict(T=-1), dict(dtype=2), dict(width=1 << 28)]
 BAD = {
     "append": CACHE_BAD + [dict(k=None), dict(v=None), dict(ks=255), dict(vs=0), dict(n_pos=-1)],
-    "read": CACHE_BAD + [dict(k=None), dict(v=None)],
+    "read": CACHE_BAD + [dict(k=None), dict(v=None), dict(k=A + 4)],
     "attn": CACHE_BAD + [dict(q=None), dict(out=None), dict(qs=1023), dict(os=1000), dict(Hq=7),
                          dict(Hq=34), dict(Hq=0), dict(n_pos=-1)],
     "beam": [dict(x=None), dict(s=None), dict(os=None), dict(ob=None), dict(ot=None),
