@@ -596,6 +596,278 @@ kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
     kv4_segment<ROWS, NP, RW, HALF, false>(a, sq, g, sm);
 }
 
+// Prompts: 128 rows to a workgroup, 32 (two column tiles) to a wave, all against the same 64 tokens
+// at a time. The waves convert a quarter of the tile's keys and values each, into LDS as bf16
+// (rows of 16-byte pieces in an order of the row's own, see `piece`), and every fragment read from
+// there serves both column tiles and all parts: 6 MFMAs (fp32) a fragment of 1 KB. The codes of
+// the next tile are loaded during the products. Of an fp32 query's three parts the last one is
+// read from LDS too: two waves a SIMD leave 256 registers.
+constexpr int kRowsRT = 128;
+template <int NP, bool HALF>
+__global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seqs sq) {
+    __shared__ __align__(16) uint16_t kt[kTile * kKv4Dim], vt[kTile * kKv4Dim];
+    __shared__ __align__(16) uint32_t qlo[NP == 3 ? 4 * 2 * 4 * 64 * 4 : 4];
+    __shared__ int pg[kMaxPages];
+    const int per_unit = sq.Hkv * a.splits;
+    // (from the last unit on: the latest rows of a prompt see the most tokens)
+    const int back = blockIdx.x / per_unit, rest = blockIdx.x - back * per_unit;
+    const int split = rest / sq.Hkv, h = rest - split * sq.Hkv;
+    int seq, tile;
+    if (!find_unit(sq, a.wgs / per_unit - 1 - back, a.G, kRowsRT, seq, tile)) return;
+    const int first = sq.cu ? sq.cu[seq] : seq;
+    const int n = sq.cu ? sq.cu[seq + 1] - first : 1;
+    const int c = sq.length(seq);
+    const int t0 = split * a.chunk, row0 = tile * kRowsRT;
+    const int last_i = min(n - 1, (row0 + kRowsRT - 1) / a.G);
+    const int t1 = min(min(t0 + a.chunk, c - n + last_i + 1), c);  // tokens that some row sees
+    if (split > 0 && t0 >= t1) return;
+
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, j = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wrow = row0 + 32 * wave;  // the wave's first row
+    const int32_t* table = sq.tables + (int64_t)seq * sq.table_stride + t0 / kKv4Page;
+    const int pages = t1 > t0 ? (t1 - t0 + kKv4Page - 1) / kKv4Page : 0;
+    auto stage_pages = [&](int from) {
+        for (int p = from + tid; p < min(pages, from + kMaxPages); p += 256) {
+            const int id = table[p];
+            pg[p - from] = id >= 0 && id < sq.n_blocks ? id : -1;
+        }
+    };
+    stage_pages(0);
+
+    // the lane's rows, and their queries as B operands (dims 32j .. 32j + 31)
+    int pos[2];
+    int64_t grow[2];
+    int head[2];
+    bool row_ok[2];
+    Frag qf[2][2][4];
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct) {
+        const int r = wrow + 16 * ct + col, i = r / a.G;
+        head[ct] = h * a.G + (r - i * a.G);
+        row_ok[ct] = i < n && first >= 0 && first + i < a.T;
+        pos[ct] = row_ok[ct] && c > 0 ? c - n + i : -1;
+        grow[ct] = (int64_t)first + i;
+        const bool turn = a.rope && pos[ct] >= 0, upper = lane >= 32;
+        const int64_t at = grow[ct] * a.q_stride + (int64_t)head[ct] * kKv4Dim + 32 * j;
+        const int64_t cs = (int64_t)max(pos[ct], 0) * kKv4Dim + 32 * (j & 1);
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, cv[4] = {1.0f, 1.0f, 1.0f, 1.0f}, sv[4] = {};
+            if (row_ok[ct]) ld_act4<HALF>(a.q, at + e, x);
+            if (turn) {
+                ld_act4<false>(a.rope, cs + e, cv);
+                ld_act4<false>(a.rope, cs + 64 + e, sv);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float lo, hi;  // the dims d and d + 64
+                lane_halves(x[k], lo, hi);
+                x[k] = upper ? __builtin_fmaf(lo, sv[k], __fmul_rn(hi, cv[k]))
+                             : __builtin_fmaf(lo, cv[k], -__fmul_rn(hi, sv[k]));
+                x[k] = __fmul_rn(x[k], kQkScale * kLog2e);
+            }
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                const uint32_t w0 = pack_hi(x[0], x[1]), w1 = pack_hi(x[2], x[3]);
+                if (p < 2) {
+                    qf[ct][p][e >> 3].w[(e >> 1) & 3] = w0;
+                    qf[ct][p][e >> 3].w[((e >> 1) & 3) + 1] = w1;
+                } else {
+                    uint32_t* dst = qlo + (((wave * 2 + ct) * 4 + (e >> 3)) * 64 + lane) * 4;
+                    *reinterpret_cast<uint2*>(dst + ((e >> 1) & 3)) = uint2{w0, w1};
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] -= masked(x[k], 0xffff0000u);
+            }
+        }
+    }
+    __syncthreads();
+
+    auto piece = [](int row, int p) {
+        return row * kKv4Dim + ((p ^ (2 * (row & 3) + (row >> 2 & 1))) << 3);
+    };
+    f32x4 acc[2][8];
+    float m[2], l[2];
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct) {
+        m[ct] = -INFINITY;
+        l[ct] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) acc[ct][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // a lane's share of a tile: 32 dims of token 16 wave + col
+    uint4 kr, vr;
+    uint32_t ks = 0, vs = 0;
+    auto load = [&](int t, int w0) {
+        const int p = min(((t - w0) >> 4) + wave, pages - 1 - ((w0 - t0) >> 4));
+        const int id = max(__builtin_amdgcn_readfirstlane(pg[p]), 0);
+        const int64_t row = (((int64_t)id * sq.n_layers + sq.layer) * sq.Hkv + h) * kKv4Page;
+        const uint32_t code = (uint32_t)(col * kKv4Row + j * 16), sc = col * kKv4Scales + j;
+        kr = *reinterpret_cast<const uint4*>(a.pk + row * kKv4Row + code);
+        vr = *reinterpret_cast<const uint4*>(a.pv + row * kKv4Row + code);
+        ks = (a.pks + row * kKv4Scales)[sc];
+        vs = (a.pvs + row * kKv4Scales)[sc];
+    };
+    auto store = [&](uint16_t* dst, uint4 codes, uint32_t scale) {
+        const float sc = e8m0_to_float(scale);
+        const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+            union {
+                bf16x2 p[4];
+                uint4 v;
+            } f;
+            f.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 0);
+            f.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 1);
+            f.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 2);
+            f.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 3);
+            *reinterpret_cast<uint4*>(dst + piece(16 * wave + col, 4 * j + st)) = f.v;
+        }
+    };
+    const int low = c - n + wrow / a.G;                             // the wave's first position
+    const int high = c - n + min(n - 1, (wrow + 31) / a.G);         // and its last
+    int w0 = t0;
+    if (t0 < t1 && sq.n_blocks > 0) load(t0, w0);
+    for (int t = t0; t < t1 && sq.n_blocks > 0; t += kTile) {
+        store(kt, kr, ks);
+        store(vt, vr, vs);
+        int ids[4];
+        bool bad = false;
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+            const int p = ((t - w0) >> 4) + tt;
+            ids[tt] = p < pages - ((w0 - t0) >> 4) ? __builtin_amdgcn_readfirstlane(pg[p]) : -1;
+            bad = bad || ids[tt] < 0;
+        }
+        __syncthreads();
+        const int next = t + kTile;
+        if (next < t1) {
+            if (next >= w0 + kMaxPages * kKv4Page) {  // (page numbers kMaxPages at a time)
+                w0 = next;
+                stage_pages((w0 - t0) / kKv4Page);
+                __syncthreads();
+            }
+            load(next, w0);
+        }
+        if (t <= high && wrow / a.G < n) {
+            f32x4 s[2][4];
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt) {
+                s[0][tt] = s[1][tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int st = 0; st < 4; ++st) {
+                    const bf16x8 kf =
+                        *reinterpret_cast<const bf16x8*>(kt + piece(16 * tt + col, 4 * j + st));
+#pragma unroll
+                    for (int ct = 0; ct < 2; ++ct) {
+                        s[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[ct][0][st].v,
+                                                                            s[ct][tt], 0, 0, 0);
+                        s[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[ct][1][st].v,
+                                                                            s[ct][tt], 0, 0, 0);
+                        if (NP == 3) {
+                            const bf16x8 q3 = *reinterpret_cast<const bf16x8*>(
+                                qlo + (((wave * 2 + ct) * 4 + st) * 64 + lane) * 4);
+                            s[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q3, s[ct][tt],
+                                                                                0, 0, 0);
+                        }
+                    }
+                }
+            }
+            const bool mask = bad || t + kTile - 1 > low;
+            Frag pf[2][2][NP];  // [column tile][32 tokens][part]
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct) {
+                if (mask)
+#pragma unroll
+                    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (ids[tt] < 0 || t + 16 * tt + 4 * j + i > pos[ct])
+                                s[ct][tt][i] = -INFINITY;
+                float top[4];
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt)
+                    top[tt] = fmaxf(fmaxf(s[ct][tt][0], s[ct][tt][1]),
+                                    fmaxf(s[ct][tt][2], s[ct][tt][3]));
+                const float mn = fmaxf(
+                    m[ct], max_quarters(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))));
+                const float base = mn == -INFINITY ? 0.0f : mn;
+                const float alpha = __builtin_amdgcn_exp2f(m[ct] - base);
+                m[ct] = mn;
+                if (__ballot(alpha != 1.0f)) {
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) acc[ct][d] *= alpha;
+                    l[ct] *= alpha;
+                }
+                float sum[4];
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        s[ct][tt][i] = __builtin_amdgcn_exp2f(s[ct][tt][i] - base);
+                    sum[tt] = (s[ct][tt][0] + s[ct][tt][1]) + (s[ct][tt][2] + s[ct][tt][3]);
+                }
+                l[ct] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        float x0 = s[ct][2 * u + (e >> 2)][e & 3];
+                        float x1 = s[ct][2 * u + (e >> 2)][(e & 3) + 1];
+#pragma unroll
+                        for (int p = 0; p < NP; ++p) {
+                            pf[ct][u][p].w[e >> 1] = pack_hi(x0, x1);
+                            x0 -= masked(x0, 0xffff0000u);
+                            x1 -= masked(x1, 0xffff0000u);
+                        }
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                    typedef __attribute__((address_space(3))) s16x4* lds4;
+                    union {
+                        s16x4 h[2];
+                        bf16x8 v;
+                    } vf;
+                    const int at = piece(32 * u + 4 * j + (col >> 2), 2 * d + (col >> 1 & 1)) +
+                                   (col & 1) * 4;
+                    vf.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vt + at));
+                    vf.h[1] =
+                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vt + at + 16 * kKv4Dim));
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+#pragma unroll
+                        for (int ct = 0; ct < 2; ++ct)
+                            acc[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                vf.v, pf[ct][u][p].v, acc[ct][d], 0, 0, 0);
+                }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct) {
+        const float L = sum_quarters(l[ct]);
+        if (!row_ok[ct]) continue;
+        if (pos[ct] < a.chunk || a.splits == 1) {
+            if (split == 0)
+#pragma unroll
+                for (int d = 0; d < 8; ++d)
+                    store4<HALF>(a, grow[ct] * a.out_stride + (int64_t)head[ct] * kKv4Dim + 16 * d +
+                                        4 * j,
+                                 acc[ct][d], L);
+        } else {
+            const int64_t at = (grow[ct] * a.Hq + head[ct]) * a.splits + split;
+#pragma unroll
+            for (int d = 0; d < 8; ++d)
+                *reinterpret_cast<f32x4*>(a.part_o + at * kKv4Dim + 16 * d + 4 * j) = acc[ct][d];
+            if (j == 0) a.part_ml[at] = make_float2(m[ct], L);
+        }
+    }
+}
+
 // Several sequences of a few rows: all their steps in a row (sequence by sequence, unit by unit)
 // and an equal share of them to each of as many workgroups as the GPU holds at once, so that
 // lengths, which only the device knows, need not be alike. A share holds the end of a unit that
@@ -774,7 +1046,7 @@ __global__ void __launch_bounds__(256) kv4_join_even_kernel(Kv4Attn a, Kv4Seqs s
 
 // Rows of a workgroup and how the tokens are dealt out, from what the host knows.
 struct Kv4Plan {
-    int rows, rw, splits, chunk;
+    int rows, rw, splits, chunk;  // rw 8: the prompts' kernel
     bool even;
     int64_t wgs;
     size_t records;
@@ -784,11 +1056,11 @@ Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, boo
     const int64_t per = cu ? ceil_div(T * G, B) : G;  // rows of an average sequence
     const int packed = half ? 8 : 4;
     p.rows = per <= packed ? packed : 16;
-    p.rw = per <= 16 ? 1 : per <= 32 ? 2 : 4;
+    p.rw = per <= 16 ? 1 : per <= 32 ? 2 : per <= 64 ? 4 : 8;
     const int rt = p.rows * p.rw;
     const int64_t units = cu ? T * G / rt + B : (int64_t)B * ceil_div(G, rt);
     const int64_t ctx = (int64_t)table_width * kKv4Page;
-    const int64_t step = kTile * (4 / p.rw);
+    const int64_t step = p.rw > 4 ? kTile : kTile * (4 / p.rw);
     const int64_t steps = ctx > 0 ? ceil_div(ctx, step) : 1;
     const int room = 768;  // workgroups that the GPU holds at once, three a CU
     const int64_t most = units * Hkv * (steps + 1);
@@ -803,7 +1075,16 @@ Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, boo
         p.records = (size_t)p.wgs * 2 * p.rows;
         return p;
     }
-    int64_t s = room / (units * Hkv);
+    const int64_t likely = cu ? (ceil_div(T * G, rt) > B ? ceil_div(T * G, rt) : B) : units;
+    int64_t s = room / (likely * Hkv);
+    if (p.rw > 4) {
+        // two workgroups a CU. A prompt's last rows see all of its tokens, its first ones few: no
+        // workgroup should have more steps than an even share of all of them
+        s = 512 / (likely * Hkv);
+        const int64_t rows = T / B / kTile < 2 * steps ? T / B / kTile : 2 * steps;
+        const int64_t share = likely * Hkv * (2 * steps - rows) / 2 / 512;
+        if (s < 2) s = ceil_div(steps, share < 1 ? 1 : share);
+    }
     s = s < 1 ? 1 : s > steps ? steps : s;
     const int64_t chunk = ceil_div(steps, s) * step;
     p.chunk = (int)(chunk < INT32_MAX / 2 ? chunk : INT32_MAX / 2 / step * step);
@@ -842,8 +1123,10 @@ int launch_kv4_plan(const Kv4Plan& p, const Kv4Attn& a, const Kv4Seqs& s, hipStr
         launch_kv4<16, NP, 1, HALF>(a, s, st);
     else if (p.rw == 2)
         launch_kv4<16, NP, 2, HALF>(a, s, st);
-    else
+    else if (p.rw == 4)
         launch_kv4<16, NP, 4, HALF>(a, s, st);
+    else
+        hipLaunchKernelGGL((kv4_attn_rows_kernel<NP, HALF>), dim3(a.wgs), dim3(256), 0, st, a, s);
     const int rc = launch_status("kv4_attn_kernel");
     if (rc || p.splits == 1) return rc;
     hipLaunchKernelGGL(kv4_join_kernel<HALF>, dim3(a.T, a.Hq), dim3(512), 0, st, a, s);

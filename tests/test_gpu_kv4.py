@@ -263,7 +263,9 @@ def test_attention_many_pages(torch_dev, ops):
 @pytest.mark.parametrize("Hq,Hkv,seqs", [
     (4, 1, [(2, 2), (3, 40), (1, 65)]), (8, 1, [(7, 100), (5, 5), (0, 30), (9, 2)]),
     (5, 1, [(33, 33), (1, 1), (64, 200)]), (4, 4, [(70, 70), (130, 131), (16, 300)]),
-    (20, 5, [(40, 90), (17, 17), (3, 0)]), (2, 1, [(300, 310)]), (16, 1, [(20, 64), (4, 4)])])
+    (20, 5, [(40, 90), (17, 17), (3, 0)]), (2, 1, [(300, 310)]), (16, 1, [(20, 64), (4, 4)]),
+    (4, 1, [(200, 230), (1, 1), (130, 100), (0, 0), (97, 2000)]), (3, 1, [(150, 150), (260, 700)]),
+    (8, 2, [(64, 1000), (65, 65)])])
 def test_attention_rows(torch_dev, ops, Hq, Hkv, seqs, dtype):
     """Several rows a sequence, each up to its own position; rows before position 0, empty
     sequences, and rows behind the last sequence that stay as they were."""
