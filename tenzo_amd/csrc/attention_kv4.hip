@@ -14,6 +14,13 @@ constexpr int kTile = 16 * kSub;    // tokens of a wave's step
 constexpr int kMaxPages = 1024;     // pages of a workgroup's part of the context
 constexpr int kQStride = 132;       // floats of a query in LDS
 
+// The prompts' kernel holds keys and values in fp16. Scale bytes whose values are exact there as
+// they are: 0.5 * 2^(s - 127) to 6 * 2^(s - 127), down to its smallest subnormal, which the matrix
+// cores take.
+constexpr int kLowScale = 104, kTopScale = 140;
+constexpr float kWeightBits = 15.0f;  // weights, at most 1, are held times 2^15
+
+
 struct Kv4Attn {
     const void* q;
     void* out;
@@ -31,7 +38,8 @@ struct Kv4Attn {
     int vec_out;        // out allows accesses of 4 elements
 };
 
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -39,6 +47,11 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 union Frag {
     uint32_t w[4];
     bf16x8 v;
+};
+union Frag16 {
+    uint32_t w[4];
+    uint4 q;
+    f16x8 v;
 };
 
 template <int CTRL>
@@ -66,6 +79,63 @@ __device__ __forceinline__ uint32_t pack_hi(float a, float b) {
 }
 __device__ __forceinline__ float masked(float v, uint32_t m) {
     return __uint_as_float(__float_as_uint(v) & m);
+}
+
+// Two floats as fp16, the first in the low half, and what that leaves of them.
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+    const f32x2 v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+}
+__device__ __forceinline__ float rest_lo(float x, uint32_t h) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    return r;
+}
+__device__ __forceinline__ float rest_hi(float x, uint32_t h) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+        : "=v"(r)
+        : "v"(h), "v"(x));
+    return r;
+}
+
+// Eight codes as fp16, times their scale (which the conversion takes the exponent of).
+__device__ __forceinline__ uint4 fp4_to_half8(uint32_t w, float scale) {
+    union {
+        f16x2 h[4];
+        uint4 q;
+    } f;
+    f.h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0);
+    f.h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1);
+    f.h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2);
+    f.h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3);
+    return f.q;
+}
+// The scale 2^(s - 127) of a byte of kLowScale .. kTopScale, or of less (about 0).
+__device__ __forceinline__ float byte_scale(int s) { return __uint_as_float((uint32_t)max(s, 1) << 23); }
+__device__ __forceinline__ float pow2(int e) {  // 2^e, 0 or the largest power where that is beyond
+    return e < -126 ? 0.0f : __uint_as_float((uint32_t)(min(e, 127) + 127) << 23);
+}
+__device__ __forceinline__ bool in_range(int s) {
+    return (uint32_t)(s - kLowScale) <= (uint32_t)(kTopScale - kLowScale);
+}
+__device__ __forceinline__ bool no_codes(uint4 c) {
+    return ((c.x | c.y | c.z | c.w) & 0x77777777u) == 0;
+}
+
+// A query row's power of two: the one that brings its largest element to 2^13 .. 2^14, so that the
+// second parts of its elements stay normal in fp16 too (2^-38 of the largest is still seen).
+__device__ __forceinline__ int row_shift(float amax) {
+    const int e = (int)(__float_as_uint(amax) >> 23);
+    return 140 - min(max(e, 14), 254);
+}
+
+// Where pieces of 8 fp16 of a row of 128 stand in LDS: rows of 256 bytes, the pieces in an order
+// of the row's own, so that eight lanes' writes or reads (8 rows, one piece) and 16 lanes'
+// transposing reads (4 rows, two pieces) meet all banks once. Only the low three bits of the
+// piece and of the row take part: 16 rows on, or 8 pieces on, is a constant away.
+__device__ __forceinline__ int piece_at(int row, int p) {
+    return row * kKv4Dim + ((p ^ (2 * (row & 3) + (row >> 2 & 1))) << 3);
 }
 
 // Four outputs, the weighted sum over the sum of weights (0 where no token was seen).
@@ -305,12 +375,12 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
     float m = -INFINITY, l = 0.0f;
 
     uint16_t* vb = smem + wave * (32 * kKv4Dim);
-    // value rows in LDS, 256 bytes each, their 16-byte pieces in an order of the row's own: eight
-    // lanes' writes (8 rows, one piece) and 16 lanes' transposing reads (4 rows, two pieces) both
-    // meet all banks once
-    auto piece = [](int row, int p) {
-        return row * kKv4Dim + ((p ^ (2 * (row & 3) + (row >> 2 & 1))) << 3);
-    };
+    int wr[4], rd[4];  // the lane's pieces of its token's row, and of the transposing reads
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        wr[k] = piece_at(col, 4 * j + k);
+        rd[k] = piece_at(4 * j + (col >> 2), 2 * k + (col >> 1 & 1)) + (col & 1) * 4;
+    }
 
     int t = t0 + kTile * tw;
     const bool any = sq.n_blocks > 0;
@@ -407,8 +477,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
         }
 #pragma unroll
         for (int tt = 0; tt < kSub; ++tt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[tt][i]);
+            top = fmaxf(top, fmaxf(fmaxf(s[tt][0], s[tt][1]), fmaxf(s[tt][2], s[tt][3])));
         const float mn = fmaxf(m, max_quarters(top));
         const float base = mn == -INFINITY ? 0.0f : mn;
         const float alpha = __builtin_amdgcn_exp2f(m - base);
@@ -420,11 +489,11 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
         }
 #pragma unroll
         for (int tt = 0; tt < kSub; ++tt)
+        {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[tt][i] = __builtin_amdgcn_exp2f(s[tt][i] - base);
-                l += s[tt][i];
-            }
+            for (int i = 0; i < 4; ++i) s[tt][i] = __builtin_amdgcn_exp2f(s[tt][i] - base);
+            l += (s[tt][0] + s[tt][1]) + (s[tt][2] + s[tt][3]);
+        }
         const uint32_t m1 = slot >= 1 ? 0xffff0000u : 0, m2 = slot >= 2 ? 0xffff0000u : 0;
 #pragma unroll
         for (int u = 0; u < kSub / 2; ++u) {
@@ -444,7 +513,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
                     f.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 1);
                     f.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 2);
                     f.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 3);
-                    *reinterpret_cast<uint4*>(vb + piece(k * 16 + col, 4 * j + st)) = f.v;
+                    *reinterpret_cast<uint4*>(vb + wr[st] + k * 16 * kKv4Dim) = f.v;
                 }
             }
             if (u == kSub / 2 - 1 && next < w1)
@@ -476,9 +545,9 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
                     bf16x8 v;
                 } vf;
                 // (lane 4r + i of 16: half a piece of row r, in return for column 4r + i)
-                const int at = piece(4 * j + (col >> 2), 2 * d + (col >> 1 & 1)) + (col & 1) * 4;
-                vf.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vb + at));
-                vf.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vb + at + 16 * kKv4Dim));
+                uint16_t* src = vb + rd[d & 3] + (d >> 2) * 64;
+                vf.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)src);
+                vf.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(src + 16 * kKv4Dim));
 #pragma unroll
                 for (int p = 0; p < NM; ++p)
                     acc[d] =
@@ -597,16 +666,22 @@ kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
 }
 
 // Prompts: 128 rows to a workgroup, 32 (two column tiles) to a wave, all against the same 64 tokens
-// at a time. The waves convert a quarter of the tile's keys and values each, into LDS as bf16
-// (rows of 16-byte pieces in an order of the row's own, see `piece`), and every fragment read from
-// there serves both column tiles and all parts: 6 MFMAs (fp32) a fragment of 1 KB. The codes of
-// the next tile are loaded during the products. Of an fp32 query's three parts the last one is
-// read from LDS too: two waves a SIMD leave 256 registers.
+// at a time. The waves convert a quarter of the tile's keys and values each, into LDS as fp16,
+// and every fragment of 1 KB read from there serves both column tiles and both parts, 4 MFMAs. The
+// codes of the next tile are loaded during the products.
+//
+// fp16 parts take two thirds of the MFMAs that bf16's would, and half of the vector work of
+// splitting the weights. Codes times scale are exact in fp16 (a token whose scales are out of its
+// range is moved by a power of two of its own: scores are multiplied back, values share one for
+// all tokens; what lies 2^37 below the largest is then lost). Queries, scaled by a power of two,
+// and weights are split into two parts, 22 bits: 2^-22 of a value is lost, little beside what fp32
+// sums lose (and of a weight 2^-40 of the largest, fp16's smallest step).
 constexpr int kRowsRT = 128;
-template <int NP, bool HALF>
+template <bool HALF>
 __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seqs sq) {
     __shared__ __align__(16) uint16_t kt[kTile * kKv4Dim], vt[kTile * kKv4Dim];
-    __shared__ __align__(16) uint32_t qlo[NP == 3 ? 4 * 2 * 4 * 64 * 4 : 4];
+    __shared__ float moved[kTile];  // 2^ the power of two that a token's keys are moved by
+    __shared__ int flags[4], tops[4];
     __shared__ int pg[kMaxPages];
     const int per_unit = sq.Hkv * a.splits;
     // (from the last unit on: the latest rows of a prompt see the most tokens)
@@ -640,7 +715,8 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
     int64_t grow[2];
     int head[2];
     bool row_ok[2];
-    Frag qf[2][2][4];
+    float unit[2];
+    Frag16 qf[2][2][4];
 #pragma unroll
     for (int ct = 0; ct < 2; ++ct) {
         const int r = wrow + 16 * ct + col, i = r / a.G;
@@ -651,10 +727,11 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
         const bool turn = a.rope && pos[ct] >= 0, upper = lane >= 32;
         const int64_t at = grow[ct] * a.q_stride + (int64_t)head[ct] * kKv4Dim + 32 * j;
         const int64_t cs = (int64_t)max(pos[ct], 0) * kKv4Dim + 32 * (j & 1);
+        float x[32], amax = 0.0f;
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
-            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, cv[4] = {1.0f, 1.0f, 1.0f, 1.0f}, sv[4] = {};
-            if (row_ok[ct]) ld_act4<HALF>(a.q, at + e, x);
+            float v[4] = {}, cv[4] = {1.0f, 1.0f, 1.0f, 1.0f}, sv[4] = {};
+            if (row_ok[ct]) ld_act4<HALF>(a.q, at + e, v);
             if (turn) {
                 ld_act4<false>(a.rope, cs + e, cv);
                 ld_act4<false>(a.rope, cs + 64 + e, sv);
@@ -662,31 +739,26 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 float lo, hi;  // the dims d and d + 64
-                lane_halves(x[k], lo, hi);
-                x[k] = upper ? __builtin_fmaf(lo, sv[k], __fmul_rn(hi, cv[k]))
+                lane_halves(v[k], lo, hi);
+                v[k] = upper ? __builtin_fmaf(lo, sv[k], __fmul_rn(hi, cv[k]))
                              : __builtin_fmaf(lo, cv[k], -__fmul_rn(hi, sv[k]));
-                x[k] = __fmul_rn(x[k], kQkScale * kLog2e);
+                x[e + k] = __fmul_rn(v[k], kQkScale * kLog2e);
+                amax = fmaxf(amax, fabsf(x[e + k]));
             }
+        }
+        const int up = row_shift(max_quarters(amax));
+        unit[ct] = pow2(-up);
 #pragma unroll
-            for (int p = 0; p < NP; ++p) {
-                const uint32_t w0 = pack_hi(x[0], x[1]), w1 = pack_hi(x[2], x[3]);
-                if (p < 2) {
-                    qf[ct][p][e >> 3].w[(e >> 1) & 3] = w0;
-                    qf[ct][p][e >> 3].w[((e >> 1) & 3) + 1] = w1;
-                } else {
-                    uint32_t* dst = qlo + (((wave * 2 + ct) * 4 + (e >> 3)) * 64 + lane) * 4;
-                    *reinterpret_cast<uint2*>(dst + ((e >> 1) & 3)) = uint2{w0, w1};
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] -= masked(x[k], 0xffff0000u);
-            }
+        for (int e = 0; e < 32; e += 2) {
+            const float x0 = x[e] * pow2(up), x1 = x[e + 1] * pow2(up);
+            const uint32_t hi = pack16(x0, x1);
+            qf[ct][0][e >> 3].w[(e >> 1) & 3] = hi;
+            qf[ct][1][e >> 3].w[(e >> 1) & 3] =
+                pack16(rest_lo(x0, hi), rest_hi(x1, hi));
         }
     }
     __syncthreads();
 
-    auto piece = [](int row, int p) {
-        return row * kKv4Dim + ((p ^ (2 * (row & 3) + (row >> 2 & 1))) << 3);
-    };
     f32x4 acc[2][8];
     float m[2], l[2];
 #pragma unroll
@@ -696,42 +768,56 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
 #pragma unroll
         for (int d = 0; d < 8; ++d) acc[ct][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    int vshift = 0, vtop = 1;
+    int wr[4], rd[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        wr[k] = piece_at(col, 4 * j + k);
+        rd[k] = piece_at(4 * j + (col >> 2), 2 * k + (col >> 1 & 1)) + (col & 1) * 4;
+    }
     // a lane's share of a tile: 32 dims of token 16 wave + col
-    uint4 kr, vr;
-    uint32_t ks = 0, vs = 0;
+    uint4 kr = {}, vr = {};
+    int ks = 0, vs = 0;
+    bool none = false;  // no one's token
     auto load = [&](int t, int w0) {
         const int p = min(((t - w0) >> 4) + wave, pages - 1 - ((w0 - t0) >> 4));
-        const int id = max(__builtin_amdgcn_readfirstlane(pg[p]), 0);
-        const int64_t row = (((int64_t)id * sq.n_layers + sq.layer) * sq.Hkv + h) * kKv4Page;
+        const int id = __builtin_amdgcn_readfirstlane(pg[p]);
+        const int64_t row = (((int64_t)max(id, 0) * sq.n_layers + sq.layer) * sq.Hkv + h) * kKv4Page;
         const uint32_t code = (uint32_t)(col * kKv4Row + j * 16), sc = col * kKv4Scales + j;
         kr = *reinterpret_cast<const uint4*>(a.pk + row * kKv4Row + code);
         vr = *reinterpret_cast<const uint4*>(a.pv + row * kKv4Row + code);
         ks = (a.pks + row * kKv4Scales)[sc];
         vs = (a.pvs + row * kKv4Scales)[sc];
+        none = id < 0 || t + 16 * wave + col >= t1;  // (looked at with the scales, when they come)
     };
-    auto store = [&](uint16_t* dst, uint4 codes, uint32_t scale) {
-        const float sc = e8m0_to_float(scale);
+    auto store = [&](uint16_t* dst, uint4 codes, int byte) {
+        const float sc = byte_scale(byte);
         const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
-        for (int st = 0; st < 4; ++st) {
-            union {
-                bf16x2 p[4];
-                uint4 v;
-            } f;
-            f.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 0);
-            f.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 1);
-            f.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 2);
-            f.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 3);
-            *reinterpret_cast<uint4*>(dst + piece(16 * wave + col, 4 * j + st)) = f.v;
-        }
+        for (int st = 0; st < 4; ++st)
+            *reinterpret_cast<uint4*>(dst + wave * 16 * kKv4Dim + wr[st]) =
+                fp4_to_half8(w[st], sc);
     };
-    const int low = c - n + wrow / a.G;                             // the wave's first position
-    const int high = c - n + min(n - 1, (wrow + 31) / a.G);         // and its last
+    const int low = c - n + wrow / a.G;                      // the wave's first position
+    const int high = c - n + min(n - 1, (wrow + 31) / a.G);  // and its last
     int w0 = t0;
     if (t0 < t1 && sq.n_blocks > 0) load(t0, w0);
     for (int t = t0; t < t1 && sq.n_blocks > 0; t += kTile) {
-        store(kt, kr, ks);
-        store(vt, vr, vs);
+        // what fp16 does not hold as it is: keys are moved token by token, values all together
+        const bool skip = none;
+        int kb = skip ? 127 : ks, vby = skip ? 127 + vshift : vs, by = 0, flag = 0;
+        if (__ballot(!in_range(kb) || !in_range(vby - vshift))) {
+            if (kb > 252 || no_codes(kr)) kb = 0;
+            if (vby > 252 || no_codes(vr)) vby = 0;
+            by = (int)max_quarters((float)kb) - kTopScale;
+            kb -= by;
+            flag = __ballot(vby > 0 && vby - vshift < kLowScale) ? 3 : 1;
+        }
+        if (!skip) vtop = max(vtop, vby);
+        store(kt, kr, kb);
+        store(vt, vr, vby - vshift);
+        if (j == 0) moved[16 * wave + col] = pow2(by);
+        if (lane == 0) flags[wave] = flag;
         int ids[4];
         bool bad = false;
 #pragma unroll
@@ -741,6 +827,27 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
             bad = bad || ids[tt] < 0;
         }
         __syncthreads();
+        flag = __builtin_amdgcn_readfirstlane(flags[0] | flags[1] | flags[2] | flags[3]);
+        const bool scaled = flag != 0;
+        if (scaled) {
+            // the values' power of two for the largest scale so far, and the tile once more
+            const int mine = (int)wave_max((float)vtop);
+            if (lane == 0) tops[wave] = mine;
+            __syncthreads();
+            vtop = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+            const int shift = vtop - kTopScale;
+            if (vtop - vshift > kTopScale || (flag > 1 && vtop - vshift < kTopScale)) {
+                const float f = pow2(vshift - shift);
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) acc[ct][d] *= f;
+                if (skip) vby += shift - vshift;
+                vshift = shift;
+                store(vt, vr, vby - vshift);
+            }
+            __syncthreads();
+        }
         const int next = t + kTile;
         if (next < t1) {
             if (next >= w0 + kMaxPages * kKv4Page) {  // (page numbers kMaxPages at a time)
@@ -757,25 +864,24 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
                 s[0][tt] = s[1][tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int st = 0; st < 4; ++st) {
-                    const bf16x8 kf =
-                        *reinterpret_cast<const bf16x8*>(kt + piece(16 * tt + col, 4 * j + st));
+                    const f16x8 kf =
+                        *reinterpret_cast<const f16x8*>(kt + wr[st] + tt * 16 * kKv4Dim);
 #pragma unroll
-                    for (int ct = 0; ct < 2; ++ct) {
-                        s[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[ct][0][st].v,
-                                                                            s[ct][tt], 0, 0, 0);
-                        s[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[ct][1][st].v,
-                                                                            s[ct][tt], 0, 0, 0);
-                        if (NP == 3) {
-                            const bf16x8 q3 = *reinterpret_cast<const bf16x8*>(
-                                qlo + (((wave * 2 + ct) * 4 + st) * 64 + lane) * 4);
-                            s[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q3, s[ct][tt],
-                                                                                0, 0, 0);
-                        }
-                    }
+                    for (int p = 0; p < 2; ++p)
+#pragma unroll
+                        for (int ct = 0; ct < 2; ++ct)
+                            s[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                kf, qf[ct][p][st].v, s[ct][tt], 0, 0, 0);
                 }
             }
+            if (scaled)
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt) {
+                    const f32x4 f = *reinterpret_cast<const f32x4*>(moved + 16 * tt + 4 * j);
+                    s[0][tt] *= f;
+                    s[1][tt] *= f;
+                }
             const bool mask = bad || t + kTile - 1 > low;
-            Frag pf[2][2][NP];  // [column tile][32 tokens][part]
 #pragma unroll
             for (int ct = 0; ct < 2; ++ct) {
                 if (mask)
@@ -791,7 +897,8 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
                     top[tt] = fmaxf(fmaxf(s[ct][tt][0], s[ct][tt][1]),
                                     fmaxf(s[ct][tt][2], s[ct][tt][3]));
                 const float mn = fmaxf(
-                    m[ct], max_quarters(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))));
+                    m[ct],
+                    unit[ct] * max_quarters(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))));
                 const float base = mn == -INFINITY ? 0.0f : mn;
                 const float alpha = __builtin_amdgcn_exp2f(m[ct] - base);
                 m[ct] = mn;
@@ -805,45 +912,43 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
                 for (int tt = 0; tt < 4; ++tt) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        s[ct][tt][i] = __builtin_amdgcn_exp2f(s[ct][tt][i] - base);
+                        s[ct][tt][i] = __builtin_amdgcn_exp2f(
+                            __builtin_fmaf(s[ct][tt][i], unit[ct], kWeightBits - base));
                     sum[tt] = (s[ct][tt][0] + s[ct][tt][1]) + (s[ct][tt][2] + s[ct][tt][3]);
                 }
                 l[ct] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int e = 0; e < 8; e += 2) {
-                        float x0 = s[ct][2 * u + (e >> 2)][e & 3];
-                        float x1 = s[ct][2 * u + (e >> 2)][(e & 3) + 1];
-#pragma unroll
-                        for (int p = 0; p < NP; ++p) {
-                            pf[ct][u][p].w[e >> 1] = pack_hi(x0, x1);
-                            x0 -= masked(x0, 0xffff0000u);
-                            x1 -= masked(x1, 0xffff0000u);
-                        }
-                    }
             }
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < 2; ++u) {
+                Frag16 pf[2][2];  // [column tile][part]
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        const float p0 = s[ct][2 * u + (e >> 2)][e & 3];
+                        const float p1 = s[ct][2 * u + (e >> 2)][(e & 3) + 1];
+                        const uint32_t hi = pack16(p0, p1);
+                        pf[ct][0].w[e >> 1] = hi;
+                        pf[ct][1].w[e >> 1] = pack16(rest_lo(p0, hi), rest_hi(p1, hi));
+                    }
 #pragma unroll
                 for (int d = 0; d < 8; ++d) {
                     typedef __attribute__((address_space(3))) s16x4* lds4;
                     union {
                         s16x4 h[2];
-                        bf16x8 v;
+                        f16x8 v;
                     } vf;
-                    const int at = piece(32 * u + 4 * j + (col >> 2), 2 * d + (col >> 1 & 1)) +
-                                   (col & 1) * 4;
-                    vf.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vt + at));
-                    vf.h[1] =
-                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vt + at + 16 * kKv4Dim));
+                    uint16_t* src = vt + rd[d & 3] + (d >> 2) * 64 + u * 32 * kKv4Dim;
+                    vf.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)src);
+                    vf.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(src + 16 * kKv4Dim));
 #pragma unroll
-                    for (int p = 0; p < NP; ++p)
+                    for (int p = 0; p < 2; ++p)
 #pragma unroll
                         for (int ct = 0; ct < 2; ++ct)
-                            acc[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                vf.v, pf[ct][u][p].v, acc[ct][d], 0, 0, 0);
+                            acc[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                vf.v, pf[ct][p].v, acc[ct][d], 0, 0, 0);
                 }
+            }
         }
         __syncthreads();
     }
@@ -851,6 +956,9 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
     for (int ct = 0; ct < 2; ++ct) {
         const float L = sum_quarters(l[ct]);
         if (!row_ok[ct]) continue;
+        if (vshift != 0)
+#pragma unroll
+            for (int d = 0; d < 8; ++d) acc[ct][d] *= pow2(vshift);
         if (pos[ct] < a.chunk || a.splits == 1) {
             if (split == 0)
 #pragma unroll
@@ -960,8 +1068,7 @@ __device__ __forceinline__ void kv4_join(const Kv4Attn& a, const Records& rc, in
         for (int s = lane; s < rc.ns; s += 64) M = fmaxf(M, a.part_ml[rc.at(s)].x);
         M = wave_max(M);
     } else {
-        for (int s = 0; s < rc.ns; ++s)
-            M = fmaxf(M, s < kAhead ? pe[0].x : a.part_ml[rc.at(s)].x);
+        for (int s = kAhead; s < rc.ns; ++s) M = fmaxf(M, a.part_ml[rc.at(s)].x);
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) M = fmaxf(M, pe[k].x);
     }
@@ -991,16 +1098,22 @@ __device__ __forceinline__ void kv4_join(const Kv4Attn& a, const Records& rc, in
     store4<HALF>(a, out_at + 4 * d4, v, L);
 }
 
-// Joins the splits of a grid: a workgroup per row and head.
-template <bool HALF>
+constexpr int kWideJoin = 1024;  // rows and heads up to which each gets a workgroup for its records
+
+// Joins the splits of a grid: a workgroup has a row's head (WIDE: few rows, many records a head,
+// shared by 16 groups of lanes) or 16 of its heads.
+template <bool HALF, bool WIDE>
 __global__ void __launch_bounds__(512) kv4_join_kernel(Kv4Attn a, Kv4Seqs sq) {
-    __shared__ f32x4 ov[16][32];
+    __shared__ f32x4 ov[WIDE ? 16 : 1][32];
     __shared__ float lv[16];
-    const int row = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
+    const int row = blockIdx.x, tid = threadIdx.x, grp = tid >> 5;
     int seq, pos;
     if (!kv4_place(sq, row, tid & 15, seq, pos) || pos < a.chunk) return;
+    const int head = WIDE ? (int)blockIdx.y : (int)blockIdx.y * 16 + grp;
+    if (head >= a.Hq) return;
     const Records rc{((int64_t)row * a.Hq + head) * a.splits, 1, 0, pos / a.chunk + 1};
-    kv4_join<HALF, 16>(a, rc, row * a.out_stride + (int64_t)head * kKv4Dim, tid >> 5, ov, lv);
+    kv4_join<HALF, WIDE ? 16 : 1>(a, rc, row * a.out_stride + (int64_t)head * kKv4Dim,
+                                  WIDE ? grp : 0, ov, lv);
 }
 
 // Joins the shares of steps dealt evenly: a workgroup has a row's head (WIDE: few rows, many
@@ -1104,7 +1217,7 @@ int launch_kv4_even(const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
     const int rc = launch_status("kv4_attn_even_kernel");
     if (rc) return rc;
     // few rows: a head to a workgroup, its records to 8 groups of lanes
-    if ((int64_t)a.T * a.Hq <= 1024)
+    if ((int64_t)a.T * a.Hq <= kWideJoin)
         hipLaunchKernelGGL((kv4_join_even_kernel<ROWS, HALF, true>), dim3(a.T, a.Hq), dim3(256), 0,
                            st, a, s);
     else
@@ -1126,10 +1239,14 @@ int launch_kv4_plan(const Kv4Plan& p, const Kv4Attn& a, const Kv4Seqs& s, hipStr
     else if (p.rw == 4)
         launch_kv4<16, NP, 4, HALF>(a, s, st);
     else
-        hipLaunchKernelGGL((kv4_attn_rows_kernel<NP, HALF>), dim3(a.wgs), dim3(256), 0, st, a, s);
+        hipLaunchKernelGGL(kv4_attn_rows_kernel<HALF>, dim3(a.wgs), dim3(256), 0, st, a, s);
     const int rc = launch_status("kv4_attn_kernel");
     if (rc || p.splits == 1) return rc;
-    hipLaunchKernelGGL(kv4_join_kernel<HALF>, dim3(a.T, a.Hq), dim3(512), 0, st, a, s);
+    if ((int64_t)a.T * a.Hq <= kWideJoin)
+        hipLaunchKernelGGL((kv4_join_kernel<HALF, true>), dim3(a.T, a.Hq), dim3(512), 0, st, a, s);
+    else
+        hipLaunchKernelGGL((kv4_join_kernel<HALF, false>), dim3(a.T, (a.Hq + 15) / 16), dim3(512),
+                           0, st, a, s);
     return launch_status("kv4_join_kernel");
 }
 

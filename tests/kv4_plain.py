@@ -78,9 +78,17 @@ def append(k, v, pools, tables, ctx, layer, rope, cu):
         pv[where], pvs[where] = quantize(np.asarray(v[r], np.float64))
 
 
+def _largest(pools, table, c, layer):
+    t = np.arange(c)
+    page = table[t // PAGE]
+    t, page = t[(page >= 0) & (page < len(pools[1]))], page[(page >= 0) & (page < len(pools[1]))]
+    v = values(pools[1][page, layer, :, t % PAGE], pools[3][page, layer, :, t % PAGE])
+    return np.abs(v).max((0, 2))
+
+
 def attention(q, pools, tables, ctx, layer, rope, cu, out, parts_eps=0.0):
     """out [T][Hq][128] and how far fp32 sums may be from it, both updated for the rows of
-    sequences. q [T][Hq][128]."""
+    sequences. q [T][Hq][128]; parts_eps: what queries and weights are rounded to."""
     pk, pv, pks, pvs = pools
     Hq, Hkv = q.shape[1], pk.shape[2]
     G = Hq // Hkv
@@ -101,6 +109,7 @@ def attention(q, pools, tables, ctx, layer, rope, cu, out, parts_eps=0.0):
             continue
         K = values(pk[page, layer, :, t % PAGE], pks[page, layer, :, t % PAGE])  # [n][Hkv][128]
         V = values(pv[page, layer, :, t % PAGE], pvs[page, layer, :, t % PAGE])
+        vmax = _largest(pools, tables[b], int(ctx[b]), layer)
         x = rotate(q[r], None if rope is None else rope[pos]) / np.sqrt(D)
         mag = np.abs(np.asarray(q[r], np.float64)).reshape(Hq, 2, 64).sum(1) / np.sqrt(D)
         mag = np.concatenate([mag, mag], -1)  # bounds a rotated element's rounding
@@ -113,12 +122,17 @@ def attention(q, pools, tables, ctx, layer, rope, cu, out, parts_eps=0.0):
             # a score: the query's roundings (rotation 3, scale 2, parts), 128 products summed;
             # a weight: its score's error twice (it and the sum's), the difference's and the
             # exponential's rounding; the sums of n weights and n products
+            # (and 2^-37 of a token's largest key element, times the query)
             ds = ((6 * u + parts_eps) * (np.abs(kk) @ mag[h]) +
-                  128 * u * (np.abs(kk) @ np.abs(x[h]))).max()
+                  128 * u * (np.abs(kk) @ np.abs(x[h])) +
+                  2.0 ** -37 * np.abs(kk).max(-1) * np.abs(x[h]).sum()).max()
             dp = 2 * ds + (8 + 2 * (s.max() - s).max()) * u + parts_eps
             tol[r, h] = (dp + 2 * (len(t) + 32) * u) * (p @ np.abs(vv))
             # weights and products below 2^-126 have no relative precision (or count as 0)
             tol[r, h] += 2.0 ** -126 * (1 + np.abs(vv)).sum(0)
+            # weights are held times 2^15 in fp16 parts, whose smallest step is 2^-24: half of it
+            tol[r, h] += 2.0 ** -40 * p.max() * np.abs(vv).sum(0)
+            tol[r, h] += 2.0 ** -37 * vmax[h // G]  # of the largest value that any row sees
     return out, tol
 
 

@@ -81,10 +81,11 @@ class Setup:
 
     def check_attention(self, out, start=None):
         want = np.zeros((self.T, self.Hq, D)) if start is None else start.astype(np.float64)
+        # (queries and weights are held to 16 bits in fp16 calls, to 22 in fp32 ones: 2^-15 and
+        # 2^-21 for the two of them)
         half = self.dtype == np.float16
-        # (queries and weights of fp16 calls are held to 16 bits)
         want, tol = plain.attention(self.q, self.pools, self.tables, self.ctx, self.layer,
-                                    self.rope, self.cu, want, 2.0 ** -15 if half else 0.0)
+                                    self.rope, self.cu, want, 2.0 ** -15 if half else 2.0 ** -21)
         got = out.reshape(want.shape).astype(np.float64)
         # half a step of the type: relative, and below its smallest normal number 2^-14 (fp16)
         # half of the constant step 2^-24 that its numbers have there
@@ -291,6 +292,52 @@ def test_attention_peaked_and_flat(torch_dev, ops, n):
     s.q[c[2]:c[3], :, 7] *= 400
     s.q[c[3]:c[4]] *= 1e-20
     s.dev(torch)
+    s.check_attention(ops.attn_kv4(s.d["q"], *s.args(), **s.opts()).cpu().numpy())
+
+
+@pytest.mark.parametrize("kind", ["keys", "values", "small", "large", "rising", "falling",
+                                  "zeros", "one_group"])
+@pytest.mark.parametrize("n,Hq", [(1, 4), (1, 12), (5, 8), (70, 4)])
+def test_attention_scale_range(torch_dev, ops, kind, n, Hq):
+    """Scales that fp16 does not span: tokens and groups 2^60 apart, everything tiny or large,
+    growing and shrinking along the sequence, groups and tokens of zeros with any scale."""
+    s = Setup([(n, 200), (n, 70)], Hq, 1, layers=1, seed=n)
+    rng = np.random.default_rng(n + Hq)
+    ks, vs = s.pools[2], s.pools[3]
+    t = np.empty(s.nb * PAGE, np.int64)  # a slot's position
+    for b in range(2):
+        for p in range(s.tables.shape[1]):
+            if s.tables[b, p] >= 0:
+                t[s.tables[b, p] * PAGE:][:PAGE] = np.arange(PAGE) + p * PAGE
+    t = t.reshape(s.nb, 1, 1, PAGE, 1)
+    some = np.broadcast_to(rng.random(ks.shape[:-1] + (1,)) < 0.1, ks.shape)
+    if kind == "keys":
+        s.q *= 1e-8
+        ks[some] = rng.integers(60, 160, some.sum())
+    elif kind == "values":
+        vs[some] = rng.integers(60, 190, some.sum())
+    elif kind == "small":
+        vs[:], ks[:] = 127 - 90, 127 - 60
+    elif kind == "large":
+        vs[:], ks[:] = 127 + 80, 127 + 60
+        s.q *= 2.0 ** -60
+    elif kind == "rising":
+        vs[:] = 100 + t // 4
+    elif kind == "falling":
+        vs[:] = 160 - t // 4
+        ks[:] = 127 - t % 30
+    elif kind == "zeros":
+        for c, e in ((s.pools[0], ks), (s.pools[1], vs)):
+            c[rng.random(c.shape[:-1]) < 0.3] = 0x80  # zeros and negative zeros
+            e[(c.reshape(*c.shape[:-1], 4, 16) & 0x77 == 0).all(-1)] = rng.choice([0, 1, 200, 255])
+    else:
+        ks[..., 2], vs[..., 1] = 127 - 35, 127 - 33
+    for e in (ks, vs):
+        for b, (_, c) in enumerate(s.seqs):
+            if c % PAGE:
+                e[s.tables[b, c // PAGE], :, :, c % PAGE:] = 252
+    s.dev(torch_dev)
+    print("attn scales", kind, n, Hq, flush=True)
     s.check_attention(ops.attn_kv4(s.d["q"], *s.args(), **s.opts()).cpu().numpy())
 
 
