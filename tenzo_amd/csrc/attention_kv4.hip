@@ -33,9 +33,15 @@ struct Kv4Attn {
     float* part_o;    // records of rows' unfinished sums: 128 sums,
     float2* part_ml;  // maximum (base 2) and sum of weights
     int G, Hq, T;
+    uint32_t g_mul;  // 2^32 / G, rounded up (0: G is 1)
     int chunk, splits;  // tokens of a split
     int wgs;            // workgroups of a call whose steps are dealt evenly
     int vec_out;        // out allows accesses of 4 elements
+
+    // r / G, exact for r < 2^28 and G up to 16 (a division is some 40 instructions).
+    __device__ __forceinline__ int token(int r) const {
+        return g_mul ? (int)__umulhi((uint32_t)r, g_mul) : r;
+    }
 };
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -292,12 +298,12 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
     const int rw = wave % RW, tw = wave / RW;
     const int n = g.n, first = g.first, c = g.c, h = g.h, t0 = g.t0;
     const int row0 = g.tile * RT;  // of the sequence's n * G
-    const int last_i = min(n - 1, (row0 + RT - 1) / a.G);
+    const int last_i = min(n - 1, a.token(row0 + RT - 1));
     const int t1 = min(min(t0 + g.len, c - n + last_i + 1), c);  // tokens that some row sees
 
     // the lane's row
     const int slot = col / ROWS, r = row0 + rw * ROWS + col % ROWS;
-    const int qi = r / a.G, head = h * a.G + (r - qi * a.G);
+    const int qi = a.token(r), head = h * a.G + (r - qi * a.G);
     const bool row_ok = qi < n && first >= 0 && first + qi < a.T;
     const int pos = row_ok && c > 0 ? c - n + qi : -1;
     const int64_t grow = (int64_t)first + qi;
@@ -313,29 +319,36 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
         }
     };
     float* qs = reinterpret_cast<float*>(smem);
+    // (no load under a condition, where it would be waited for: rows and positions that are not
+    // there read others, whose results nobody writes)
     constexpr int QT = RT / 4;
-    float x0[QT], x1[QT];
+    float x0[QT], x1[QT], cv[QT], sv[QT];
+    const int last_row = n * a.G - 1;
 #pragma unroll
     for (int k = 0; k < QT; ++k) {
-        const int r2 = row0 + wave + 4 * k, i2 = r2 / a.G, p2 = c - n + i2;
-        x0[k] = x1[k] = 0.0f;
-        if (i2 < n && first >= 0 && first + i2 < a.T && p2 >= 0) {
-            const int64_t at = ((int64_t)first + i2) * a.q_stride +
-                               (int64_t)(h * a.G + (r2 - i2 * a.G)) * kKv4Dim + lane;
-            x0[k] = ld_act<HALF>(a.q, at);
-            x1[k] = ld_act<HALF>(a.q, at + 64);
-        }
+        const int r2 = min(row0 + wave + 4 * k, last_row), i2 = a.token(r2);
+        const int64_t at = (int64_t)min(max(first + i2, 0), a.T - 1) * a.q_stride +
+                           (int64_t)(h * a.G + (r2 - i2 * a.G)) * kKv4Dim + lane;
+        x0[k] = ld_act<HALF>(a.q, at);
+        x1[k] = ld_act<HALF>(a.q, at + 64);
+        cv[k] = 1.0f;
+        sv[k] = 0.0f;
     }
+    if (a.rope && c > 0)
+#pragma unroll
+        for (int k = 0; k < QT; ++k) {
+            const int p2 = c - n + a.token(min(row0 + wave + 4 * k, last_row));
+            const float* cs = a.rope + (int64_t)min(max(p2, 0), c - 1) * kKv4Dim + lane;
+            cv[k] = cs[0];
+            sv[k] = cs[64];
+        }
     stage_pages(0);
 #pragma unroll
     for (int k = 0; k < QT; ++k) {
-        const int rr = wave + 4 * k, p2 = c - n + (row0 + rr) / a.G;
-        if (a.rope && p2 >= 0 && p2 < c) {
-            const float* cs = a.rope + (int64_t)p2 * kKv4Dim + lane;
-            const float cv = cs[0], sv = cs[64], y0 = x0[k];
-            x0[k] = __builtin_fmaf(y0, cv, -__fmul_rn(x1[k], sv));
-            x1[k] = __builtin_fmaf(y0, sv, __fmul_rn(x1[k], cv));
-        }
+        const int rr = wave + 4 * k;
+        const float y0 = x0[k];
+        x0[k] = __builtin_fmaf(y0, cv[k], -__fmul_rn(x1[k], sv[k]));
+        x1[k] = __builtin_fmaf(y0, sv[k], __fmul_rn(x1[k], cv[k]));
         qs[rr * kQStride + lane] = __fmul_rn(x0[k], kQkScale * kLog2e);
         qs[rr * kQStride + lane + 64] = __fmul_rn(x1[k], kQkScale * kLog2e);
     }
@@ -468,7 +481,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
                 s[tt][i] = v;
             }
         // a step that a row may not see whole: past its position, or absent pages
-        if (bad || t + kTile - 1 > c - n + row0 / a.G) {
+        if (bad || t + kTile - 1 > c - n + a.token(row0)) {
 #pragma unroll
             for (int tt = 0; tt < kSub; ++tt)
 #pragma unroll
@@ -598,7 +611,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
         __syncthreads();
         for (int it = tid; it < RT * 32; it += 256) {
             const int rr = it >> 5, d4 = it & 31, grp = rr / ROWS, cc = rr % ROWS;
-            const int r2 = row0 + rr, i2 = r2 / a.G;
+            const int r2 = row0 + rr, i2 = a.token(r2);
             if (i2 >= n || first < 0 || first + i2 >= a.T) continue;
             float M = -INFINITY, L = 0.0f;
             f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -660,7 +673,7 @@ kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
     g.c = sq.length(g.seq);
     g.t0 = g.split * a.chunk;
     g.len = a.chunk;
-    const int last_i = min(g.n - 1, (g.tile * ROWS * RW + ROWS * RW - 1) / a.G);
+    const int last_i = min(g.n - 1, a.token(g.tile * ROWS * RW + ROWS * RW - 1));
     if (g.split > 0 && g.t0 >= min(g.c - g.n + last_i + 1, g.c)) return;
     kv4_segment<ROWS, NP, RW, HALF, false>(a, sq, g, sm);
 }
@@ -668,7 +681,8 @@ kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
 // Prompts: 128 rows to a workgroup, 32 (two column tiles) to a wave, all against the same 64 tokens
 // at a time. The waves convert a quarter of the tile's keys and values each, into LDS as fp16,
 // and every fragment of 1 KB read from there serves both column tiles and both parts, 4 MFMAs. The
-// codes of the next tile are loaded during the products.
+// codes of the next tile are loaded during the products and go into the other half of LDS after
+// them: one barrier a tile.
 //
 // fp16 parts take two thirds of the MFMAs that bf16's would, and half of the vector work of
 // splitting the weights. Codes times scale are exact in fp16 (a token whose scales are out of its
@@ -679,9 +693,10 @@ kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
 constexpr int kRowsRT = 128;
 template <bool HALF>
 __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seqs sq) {
-    __shared__ __align__(16) uint16_t kt[kTile * kKv4Dim], vt[kTile * kKv4Dim];
-    __shared__ float moved[kTile];  // 2^ the power of two that a token's keys are moved by
-    __shared__ int flags[4], tops[4];
+    // two tiles' keys and values (the first is the queries' on their way to registers before)
+    __shared__ __align__(16) uint16_t tiles[2][2][kTile * kKv4Dim];
+    __shared__ float moved[2][kTile];  // 2^ the power of two that a token's keys are moved by
+    __shared__ int flags[2][4], tops[4];
     __shared__ int pg[kMaxPages];
     const int per_unit = sq.Hkv * a.splits;
     // (from the last unit on: the latest rows of a prompt see the most tokens)
@@ -693,7 +708,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
     const int n = sq.cu ? sq.cu[seq + 1] - first : 1;
     const int c = sq.length(seq);
     const int t0 = split * a.chunk, row0 = tile * kRowsRT;
-    const int last_i = min(n - 1, (row0 + kRowsRT - 1) / a.G);
+    const int last_i = min(n - 1, a.token(row0 + kRowsRT - 1));
     const int t1 = min(min(t0 + a.chunk, c - n + last_i + 1), c);  // tokens that some row sees
     if (split > 0 && t0 >= t1) return;
 
@@ -710,7 +725,9 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
     };
     stage_pages(0);
 
-    // the lane's rows, and their queries as B operands (dims 32j .. 32j + 31)
+    // the lane's rows, and their queries as B operands (dims 32j .. 32j + 31; no load under a
+    // condition, as above)
+    const int last_row = n * a.G - 1;
     int pos[2];
     int64_t grow[2];
     int head[2];
@@ -719,42 +736,61 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
     Frag16 qf[2][2][4];
 #pragma unroll
     for (int ct = 0; ct < 2; ++ct) {
-        const int r = wrow + 16 * ct + col, i = r / a.G;
+        const int r = wrow + 16 * ct + col, i = a.token(r);
         head[ct] = h * a.G + (r - i * a.G);
         row_ok[ct] = i < n && first >= 0 && first + i < a.T;
         pos[ct] = row_ok[ct] && c > 0 ? c - n + i : -1;
         grow[ct] = (int64_t)first + i;
-        const bool turn = a.rope && pos[ct] >= 0, upper = lane >= 32;
-        const int64_t at = grow[ct] * a.q_stride + (int64_t)head[ct] * kKv4Dim + 32 * j;
-        const int64_t cs = (int64_t)max(pos[ct], 0) * kKv4Dim + 32 * (j & 1);
-        float x[32], amax = 0.0f;
+        // 16 rows by way of the wave's own 8 KB: rows of 512 bytes in, a lane's 32 dims out
+        float* qs = reinterpret_cast<float*>(tiles[0][0]) + wave * (16 * kKv4Dim);
+        auto place = [](int row, int d) { return row * kKv4Dim + (d ^ ((row & 7) << 2)); };
+        float x0[16], x1[16], cv[16], sv[16];
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-            float v[4] = {}, cv[4] = {1.0f, 1.0f, 1.0f, 1.0f}, sv[4] = {};
-            if (row_ok[ct]) ld_act4<HALF>(a.q, at + e, v);
-            if (turn) {
-                ld_act4<false>(a.rope, cs + e, cv);
-                ld_act4<false>(a.rope, cs + 64 + e, sv);
+        for (int rr = 0; rr < 16; ++rr) {
+            const int r2 = min(wrow + 16 * ct + rr, last_row), i2 = a.token(r2);
+            const int64_t at = (int64_t)min(max(first + i2, 0), a.T - 1) * a.q_stride +
+                               (int64_t)(h * a.G + (r2 - i2 * a.G)) * kKv4Dim + lane;
+            x0[rr] = ld_act<HALF>(a.q, at);
+            x1[rr] = ld_act<HALF>(a.q, at + 64);
+            cv[rr] = 1.0f;
+            sv[rr] = 0.0f;
+        }
+        if (a.rope && c > 0)
+#pragma unroll
+            for (int rr = 0; rr < 16; ++rr) {
+                const int p2 = c - n + a.token(min(wrow + 16 * ct + rr, last_row));
+                const float* cs = a.rope + (int64_t)min(max(p2, 0), c - 1) * kKv4Dim + lane;
+                cv[rr] = cs[0];
+                sv[rr] = cs[64];
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float lo, hi;  // the dims d and d + 64
-                lane_halves(v[k], lo, hi);
-                v[k] = upper ? __builtin_fmaf(lo, sv[k], __fmul_rn(hi, cv[k]))
-                             : __builtin_fmaf(lo, cv[k], -__fmul_rn(hi, sv[k]));
-                x[e + k] = __fmul_rn(v[k], kQkScale * kLog2e);
-                amax = fmaxf(amax, fabsf(x[e + k]));
-            }
+        for (int rr = 0; rr < 16; ++rr) {
+            const float y0 = x0[rr];
+            x0[rr] = __builtin_fmaf(y0, cv[rr], -__fmul_rn(x1[rr], sv[rr]));
+            x1[rr] = __builtin_fmaf(y0, sv[rr], __fmul_rn(x1[rr], cv[rr]));
+            qs[place(rr, lane)] = __fmul_rn(x0[rr], kQkScale * kLog2e);
+            qs[place(rr, lane + 64)] = __fmul_rn(x1[rr], kQkScale * kLog2e);
+        }
+        f32x4 x[8];
+        float amax = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[e] = *reinterpret_cast<const f32x4*>(qs + place(col, 32 * j + 4 * e));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) amax = fmaxf(amax, fabsf(x[e][k]));
         }
         const int up = row_shift(max_quarters(amax));
         unit[ct] = pow2(-up);
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-            const float x0 = x[e] * pow2(up), x1 = x[e + 1] * pow2(up);
-            const uint32_t hi = pack16(x0, x1);
-            qf[ct][0][e >> 3].w[(e >> 1) & 3] = hi;
-            qf[ct][1][e >> 3].w[(e >> 1) & 3] =
-                pack16(rest_lo(x0, hi), rest_hi(x1, hi));
+        for (int e = 0; e < 8; ++e) {
+            x[e] *= pow2(up);
+#pragma unroll
+            for (int k = 0; k < 4; k += 2) {
+                const uint32_t hi = pack16(x[e][k], x[e][k + 1]);
+                qf[ct][0][e >> 1].w[2 * (e & 1) + k / 2] = hi;
+                qf[ct][1][e >> 1].w[2 * (e & 1) + k / 2] =
+                    pack16(rest_lo(x[e][k], hi), rest_hi(x[e][k + 1], hi));
+            }
         }
     }
     __syncthreads();
@@ -798,14 +834,16 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
             *reinterpret_cast<uint4*>(dst + wave * 16 * kKv4Dim + wr[st]) =
                 fp4_to_half8(w[st], sc);
     };
-    const int low = c - n + wrow / a.G;                      // the wave's first position
-    const int high = c - n + min(n - 1, (wrow + 31) / a.G);  // and its last
-    int w0 = t0;
-    if (t0 < t1 && sq.n_blocks > 0) load(t0, w0);
-    for (int t = t0; t < t1 && sq.n_blocks > 0; t += kTile) {
-        // what fp16 does not hold as it is: keys are moved token by token, values all together
-        const bool skip = none;
-        int kb = skip ? 127 : ks, vby = skip ? 127 + vshift : vs, by = 0, flag = 0;
+    const int low = c - n + a.token(wrow);                      // the wave's first position
+    const int high = c - n + min(n - 1, a.token(wrow + 31));  // and its last
+    // A tile into its half of LDS. What fp16 does not hold as it is: keys are moved token by token;
+    // values all together, which waits for the tile's turn (the values then go in again).
+    int vby = 0;
+    bool skip = false;
+    auto convert = [&](int half) {
+        skip = none;
+        int kb = skip ? 127 : ks, by = 0, flag = 0;
+        vby = skip ? 127 + vshift : vs;
         if (__ballot(!in_range(kb) || !in_range(vby - vshift))) {
             if (kb > 252 || no_codes(kr)) kb = 0;
             if (vby > 252 || no_codes(vr)) vby = 0;
@@ -814,10 +852,19 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
             flag = __ballot(vby > 0 && vby - vshift < kLowScale) ? 3 : 1;
         }
         if (!skip) vtop = max(vtop, vby);
-        store(kt, kr, kb);
-        store(vt, vr, vby - vshift);
-        if (j == 0) moved[16 * wave + col] = pow2(by);
-        if (lane == 0) flags[wave] = flag;
+        store(tiles[half][0], kr, kb);
+        store(tiles[half][1], vr, vby - vshift);
+        if (j == 0) moved[half][16 * wave + col] = pow2(by);
+        if (lane == 0) flags[half][wave] = flag;
+    };
+    int w0 = t0;
+    const bool any = t0 < t1 && sq.n_blocks > 0;
+    __syncthreads();
+    if (any) {
+        load(t0, w0);
+        convert(0);
+    }
+    for (int t = t0, half = 0; t < t1 && any; t += kTile, half ^= 1) {
         int ids[4];
         bool bad = false;
 #pragma unroll
@@ -827,7 +874,10 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
             bad = bad || ids[tt] < 0;
         }
         __syncthreads();
-        flag = __builtin_amdgcn_readfirstlane(flags[0] | flags[1] | flags[2] | flags[3]);
+        const uint16_t* kt = tiles[half][0];
+        uint16_t* vt = tiles[half][1];
+        const int* fl = flags[half];
+        const int flag = __builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]);
         const bool scaled = flag != 0;
         if (scaled) {
             // the values' power of two for the largest scale so far, and the tile once more
@@ -857,7 +907,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
             }
             load(next, w0);
         }
-        if (t <= high && wrow / a.G < n) {
+        if (t <= high && a.token(wrow) < n) {
             f32x4 s[2][4];
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt) {
@@ -877,7 +927,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
             if (scaled)
 #pragma unroll
                 for (int tt = 0; tt < 4; ++tt) {
-                    const f32x4 f = *reinterpret_cast<const f32x4*>(moved + 16 * tt + 4 * j);
+                    const f32x4 f = *reinterpret_cast<const f32x4*>(moved[half] + 16 * tt + 4 * j);
                     s[0][tt] *= f;
                     s[1][tt] *= f;
                 }
@@ -950,7 +1000,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
                 }
             }
         }
-        __syncthreads();
+        if (next < t1) convert(half ^ 1);
     }
 #pragma unroll
     for (int ct = 0; ct < 2; ++ct) {
@@ -1309,6 +1359,7 @@ TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,
     a.part_ml = (float2*)((char*)ws + p.records * kKv4Dim * 4);
     a.wgs = (int)p.wgs;
     a.G = G;
+    a.g_mul = G == 1 ? 0 : (uint32_t)((0x100000000ull + G - 1) / G);
     a.Hq = Hq;
     a.T = (int)T;
     a.chunk = p.chunk;
