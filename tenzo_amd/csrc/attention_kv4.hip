@@ -436,26 +436,35 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
     for (; t < w1 && any; t += kTile * TW) {
         const int next = t + kTile * TW;
         f32x4 s[kSub];
+        // (the steps outermost: an MFMA waits some 60 cycles for the sum that it adds to, so
+        // neighbours have different ones)
+        float sc[kSub];
 #pragma unroll
         for (int tt = 0; tt < kSub; ++tt) {
-            const float sc = e8m0_to_float(ksc[tt]);
-            const uint32_t w[4] = {kr[tt].x, kr[tt].y, kr[tt].z, kr[tt].w};
+            sc[tt] = e8m0_to_float(ksc[tt]);
             s[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
 #pragma unroll
-            for (int st = 0; st < 4; ++st) {
-                union {
-                    bf16x2 p[4];
-                    bf16x8 v;
-                } kf;
-                kf.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 0);
-                kf.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 1);
-                kf.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 2);
-                kf.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 3);
+        for (int st = 0; st < 4; ++st) {
+            union {
+                bf16x2 p[4];
+                bf16x8 v;
+            } kf[kSub];
 #pragma unroll
-                for (int p = 0; p < NM; ++p)
-                    s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf.v, qf[p][st].v, s[tt], 0, 0,
-                                                                    0);
+            for (int tt = 0; tt < kSub; ++tt) {
+                const uint32_t w = st == 0 ? kr[tt].x : st == 1 ? kr[tt].y : st == 2 ? kr[tt].z
+                                                                                   : kr[tt].w;
+                kf[tt].p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc[tt], 0);
+                kf[tt].p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc[tt], 1);
+                kf[tt].p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc[tt], 2);
+                kf[tt].p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc[tt], 3);
             }
+#pragma unroll
+            for (int p = 0; p < NM; ++p)
+#pragma unroll
+                for (int tt = 0; tt < kSub; ++tt)
+                    s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[tt].v, qf[p][st].v, s[tt],
+                                                                    0, 0, 0);
         }
         bool bad = false;
         int id_now[kSub];
@@ -551,20 +560,26 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
                     p8[e + 1] -= masked(p8[e + 1], 0xffff0000u);
                 }
 #pragma unroll
-            for (int d = 0; d < 8; ++d) {
+            for (int d0 = 0; d0 < 8; d0 += 4) {
                 typedef __attribute__((address_space(3))) s16x4* lds4;
                 union {
                     s16x4 h[2];
                     bf16x8 v;
-                } vf;
-                // (lane 4r + i of 16: half a piece of row r, in return for column 4r + i)
-                uint16_t* src = vb + rd[d & 3] + (d >> 2) * 64;
-                vf.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)src);
-                vf.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(src + 16 * kKv4Dim));
+                } vf[4];
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    // (lane 4r + i of 16: half a piece of row r, in return for column 4r + i)
+                    uint16_t* src = vb + rd[d] + (d0 >> 2) * 64;
+                    vf[d].h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)src);
+                    vf[d].h[1] =
+                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(src + 16 * kKv4Dim));
+                }
 #pragma unroll
                 for (int p = 0; p < NM; ++p)
-                    acc[d] =
-                        __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.v, pf[p].v, acc[d], 0, 0, 0);
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+                        acc[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            vf[d].v, pf[p].v, acc[d0 + d], 0, 0, 0);
             }
         }
     }
@@ -657,7 +672,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
 
 // A grid of (unit, split, kv head): every workgroup one piece.
 template <int ROWS, int NP, int RW, bool HALF>
-__global__ void __launch_bounds__(256, ROWS == 16 && NP == 3 ? 2 : 3)
+__global__ void __launch_bounds__(256, ROWS == 16 ? 2 : 3)
 kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
     __shared__ Kv4Smem<ROWS, NP, RW, HALF> sm;
     const int per_unit = sq.Hkv * a.splits;
@@ -678,6 +693,56 @@ kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
     kv4_segment<ROWS, NP, RW, HALF, false>(a, sq, g, sm);
 }
 
+constexpr int kRowsRT = 128;
+
+// Sequence and row tile of a work unit of the prompts' kernel, those that see the most tokens first
+// whatever their sequence: tile k of a sequence starts at position length - rows + 128 k / G, and
+// the unit-th largest start is found by bisection (a lane a sequence; one sequence, or over 64 in
+// their order, from the last unit on). 3 prompts of 500 to 2000 tokens, 20 / 5 heads: 103 us, in
+// the order of the rows 119.
+__device__ __forceinline__ bool find_unit_latest(const Kv4Seqs& sq, int unit, int units, int G,
+                                                 int& seq, int& tile) {
+    if (!sq.cu || sq.B == 1 || sq.B > 64)
+        return find_unit(sq, units - 1 - unit, G, kRowsRT, seq, tile);
+    const int lane = threadIdx.x & 63;
+    int n = 0, c = 0;
+    if (lane < sq.B) {
+        n = max(0, sq.cu[lane + 1] - sq.cu[lane]);
+        c = sq.length(lane);
+    }
+    const int tiles = (int)(((int64_t)n * G + kRowsRT - 1) / kRowsRT), prior = max(c - n, 0);
+    // tiles of the lane's sequence that start past x
+    auto past = [&](int x) {
+        if (x < prior) return tiles;
+        return (int)max((int64_t)tiles - 1 - (int64_t)(x - prior) * G / kRowsRT, (int64_t)0);
+    };
+    if (unit >= wave_sum_i32(tiles)) return false;
+    int lo = 0, hi = max(c, n);  // (no tile starts past the largest)
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) hi = max(hi, __shfl_xor(hi, d));
+    while (lo < hi) {  // the smallest start that at most `unit` tiles lie past
+        const int x = lo + (hi - lo) / 2;
+        if (wave_sum_i32(past(x)) <= unit)
+            hi = x;
+        else
+            lo = x + 1;
+    }
+    const int later = past(lo), here = past(lo - 1) - later;
+    int rank = unit - wave_sum_i32(later), incl = here;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(incl, d);
+        if (lane >= d) incl += o;
+    }
+    const uint64_t mine = __ballot(incl > rank);
+    if (!mine) return false;
+    const int l = __ffsll((unsigned long long)mine) - 1;
+    seq = l;
+    rank -= __builtin_amdgcn_readlane(incl - here, l);
+    tile = __builtin_amdgcn_readlane(tiles - 1 - later, l) - rank;
+    return true;
+}
+
 // Prompts: 128 rows to a workgroup, 32 (two column tiles) to a wave, all against the same 64 tokens
 // at a time. The waves convert a quarter of the tile's keys and values each, into LDS as fp16,
 // and every fragment of 1 KB read from there serves both column tiles and both parts, 4 MFMAs. The
@@ -690,7 +755,6 @@ kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
 // all tokens; what lies 2^37 below the largest is then lost). Queries, scaled by a power of two,
 // and weights are split into two parts, 22 bits: 2^-22 of a value is lost, little beside what fp32
 // sums lose (and of a weight 2^-40 of the largest, fp16's smallest step).
-constexpr int kRowsRT = 128;
 template <bool HALF>
 __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seqs sq) {
     // two tiles' keys and values (the first is the queries' on their way to registers before)
@@ -699,11 +763,10 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
     __shared__ int flags[2][4], tops[4];
     __shared__ int pg[kMaxPages];
     const int per_unit = sq.Hkv * a.splits;
-    // (from the last unit on: the latest rows of a prompt see the most tokens)
-    const int back = blockIdx.x / per_unit, rest = blockIdx.x - back * per_unit;
+    const int nth = blockIdx.x / per_unit, rest = blockIdx.x - nth * per_unit;
     const int split = rest / sq.Hkv, h = rest - split * sq.Hkv;
     int seq, tile;
-    if (!find_unit(sq, a.wgs / per_unit - 1 - back, a.G, kRowsRT, seq, tile)) return;
+    if (!find_unit_latest(sq, nth, a.wgs / per_unit, a.G, seq, tile)) return;
     const int first = sq.cu ? sq.cu[seq] : seq;
     const int n = sq.cu ? sq.cu[seq + 1] - first : 1;
     const int c = sq.length(seq);
@@ -909,20 +972,23 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
         }
         if (t <= high && a.token(wrow) < n) {
             f32x4 s[2][4];
+            // (neighbouring MFMAs add to different sums, as above)
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt) {
-                s[0][tt] = s[1][tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int tt = 0; tt < 4; ++tt) s[0][tt] = s[1][tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int st = 0; st < 4; ++st) {
-                    const f16x8 kf =
-                        *reinterpret_cast<const f16x8*>(kt + wr[st] + tt * 16 * kKv4Dim);
+            for (int st = 0; st < 4; ++st) {
+                f16x8 kf[4];
 #pragma unroll
-                    for (int p = 0; p < 2; ++p)
+                for (int tt = 0; tt < 4; ++tt)
+                    kf[tt] = *reinterpret_cast<const f16x8*>(kt + wr[st] + tt * 16 * kKv4Dim);
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
                         for (int ct = 0; ct < 2; ++ct)
                             s[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                kf, qf[ct][p][st].v, s[ct][tt], 0, 0, 0);
-                }
+                                kf[tt], qf[ct][p][st].v, s[ct][tt], 0, 0, 0);
             }
             if (scaled)
 #pragma unroll
@@ -982,21 +1048,27 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
                         pf[ct][1].w[e >> 1] = pack16(rest_lo(p0, hi), rest_hi(p1, hi));
                     }
 #pragma unroll
-                for (int d = 0; d < 8; ++d) {
+                for (int d0 = 0; d0 < 8; d0 += 4) {
                     typedef __attribute__((address_space(3))) s16x4* lds4;
                     union {
                         s16x4 h[2];
                         f16x8 v;
-                    } vf;
-                    uint16_t* src = vt + rd[d & 3] + (d >> 2) * 64 + u * 32 * kKv4Dim;
-                    vf.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)src);
-                    vf.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(src + 16 * kKv4Dim));
+                    } vf[4];
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        uint16_t* src = vt + rd[d] + (d0 >> 2) * 64 + u * 32 * kKv4Dim;
+                        vf[d].h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)src);
+                        vf[d].h[1] =
+                            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(src + 16 * kKv4Dim));
+                    }
 #pragma unroll
                     for (int p = 0; p < 2; ++p)
 #pragma unroll
-                        for (int ct = 0; ct < 2; ++ct)
-                            acc[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                vf.v, pf[ct][p].v, acc[ct][d], 0, 0, 0);
+                        for (int d = 0; d < 4; ++d)
+#pragma unroll
+                            for (int ct = 0; ct < 2; ++ct)
+                                acc[ct][d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    vf[d].v, pf[ct][p].v, acc[ct][d0 + d], 0, 0, 0);
                 }
             }
         }
@@ -1031,7 +1103,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
 // lengths, which only the device knows, need not be alike. A share holds the end of a unit that
 // an earlier workgroup began, whole units and the beginning of one: two records at most.
 template <int ROWS, int NP, bool HALF>
-__global__ void __launch_bounds__(256, ROWS == 16 && NP == 3 ? 2 : 3)
+__global__ void __launch_bounds__(256, ROWS == 16 ? 2 : 3)
 kv4_attn_even_kernel(Kv4Attn a, Kv4Seqs sq) {
     __shared__ Kv4Smem<ROWS, NP, 1, HALF> sm;
     __shared__ int wsum[4], at_base, at_seq;
@@ -1239,15 +1311,7 @@ Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, boo
         return p;
     }
     const int64_t likely = cu ? (ceil_div(T * G, rt) > B ? ceil_div(T * G, rt) : B) : units;
-    int64_t s = room / (likely * Hkv);
-    if (p.rw > 4) {
-        // two workgroups a CU. A prompt's last rows see all of its tokens, its first ones few: no
-        // workgroup should have more steps than an even share of all of them
-        s = 512 / (likely * Hkv);
-        const int64_t rows = T / B / kTile < 2 * steps ? T / B / kTile : 2 * steps;
-        const int64_t share = likely * Hkv * (2 * steps - rows) / 2 / 512;
-        if (s < 2) s = ceil_div(steps, share < 1 ? 1 : share);
-    }
+    int64_t s = (p.rw > 4 ? 512 : room) / (likely * Hkv);  // (the prompts' kernel: two a CU)
     s = s < 1 ? 1 : s > steps ? steps : s;
     const int64_t chunk = ceil_div(steps, s) * step;
     p.chunk = (int)(chunk < INT32_MAX / 2 ? chunk : INT32_MAX / 2 / step * step);
