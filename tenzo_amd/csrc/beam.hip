@@ -246,27 +246,36 @@ __device__ __forceinline__ bool before(const BeamCand& a, const BeamCand& b) {
     return a.t < b.t;
 }
 
-// Stage 2, a workgroup per request: the rows' log-sums, then the best k of the slices' lists.
-// As in stage 1 the heads of the lists give a bound that k candidates reach (in fp32, rounded
-// down: it keeps too many rather than too few), and those that do are ranked by counting; where
-// they are many (equal scores, masked beams) the k best are taken one after the other.
+// The 64 largest of two descending lists, a value a lane, in order.
+__device__ __forceinline__ float merge64(float v, float reversed) {
+    v = sort_step<32>(fmaxf(v, reversed));
+    return sort_step<1>(sort_step<2>(sort_step<4>(sort_step<8>(sort_step<16>(v)))));
+}
+
+// Stage 2, a workgroup per request: the rows' log-sums, then the best k of the slices' lists. The
+// first few of every list, 1024 in all, are put in order (sorted by waves, merged in pairs), and
+// their k-th is a bound that k candidates reach (in fp32, rounded down: it keeps too many rather
+// than too few). Those that do are ranked by counting; where they are many (equal scores, masked
+// beams) the k best are taken one after the other.
 __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
     __shared__ double lse[kBeamMax], own[kBeamMax];
     __shared__ double ls[kPickCand];
-    __shared__ float lx[kPickCand], bound[16], tops[64];
-    __shared__ int lw[kPickCand], lt[kPickCand], cnt;
+    __shared__ float lx[kPickCand], tops[16][64];
+    __shared__ int lw[kPickCand], lt[kPickCand], open[kPickCand], cnt, opened;
     __shared__ BeamCand best[16];
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int per = a.ns * a.k, total = a.W * per, lists = a.W * a.ns;
     const float2* cand = a.cand + (int64_t)b * total;
-    const float2 head = tid < lists ? cand[tid * a.k] : make_float2(-INFINITY, 0.0f);
-    constexpr int kOwn = 4;  // a thread's first candidates, on their way during the log-sums
+    const int depth = max(1, min(a.k, 1024 / lists)), first = tid / depth * a.k + tid % depth;
+    const float2 none2 = make_float2(-INFINITY, __int_as_float(INT_MAX));
+    const float2 head = tid < lists * depth ? cand[first] : none2;
+    constexpr int kOwn = 4;  // a thread's candidates where they are few, loaded during the log-sums
+    const bool few = total <= 1024 * kOwn;
     float2 mine[kOwn];
 #pragma unroll
     for (int i = 0; i < kOwn; ++i)
-        mine[i] = tid + 1024 * i < total ? cand[tid + 1024 * i]
-                                         : make_float2(-INFINITY, __int_as_float(INT_MAX));
+        mine[i] = few && tid + 1024 * i < total ? cand[tid + 1024 * i] : none2;
     for (int w = wave; w < a.W; w += 16) {
         const double2* sums = a.sums + ((int64_t)b * a.W + w) * a.ns;
         double m = -INFINITY;
@@ -281,7 +290,7 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
             own[w] = beam_logit(a.scores[b * a.W + w]);
         }
     }
-    if (tid == 0) cnt = 0;
+    if (tid == 0) cnt = opened = 0;
     __syncthreads();
     const auto get = [&](int c, float2 e) {
         BeamCand r;
@@ -292,18 +301,20 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
         return r;
     };
     float top = -INFINITY;
-    if (tid < lists) top = __double2float_rd(get(tid * a.k, head).s);
+    if (tid < lists * depth) top = __double2float_rd(get(first, head).s);
     for (int i = tid + 1024; i < lists; i += 1024)
         top = fmaxf(top, __double2float_rd(get(i * a.k, cand[i * a.k]).s));
-    // two such bounds, the larger one holds: the k-th of a wave's 64 lanes, and the k-th of the
-    // 4 best lanes of every wave
-    const float sorted = sort64_desc(top);
-    if (lane < 4) tops[wave * 4 + lane] = sorted;
-    if (lane == 0) bound[wave] = lane_f(sorted, a.k - 1);
+    float sorted = sort64_desc(top);
+    tops[wave][lane] = sorted;
     __syncthreads();
-    float tau = lane_f(sort64_desc(tops[lane]), a.k - 1);
-#pragma unroll
-    for (int w = 0; w < 16; ++w) tau = fmaxf(tau, bound[w]);
+    for (int half = lists * depth > 512 ? 8 : lists * depth > 128 ? 4 : 1; half > 0; half >>= 1) {
+        if (wave < half) {
+            sorted = merge64(sorted, tops[wave + half][63 - lane]);
+            tops[wave][lane] = sorted;
+        }
+        __syncthreads();
+    }
+    const float tau = tops[0][a.k - 1];
     const auto keep = [&](const BeamCand& c) {
         if (c.t == INT_MAX || __double2float_rd(c.s) < tau) return;
         const int at = atomicAdd(&cnt, 1);
@@ -311,11 +322,22 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
     };
 #pragma unroll
     for (int i = 0; i < kOwn; ++i)
-        if (tid + 1024 * i < total) keep(get(tid + 1024 * i, mine[i]));
-    for (int c = tid + 1024 * kOwn; c < total; c += 1024) keep(get(c, cand[c]));
+        if (few && tid + 1024 * i < total) keep(get(tid + 1024 * i, mine[i]));
+    if (!few) {  // only the lists whose first candidate reaches the bound
+        for (int i = tid; i < lists; i += 1024)
+            if (__double2float_rd(get(i * a.k, cand[i * a.k]).s) >= tau) {
+                const int at = atomicAdd(&opened, 1);
+                if (at < kPickCand) open[at] = i * a.k;
+            }
+        __syncthreads();
+        for (int e = tid; e < min(opened, kPickCand) * a.k; e += 1024) {
+            const int c = open[e / a.k] + e % a.k;
+            keep(get(c, cand[c]));
+        }
+    }
     __syncthreads();
     const int n = cnt;
-    if (n <= kPickCand) {
+    if (n <= kPickCand && opened <= kPickCand) {
         // four lanes to a candidate; equal scores are rare and looked at in full
         const int q = tid & 3;
         for (int i0 = 0; i0 < n; i0 += 256) {
@@ -384,27 +406,24 @@ struct BeamReorder {
 
 constexpr int kPageTokens = 16;
 
-// What slot i of a request takes: from which page to which (in progress), or nothing.
-template <int WMAX>
-struct Moves {
-    int64_t from[WMAX], to[WMAX];  // first row of the pages' planes, -1: stays
-};
-
 // One piece of the page in progress (bytes `at` of pages of `size`), for all slots of a request:
 // every parent's is read before the first is written, so no slot's is lost whatever the
-// permutation, and no two threads touch the same piece.
+// permutation, and no two threads touch the same piece. Lane i of `from` and `to` has slot i's
+// pages, from -1 where it stays.
 template <int WMAX, typename P>
-__device__ __forceinline__ void move_piece(const Moves<WMAX>& m, uint8_t* pool, int64_t size,
+__device__ __forceinline__ void move_piece(int from, int to, uint8_t* pool, int64_t size,
                                            int64_t at) {
     P v[WMAX];
 #pragma unroll
     for (int i = 0; i < WMAX; ++i) {
+        const int page = __builtin_amdgcn_readlane(from, i);
         v[i] = P{};
-        if (m.from[i] >= 0) v[i] = *reinterpret_cast<const P*>(pool + m.from[i] * size + at);
+        if (page >= 0) v[i] = *reinterpret_cast<const P*>(pool + page * size + at);
     }
 #pragma unroll
     for (int i = 0; i < WMAX; ++i)
-        if (m.from[i] >= 0) *reinterpret_cast<P*>(pool + m.to[i] * size + at) = v[i];
+        if (__builtin_amdgcn_readlane(from, i) >= 0)
+            *reinterpret_cast<P*>(pool + __builtin_amdgcn_readlane(to, i) * size + at) = v[i];
 }
 
 // In place: slot i of a request takes the cached tokens of slot parents[i]. The pages that are
@@ -441,20 +460,14 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(BeamReorder a) {
         return;
     }
     if (fill == 0) return;
-    Moves<WMAX> m;
-#pragma unroll
-    for (int i = 0; i < WMAX; ++i) {
-        m.from[i] = m.to[i] = -1;
-        if (i < a.W) {
-            const int par = parents[i];
-            const bool other = par >= 0 && par < a.W && par != i;
-            const int64_t from = table[(other ? par : i) * a.table_stride + full];
-            const int64_t to = table[i * a.table_stride + full];
-            if (other && from >= 0 && from < a.n_blocks && to >= 0 && to < a.n_blocks) {
-                m.from[i] = from * a.planes;
-                m.to[i] = to * a.planes;
-            }
-        }
+    const int slot = threadIdx.x & 63;
+    int from = -1, to = -1;
+    if (slot < a.W) {
+        const int par = parents[slot];
+        const bool other = par >= 0 && par < a.W && par != slot;
+        from = table[(other ? par : slot) * a.table_stride + full];
+        to = table[slot * a.table_stride + full];
+        if (!other || from >= a.n_blocks || to < 0 || to >= a.n_blocks) from = -1;
     }
     const int step = a.copiers * 256, first = blockIdx.x * 256 + threadIdx.x;
     // codes: row_bytes pieces a plane, token by token
@@ -463,15 +476,15 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(BeamReorder a) {
     for (int w = 0; w < 2; ++w)
         for (int p = first; p < pieces; p += step)
             if ((p & (a.row_bytes - 1)) >> (shift - 4) < fill)
-                move_piece<WMAX, uint4>(m, w ? a.codes[1] : a.codes[0], a.row_bytes * kPageTokens,
-                                        (int64_t)p * 16);
+                move_piece<WMAX, uint4>(from, to, w ? a.codes[1] : a.codes[0],
+                                        a.planes * a.row_bytes * kPageTokens, (int64_t)p * 16);
     const int rows = (int)a.planes * kPageTokens;
 #pragma unroll
     for (int w = 0; w < 2; ++w)
         for (int p = first; p < rows; p += step)
             if ((p & (kPageTokens - 1)) < fill)
-                move_piece<WMAX, uint32_t>(m, w ? a.scales[1] : a.scales[0], 4 * kPageTokens,
-                                           (int64_t)p * 4);
+                move_piece<WMAX, uint32_t>(from, to, w ? a.scales[1] : a.scales[0],
+                                           a.planes * 4 * kPageTokens, (int64_t)p * 4);
 }
 
 }  // namespace
