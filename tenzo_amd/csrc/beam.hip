@@ -4,7 +4,8 @@
 // Selection: candidate (w, t) has the score s_w + x_wt - log sum_u exp(x_wu), in 64 bits (two
 // beams' candidates can lie closer than fp32 tells apart); the k largest are taken, among equal
 // ones the lower beam, then the larger logit, then the lower token. So a beam's candidates come
-// in the order of (logit, token) and the first k of each beam hold the answer. A logit that is not below +inf (NaN, +inf) counts as -inf.
+// in the order of (logit, token) and the first k of each beam hold the answer. A logit that is
+// not below +inf (NaN, +inf) counts as -inf.
 #include <climits>
 
 #include "common.h"
@@ -15,6 +16,11 @@ namespace {
 constexpr int kBeamMax = 64;      // beams and candidates, upper bounds
 constexpr int kSliceCand = 1024;  // a slice's candidates in LDS
 constexpr int kPickCand = 512;    // the candidates that the last step ranks
+
+// Up to here a slice's bound is the best of its waves' own, above it that of their merged order:
+// 19 x 16 beams over 154773 logits, 32 candidates, 58 us merged and 70 not, 8 beams over 128256,
+// 64 candidates, 15 and 67; 48 x 8 beams over 128256, 16 candidates, 55.6 and 54.2.
+constexpr int kWaveBound = 16;
 
 struct BeamSelect {
     const float* logits;
@@ -90,19 +96,26 @@ __device__ __forceinline__ float sort64_desc(float v) {
         sort_step<2>(sort_step<4>(sort_step<8>(sort_step<16>(sort_step<63>(v))))));
 }
 
+// The 64 largest of two descending lists, a value a lane, in order.
+__device__ __forceinline__ float merge64(float v, float reversed) {
+    v = sort_step<32>(fmaxf(v, reversed));
+    return sort_step<1>(sort_step<2>(sort_step<4>(sort_step<8>(sort_step<16>(v)))));
+}
+
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 // Stage 1, a workgroup per slice of 256 * E logits of a row, held in registers: the slice's
-// maximum and sum of exponentials, and its k best logits in order. The k-th largest of a wave's
-// 64 lane maxima is a bound that at least k of the slice reach, and the largest of the four
-// waves' bounds keeps the list of those that do short (about 2k of 8192 ordinary logits); the
-// list is put in order by counting. Where too many reach it (equal logits, masked vocabularies:
-// -inf is no bound) the k-th largest is found bit by bit instead, and among its equals the
-// lowest tokens.
+// maximum and sum of exponentials, and its k best logits in order. The k-th largest of 64 lanes'
+// maxima (a wave's, or of the waves' merged order) is a bound that at least k of the slice reach;
+// the list of those that do is short (about 2k of 4096 ordinary logits) and put in order by
+// counting. Where too many reach it (equal logits, masked vocabularies: -inf is no bound) the k-th
+// largest is found bit by bit instead, and among its equals the lowest tokens. Bound by reading
+// the logits, 8 waves a SIMD (64 registers) keep the loads coming: 48 x 8 beams over 128256
+// logits 45 us, 4.4 TB/s.
 template <int E>
 __global__ void __launch_bounds__(256, 8) beam_slice_kernel(BeamSelect a) {
     __shared__ uint64_t list[kSliceCand];
-    __shared__ float bound[4], tops[4];
+    __shared__ float tops[4][64];
     __shared__ double part[4];
     __shared__ int cnt, red[4];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -133,12 +146,18 @@ __global__ void __launch_bounds__(256, 8) beam_slice_kernel(BeamSelect a) {
         v[i] = beam_logit(v[i]);
         top = fmaxf(top, v[i]);
     }
-    const float sorted = sort64_desc(top);
-    const float bw = lane_f(sorted, a.k - 1);
-    if (lane == 0) bound[wave] = bw, tops[wave] = sorted;
+    tops[wave][lane] = sort64_desc(top);
     __syncthreads();
-    const float M = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    const float tau = fmaxf(fmaxf(bound[0], bound[1]), fmaxf(bound[2], bound[3]));
+    const float M = fmaxf(fmaxf(tops[0][0], tops[1][0]), fmaxf(tops[2][0], tops[3][0]));
+    float tau;
+    if (a.k > kWaveBound) {
+        const float lo = merge64(tops[0][lane], tops[1][63 - lane]);
+        const float hi = merge64(tops[2][lane], tops[3][63 - lane]);
+        tau = lane_f(merge64(lo, lane_xor<63>(hi)), a.k - 1);
+    } else {
+        tau = fmaxf(fmaxf(tops[0][a.k - 1], tops[1][a.k - 1]),
+                    fmaxf(tops[2][a.k - 1], tops[3][a.k - 1]));
+    }
     const float ref = M == -INFINITY ? 0.0f : M;
 
     // few terms are added in 32 bits, their sums in 64
@@ -246,17 +265,12 @@ __device__ __forceinline__ bool before(const BeamCand& a, const BeamCand& b) {
     return a.t < b.t;
 }
 
-// The 64 largest of two descending lists, a value a lane, in order.
-__device__ __forceinline__ float merge64(float v, float reversed) {
-    v = sort_step<32>(fmaxf(v, reversed));
-    return sort_step<1>(sort_step<2>(sort_step<4>(sort_step<8>(sort_step<16>(v)))));
-}
-
 // Stage 2, a workgroup per request: the rows' log-sums, then the best k of the slices' lists. The
 // first few of every list, 1024 in all, are put in order (sorted by waves, merged in pairs), and
 // their k-th is a bound that k candidates reach (in fp32, rounded down: it keeps too many rather
 // than too few). Those that do are ranked by counting; where they are many (equal scores, masked
-// beams) the k best are taken one after the other.
+// beams) the k best are taken one after the other. 48 x 8 beams, 32 slices, 16 candidates: 9 us,
+// latency from end to end.
 __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
     __shared__ double lse[kBeamMax], own[kBeamMax];
     __shared__ double ls[kPickCand];
@@ -388,8 +402,11 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
     }
 }
 
-// Logits a thread of stage 1 holds: 16 where that fills the GPU, 8 for few rows.
-int beam_elems(int64_t rows, int64_t V) { return rows * ceil_div(V, 256 * 16) >= 256 ? 16 : 8; }
+// Logits a thread of stage 1 holds: 8 where 16 would leave fewer than four workgroups a CU. 8 x
+// 128256 logits 13.2 us with 8 and 14.7 with 16, 192 x 32089 23.3 and 20.8, 384 x 128256 74 and 54.
+int beam_elems(int64_t rows, int64_t V) {
+    return rows * ceil_div(V, 256 * 16) >= 1024 ? 16 : 8;
+}
 
 // ------------------------------------------------------------- reordering --
 
@@ -431,7 +448,7 @@ __device__ __forceinline__ void move_piece(int from, int to, uint8_t* pool, int6
 // the rows of the page in progress are copied into the slot's own page, in pieces of 16 bytes of
 // codes and 4 of scales. A page's planes lie side by side, so a request's moves are a few long
 // copies; each of its a.copiers workgroups takes pieces in turn (the page numbers, a chain of
-// three loads, are found once for all of them). 48 x 8 beams, 150 planes, 14 rows: 46 us, 4.4 TB/s
+// three loads, are found once for all of them). 48 x 8 beams, 150 planes, 14 rows: 43 us, 4.1 TB/s
 // read and written (a workgroup for every 256 pieces, each finding its pages: 86).
 template <int WMAX>
 __global__ void __launch_bounds__(256) beam_reorder_kernel(BeamReorder a) {

@@ -105,6 +105,25 @@ def test_select_orders(torch_dev, ops, kind, V):
     check(run(torch_dev, ops, x, s, k), x, s, k)
 
 
+@pytest.mark.parametrize("B,W,V,k", [(1, 16, 2723, 32), (3, 16, 70000, 32), (2, 32, 20000, 64),
+                                     (2, 1, 50000, 64), (1, 64, 40000, 64), (2, 5, 90001, 64)])
+@pytest.mark.parametrize("kind", ["alike", "one_beam", "first_step", "one_place"])
+def test_select_many(torch_dev, ops, B, W, V, k, kind):
+    """Many candidates from many lists: of beams alike, of one beam far above the others, of one
+    beam alone, and all side by side in the vocabulary."""
+    print("beam", B, W, V, k, kind, flush=True)
+    rng = np.random.default_rng(V + k)
+    x = (2 * rng.standard_normal((B, W, V))).astype(np.float32)
+    s = (-3 * rng.random((B, W))).astype(np.float32)
+    if kind == "one_beam":
+        s[:, 1:] -= 30
+    elif kind == "first_step":
+        s[:, 1:] = -np.inf
+    elif kind == "one_place":
+        x[:, :, V // 2:V // 2 + k] += 20
+    check(run(torch_dev, ops, x, s, k), x, s, k)
+
+
 def test_select_strides(torch_dev, ops):
     """Rows of a padded vocabulary, at an odd stride and offset."""
     torch = torch_dev
