@@ -7,7 +7,6 @@ namespace tz {
 namespace {
 
 constexpr float kQkScale = 0.08838834764831845f;  // 1/sqrt(128)
-
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kSub = 4;             // 16-token pages of a wave's step
 constexpr int kTile = 16 * kSub;    // tokens of a wave's step
@@ -19,7 +18,6 @@ constexpr int kQStride = 132;       // floats of a query in LDS
 // cores take.
 constexpr int kLowScale = 104, kTopScale = 140;
 constexpr float kWeightBits = 15.0f;  // weights, at most 1, are held times 2^15
-
 
 struct Kv4Attn {
     const void* q;
@@ -118,7 +116,9 @@ __device__ __forceinline__ uint4 fp4_to_half8(uint32_t w, float scale) {
     return f.q;
 }
 // The scale 2^(s - 127) of a byte of kLowScale .. kTopScale, or of less (about 0).
-__device__ __forceinline__ float byte_scale(int s) { return __uint_as_float((uint32_t)max(s, 1) << 23); }
+__device__ __forceinline__ float byte_scale(int s) {
+    return __uint_as_float((uint32_t)max(s, 1) << 23);
+}
 __device__ __forceinline__ float pow2(int e) {  // 2^e, 0 or the largest power where that is beyond
     return e < -126 ? 0.0f : __uint_as_float((uint32_t)(min(e, 127) + 127) << 23);
 }
@@ -147,9 +147,10 @@ __device__ __forceinline__ int piece_at(int row, int p) {
 // Four outputs, the weighted sum over the sum of weights (0 where no token was seen).
 template <bool HALF>
 __device__ __forceinline__ void store4(const Kv4Attn& a, int64_t at, f32x4 v, float l) {
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // (2^-24 of the output; a division each: 1 us)
     float o[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] = l != 0.0f ? v[k] / l : 0.0f;
+    for (int k = 0; k < 4; ++k) o[k] = v[k] * inv;
     if (!a.vec_out) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) st_act<HALF>(a.out, at + k, o[k]);
@@ -176,8 +177,8 @@ __device__ __forceinline__ bool find_unit(const Kv4Seqs& sq, int unit, int G, in
     const int lane = threadIdx.x & 63;
     for (int base = 0; base < sq.B; base += 64) {
         const int b = base + lane;
-        int n = 0;
-        if (b < sq.B) n = max(0, sq.cu[b + 1] - sq.cu[b]);
+        int n = 0, first;
+        if (b < sq.B) n = sq.rows(b, first);
         const int nt = (int)(((int64_t)n * G + RT - 1) / RT);
         int incl = nt;
 #pragma unroll
@@ -204,8 +205,7 @@ constexpr int kStep = 4 * kTile;
 struct SeqWork {
     int first, n, c, steps, tiles;
     __device__ __forceinline__ SeqWork(const Kv4Seqs& sq, int b, int G, int RT) {
-        first = sq.cu ? sq.cu[b] : b;
-        n = sq.cu ? max(0, sq.cu[b + 1] - first) : 1;
+        n = sq.rows(b, first);
         c = sq.length(b);
         steps = (c + kStep - 1) / kStep;
         tiles = (n * G + RT - 1) / RT;
@@ -304,7 +304,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
     // the lane's row
     const int slot = col / ROWS, r = row0 + rw * ROWS + col % ROWS;
     const int qi = a.token(r), head = h * a.G + (r - qi * a.G);
-    const bool row_ok = qi < n && first >= 0 && first + qi < a.T;
+    const bool row_ok = qi < n;
     const int pos = row_ok && c > 0 ? c - n + qi : -1;
     const int64_t grow = (int64_t)first + qi;
 
@@ -327,7 +327,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
 #pragma unroll
     for (int k = 0; k < QT; ++k) {
         const int r2 = min(row0 + wave + 4 * k, last_row), i2 = a.token(r2);
-        const int64_t at = (int64_t)min(max(first + i2, 0), a.T - 1) * a.q_stride +
+        const int64_t at = (int64_t)(first + i2) * a.q_stride +
                            (int64_t)(h * a.G + (r2 - i2 * a.G)) * kKv4Dim + lane;
         x0[k] = ld_act<HALF>(a.q, at);
         x1[k] = ld_act<HALF>(a.q, at + 64);
@@ -432,169 +432,168 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
     __syncthreads();
     // (kMaxPages pages at a time: page numbers in LDS)
     for (int w0 = t0;;) {
-    const int w1 = min(t1, w0 + kMaxPages * kKv4Page);
-    for (; t < w1 && any; t += kTile * TW) {
-        const int next = t + kTile * TW;
-        f32x4 s[kSub];
-        // (the steps outermost: an MFMA waits some 60 cycles for the sum that it adds to, so
-        // neighbours have different ones)
-        float sc[kSub];
-#pragma unroll
-        for (int tt = 0; tt < kSub; ++tt) {
-            sc[tt] = e8m0_to_float(ksc[tt]);
-            s[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-#pragma unroll
-        for (int st = 0; st < 4; ++st) {
-            union {
-                bf16x2 p[4];
-                bf16x8 v;
-            } kf[kSub];
+        const int w1 = min(t1, w0 + kMaxPages * kKv4Page);
+        for (; t < w1 && any; t += kTile * TW) {
+            const int next = t + kTile * TW;
+            f32x4 s[kSub];
+            // (the steps outermost: an MFMA waits some 60 cycles for the sum that it adds to, so
+            // neighbours have different ones)
+            float sc[kSub];
 #pragma unroll
             for (int tt = 0; tt < kSub; ++tt) {
-                const uint32_t w = st == 0 ? kr[tt].x : st == 1 ? kr[tt].y : st == 2 ? kr[tt].z
-                                                                                   : kr[tt].w;
-                kf[tt].p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc[tt], 0);
-                kf[tt].p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc[tt], 1);
-                kf[tt].p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc[tt], 2);
-                kf[tt].p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc[tt], 3);
+                sc[tt] = e8m0_to_float(ksc[tt]);
+                s[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }
 #pragma unroll
-            for (int p = 0; p < NM; ++p)
-#pragma unroll
-                for (int tt = 0; tt < kSub; ++tt)
-                    s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[tt].v, qf[p][st].v, s[tt],
-                                                                    0, 0, 0);
-        }
-        bool bad = false;
-        int id_now[kSub];
-#pragma unroll
-        for (int tt = 0; tt < kSub; ++tt) {
-            id_now[tt] = ((t - t0) >> 4) + tt < pages ? id_next[tt] : -1;
-            bad = bad || id_now[tt] < 0;
-        }
-        if (next < w1) {
-            next_ids(next, w0);
-#pragma unroll
-            for (int tt = 0; tt < kSub; ++tt) load_k(tt, id_next[tt]);
-        }
-        float top = -INFINITY;
-#pragma unroll
-        for (int tt = 0; tt < kSub; ++tt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float v = s[tt][i];
-                if (ROWS == 4) v += ror16<kDppRor8>(v);
-                if (ROWS == 4) v += ror16<kDppRor4>(v);
-                if (ROWS == 8) v += ror16<kDppRor8>(v);
-                s[tt][i] = v;
-            }
-        // a step that a row may not see whole: past its position, or absent pages
-        if (bad || t + kTile - 1 > c - n + a.token(row0)) {
-#pragma unroll
-            for (int tt = 0; tt < kSub; ++tt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (id_now[tt] < 0 || t + 16 * tt + 4 * j + i > pos) s[tt][i] = -INFINITY;
-        }
-#pragma unroll
-        for (int tt = 0; tt < kSub; ++tt)
-            top = fmaxf(top, fmaxf(fmaxf(s[tt][0], s[tt][1]), fmaxf(s[tt][2], s[tt][3])));
-        const float mn = fmaxf(m, max_quarters(top));
-        const float base = mn == -INFINITY ? 0.0f : mn;
-        const float alpha = __builtin_amdgcn_exp2f(m - base);
-        m = mn;
-        if (__ballot(alpha != 1.0f)) {
-#pragma unroll
-            for (int d = 0; d < 8; ++d) acc[d] *= alpha;
-            l *= alpha;
-        }
-#pragma unroll
-        for (int tt = 0; tt < kSub; ++tt)
-        {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[tt][i] = __builtin_amdgcn_exp2f(s[tt][i] - base);
-            l += (s[tt][0] + s[tt][1]) + (s[tt][2] + s[tt][3]);
-        }
-        const uint32_t m1 = slot >= 1 ? 0xffff0000u : 0, m2 = slot >= 2 ? 0xffff0000u : 0;
-#pragma unroll
-        for (int u = 0; u < kSub / 2; ++u) {
-            // 32 value rows, by two 16-token pages
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int tt = 2 * u + k;
-                const float sc = e8m0_to_float(vsc[tt]);
-                const uint32_t w[4] = {vr[tt].x, vr[tt].y, vr[tt].z, vr[tt].w};
-#pragma unroll
-                for (int st = 0; st < 4; ++st) {
-                    union {
-                        bf16x2 p[4];
-                        uint4 v;
-                    } f;
-                    f.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 0);
-                    f.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 1);
-                    f.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 2);
-                    f.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 3);
-                    *reinterpret_cast<uint4*>(vb + wr[st] + k * 16 * kKv4Dim) = f.v;
-                }
-            }
-            if (u == kSub / 2 - 1 && next < w1)
-#pragma unroll
-                for (int tt = 0; tt < kSub; ++tt) load_v(tt, id_next[tt]);
-            Frag pf[NM];
-            float p8[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                p8[e] = s[2 * u + (e >> 2)][e & 3];
-                if (SLOTS > 1) {
-                    p8[e] -= masked(p8[e], m1);
-                    if (NP == 3) p8[e] -= masked(p8[e], m2);
-                }
-            }
-#pragma unroll
-            for (int p = 0; p < NM; ++p)
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    pf[p].w[e >> 1] = pack_hi(p8[e], p8[e + 1]);
-                    p8[e] -= masked(p8[e], 0xffff0000u);
-                    p8[e + 1] -= masked(p8[e + 1], 0xffff0000u);
-                }
-#pragma unroll
-            for (int d0 = 0; d0 < 8; d0 += 4) {
-                typedef __attribute__((address_space(3))) s16x4* lds4;
+            for (int st = 0; st < 4; ++st) {
                 union {
-                    s16x4 h[2];
+                    bf16x2 p[4];
                     bf16x8 v;
-                } vf[4];
+                } kf[kSub];
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    // (lane 4r + i of 16: half a piece of row r, in return for column 4r + i)
-                    uint16_t* src = vb + rd[d] + (d0 >> 2) * 64;
-                    vf[d].h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)src);
-                    vf[d].h[1] =
-                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(src + 16 * kKv4Dim));
+                for (int tt = 0; tt < kSub; ++tt) {
+                    const uint32_t w = st == 0 ? kr[tt].x : st == 1 ? kr[tt].y : st == 2 ? kr[tt].z
+                                                                                       : kr[tt].w;
+                    kf[tt].p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc[tt], 0);
+                    kf[tt].p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc[tt], 1);
+                    kf[tt].p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc[tt], 2);
+                    kf[tt].p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc[tt], 3);
                 }
 #pragma unroll
                 for (int p = 0; p < NM; ++p)
 #pragma unroll
-                    for (int d = 0; d < 4; ++d)
-                        acc[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            vf[d].v, pf[p].v, acc[d0 + d], 0, 0, 0);
+                    for (int tt = 0; tt < kSub; ++tt)
+                        s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            kf[tt].v, qf[p][st].v, s[tt], 0, 0, 0);
+            }
+            bool bad = false;
+            int id_now[kSub];
+#pragma unroll
+            for (int tt = 0; tt < kSub; ++tt) {
+                id_now[tt] = ((t - t0) >> 4) + tt < pages ? id_next[tt] : -1;
+                bad = bad || id_now[tt] < 0;
+            }
+            if (next < w1) {
+                next_ids(next, w0);
+#pragma unroll
+                for (int tt = 0; tt < kSub; ++tt) load_k(tt, id_next[tt]);
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int tt = 0; tt < kSub; ++tt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float v = s[tt][i];
+                    if (ROWS == 4) v += ror16<kDppRor8>(v);
+                    if (ROWS == 4) v += ror16<kDppRor4>(v);
+                    if (ROWS == 8) v += ror16<kDppRor8>(v);
+                    s[tt][i] = v;
+                }
+            // a step that a row may not see whole: past its position, or absent pages
+            if (bad || t + kTile - 1 > c - n + a.token(row0)) {
+#pragma unroll
+                for (int tt = 0; tt < kSub; ++tt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (id_now[tt] < 0 || t + 16 * tt + 4 * j + i > pos) s[tt][i] = -INFINITY;
+            }
+#pragma unroll
+            for (int tt = 0; tt < kSub; ++tt)
+                top = fmaxf(top, fmaxf(fmaxf(s[tt][0], s[tt][1]), fmaxf(s[tt][2], s[tt][3])));
+            const float mn = fmaxf(m, max_quarters(top));
+            const float base = mn == -INFINITY ? 0.0f : mn;
+            const float alpha = __builtin_amdgcn_exp2f(m - base);
+            m = mn;
+            if (__ballot(alpha != 1.0f)) {
+#pragma unroll
+                for (int d = 0; d < 8; ++d) acc[d] *= alpha;
+                l *= alpha;
+            }
+#pragma unroll
+            for (int tt = 0; tt < kSub; ++tt) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[tt][i] = __builtin_amdgcn_exp2f(s[tt][i] - base);
+                l += (s[tt][0] + s[tt][1]) + (s[tt][2] + s[tt][3]);
+            }
+            const uint32_t m1 = slot >= 1 ? 0xffff0000u : 0, m2 = slot >= 2 ? 0xffff0000u : 0;
+#pragma unroll
+            for (int u = 0; u < kSub / 2; ++u) {
+                // 32 value rows, by two 16-token pages
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int tt = 2 * u + k;
+                    const float sc = e8m0_to_float(vsc[tt]);
+                    const uint32_t w[4] = {vr[tt].x, vr[tt].y, vr[tt].z, vr[tt].w};
+#pragma unroll
+                    for (int st = 0; st < 4; ++st) {
+                        union {
+                            bf16x2 p[4];
+                            uint4 v;
+                        } f;
+                        f.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 0);
+                        f.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 1);
+                        f.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 2);
+                        f.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[st], sc, 3);
+                        *reinterpret_cast<uint4*>(vb + wr[st] + k * 16 * kKv4Dim) = f.v;
+                    }
+                }
+                if (u == kSub / 2 - 1 && next < w1)
+#pragma unroll
+                    for (int tt = 0; tt < kSub; ++tt) load_v(tt, id_next[tt]);
+                Frag pf[NM];
+                float p8[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    p8[e] = s[2 * u + (e >> 2)][e & 3];
+                    if (SLOTS > 1) {
+                        p8[e] -= masked(p8[e], m1);
+                        if (NP == 3) p8[e] -= masked(p8[e], m2);
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < NM; ++p)
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        pf[p].w[e >> 1] = pack_hi(p8[e], p8[e + 1]);
+                        p8[e] -= masked(p8[e], 0xffff0000u);
+                        p8[e + 1] -= masked(p8[e + 1], 0xffff0000u);
+                    }
+#pragma unroll
+                for (int d0 = 0; d0 < 8; d0 += 4) {
+                    typedef __attribute__((address_space(3))) s16x4* lds4;
+                    union {
+                        s16x4 h[2];
+                        bf16x8 v;
+                    } vf[4];
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        // (lane 4r + i of 16: half a piece of row r, in return for column 4r + i)
+                        uint16_t* src = vb + rd[d] + (d0 >> 2) * 64;
+                        vf[d].h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)src);
+                        vf[d].h[1] =
+                            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(src + 16 * kKv4Dim));
+                    }
+#pragma unroll
+                    for (int p = 0; p < NM; ++p)
+#pragma unroll
+                        for (int d = 0; d < 4; ++d)
+                            acc[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                vf[d].v, pf[p].v, acc[d0 + d], 0, 0, 0);
+                }
             }
         }
-    }
-    w0 += kMaxPages * kKv4Page;
-    if (w0 >= t1 || !any) break;
-    __syncthreads();
-    stage_pages((w0 - t0) / kKv4Page);
-    __syncthreads();
-    if (t < t1) {
-        next_ids(t, w0);
+        w0 += kMaxPages * kKv4Page;
+        if (w0 >= t1 || !any) break;
+        __syncthreads();
+        stage_pages((w0 - t0) / kKv4Page);
+        __syncthreads();
+        if (t < t1) {
+            next_ids(t, w0);
 #pragma unroll
-        for (int tt = 0; tt < kSub; ++tt) load_k(tt, id_next[tt]);
+            for (int tt = 0; tt < kSub; ++tt) load_k(tt, id_next[tt]);
 #pragma unroll
-        for (int tt = 0; tt < kSub; ++tt) load_v(tt, id_next[tt]);
-    }
+            for (int tt = 0; tt < kSub; ++tt) load_v(tt, id_next[tt]);
+        }
     }
 
     l = sum_quarters(l);
@@ -627,7 +626,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
         for (int it = tid; it < RT * 32; it += 256) {
             const int rr = it >> 5, d4 = it & 31, grp = rr / ROWS, cc = rr % ROWS;
             const int r2 = row0 + rr, i2 = a.token(r2);
-            if (i2 >= n || first < 0 || first + i2 >= a.T) continue;
+            if (i2 >= n) continue;
             float M = -INFINITY, L = 0.0f;
             f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -638,9 +637,9 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
                 const float2 e = sm.ml[w * RW + grp][cc];
                 const float f = __builtin_amdgcn_exp2f(e.x - base);
                 L += e.y * f;
-                v += f * *reinterpret_cast<const f32x4*>(
-                             reinterpret_cast<const float*>(smem + (w * RW + grp) * (32 * kKv4Dim)) +
-                             cc * kKv4Dim + 4 * d4);
+                const float* from =
+                    reinterpret_cast<const float*>(smem + (w * RW + grp) * (32 * kKv4Dim));
+                v += f * *reinterpret_cast<const f32x4*>(from + cc * kKv4Dim + 4 * d4);
             }
             const int64_t g2 = (int64_t)first + i2, hd = h * a.G + (r2 - i2 * a.G);
             if (direct(c - n + i2)) {
@@ -683,8 +682,7 @@ kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
     g.split = rest / sq.Hkv;
     g.h = rest - g.split * sq.Hkv;
     if (!find_unit(sq, unit, a.G, ROWS * RW, g.seq, g.tile)) return;
-    g.first = sq.cu ? sq.cu[g.seq] : g.seq;
-    g.n = sq.cu ? sq.cu[g.seq + 1] - g.first : 1;
+    g.n = sq.rows(g.seq, g.first);
     g.c = sq.length(g.seq);
     g.t0 = g.split * a.chunk;
     g.len = a.chunk;
@@ -697,27 +695,27 @@ constexpr int kRowsRT = 128;
 
 // Sequence and row tile of a work unit of the prompts' kernel, those that see the most tokens first
 // whatever their sequence: tile k of a sequence starts at position length - rows + 128 k / G, and
-// the unit-th largest start is found by bisection (a lane a sequence; one sequence, or over 64 in
-// their order, from the last unit on). 3 prompts of 500 to 2000 tokens, 20 / 5 heads: 103 us, in
-// the order of the rows 119.
+// the unit-th largest start, in 64 tokens, is found by bisection (a lane a sequence; one sequence,
+// or over 64 in their order, from the last unit on). 3 prompts of 500 to 2000 tokens, 20 / 5 heads:
+// 103 us, in the order of the rows 119.
 __device__ __forceinline__ bool find_unit_latest(const Kv4Seqs& sq, int unit, int units, int G,
                                                  int& seq, int& tile) {
     if (!sq.cu || sq.B == 1 || sq.B > 64)
         return find_unit(sq, units - 1 - unit, G, kRowsRT, seq, tile);
     const int lane = threadIdx.x & 63;
-    int n = 0, c = 0;
+    int n = 0, c = 0, first;
     if (lane < sq.B) {
-        n = max(0, sq.cu[lane + 1] - sq.cu[lane]);
+        n = sq.rows(lane, first);
         c = sq.length(lane);
     }
     const int tiles = (int)(((int64_t)n * G + kRowsRT - 1) / kRowsRT), prior = max(c - n, 0);
-    // tiles of the lane's sequence that start past x
+    // tiles of the lane's sequence that start past 64 x
     auto past = [&](int x) {
-        if (x < prior) return tiles;
-        return (int)max((int64_t)tiles - 1 - (int64_t)(x - prior) * G / kRowsRT, (int64_t)0);
+        const int64_t ahead = ((int64_t)x * 64 - prior) * G / kRowsRT;
+        return (int64_t)x * 64 < prior ? tiles : (int)max((int64_t)tiles - 1 - ahead, (int64_t)0);
     };
     if (unit >= wave_sum_i32(tiles)) return false;
-    int lo = 0, hi = max(c, n);  // (no tile starts past the largest)
+    int lo = 0, hi = max(c, n) / 64 + 1;  // (no tile starts past the largest)
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) hi = max(hi, __shfl_xor(hi, d));
     while (lo < hi) {  // the smallest start that at most `unit` tiles lie past
@@ -767,8 +765,8 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
     const int split = rest / sq.Hkv, h = rest - split * sq.Hkv;
     int seq, tile;
     if (!find_unit_latest(sq, nth, a.wgs / per_unit, a.G, seq, tile)) return;
-    const int first = sq.cu ? sq.cu[seq] : seq;
-    const int n = sq.cu ? sq.cu[seq + 1] - first : 1;
+    int first;
+    const int n = sq.rows(seq, first);
     const int c = sq.length(seq);
     const int t0 = split * a.chunk, row0 = tile * kRowsRT;
     const int last_i = min(n - 1, a.token(row0 + kRowsRT - 1));
@@ -801,7 +799,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
     for (int ct = 0; ct < 2; ++ct) {
         const int r = wrow + 16 * ct + col, i = a.token(r);
         head[ct] = h * a.G + (r - i * a.G);
-        row_ok[ct] = i < n && first >= 0 && first + i < a.T;
+        row_ok[ct] = i < n;
         pos[ct] = row_ok[ct] && c > 0 ? c - n + i : -1;
         grow[ct] = (int64_t)first + i;
         // 16 rows by way of the wave's own 8 KB: rows of 512 bytes in, a lane's 32 dims out
@@ -811,7 +809,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
 #pragma unroll
         for (int rr = 0; rr < 16; ++rr) {
             const int r2 = min(wrow + 16 * ct + rr, last_row), i2 = a.token(r2);
-            const int64_t at = (int64_t)min(max(first + i2, 0), a.T - 1) * a.q_stride +
+            const int64_t at = (int64_t)(first + i2) * a.q_stride +
                                (int64_t)(h * a.G + (r2 - i2 * a.G)) * kKv4Dim + lane;
             x0[rr] = ld_act<HALF>(a.q, at);
             x1[rr] = ld_act<HALF>(a.q, at + 64);
@@ -881,7 +879,8 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
     auto load = [&](int t, int w0) {
         const int p = min(((t - w0) >> 4) + wave, pages - 1 - ((w0 - t0) >> 4));
         const int id = __builtin_amdgcn_readfirstlane(pg[p]);
-        const int64_t row = (((int64_t)max(id, 0) * sq.n_layers + sq.layer) * sq.Hkv + h) * kKv4Page;
+        const int64_t row =
+            (((int64_t)max(id, 0) * sq.n_layers + sq.layer) * sq.Hkv + h) * kKv4Page;
         const uint32_t code = (uint32_t)(col * kKv4Row + j * 16), sc = col * kKv4Scales + j;
         kr = *reinterpret_cast<const uint4*>(a.pk + row * kKv4Row + code);
         vr = *reinterpret_cast<const uint4*>(a.pv + row * kKv4Row + code);
@@ -971,6 +970,9 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
             load(next, w0);
         }
         if (t <= high && a.token(wrow) < n) {
+            // (a wave at its products goes first: two of a SIMD then take turns, one at products,
+            // the other at its weights; 512 rows at 8500 tokens 101 us, 105 without)
+            __builtin_amdgcn_s_setprio(1);
             f32x4 s[2][4];
             // (neighbouring MFMAs add to different sums, as above)
 #pragma unroll
@@ -997,6 +999,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
                     s[0][tt] *= f;
                     s[1][tt] *= f;
                 }
+            __builtin_amdgcn_s_setprio(0);
             const bool mask = bad || t + kTile - 1 > low;
 #pragma unroll
             for (int ct = 0; ct < 2; ++ct) {
@@ -1034,6 +1037,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
                 }
                 l[ct] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 Frag16 pf[2][2];  // [column tile][part]
@@ -1071,6 +1075,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
                                     vf[d].v, pf[ct][p].v, acc[ct][d0 + d], 0, 0, 0);
                 }
             }
+            __builtin_amdgcn_s_setprio(0);
         }
         if (next < t1) convert(half ^ 1);
     }
@@ -1111,6 +1116,7 @@ kv4_attn_even_kernel(Kv4Attn a, Kv4Seqs sq) {
     int mine = 0, total;
     for (int b = b0; b < min(sq.B, b0 + per); ++b)
         mine += SeqWork(sq, b, a.G, ROWS).total(sq.Hkv);
+    if (threadIdx.x == 0) at_seq = sq.B;
     int base = block_scan<4>(mine, wsum, total);
     total = uniform(total);
     const int begin = wg_start(blockIdx.x, total, a.wgs);
@@ -1129,7 +1135,7 @@ kv4_attn_even_kernel(Kv4Attn a, Kv4Seqs sq) {
     __syncthreads();
     int b = uniform(at_seq);
     base = uniform(at_base);
-    for (int at = begin; at < end;) {
+    for (int at = begin; at < end && b < sq.B;) {
         const SeqWork w(sq, b, a.G, ROWS);
         const int past = at - base;
         if (past >= w.total(sq.Hkv)) {
@@ -1255,7 +1261,7 @@ __global__ void __launch_bounds__(256) kv4_join_even_kernel(Kv4Attn a, Kv4Seqs s
     int base = block_scan<4>(mine, wsum, total);
     for (int b = b0; b < min(sq.B, b0 + per); ++b) {
         const SeqWork w(sq, b, a.G, ROWS);
-        if (w.first >= 0 && row >= w.first && row < w.first + w.n) at_seq = b, at_base = base;
+        if (row >= w.first && row < w.first + w.n) at_seq = b, at_base = base;
         base += w.total(sq.Hkv);
     }
     __syncthreads();
@@ -1291,13 +1297,24 @@ Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, boo
     const int64_t per = cu ? ceil_div(T * G, B) : G;  // rows of an average sequence
     const int packed = half ? 8 : 4;
     p.rows = per <= packed ? packed : 16;
-    p.rw = per <= 16 ? 1 : per <= 32 ? 2 : per <= 64 ? 4 : 8;
+    const int64_t ctx = (int64_t)table_width * kKv4Page;
+    // Rows of a workgroup: 16 against 256 tokens at a time spread few rows over the GPU; the
+    // prompts' kernel, once it has work for a while (16 us go into its queries and outputs), reads
+    // and converts a token once for 128; between, many rows of few tokens, 32. Measured in us, 20 /
+    // 5 heads, 16 rows | 32 | 128: a prompt of 100 tokens 7.5 | 8.9 | 21, one of 1000 38 | 34 | 44,
+    // 32 of up to 128 44 | 32 | 21; 128 tokens after 4000 33 | 37 | 38, 200 after 7800 63 | 66 |
+    // 56, 512 after 8000 160 | 200 | 102.
+    const double units128 = (double)T * G * Hkv / kRowsRT;
+    p.rw = 1;
+    if (per > 64 && (units128 > 320 || units128 * ctx > 3500 * kTile))
+        p.rw = 8;
+    else if (per > 16 && T * G / 16 * Hkv > 512 && ctx <= 1024)
+        p.rw = 2;
     const int rt = p.rows * p.rw;
     const int64_t units = cu ? T * G / rt + B : (int64_t)B * ceil_div(G, rt);
-    const int64_t ctx = (int64_t)table_width * kKv4Page;
     const int64_t step = p.rw > 4 ? kTile : kTile * (4 / p.rw);
     const int64_t steps = ctx > 0 ? ceil_div(ctx, step) : 1;
-    const int room = 768;  // workgroups that the GPU holds at once, three a CU
+    const int room = p.rows == 16 ? 512 : 768;  // workgroups that the GPU holds at once
     const int64_t most = units * Hkv * (steps + 1);
     // Units that fill the GPU twice over are balanced by its own scheduling, and where every
     // workgroup has a step at most there is nothing to balance. Between: 48 sequences of up to 8190
@@ -1311,10 +1328,13 @@ Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, boo
         return p;
     }
     const int64_t likely = cu ? (ceil_div(T * G, rt) > B ? ceil_div(T * G, rt) : B) : units;
-    int64_t s = (p.rw > 4 ? 512 : room) / (likely * Hkv);  // (the prompts' kernel: two a CU)
-    s = s < 1 ? 1 : s > steps ? steps : s;
-    const int64_t chunk = ceil_div(steps, s) * step;
-    p.chunk = (int)(chunk < INT32_MAX / 2 ? chunk : INT32_MAX / 2 / step * step);
+    // (of a prompt's splits, those past its earlier rows have nothing to do)
+    const double own = ctx > 0 ? (double)T / B / ctx : 0.0;  // of a sequence's tokens, its rows'
+    const double some = 1.0 - 0.5 * (own < 1.0 ? own : 1.0);
+    const double fits = (double)room / (likely * Hkv);
+    int64_t s = fits > 1.0 ? 1 + (int64_t)((fits - 1.0) / some) : 1;
+    s = s > steps ? steps : s;
+    p.chunk = (int)(ceil_div(steps, s) * step);
     p.splits = ctx > 0 ? (int)ceil_div(ctx, p.chunk) : 1;
     p.wgs = units * p.splits * Hkv;
     p.records = p.splits > 1 ? (size_t)T * G * Hkv * p.splits : 0;
@@ -1350,8 +1370,6 @@ int launch_kv4_plan(const Kv4Plan& p, const Kv4Attn& a, const Kv4Seqs& s, hipStr
         launch_kv4<16, NP, 1, HALF>(a, s, st);
     else if (p.rw == 2)
         launch_kv4<16, NP, 2, HALF>(a, s, st);
-    else if (p.rw == 4)
-        launch_kv4<16, NP, 4, HALF>(a, s, st);
     else
         hipLaunchKernelGGL(kv4_attn_rows_kernel<HALF>, dim3(a.wgs), dim3(256), 0, st, a, s);
     const int rc = launch_status("kv4_attn_kernel");

@@ -36,7 +36,9 @@ struct BeamSelect {
 };
 
 // NaN and +inf count as -inf; -0 as 0.
-__device__ __forceinline__ float beam_logit(float x) { return (x < INFINITY ? x : -INFINITY) + 0.0f; }
+__device__ __forceinline__ float beam_logit(float x) {
+    return (x < INFINITY ? x : -INFINITY) + 0.0f;
+}
 
 // Bits in the order of the values.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -250,7 +252,8 @@ __global__ void __launch_bounds__(256, 8) beam_slice_kernel(BeamSelect a) {
             a.cand[at * a.k + rank] = make_float2(
                 from_ordered((uint32_t)(me >> 32)), __int_as_float(INT_MAX - (int)(uint32_t)me));
     }
-    if (tid >= n && tid < a.k) a.cand[at * a.k + tid] = make_float2(-INFINITY, __int_as_float(INT_MAX));
+    if (tid >= n && tid < a.k)
+        a.cand[at * a.k + tid] = make_float2(-INFINITY, __int_as_float(INT_MAX));
 }
 
 struct BeamCand {

@@ -22,20 +22,30 @@ constexpr int kKv4Scales = 4;  // scale bytes of a row
 // The sequences of a call. Row r of the T rows belongs to sequence s with cu[s] <= r < cu[s + 1]
 // (cu null: row r is sequence r's only one) and stands at position ctx[s] - n + (r - cu[s]), n
 // the sequence's rows. What the device finds in these arrays is checked before it is used: a
-// length above `limit` (the table's width, the rotation's rows) counts as 0, a page outside the
-// pool as absent.
+// length above `limit` (the table's width, the rotation's rows) counts as 0, a range outside the T
+// rows as empty, a page outside the pool as absent.
 struct Kv4Seqs {
     const int32_t* tables;
     const int32_t* ctx;
     const int32_t* cu;
     int64_t table_stride;
     int64_t n_blocks;
-    int B, limit;
+    int B, limit, T;
     int n_layers, layer, Hkv;
 
     __device__ __forceinline__ int length(int s) const {
         const int c = ctx[s];
         return c > 0 && c <= limit ? c : 0;
+    }
+    // Rows of sequence s (none where cu has no range of the T rows there), and its first.
+    __device__ __forceinline__ int rows(int s, int& first) const {
+        if (!cu) {
+            first = s;
+            return 1;
+        }
+        const int begin = cu[s], end = cu[s + 1];
+        first = begin;
+        return begin >= 0 && end > begin && end <= T ? end - begin : 0;
     }
     // Row (of 16-token pages) of head 0 in logical page `p` of sequence s, or -1.
     __device__ __forceinline__ int64_t page_base(int s, int p) const {
@@ -64,8 +74,8 @@ __device__ __forceinline__ bool kv4_place(const Kv4Seqs& q, int r, int lane16, i
     if (q.cu) {
         seq = kv4_seq_of_row(q, r, lane16);
         if (seq >= q.B) return false;
-        const int first = q.cu[seq];
-        n = q.cu[seq + 1] - first;
+        int first;
+        n = q.rows(seq, first);
         i = r - first;
     }
     const int c = q.length(seq);

@@ -174,7 +174,7 @@ int kv4_check(const char* what, const void* pk, const void* pv, const void* pks,
              n_layers);
     TZ_CHECK(n_blocks >= 0 && n_blocks <= INT32_MAX, "%s: %lld blocks", what,
              (long long)n_blocks);
-    TZ_CHECK(table_width >= 0 && table_width <= INT32_MAX / kKv4Page &&
+    TZ_CHECK(table_width >= 0 && table_width <= (1 << 26) &&
                  (table_stride >= table_width || B <= 1),
              "%s: block tables of %d pages, %lld apart", what, table_width,
              (long long)table_stride);
@@ -186,6 +186,7 @@ int kv4_check(const char* what, const void* pk, const void* pv, const void* pks,
     q.table_stride = table_stride;
     q.n_blocks = n_blocks;
     q.B = B;
+    q.T = (int)T;
     q.limit = table_width * kKv4Page;
     if (rope_cs && n_pos < q.limit) q.limit = n_pos;
     q.n_layers = n_layers;
