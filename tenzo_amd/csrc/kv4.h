@@ -54,16 +54,18 @@ struct Kv4Seqs {
     }
 };
 
-// The sequence of row r: how many of cu[1 .. B] are <= r, counted by the 16 lanes of a DPP row
-// (all of them active and with the same r). B or a sequence whose range does not hold r: none.
+// The sequence whose range holds row r, looked for by the 16 lanes of a DPP row (all of them
+// active and with the same r); -1: none.
 __device__ __forceinline__ int kv4_seq_of_row(const Kv4Seqs& q, int r, int lane16) {
-    int n = 0;
-    for (int b = lane16; b < q.B; b += 16) n += q.cu[b + 1] <= r ? 1 : 0;
-    n += dpp_i<kDppXor1>(n);
-    n += dpp_i<kDppXor2>(n);
-    n += dpp_i<kDppHalfMirror>(n);
-    n += dpp_i<kDppMirror>(n);
-    return n;
+    int s = -1, first;
+    for (int b = lane16; b < q.B; b += 16) {
+        const int n = q.rows(b, first);
+        if (r >= first && r < first + n) s = b;
+    }
+    s = max(s, dpp_i<kDppXor1>(s));
+    s = max(s, dpp_i<kDppXor2>(s));
+    s = max(s, dpp_i<kDppHalfMirror>(s));
+    return max(s, dpp_i<kDppMirror>(s));
 }
 
 // Position of row r and its sequence; false where it stands nowhere (padding).
@@ -73,7 +75,7 @@ __device__ __forceinline__ bool kv4_place(const Kv4Seqs& q, int r, int lane16, i
     seq = r;
     if (q.cu) {
         seq = kv4_seq_of_row(q, r, lane16);
-        if (seq >= q.B) return false;
+        if (seq < 0) return false;
         int first;
         n = q.rows(seq, first);
         i = r - first;
