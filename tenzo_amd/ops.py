@@ -12,6 +12,7 @@ libtenzo_hip.so on the current torch stream; tensors must live on the GPU.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -242,6 +243,16 @@ KV4_PAGE = 16
 _dev = torch._C._cuda_getDevice
 
 
+@functools.lru_cache(4096)
+def _attn_kv4_ws(*args: int) -> int:
+    return _lib.load().tenzo_hip_attn_kv4_ws_bytes(*args)
+
+
+@functools.lru_cache(4096)
+def _beam_select_ws(*args: int) -> int:
+    return _lib.load().tenzo_hip_beam_select_ws_bytes(*args)
+
+
 def _on(t: torch.Tensor, dev: int, dtype: torch.dtype, name: str) -> int:
     """The address of a tensor of the current device (the kernels run on its stream)."""
     if t.get_device() != dev:
@@ -275,9 +286,10 @@ def kv4_pool(n_blocks: int, n_layers: int, n_kv_heads: int, device="cuda"):
                  for w in (64, 64, 4, 4))
 
 
-# (The calls on a cache check a dozen tensors, and the smallest run for 3 us on the GPU: each
+# (The calls on a cache check a dozen tensors, and the smallest run for 4 us on the GPU: each
 # property is asked for once and the words for what is wrong are looked for afterwards. Host side
-# of a call, us, checked tensor by tensor | so: append 13.8 | 8.0, attn 19.5 | 12.2.)
+# of a call: append 9 us, attn 16, select 14 (two launches each), reorder 8; the sizes of workspaces, a function of
+# the arguments, are asked for once.)
 _U8, _I32, _F32 = torch.uint8, torch.int32, torch.float32
 
 
@@ -399,7 +411,7 @@ def attn_kv4(q, pk, pv, pks, pvs, block_tables, ctx_lens, layer: int, rope_cs=No
         return out
     L, Hq = _lib.load(), cols // 128
     os = _row_stride(out, cols, "out")
-    nbytes = L.tenzo_hip_attn_kv4_ws_bytes(T, seqs[5], Hq, Hkv, seqs[2], cu_q is not None, dt)
+    nbytes = _attn_kv4_ws(T, seqs[5], Hq, Hkv, seqs[2], cu_q is not None, dt)
     ws = pk.new_empty(nbytes) if nbytes else None  # (held until the launch)
     _lib.check(L.tenzo_hip_attn_kv4(
         _on(q, dev, q.dtype, "q"), dt, qs, *pools, *where[:3], Hq, Hkv, *seqs,
@@ -537,10 +549,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int):
     lp = _on(logits, dev, torch.float32, "logits")
     sp = _whole(scores, dev, torch.float32, "scores")
     L = _lib.load()
-    nbytes = L.tenzo_hip_beam_select_ws_bytes(B, W, V, k)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
-    out = torch.empty((B, k), dtype=torch.float32, device=logits.device)
-    beams = torch.empty((B, k), dtype=torch.int32, device=logits.device)
+    nbytes = _beam_select_ws(B, W, V, k)
+    ws = logits.new_empty(nbytes // 4)  # (whole numbers of 8 bytes; held until the launch)
+    out = scores.new_empty((B, k))
+    beams = torch.empty_like(out, dtype=torch.int32)
     tokens = torch.empty_like(beams)
     _lib.check(L.tenzo_hip_beam_select(lp, ld, sp, B, W, V, k, out.data_ptr(), beams.data_ptr(),
                                        tokens.data_ptr(), ws.data_ptr(), nbytes, _stream()),
