@@ -1178,18 +1178,17 @@ template <bool HALF, int GROUPS>
 __device__ __forceinline__ void kv4_join(const Kv4Attn& a, const Records& rc, int64_t out_at, int g,
                                          f32x4 (*ov)[32], float* lv) {
     const int lane = threadIdx.x & 63, d4 = threadIdx.x & 31;
-    constexpr int kAhead = 4;  // a group's first sums on their way while the maximum is found
+    // a group's first sums are on their way while the maximum is found
+    constexpr int kAhead = GROUPS > 1 ? 1 : 6;
     f32x4 pv[kAhead];
     float2 pe[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
         const int s = g + GROUPS * k;
-        pv[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        pe[k] = make_float2(-INFINITY, 0.0f);
-        if (s < rc.ns) {
-            pv[k] = *reinterpret_cast<const f32x4*>(a.part_o + rc.at(s) * kKv4Dim + 4 * d4);
-            pe[k] = a.part_ml[rc.at(s)];
-        }
+        const int64_t at = rc.at(min(s, rc.ns - 1));  // (no load under a condition)
+        pv[k] = *reinterpret_cast<const f32x4*>(a.part_o + at * kKv4Dim + 4 * d4);
+        pe[k] = a.part_ml[at];
+        if (s >= rc.ns) pe[k] = make_float2(-INFINITY, 0.0f);
     }
     float M = -INFINITY;
     if (GROUPS > 1) {
