@@ -970,9 +970,6 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
             load(next, w0);
         }
         if (t <= high && a.token(wrow) < n) {
-            // (a wave at its products goes first: two of a SIMD then take turns, one at products,
-            // the other at its weights; 512 rows at 8500 tokens 101 us, 105 without)
-            __builtin_amdgcn_s_setprio(1);
             f32x4 s[2][4];
             // (neighbouring MFMAs add to different sums, as above)
 #pragma unroll
@@ -999,8 +996,8 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
                     s[0][tt] *= f;
                     s[1][tt] *= f;
                 }
-            __builtin_amdgcn_s_setprio(0);
             const bool mask = bad || t + kTile - 1 > low;
+            float shift[2];
 #pragma unroll
             for (int ct = 0; ct < 2; ++ct) {
                 if (mask)
@@ -1021,28 +1018,34 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
                 const float base = mn == -INFINITY ? 0.0f : mn;
                 const float alpha = __builtin_amdgcn_exp2f(m[ct] - base);
                 m[ct] = mn;
+                shift[ct] = kWeightBits - base;
                 if (__ballot(alpha != 1.0f)) {
 #pragma unroll
                     for (int d = 0; d < 8; ++d) acc[ct][d] *= alpha;
                     l[ct] *= alpha;
                 }
-                float sum[4];
-#pragma unroll
-                for (int tt = 0; tt < 4; ++tt) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        s[ct][tt][i] = __builtin_amdgcn_exp2f(
-                            __builtin_fmaf(s[ct][tt][i], unit[ct], kWeightBits - base));
-                    sum[tt] = (s[ct][tt][0] + s[ct][tt][1]) + (s[ct][tt][2] + s[ct][tt][3]);
-                }
-                l[ct] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
-            __builtin_amdgcn_s_setprio(1);
+            // (parts of tokens are alike: a wave at its products goes first, and the two of a SIMD
+            // take turns. 512 rows after 8000 tokens 95 us, 104 without; whole prompts of up to
+            // 2000 tokens, which are not alike, 103.4 and 101.9.)
+            if (a.splits > 1) __builtin_amdgcn_s_setprio(1);
+            // (the weights of the second 32 tokens between the products of the first)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 Frag16 pf[2][2];  // [column tile][part]
 #pragma unroll
-                for (int ct = 0; ct < 2; ++ct)
+                for (int ct = 0; ct < 2; ++ct) {
+                    float sum[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        f32x4& w = s[ct][2 * u + k];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            w[i] = __builtin_amdgcn_exp2f(
+                                __builtin_fmaf(w[i], unit[ct], shift[ct]));
+                        sum[k] = (w[0] + w[1]) + (w[2] + w[3]);
+                    }
+                    l[ct] += sum[0] + sum[1];
 #pragma unroll
                     for (int e = 0; e < 8; e += 2) {
                         const float p0 = s[ct][2 * u + (e >> 2)][e & 3];
@@ -1051,6 +1054,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
                         pf[ct][0].w[e >> 1] = hi;
                         pf[ct][1].w[e >> 1] = pack16(rest_lo(p0, hi), rest_hi(p1, hi));
                     }
+                }
 #pragma unroll
                 for (int d0 = 0; d0 < 8; d0 += 4) {
                     typedef __attribute__((address_space(3))) s16x4* lds4;
@@ -1075,7 +1079,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
                                     vf[d].v, pf[ct][p].v, acc[ct][d0 + d], 0, 0, 0);
                 }
             }
-            __builtin_amdgcn_s_setprio(0);
+            if (a.splits > 1) __builtin_amdgcn_s_setprio(0);
         }
         if (next < t1) convert(half ^ 1);
     }
