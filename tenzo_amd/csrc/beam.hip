@@ -269,11 +269,11 @@ __device__ __forceinline__ bool before(const BeamCand& a, const BeamCand& b) {
 }
 
 // Stage 2, a workgroup per request: the rows' log-sums, then the best k of the slices' lists. The
-// first few of every list, 1024 in all, are put in order (sorted by waves, merged in pairs), and
-// their k-th is a bound that k candidates reach (in fp32, rounded down: it keeps too many rather
-// than too few). Those that do are ranked by counting; where they are many (equal scores, masked
-// beams) the k best are taken one after the other. 48 x 8 beams, 32 slices, 16 candidates: 9 us,
-// latency from end to end.
+// first few of every list (2k of a beam's or more, up to 1024 in all) are put in order (sorted by
+// waves, merged in pairs), and their k-th is a bound that k candidates reach (in fp32, rounded
+// down: it keeps too many rather than too few). Those that do are ranked by counting; where they
+// are many (equal scores, masked beams) the k best are taken one after the other. 48 x 8 beams, 32
+// slices, 16 candidates: 9 us, latency from end to end.
 __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
     __shared__ double lse[kBeamMax], own[kBeamMax];
     __shared__ double ls[kPickCand];
@@ -284,27 +284,30 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int per = a.ns * a.k, total = a.W * per, lists = a.W * a.ns;
     const float2* cand = a.cand + (int64_t)b * total;
-    const int depth = max(1, min(a.k, 1024 / lists)), first = tid / depth * a.k + tid % depth;
-    const float2 none2 = make_float2(-INFINITY, __int_as_float(INT_MAX));
-    const float2 head = tid < lists * depth ? cand[first] : none2;
+    const int depth = max(1, min(min(a.k, 1024 / lists), (2 * a.k + a.ns - 1) / a.ns));
+    const int heads = lists * depth, first = min(tid, heads - 1) / depth * a.k + tid % depth;
+    // (loads whose places are clamped, none under a condition, where it would be waited for)
+    const float2 head = cand[first];
     constexpr int kOwn = 4;  // a thread's candidates where they are few, loaded during the log-sums
     const bool few = total <= 1024 * kOwn;
     float2 mine[kOwn];
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i)
-        mine[i] = few && tid + 1024 * i < total ? cand[tid + 1024 * i] : none2;
+    for (int i = 0; i < kOwn; ++i) mine[i] = cand[min(tid + 1024 * i, total - 1)];
     for (int w = wave; w < a.W; w += 16) {
         const double2* sums = a.sums + ((int64_t)b * a.W + w) * a.ns;
-        double m = -INFINITY;
-        for (int i = lane; i < a.ns; i += 64) m = fmax(m, sums[i].x);
+        const float score = a.scores[b * a.W + w];
+        double2 e = sums[min(lane, a.ns - 1)];
+        if (lane >= a.ns) e.x = -INFINITY;
+        double m = e.x;
+        for (int i = lane + 64; i < a.ns; i += 64) m = fmax(m, sums[i].x);
         for (int d = 32; d > 0; d >>= 1) m = fmax(m, __shfl_xor(m, d));
-        double s = 0.0;
-        for (int i = lane; i < a.ns; i += 64)
+        double s = e.x > -INFINITY ? e.y * exp(e.x - m) : 0.0;
+        for (int i = lane + 64; i < a.ns; i += 64)
             if (sums[i].x > -INFINITY) s += sums[i].y * exp(sums[i].x - m);
         for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
         if (lane == 0) {
             lse[w] = m > -INFINITY ? m + log(s) : 0.0;
-            own[w] = beam_logit(a.scores[b * a.W + w]);
+            own[w] = beam_logit(score);
         }
     }
     if (tid == 0) cnt = opened = 0;
@@ -318,13 +321,13 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
         return r;
     };
     float top = -INFINITY;
-    if (tid < lists * depth) top = __double2float_rd(get(first, head).s);
+    if (tid < heads) top = __double2float_rd(get(first, head).s);
     for (int i = tid + 1024; i < lists; i += 1024)
         top = fmaxf(top, __double2float_rd(get(i * a.k, cand[i * a.k]).s));
     float sorted = sort64_desc(top);
     tops[wave][lane] = sorted;
     __syncthreads();
-    for (int half = lists * depth > 512 ? 8 : lists * depth > 128 ? 4 : 1; half > 0; half >>= 1) {
+    for (int half = heads > 512 ? 8 : heads > 128 ? 4 : 1; half > 0; half >>= 1) {
         if (wave < half) {
             sorted = merge64(sorted, tops[wave + half][63 - lane]);
             tops[wave][lane] = sorted;
