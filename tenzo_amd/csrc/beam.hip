@@ -80,6 +80,31 @@ __device__ __forceinline__ float lane_xor(float v) {
     }
 }
 
+template <int M>
+__device__ __forceinline__ double lane_xor(double v) {
+    const uint64_t b = __double_as_longlong(v);
+    const uint32_t lo = __float_as_uint(lane_xor<M>(__uint_as_float((uint32_t)b)));
+    const uint32_t hi = __float_as_uint(lane_xor<M>(__uint_as_float((uint32_t)(b >> 32))));
+    return __longlong_as_double((uint64_t)hi << 32 | lo);
+}
+// Over the 64 lanes, in all of them.
+__device__ __forceinline__ double lanes_sum(double v) {
+    v += lane_xor<32>(v);
+    v += lane_xor<16>(v);
+    v += lane_xor<8>(v);
+    v += lane_xor<4>(v);
+    v += lane_xor<2>(v);
+    return v + lane_xor<1>(v);
+}
+__device__ __forceinline__ double lanes_max(double v) {
+    v = fmax(v, lane_xor<32>(v));
+    v = fmax(v, lane_xor<16>(v));
+    v = fmax(v, lane_xor<8>(v));
+    v = fmax(v, lane_xor<4>(v));
+    v = fmax(v, lane_xor<2>(v));
+    return fmax(v, lane_xor<1>(v));
+}
+
 // One step of a descending bitonic sort over the 64 lanes: lane l and l ^ M, the one without
 // the mask's top bit keeps the larger.
 template <int M>
@@ -172,7 +197,7 @@ __global__ void __launch_bounds__(256, 8) beam_slice_kernel(BeamSelect a) {
             e[c] = __builtin_amdgcn_exp2f((v[i + c] - ref) * 1.4426950408889634f);
         sum += (double)(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])));
     }
-    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+    sum = lanes_sum(sum);
     if (lane == 0) part[wave] = sum;
 
     const auto token = [&](int i) { return base + 1024 * (i / 4) + i % 4; };
@@ -300,11 +325,11 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
         if (lane >= a.ns) e.x = -INFINITY;
         double m = e.x;
         for (int i = lane + 64; i < a.ns; i += 64) m = fmax(m, sums[i].x);
-        for (int d = 32; d > 0; d >>= 1) m = fmax(m, __shfl_xor(m, d));
+        m = lanes_max(m);
         double s = e.x > -INFINITY ? e.y * exp(e.x - m) : 0.0;
         for (int i = lane + 64; i < a.ns; i += 64)
             if (sums[i].x > -INFINITY) s += sums[i].y * exp(sums[i].x - m);
-        for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
+        s = lanes_sum(s);
         if (lane == 0) {
             lse[w] = m > -INFINITY ? m + log(s) : 0.0;
             own[w] = beam_logit(score);
