@@ -539,12 +539,13 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int):
     larger logit, then the lower token comes first. NaN and +inf count as -inf, which comes
     last."""
     dev = _dev()
-    if logits.dim() != 3 or scores.shape != logits.shape[:2]:
-        raise ValueError(f"logits [B][W][V] and scores [B][W]: {tuple(logits.shape)}, "
+    shape = logits.shape
+    if len(shape) != 3 or scores.shape != shape[:2]:
+        raise ValueError(f"logits [B][W][V] and scores [B][W]: {tuple(shape)}, "
                          f"{tuple(scores.shape)}")
-    B, W, V = logits.shape
-    ld = logits.stride(1) if W > 1 else logits.stride(0) if B > 1 else V
-    if (V > 1 and logits.stride(2) != 1) or (B > 1 and logits.stride(0) != W * ld):
+    (B, W, V), (between, ld, step) = shape, logits.stride()
+    ld = ld if W > 1 else between if B > 1 else V
+    if (V > 1 and step != 1) or (B > 1 and between != W * ld):
         raise ValueError(f"logits: strides {logits.stride()}")
     lp = _on(logits, dev, torch.float32, "logits")
     sp = _whole(scores, dev, torch.float32, "scores")
