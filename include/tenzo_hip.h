@@ -246,7 +246,9 @@ TENZO_HIP_API int tenzo_hip_kv4_read(const uint8_t* pk, const uint8_t* pv, const
  * apart, rotated at their positions; row r's head h attends with scale
  * 1/sqrt(128) to kv head h / (Hq/Hkv) at positions 0 .. its own (the cache has
  * to hold them: append first), out likewise out_stride apart. A row that sees
- * no token is zero. Hq / Hkv 1 to 16. out must not overlap q. ws: a workspace
+ * no token is zero; sums are held in fp32 until they are divided, so scores or
+ * sums of weighted values past its range give infinities and NaN in the rows
+ * concerned. Hq / Hkv 1 to 16. out must not overlap q. ws: a workspace
  * of tenzo_hip_attn_kv4_ws_bytes(...) bytes, 16-byte aligned, of this call
  * alone until it has run (null where that is 0); has_cu: cu_q is not null. The
  * split of rows and tokens over workgroups follows from T, B, the heads, the
