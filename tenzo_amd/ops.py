@@ -393,8 +393,8 @@ def attn_kv4(q, pk, pv, pks, pvs, block_tables, ctx_lens, layer: int, rope_cs=No
     """Attention over a paged cache in 4 bits: q [T][Hq*128] (or [T][Hq][128]) fp32 or fp16,
     rotated at its rows' positions (rope_cs, None: not), each row attending to the positions
     up to its own; the other arguments as kv4_append, which comes first. Returns out like q
-    (into `out` when given: rows behind the last sequence stay as they are; they are not
-    initialised otherwise). Rows that see no token are zeros."""
+    (into `out` when given, which must not overlap q: rows behind the last sequence stay as they
+    are; they are not initialised otherwise). Rows that see no token are zeros."""
     dev = _dev()
     T = q.shape[0]
     pools, where, seqs = _kv4_cache(pk, pv, pks, pvs, block_tables, ctx_lens, cu_q, layer, T, dev)
