@@ -15,6 +15,7 @@ namespace {
 
 constexpr int kBeamMax = 64;      // beams and candidates, upper bounds
 constexpr int kSliceCand = 1024;  // a slice's candidates in LDS
+constexpr int kSliceFew = 256;    // logits above -inf that are put in order as they are
 constexpr int kPickCand = 512;    // the candidates that the last step ranks
 
 // Up to here a slice's bound is the best of its waves' own, above it that of their merged order:
@@ -135,10 +136,10 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 // maximum and sum of exponentials, and its k best logits in order. The k-th largest of 64 lanes'
 // maxima (a wave's, or of the waves' merged order) is a bound that at least k of the slice reach;
 // the list of those that do is short (about 2k of 4096 ordinary logits) and put in order by
-// counting. Where too many reach it (equal logits, masked vocabularies: -inf is no bound) the k-th
-// largest is found bit by bit instead, and among its equals the lowest tokens. Bound by reading
-// the logits, 8 waves a SIMD (64 registers) keep the loads coming: 48 x 8 beams over 128256
-// logits 45 us, 4.4 TB/s.
+// counting. Where too many reach it (equal logits, masked vocabularies: -inf is no bound) and
+// more than 256 are above -inf the k-th largest is found bit by bit instead, and among its equals
+// the lowest tokens. Bound by reading the logits, 8 waves a SIMD (64 registers) keep the loads
+// coming: 48 x 8 beams over 128256 logits 45 us, 4.4 TB/s.
 template <int E>
 __global__ void __launch_bounds__(256, 8) beam_slice_kernel(BeamSelect a) {
     __shared__ uint64_t list[kSliceCand];
@@ -231,7 +232,9 @@ __global__ void __launch_bounds__(256, 8) beam_slice_kernel(BeamSelect a) {
         }
         const int want = min(a.k, total(mine));
         uint32_t bar = ordered(-INFINITY);
-        if (total(real) >= want) {  // the want-th largest value, from its highest bit on
+        real = total(real);
+        // the want-th largest value, from its highest bit on; a few are listed all
+        if (real >= want && real > kSliceFew) {
             bar = 0;
             for (int bit = 31; bit >= 0; --bit) {
                 const uint32_t up = bar | 1u << bit;
@@ -248,15 +251,18 @@ __global__ void __launch_bounds__(256, 8) beam_slice_kernel(BeamSelect a) {
         const int need = want - total(c);
         // its equals below token `until` are the ones needed
         const int from = slice * (256 * E);
-        int below = 0;
-        for (int step = 256 * E; step > 0; step >>= 1) {
-            c = 0;
+        int until = from;
+        if (need > 0) {
+            int below = 0;
+            for (int step = 256 * E; step > 0; step >>= 1) {
+                c = 0;
 #pragma unroll
-            for (int i = 0; i < E; ++i)
-                c += v[i] == least && token(i) < a.V && token(i) < from + below + step ? 1 : 0;
-            if (total(c) < need) below += step;
+                for (int i = 0; i < E; ++i)
+                    c += v[i] == least && token(i) < a.V && token(i) < from + below + step ? 1 : 0;
+                if (total(c) < need) below += step;
+            }
+            until = from + below + 1;
         }
-        const int until = from + below + 1;
         __syncthreads();
         if (tid == 0) cnt = 0;
         __syncthreads();

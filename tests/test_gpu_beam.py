@@ -124,6 +124,23 @@ def test_select_many(torch_dev, ops, B, W, V, k, kind):
     check(run(torch_dev, ops, x, s, k), x, s, k)
 
 
+@pytest.mark.parametrize("V,k", [(2049, 1), (2069, 20), (2048 + 255, 64), (4096 + 300, 64),
+                                 (20000, 16), (20000, 64)])
+@pytest.mark.parametrize("allowed", [None, 3, 200, 300])
+def test_select_few(torch_dev, ops, V, k, allowed):
+    """A last slice of few logits, and vocabularies of which all but a few are masked."""
+    print("beam few", V, k, allowed, flush=True)
+    rng = np.random.default_rng(V + k)
+    x = rng.standard_normal((2, 3, V)).astype(np.float32)
+    if allowed:
+        keep = np.zeros(V, bool)
+        keep[rng.permutation(V)[:allowed // 2]] = True
+        keep[100:100 + allowed // 2] = True
+        x[..., ~keep] = -np.inf
+    s = (-rng.random((2, 3))).astype(np.float32)
+    check(run(torch_dev, ops, x, s, k), x, s, k)
+
+
 def test_select_strides(torch_dev, ops):
     """Rows of a padded vocabulary, at an odd stride and offset."""
     torch = torch_dev
