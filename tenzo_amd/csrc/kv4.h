@@ -54,35 +54,34 @@ struct Kv4Seqs {
     }
 };
 
-// The sequence whose range holds row r, looked for by the 16 lanes of a DPP row (all of them
-// active and with the same r); -1: none.
-__device__ __forceinline__ int kv4_seq_of_row(const Kv4Seqs& q, int r, int lane16) {
-    int s = -1, first;
-    for (int b = lane16; b < q.B; b += 16) {
-        const int n = q.rows(b, first);
-        if (r >= first && r < first + n) s = b;
-    }
-    s = max(s, dpp_i<kDppXor1>(s));
-    s = max(s, dpp_i<kDppXor2>(s));
-    s = max(s, dpp_i<kDppHalfMirror>(s));
-    return max(s, dpp_i<kDppMirror>(s));
+__device__ __forceinline__ int max_row16(int v) {  // over the 16 lanes of a DPP row
+    v = max(v, dpp_i<kDppXor1>(v));
+    v = max(v, dpp_i<kDppXor2>(v));
+    v = max(v, dpp_i<kDppHalfMirror>(v));
+    return max(v, dpp_i<kDppMirror>(v));
 }
 
-// Position of row r and its sequence; false where it stands nowhere (padding).
+// Position of row r and its sequence; false where it stands nowhere (padding). The sequence is
+// looked for by the 16 lanes of a DPP row, all of them active and with the same r.
 __device__ __forceinline__ bool kv4_place(const Kv4Seqs& q, int r, int lane16, int& seq,
                                           int& pos) {
-    int n = 1, i = 0;
-    seq = r;
-    if (q.cu) {
-        seq = kv4_seq_of_row(q, r, lane16);
-        if (seq < 0) return false;
-        int first;
-        n = q.rows(seq, first);
-        i = r - first;
+    if (!q.cu) {
+        seq = r;
+        pos = q.length(r) - 1;
+        return pos >= 0;
     }
-    const int c = q.length(seq);
-    pos = c - n + i;
-    return i >= 0 && i < n && pos >= 0 && pos < c;
+    seq = pos = -1;
+    for (int b = lane16; b < q.B; b += 16) {
+        int first;
+        const int n = q.rows(b, first), c = q.length(b);
+        if (r >= first && r < first + n) {
+            seq = b;
+            pos = c - n + (r - first);
+        }
+    }
+    seq = max_row16(seq);
+    pos = max_row16(pos);
+    return pos >= 0;
 }
 
 // 2^(s - 127) as fp32. Bytes above 252, which no append writes, count as 0: whatever a pool holds
