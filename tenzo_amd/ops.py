@@ -278,6 +278,16 @@ def _row_stride(t: torch.Tensor, cols: int, name: str) -> int:
     raise ValueError(f"{name}: {tuple(shape)} with strides {st}, not rows of {cols}")
 
 
+def _row_args(t: torch.Tensor, cols: int, dev: int, dtype: torch.dtype, name: str):
+    """The address of t and the elements between its rows, checked."""
+    shape = t.shape
+    if len(shape) == 2 and shape[1] == cols and t.dtype is dtype and t.get_device() == dev:
+        between, step = t.stride()
+        if step == 1:
+            return t.data_ptr(), between if shape[0] > 1 else cols
+    return _on(t, dev, dtype, name), _row_stride(t, cols, name)
+
+
 def kv4_pool(n_blocks: int, n_layers: int, n_kv_heads: int, device="cuda"):
     """Empty pools (pk, pv, pks, pvs) of n_blocks 16-token pages of a cache in 4 bits: codes
     [blocks][layers][kv heads][16][64] and scales [blocks][layers][kv heads][16][4], uint8."""
@@ -288,7 +298,7 @@ def kv4_pool(n_blocks: int, n_layers: int, n_kv_heads: int, device="cuda"):
 
 # (The calls on a cache check a dozen tensors, and the smallest run for 4 us on the GPU: each
 # property is asked for once and the words for what is wrong are looked for afterwards. Host side
-# of a call: append 9 us, attn 16, select 14 (two launches each), reorder 8; the sizes of workspaces, a function of
+# of a call: append 9 us, attn 15, select 14 (two launches each), reorder 8; the sizes of workspaces, a function of
 # the arguments, are asked for once.)
 _U8, _I32, _F32 = torch.uint8, torch.int32, torch.float32
 
@@ -342,6 +352,8 @@ def _rope_rows(rope_cs, dev):
     shape = rope_cs.shape
     if len(shape) != 2 or shape[1] != 128:
         raise ValueError(f"rope_cs: {tuple(shape)}, not [positions][128]")
+    if rope_cs.dtype is _F32 and rope_cs.get_device() == dev and rope_cs.is_contiguous():
+        return rope_cs.data_ptr(), shape[0]
     return _whole(rope_cs, dev, _F32, "rope_cs"), shape[0]
 
 
@@ -359,14 +371,15 @@ def kv4_append(k, v, pk, pv, pks, pvs, block_tables, ctx_lens, layer: int, rope_
     dev = _dev()
     T = k.shape[0]
     pools, where, seqs = _kv4_cache(pk, pv, pks, pvs, block_tables, ctx_lens, cu_q, layer, T, dev)
-    dt = _dtype_code(k)
-    cols = where[3] * 128
-    ks, vs = _row_stride(k, cols, "k"), _row_stride(v, cols, "v")
+    dt, dtype, cols = _dtype_code(k), k.dtype, where[3] * 128
+    kp, ks = _row_args(k, cols, dev, dtype, "k")
+    vp, vs = _row_args(v, cols, dev, dtype, "v")
     if v.shape[0] != T:
         raise ValueError(f"{T} rows of k, {v.shape[0]} of v")
-    _lib.check(_lib.load().tenzo_hip_kv4_append(
-        _on(k, dev, k.dtype, "k"), _on(v, dev, k.dtype, "v"), dt, ks, vs, *pools, *where, *seqs,
-        *_rope_rows(rope_cs, dev), _stream()), "kv4_append")
+    rc = _lib.load().tenzo_hip_kv4_append(kp, vp, dt, ks, vs, *pools, *where, *seqs,
+                                          *_rope_rows(rope_cs, dev), _stream())
+    if rc:
+        _lib.check(rc, "kv4_append")
 
 
 def kv4_read(pk, pv, pks, pvs, block_tables, ctx_lens, layer: int, rows: int | None = None,
@@ -402,22 +415,25 @@ def attn_kv4(q, pk, pv, pks, pvs, block_tables, ctx_lens, layer: int, rope_cs=No
     Hkv = where[3]
     if Hkv < 1 or cols % 128 or (cols // 128) % Hkv:
         raise ValueError(f"q: {tuple(q.shape)}, not rows of heads of 128 over {Hkv} kv heads")
-    dt, qs = _dtype_code(q), _row_stride(q, cols, "q")
+    dt, dtype = _dtype_code(q), q.dtype
+    qp, qs = _row_args(q, cols, dev, dtype, "q")
     if out is None:
         out = q.new_empty(q.shape)
-    elif out.shape != q.shape:
+        op, os = out.data_ptr(), cols
+    elif out.shape == q.shape:
+        op, os = _row_args(out, cols, dev, dtype, "out")
+    else:
         raise ValueError(f"out: {tuple(out.shape)}, q: {tuple(q.shape)}")
     if not T:
         return out
-    L, Hq = _lib.load(), cols // 128
-    os = _row_stride(out, cols, "out")
+    Hq = cols // 128
     nbytes = _attn_kv4_ws(T, seqs[5], Hq, Hkv, seqs[2], cu_q is not None, dt)
     ws = pk.new_empty(nbytes) if nbytes else None  # (held until the launch)
-    _lib.check(L.tenzo_hip_attn_kv4(
-        _on(q, dev, q.dtype, "q"), dt, qs, *pools, *where[:3], Hq, Hkv, *seqs,
-        *_rope_rows(rope_cs, dev), _on(out, dev, q.dtype, "out"), os,
-        None if ws is None else ws.data_ptr(), nbytes, _stream()),
-        "attn_kv4")
+    rc = _lib.load().tenzo_hip_attn_kv4(qp, dt, qs, *pools, *where[:3], Hq, Hkv, *seqs,
+                                        *_rope_rows(rope_cs, dev), op, os,
+                                        ws.data_ptr() if nbytes else None, nbytes, _stream())
+    if rc:
+        _lib.check(rc, "attn_kv4")
     return out
 
 
