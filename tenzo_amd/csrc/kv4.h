@@ -93,12 +93,12 @@ __device__ __forceinline__ float e8m0_to_float(uint32_t s) {
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// The eight values of a word of codes, in order.
-__device__ __forceinline__ void fp4_to_float8(uint32_t w, float scale, float (&v)[8]) {
-    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 0);
-    const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 1);
-    const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 2);
-    const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 3);
+// Eight codes of two groups, the low four times `lo`, the upper four times `hi`.
+__device__ __forceinline__ void fp4_to_float8(uint32_t w, float lo, float hi, float (&v)[8]) {
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, lo, 0);
+    const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, lo, 1);
+    const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, hi, 2);
+    const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, hi, 3);
     v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
     v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
 }
