@@ -30,14 +30,27 @@ __device__ __forceinline__ float round_sticky(double r) {
     return __uint_as_float(b);
 }
 
+// The same where r lies within fp32's normal numbers (`high`, its upper word without the sign, in
+// kHighLow .. kHighTop): its upper 23 bits of fraction, with the exponent of fp32.
+constexpr uint32_t kHighLow = 897u << 20, kHighTop = (1151u << 20) - 1;
+__device__ __forceinline__ uint32_t high_word(double r) {
+    return (uint32_t)__double2hiint(r) & 0x7fffffffu;
+}
+__device__ __forceinline__ float cut_sticky(double r) {
+    const uint32_t hi = (uint32_t)__double2hiint(r), lo = (uint32_t)__double2loint(r);
+    const uint32_t b = __builtin_amdgcn_alignbit(hi, lo, 29) - (896u << 23);
+    return __uint_as_float((b & 0x7fffffffu) | (hi & 0x80000000u) | min(lo & 0x1fffffffu, 1u));
+}
+
 __device__ __forceinline__ float tame(float x) {  // NaN counts as 0, what is beyond is held there
     return x == x ? fminf(fmaxf(x, -kKv4Max), kKv4Max) : 0.0f;
 }
 
-// The scale byte of a group: the smallest e with amax <= 7 * 2^(e - 127) (codes up to 7 go to 6,
-// the last one), at least 1. In the bits: the exponent field less 2, one more above 1.75.
-__device__ __forceinline__ int group_scale(float amax) {
-    return max((int)((__float_as_uint(amax) + 0x1FFFFFu) >> 23) - 2, 1);
+// The scale byte of a group whose largest magnitude has the bits `top`: the smallest e with top <=
+// 7 * 2^(e - 127) (codes up to 7 go to 6, the last one), at least 1: the exponent field less 2, one
+// more above 1.75.
+__device__ __forceinline__ int group_scale(uint32_t top) {
+    return max((int)((top + 0x1FFFFFu) >> 23) - 2, 1);
 }
 
 // Four values of one group as codes, the first in the low nibble.
@@ -48,22 +61,31 @@ __device__ __forceinline__ uint32_t codes4(const float (&x)[4], int e) {
     return w & 0xffffu;
 }
 
-__device__ __forceinline__ float max8(float m) {  // over the 8 lanes of a half DPP row
-    m = fmaxf(m, dpp_f<kDppXor1>(m));
-    m = fmaxf(m, dpp_f<kDppXor2>(m));
-    return fmaxf(m, dpp_f<kDppHalfMirror>(m));
+__device__ __forceinline__ uint32_t max8(uint32_t m) {  // over the 8 lanes of a half DPP row
+    m = max(m, (uint32_t)dpp_i<kDppXor1>((int)m));
+    m = max(m, (uint32_t)dpp_i<kDppXor2>((int)m));
+    return max(m, (uint32_t)dpp_i<kDppHalfMirror>((int)m));
+}
+// Of four values, the bits of the largest magnitude (a NaN's are above all numbers').
+__device__ __forceinline__ uint32_t top4(const float (&x)[4]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+    return m;
 }
 
 // A row's codes and scales to its place: lane l of 16 has dims 4l .. 4l + 3 and 64 + 4l .. + 3.
 __device__ __forceinline__ void write_row(float (&lo)[4], float (&hi)[4], int l, uint8_t* codes,
                                           uint8_t* scales) {
-    float ml = 0.0f, mh = 0.0f;
+    uint32_t ml = top4(lo), mh = top4(hi);
+    if (__ballot(max(ml, mh) > __float_as_uint(kKv4Max))) {  // (rare)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        lo[j] = tame(lo[j]);
-        hi[j] = tame(hi[j]);
-        ml = fmaxf(ml, fabsf(lo[j]));
-        mh = fmaxf(mh, fabsf(hi[j]));
+        for (int j = 0; j < 4; ++j) {
+            lo[j] = tame(lo[j]);
+            hi[j] = tame(hi[j]);
+        }
+        ml = top4(lo);
+        mh = top4(hi);
     }
     const int el = group_scale(max8(ml)), eh = group_scale(max8(mh));
     reinterpret_cast<uint16_t*>(codes)[l] = (uint16_t)codes4(lo, el);
@@ -76,9 +98,9 @@ __device__ __forceinline__ void write_row(float (&lo)[4], float (&hi)[4], int l,
 
 // 16 lanes to a head of a row, its key and its value: lane l has dims 4l .. 4l + 3 and 64 + 4l
 // .. 64 + 4l + 3, so that a dim and its partner of the rotation meet in one lane and a group of
-// 32 lies in 8 lanes. Bound by the bytes read, in loads of 16: 9245 rows of 5 kv heads, fp32, 15.5
-// us, 3.5 TB/s (with the read of them 28.4; loads of 4, keys and values apart, 30.3); one row 2.4
-// us, a chain of four loads.
+// 32 lies in 8 lanes. Bound by the vector work beside the bytes: 9245 rows of 5 kv heads, fp32, 14.4
+// us, 3.7 TB/s (15.5 where fp64 is converted rather than cut to fp32 by its bits, and NaN and
+// infinities are looked at one by one); one row 2.4 us, a chain of four loads.
 template <bool HALF>
 __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4Append a, Kv4Seqs sq) {
     const int l = threadIdx.x & 15;
@@ -103,11 +125,28 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4Append a, Kv4Seqs sq
         float c4[4], s4[4];
         ld_act4<false>(a.rope, (int64_t)pos * kKv4Dim + 4 * l, c4);
         ld_act4<false>(a.rope, (int64_t)pos * kKv4Dim + 64 + 4 * l, s4);
+        double a0[4], a1[4];
+        uint32_t low = 0xffffffffu, top = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const double c = c4[j], s = s4[j], x0 = klo[j], x1 = khi[j];
-            klo[j] = round_sticky(__builtin_fma(-x1, s, x0 * c));
-            khi[j] = round_sticky(__builtin_fma(x1, c, x0 * s));
+            a0[j] = __builtin_fma(-x1, s, x0 * c);
+            a1[j] = __builtin_fma(x1, c, x0 * s);
+            low = min(low, min(high_word(a0[j]), high_word(a1[j])));
+            top = max(top, max(high_word(a0[j]), high_word(a1[j])));
+        }
+        if (__ballot(low < kHighLow || top > kHighTop)) {  // (zeros, mostly)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                klo[j] = round_sticky(a0[j]);
+                khi[j] = round_sticky(a1[j]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                klo[j] = cut_sticky(a0[j]);
+                khi[j] = cut_sticky(a1[j]);
+            }
         }
     }
     write_row(klo, khi, l, a.pk + dst * kKv4Row, a.pks + dst * kKv4Scales);

@@ -184,6 +184,21 @@ def test_append_rotated_borders(torch_dev, ops):
     pools_equal(s, s.dp)
 
 
+def test_append_rotated_range(torch_dev, ops):
+    """Rotated keys of every magnitude that fp32 has, its subnormal numbers among them, alone and
+    beside zeros."""
+    torch = torch_dev
+    T = 270
+    s = Setup([(T, T)], 1, 1, seed=11)
+    s.k = np.ldexp(s.rng.uniform(-2, 2, (T, 1, D)), np.arange(-148, T - 148)[:, None, None]).astype(
+        np.float32)
+    s.k[::3, 0, 5::9] = 0
+    s.dev(torch)
+    ops.kv4_append(s.d["k"], s.d["v"], *s.args(), **s.opts())
+    plain.append(s.k, s.v, s.pools, s.tables, s.ctx, s.layer, s.rope, s.cu)
+    pools_equal(s, s.dp)
+
+
 def test_append_strides_and_bad_pages(torch_dev, ops):
     """Keys and values as slices of a fused projection at an odd stride and offset; pages out of
     the pool, lengths above the tables' and the rotation's rows: nothing is written there."""
