@@ -251,9 +251,9 @@ TENZO_HIP_API int tenzo_hip_kv4_read(const uint8_t* pk, const uint8_t* pv, const
  * concerned. Hq / Hkv 1 to 16. out must not overlap q. ws: a workspace
  * of tenzo_hip_attn_kv4_ws_bytes(...) bytes, 16-byte aligned, of this call
  * alone until it has run (null where that is 0); has_cu: cu_q is not null. The
- * split of rows and tokens over workgroups follows from T, B, the heads, the
- * dtype and table_width (the longest context that the call can have), so a
- * row's sums may be rounded differently in another batch. */
+ * split of rows and tokens over workgroups follows from T, B, the heads and
+ * table_width (the longest context that the call can have), so a row's sums
+ * may be rounded differently in another batch. */
 TENZO_HIP_API size_t tenzo_hip_attn_kv4_ws_bytes(int64_t T, int B, int Hq, int Hkv,
                                                  int table_width, int has_cu, int dtype);
 TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,

@@ -12,6 +12,7 @@ constexpr int kSub = 4;             // 16-token pages of a wave's step
 constexpr int kTile = 16 * kSub;    // tokens of a wave's step
 constexpr int kMaxPages = 1024;     // pages of a workgroup's part of the context
 constexpr int kQStride = 132;       // floats of a query in LDS
+constexpr int kParts = 3;           // parts of 8 bits of an fp32 value: every bit
 
 // The prompts' kernel holds keys and values in fp16. Scale bytes whose values are exact there as
 // they are: 0.5 * 2^(s - 127) to 6 * 2^(s - 127), down to its smallest subnormal, which the matrix
@@ -269,14 +270,16 @@ struct Segment {
 // which is what the B operand of O^T = V^T P^T wants when the value rows are taken in the same
 // order: no weight changes lanes. V^T comes from value rows in LDS (bf16, private to the wave)
 // by transposing reads. Codes times scale are exact in bf16; queries and weights are split into
-// NP parts of 8 bits (fp32: 3, every bit; fp16: 2). With ROWS < 16 the parts stand in columns
-// side by side (column = part * ROWS + row) and one MFMA serves all of them.
+// three parts of 8 bits, every bit that fp32 holds, whatever the type of the call (with two in fp16
+// calls, a part in 2^15 at worst, scores of 50 were wrong by 2^-10 of an output; the two save 1%
+// of a batch of tokens with 4 query heads a kv head, 12% with 8 and 4% of drafts). With 4 rows the
+// parts stand in columns side by side (column = part * ROWS + row) and one MFMA serves all of them.
 //
 // A step loads 136 bytes a token straight to registers, the next step's during the products.
 // 130000 tokens of one sequence, 20 / 5 heads: 23.4 us, 3.8 TB/s (and 3 for the join), bound by
 // the vector work on codes and weights beside the loads; up to 256 tokens 6 us, a chain of loads
 // (length, page number, codes), the products' latency and the waves' meeting.
-template <int ROWS, int NP, int RW, bool HALF>
+template <int ROWS, int RW>
 struct Kv4Smem {
     static constexpr int RT = ROWS * RW;
     // the queries first, then 32 value rows (bf16) a wave, at last the rows' sums
@@ -287,11 +290,11 @@ struct Kv4Smem {
     int pg[kMaxPages];
 };
 
-template <int ROWS, int NP, int RW, bool HALF, bool EVEN>
+template <int ROWS, int RW, bool HALF, bool EVEN>
 __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq, const Segment& g,
-                                            Kv4Smem<ROWS, NP, RW, HALF>& sm) {
-    constexpr int SLOTS = 16 / ROWS, NM = SLOTS == 1 ? NP : 1, TW = 4 / RW, RT = ROWS * RW;
-    static_assert(SLOTS == 1 || SLOTS >= NP, "a column for each part");
+                                            Kv4Smem<ROWS, RW>& sm) {
+    constexpr int SLOTS = 16 / ROWS, NM = SLOTS == 1 ? kParts : 1, TW = 4 / RW, RT = ROWS * RW;
+    static_assert(SLOTS == 1 || SLOTS > kParts, "a column for each part");
     static_assert(32 * kKv4Dim * 2 >= 16 * kKv4Dim * 4, "the rows' sums fit a wave's values");
     uint16_t* smem = sm.main;
     int* pg = sm.pg;
@@ -422,8 +425,8 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     x[k] -= masked(x[k], m1);
-                    if (NP == 3) x[k] -= masked(x[k], m2);
-                    if (SLOTS > NP && slot >= NP) x[k] = 0.0f;
+                    x[k] -= masked(x[k], m2);
+                    if (slot >= kParts) x[k] = 0.0f;
                 }
 #pragma unroll
             for (int p = 0; p < NM; ++p) {
@@ -489,9 +492,8 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float v = s[tt][i];
-                    if (ROWS == 4) v += ror16<kDppRor8>(v);
-                    if (ROWS == 4) v += ror16<kDppRor4>(v);
-                    if (ROWS == 8) v += ror16<kDppRor8>(v);
+                    if (SLOTS > 1) v += ror16<kDppRor8>(v);
+                    if (SLOTS > 1) v += ror16<kDppRor4>(v);
                     s[tt][i] = v;
                 }
             // a step that a row may not see whole: past its position, or absent pages
@@ -552,7 +554,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
                     p8[e] = s[2 * u + (e >> 2)][e & 3];
                     if (SLOTS > 1) {
                         p8[e] -= masked(p8[e], m1);
-                        if (NP == 3) p8[e] -= masked(p8[e], m2);
+                        p8[e] -= masked(p8[e], m2);
                     }
                 }
 #pragma unroll
@@ -607,9 +609,9 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
         for (int d = 0; d < 8; ++d)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float v = slot < NP ? acc[d][i] : 0.0f;
+                float v = slot < kParts ? acc[d][i] : 0.0f;
                 v += ror16<kDppRor8>(v);
-                if (ROWS == 4) v += ror16<kDppRor4>(v);
+                v += ror16<kDppRor4>(v);
                 acc[d][i] = v;
             }
     }
@@ -675,10 +677,10 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
 }
 
 // A grid of (unit, split, kv head): every workgroup one piece.
-template <int ROWS, int NP, int RW, bool HALF>
+template <int ROWS, int RW, bool HALF>
 __global__ void __launch_bounds__(256, ROWS == 16 ? 2 : 3)
 kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
-    __shared__ Kv4Smem<ROWS, NP, RW, HALF> sm;
+    __shared__ Kv4Smem<ROWS, RW> sm;
     const int per_unit = sq.Hkv * a.splits;
     // (from the last unit on: the latest rows of a prompt see the most tokens)
     const int back = blockIdx.x / per_unit, rest = blockIdx.x - back * per_unit;
@@ -693,7 +695,7 @@ kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
     g.len = a.chunk;
     const int last_i = min(g.n - 1, a.token(g.tile * ROWS * RW + ROWS * RW - 1));
     if (g.split > 0 && g.t0 >= min(g.c - g.n + last_i + 1, g.c)) return;
-    kv4_segment<ROWS, NP, RW, HALF, false>(a, sq, g, sm);
+    kv4_segment<ROWS, RW, HALF, false>(a, sq, g, sm);
 }
 
 constexpr int kRowsRT = 128;
@@ -1122,10 +1124,10 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
 // lengths, which only the device knows, need not be alike. A share holds the end of a unit that
 // an earlier workgroup began, whole units and the beginning of one: two records at most. 48
 // sequences of up to 8190 tokens (223127 in all), 32 / 8 heads, fp16: 55 us, 4.4 TB/s.
-template <int ROWS, int NP, bool HALF>
+template <int ROWS, bool HALF>
 __global__ void __launch_bounds__(256, ROWS == 16 ? 2 : 3)
 kv4_attn_even_kernel(Kv4Attn a, Kv4Seqs sq) {
-    __shared__ Kv4Smem<ROWS, NP, 1, HALF> sm;
+    __shared__ Kv4Smem<ROWS, 1> sm;
     __shared__ int wsum[4], at_base, at_seq;
     const int per = (sq.B + 255) / 256, b0 = threadIdx.x * per;
     int mine = 0, total;
@@ -1176,7 +1178,7 @@ kv4_attn_even_kernel(Kv4Attn a, Kv4Seqs sq) {
         g.whole = to - from == w.steps;
         g.rec = ((int64_t)blockIdx.x * 2 + (from == 0 ? 1 : 0)) * ROWS;
         g.split = 0;
-        kv4_segment<ROWS, NP, 1, HALF, true>(a, sq, g, sm);
+        kv4_segment<ROWS, 1, HALF, true>(a, sq, g, sm);
     }
 }
 
@@ -1308,11 +1310,10 @@ struct Kv4Plan {
     int64_t wgs;
     size_t records;
 };
-Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, bool half) {
+Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu) {
     Kv4Plan p{};
     const int64_t per = cu ? ceil_div(T * G, B) : G;  // rows of an average sequence
-    const int packed = half ? 8 : 4;
-    p.rows = per <= packed ? packed : 16;
+    p.rows = per <= 4 ? 4 : 16;
     const int64_t ctx = (int64_t)table_width * kKv4Page;
     // Rows of a workgroup: 16 against 256 tokens at a time spread few rows over the GPU; the
     // prompts' kernel, once it has work for a while (16 us go into its queries and outputs), reads
@@ -1357,13 +1358,13 @@ Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, boo
     return p;
 }
 
-template <int ROWS, int NP, int RW, bool HALF>
+template <int ROWS, int RW, bool HALF>
 void launch_kv4(const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
-    hipLaunchKernelGGL((kv4_attn_kernel<ROWS, NP, RW, HALF>), dim3(a.wgs), dim3(256), 0, st, a, s);
+    hipLaunchKernelGGL((kv4_attn_kernel<ROWS, RW, HALF>), dim3(a.wgs), dim3(256), 0, st, a, s);
 }
-template <int ROWS, int NP, bool HALF>
+template <int ROWS, bool HALF>
 int launch_kv4_even(const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
-    hipLaunchKernelGGL((kv4_attn_even_kernel<ROWS, NP, HALF>), dim3(a.wgs), dim3(256), 0, st, a, s);
+    hipLaunchKernelGGL((kv4_attn_even_kernel<ROWS, HALF>), dim3(a.wgs), dim3(256), 0, st, a, s);
     const int rc = launch_status("kv4_attn_even_kernel");
     if (rc) return rc;
     // few rows: a head to a workgroup, its records to 8 groups of lanes
@@ -1375,17 +1376,17 @@ int launch_kv4_even(const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
                            dim3(a.T, (a.Hq + 7) / 8), dim3(256), 0, st, a, s);
     return launch_status("kv4_join_even_kernel");
 }
-template <int PACKED, int NP, bool HALF>
+template <bool HALF>
 int launch_kv4_plan(const Kv4Plan& p, const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
     if (p.even)
-        return p.rows == PACKED ? launch_kv4_even<PACKED, NP, HALF>(a, s, st)
-                                : launch_kv4_even<16, NP, HALF>(a, s, st);
-    if (p.rows == PACKED)
-        launch_kv4<PACKED, NP, 1, HALF>(a, s, st);
+        return p.rows == 4 ? launch_kv4_even<4, HALF>(a, s, st)
+                           : launch_kv4_even<16, HALF>(a, s, st);
+    if (p.rows == 4)
+        launch_kv4<4, 1, HALF>(a, s, st);
     else if (p.rw == 1)
-        launch_kv4<16, NP, 1, HALF>(a, s, st);
+        launch_kv4<16, 1, HALF>(a, s, st);
     else if (p.rw == 2)
-        launch_kv4<16, NP, 2, HALF>(a, s, st);
+        launch_kv4<16, 2, HALF>(a, s, st);
     else
         hipLaunchKernelGGL(kv4_attn_rows_kernel<HALF>, dim3(a.wgs), dim3(256), 0, st, a, s);
     const int rc = launch_status("kv4_attn_kernel");
@@ -1406,9 +1407,9 @@ using namespace tz;
 extern "C" {
 
 TENZO_HIP_API size_t tenzo_hip_attn_kv4_ws_bytes(int64_t T, int B, int Hq, int Hkv,
-                                                 int table_width, int has_cu, int dtype) {
+                                                 int table_width, int has_cu, int /*dtype*/) {
     if (T <= 0 || B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || table_width < 0) return 0;
-    const Kv4Plan p = kv4_plan(T, B, Hq / Hkv, Hkv, table_width, has_cu != 0, dtype != 0);
+    const Kv4Plan p = kv4_plan(T, B, Hq / Hkv, Hkv, table_width, has_cu != 0);
     return p.records * (kKv4Dim * 4 + 8);
 }
 
@@ -1440,7 +1441,7 @@ TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,
              "attn_kv4: %zu bytes of workspace needed, 16-byte aligned, %zu given", need,
              ws ? ws_bytes : 0);
     const int G = Hq / Hkv;
-    const Kv4Plan p = kv4_plan(T, B, G, Hkv, table_width, cu_q != nullptr, dtype != 0);
+    const Kv4Plan p = kv4_plan(T, B, G, Hkv, table_width, cu_q != nullptr);
     TZ_CHECK(p.wgs <= 0xffffff && T <= 0x7fffff && Hq <= 65535, "attn_kv4: %lld rows of %d heads",
              (long long)T, Hq);
     Kv4Attn a{};
@@ -1463,8 +1464,8 @@ TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,
     a.chunk = p.chunk;
     a.splits = p.splits;
     a.vec_out = (((uintptr_t)out | (uintptr_t)(out_stride * (dtype ? 2 : 4))) & 15) == 0;
-    return dtype ? launch_kv4_plan<8, 2, true>(p, a, s, (hipStream_t)stream)
-                 : launch_kv4_plan<4, 3, false>(p, a, s, (hipStream_t)stream);
+    return dtype ? launch_kv4_plan<true>(p, a, s, (hipStream_t)stream)
+                 : launch_kv4_plan<false>(p, a, s, (hipStream_t)stream);
 }
 
 }  // extern "C"
