@@ -362,9 +362,11 @@ TENZO_HIP_API int tenzo_hip_sample_top_k_top_p(const float* logits, int64_t V, i
  * each of B requests with W beams. Candidate (w, t) of a request has the score
  * scores[b][w] + log_softmax(logits[b][w])[t] (row b * W + w of the logits at
  * row_stride elements); the k largest, in order, go to out_scores, out_beams
- * (w) and out_tokens (t), each [B][k]. Scores are compared in 64 bits; among
- * equal ones the lower beam comes first, then the larger logit, then the lower
- * token. A logit or a score that is not below +inf (NaN too) counts as -inf;
+ * (w) and out_tokens (t), each [B][k]. The order is that of scores in 64 bits
+ * (log-sums come from exponentials in fp32, and anew from 64-bit ones where
+ * beams' candidates are within 2.5e-6); among equal ones the lower beam comes
+ * first, then the larger logit, then the lower token. A score written is off
+ * by at most 1.25e-6 and its rounding to fp32. A logit or a score that is not below +inf (NaN too) counts as -inf;
  * -inf candidates come last. W and k up to 64, k <= W * V, V up to 2^30 and
  * W * V below 2^31. ws: as above, tenzo_hip_beam_select_ws_bytes(...) bytes. */
 TENZO_HIP_API size_t tenzo_hip_beam_select_ws_bytes(int B, int W, int64_t V, int k);

@@ -1,11 +1,11 @@
 // Beam search on the device: the best k continuations of a request's W beams over the
 // vocabulary, and the reordering of the beams' paged caches.
 //
-// Selection: candidate (w, t) has the score s_w + x_wt - log sum_u exp(x_wu), in 64 bits (two
-// beams' candidates can lie closer than fp32 tells apart); the k largest are taken, among equal
-// ones the lower beam, then the larger logit, then the lower token. So a beam's candidates come
-// in the order of (logit, token) and the first k of each beam hold the answer. A logit that is
-// not below +inf (NaN, +inf) counts as -inf.
+// Selection: candidate (w, t) has the score s_w + x_wt - log sum_u exp(x_wu); the k largest are
+// taken, among equal ones the lower beam, then the larger logit, then the lower token. So a beam's
+// candidates come in the order of (logit, token) and the first k of each beam hold the answer. A
+// logit that is not below +inf (NaN, +inf) counts as -inf. Two beams' candidates can lie closer
+// than exponentials in fp32 tell apart; where they do, the log-sums are taken anew in 64 bits.
 #include <climits>
 
 #include "common.h"
@@ -17,6 +17,12 @@ constexpr int kBeamMax = 64;      // beams and candidates, upper bounds
 constexpr int kSliceCand = 1024;  // a slice's candidates in LDS
 constexpr int kSliceFew = 256;    // logits above -inf that are put in order as they are
 constexpr int kPickCand = 512;    // the candidates that the last step ranks
+
+// A row's log-sum from fp32 exponentials is nearer than this to the true one. x - max and its
+// product with log2 e are rounded to 2^-24 of themselves each, in base 2 at most 8.1 of them on a
+// slice's average (5 of 6 parts of the weight at 4095 logits 9.7 below one), 6.7e-7; log2 e
+// itself 7e-8, the exponential's step 1.2e-7, eight of them added in fp32 1.8e-7. (Seen: 2.8e-7.)
+constexpr double kLogSumError = 1.25e-6;
 
 // Up to here a slice's bound is the best of its waves' own, above it that of their merged order:
 // 19 x 16 beams over 154773 logits, 32 candidates, 58 us merged and 70 not, 8 beams over 128256,
@@ -106,6 +112,24 @@ __device__ __forceinline__ double lanes_max(double v) {
     return fmax(v, lane_xor<1>(v));
 }
 
+// exp(x) of x up to 0, within 2^-50: x log2 e = n + f, and 2^f by the polynomial of degree 10
+// through its values at the Chebyshev nodes of [-1/2, 1/2] (4.5e-16 of it). 128256 of them by a
+// workgroup take 8 us less than the library's, which takes any x.
+__device__ __forceinline__ double exp64(double x) {
+    constexpr double kC[] = {
+        0x1.e6063f7217bc6p-28, 0x1.b675bca4eeebbp-24, 0x1.62bfd47773353p-20, 0x1.ffcb54062e698p-17,
+        0x1.430913096fd9fp-13, 0x1.5d87fe9d7a584p-10, 0x1.3b2ab6fba1ddap-7, 0x1.c6b08d703ce49p-5,
+        0x1.ebfbdff82c598p-3, 0x1.62e42fefa3a19p-1, 0x1.0000000000000p+0};
+    constexpr double kLog2e = 0x1.71547652b82fep0, kRound = 0x1.8p52;  // (a sum's low word is n)
+    x = fmax(x, -1000.0);  // (0 from there on)
+    const double t = __builtin_fma(x, kLog2e, kRound);
+    const double f = __builtin_fma(x, kLog2e, kRound - t);
+    double p = kC[0];
+#pragma unroll
+    for (int i = 1; i <= 10; ++i) p = __builtin_fma(p, f, kC[i]);
+    return __builtin_ldexp(p, __double2loint(t));
+}
+
 // One step of a descending bitonic sort over the 64 lanes: lane l and l ^ M, the one without
 // the mask's top bit keeps the larger.
 template <int M>
@@ -188,7 +212,8 @@ __global__ void __launch_bounds__(256, 8) beam_slice_kernel(BeamSelect a) {
     }
     const float ref = M == -INFINITY ? 0.0f : M;
 
-    // few terms are added in 32 bits, their sums in 64
+    // few terms are added in 32 bits, their sums in 64 (with exponentials in 64 bits, to 2e-9, the
+    // selection of 48 x 8 beams takes 66 us in place of 53)
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < E; i += 8) {
@@ -301,15 +326,19 @@ __device__ __forceinline__ bool before(const BeamCand& a, const BeamCand& b) {
 
 // Stage 2, a workgroup per request: the rows' log-sums, then the best k of the slices' lists. The
 // first few of every list (2k of a beam's or more, up to 1024 in all) are put in order (sorted by
-// waves, merged in pairs), and their k-th is a bound that k candidates reach (in fp32, rounded
-// down: it keeps too many rather than too few). Those that do are ranked by counting; where they
-// are many (equal scores, masked beams) the k best are taken one after the other. 48 x 8 beams, 32
-// slices, 16 candidates: 8 us, latency from end to end.
+// waves, merged in pairs), and their k-th (in fp32, rounded
+// down), less what the log-sums may be off by, is a bound that the k best reach. Those that
+// do are ranked by counting. Where one of the k best has another beam's candidate so near that the
+// log-sums leave their order open, theirs are summed in 64 bits from the logits (27 us a beam of
+// 128256) and all are ranked once more. Where candidates are many (equal scores, masked beams) all
+// beams' are, and the k best are taken one after the other. 48 x 8 beams, 32 slices, 16 candidates:
+// 8 us, latency from end to end.
 __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
-    __shared__ double lse[kBeamMax], own[kBeamMax];
+    __shared__ double lse[kBeamMax], own[kBeamMax], peak[kBeamMax], part[16];
     __shared__ double ls[kPickCand];
+    __shared__ uint32_t near[2];  // beams whose log-sums are needed in 64 bits
     __shared__ float lx[kPickCand], tops[16][64];
-    __shared__ int lw[kPickCand], lt[kPickCand], open[kPickCand], cnt, opened;
+    __shared__ int lw[kPickCand], lt[kPickCand], lr[kPickCand], open[kPickCand], cnt, opened;
     __shared__ BeamCand best[16];
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -338,10 +367,11 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
         s = lanes_sum(s);
         if (lane == 0) {
             lse[w] = m > -INFINITY ? m + log(s) : 0.0;
+            peak[w] = m;
             own[w] = beam_logit(score);
         }
     }
-    if (tid == 0) cnt = opened = 0;
+    if (tid == 0) cnt = opened = near[0] = near[1] = 0;
     __syncthreads();
     const auto get = [&](int c, float2 e) {
         BeamCand r;
@@ -365,9 +395,9 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
         }
         __syncthreads();
     }
-    const float tau = tops[0][a.k - 1];
+    const double bound = (double)tops[0][a.k - 1] - 2 * kLogSumError;
     const auto keep = [&](const BeamCand& c) {
-        if (c.t == INT_MAX || __double2float_rd(c.s) < tau) return;
+        if (c.t == INT_MAX || c.s < bound) return;
         const int at = atomicAdd(&cnt, 1);
         if (at < kPickCand) ls[at] = c.s, lx[at] = c.x, lw[at] = c.w, lt[at] = c.t;
     };
@@ -376,7 +406,7 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
         if (few && tid + 1024 * i < total) keep(get(tid + 1024 * i, mine[i]));
     if (!few) {  // only the lists whose first candidate reaches the bound
         for (int i = tid; i < lists; i += 1024)
-            if (__double2float_rd(get(i * a.k, cand[i * a.k]).s) >= tau) {
+            if (get(i * a.k, cand[i * a.k]).s >= bound) {
                 const int at = atomicAdd(&opened, 1);
                 if (at < kPickCand) open[at] = i * a.k;
             }
@@ -387,30 +417,81 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
         }
     }
     __syncthreads();
+    // a beam's log-sum in 64 bits (a beam without candidates: nothing to do)
+    const auto sum_exactly = [&](int w) {
+        const double m = peak[w];
+        if (m == -INFINITY || own[w] == -INFINITY) return;
+        const float* x = a.logits + ((int64_t)b * a.W + w) * a.stride;
+        double s = 0.0;
+        float v[8], next[8];  // (the next ones are loaded during the sums)
+        const auto load = [&](int t0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) next[i] = x[min(t0 + 1024 * i, a.V - 1)];
+        };
+        load(tid);
+        for (int t0 = tid; t0 < a.V; t0 += 8 * 1024) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = t0 + 1024 * i < a.V ? next[i] : -INFINITY;
+            load(t0 + 8 * 1024);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += exp64((double)beam_logit(v[i]) - m);
+        }
+        s = lanes_sum(s);
+        if (lane == 0) part[wave] = s;
+        __syncthreads();
+        if (tid == 0) {
+            s = 0.0;
+            for (int i = 0; i < 16; ++i) s += part[i];
+            lse[w] = m + log(s);
+        }
+        __syncthreads();
+    };
     const int n = cnt;
     if (n <= kPickCand && opened <= kPickCand) {
-        // four lanes to a candidate; equal scores are rare and looked at in full
-        const int q = tid & 3;
-        for (int i0 = 0; i0 < n; i0 += 256) {
-            const int i = i0 + (tid >> 2);
-            const double me = ls[min(i, n - 1)];
-            int rank = 0;
-            for (int o = q; o < n; o += 4) {
-                rank += ls[o] > me ? 1 : 0;
-                if (ls[o] == me && i < n &&
-                    before(BeamCand{me, lx[o], lw[o], lt[o]}, BeamCand{me, lx[i], lw[i], lt[i]}))
-                    ++rank;
+        for (bool first = a.W > 1;; first = false) {
+            // four lanes to a candidate; equal scores are rare and looked at in full
+            const int q = tid & 3;
+            for (int i0 = 0; i0 < n; i0 += 256) {
+                const int i = i0 + (tid >> 2);
+                const double me = ls[min(i, n - 1)];
+                int rank = 0;
+                uint64_t beams = 0;  // that have a candidate next to this one
+                for (int o = q; o < n; o += 4) {
+                    rank += ls[o] > me ? 1 : 0;
+                    if (fabs(ls[o] - me) <= 2 * kLogSumError && i < n) {
+                        if (lw[o] != lw[i]) beams |= 1ull << lw[o] | 1ull << lw[i];
+                    }
+                    if (ls[o] == me && i < n &&
+                        before(BeamCand{me, lx[o], lw[o], lt[o]},
+                               BeamCand{me, lx[i], lw[i], lt[i]}))
+                        ++rank;
+                }
+                rank += dpp_i<kDppXor1>(rank);
+                rank += dpp_i<kDppXor2>(rank);
+                if (i < n && q == 0) lr[i] = rank;
+                if (first && beams && rank < a.k) {
+                    atomicOr(&near[0], (uint32_t)beams);
+                    atomicOr(&near[1], (uint32_t)(beams >> 32));
+                }
             }
-            rank += dpp_i<kDppXor1>(rank);
-            rank += dpp_i<kDppXor2>(rank);
-            if (i < n && q == 0 && rank < a.k) {
-                a.out_scores[b * a.k + rank] = (float)me;
-                a.out_beams[b * a.k + rank] = lw[i];
-                a.out_tokens[b * a.k + rank] = lt[i];
-            }
+            __syncthreads();
+            if (!first || !(near[0] | near[1])) break;
+            for (int w = 0; w < a.W; ++w)
+                if (near[w >> 5] >> (w & 31) & 1) sum_exactly(w);
+            for (int i = tid; i < n; i += 1024)
+                if (ls[i] > -INFINITY) ls[i] = ((double)lx[i] - lse[lw[i]]) + own[lw[i]];
+            __syncthreads();
         }
+        for (int i = tid; i < n; i += 1024)
+            if (lr[i] < a.k) {
+                a.out_scores[b * a.k + lr[i]] = (float)ls[i];
+                a.out_beams[b * a.k + lr[i]] = lw[i];
+                a.out_tokens[b * a.k + lr[i]] = lt[i];
+            }
         return;
     }
+    if (a.W > 1)
+        for (int w = 0; w < a.W; ++w) sum_exactly(w);
     BeamCand last{INFINITY, INFINITY, -1, -1};
     const BeamCand none{-INFINITY, -INFINITY, INT_MAX, INT_MAX};
     for (int j = 0; j < a.k; ++j) {

@@ -551,9 +551,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int):
     """The best k continuations of each request: logits [B][W][V] fp32 (beams any stride
     apart), scores [B][W] fp32, the beams' running log-probabilities. Returns (scores [B][k]
     fp32, beams [B][k] int32, tokens [B][k] int32) of the candidates scores + log_softmax(
-    logits), compared in 64 bits, in falling order; among equal ones the lower beam, then the
-    larger logit, then the lower token comes first. NaN and +inf count as -inf, which comes
-    last."""
+    logits), in the falling order that they have in 64 bits; among equal ones the lower beam,
+    then the larger logit, then the lower token comes first. Scores are within 1.25e-6 and half
+    a step of fp32. NaN and +inf count as -inf, which comes last."""
     dev = _dev()
     shape = logits.shape
     if len(shape) != 3 or scores.shape != shape[:2]:
