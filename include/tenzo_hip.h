@@ -248,7 +248,12 @@ TENZO_HIP_API int tenzo_hip_kv4_read(const uint8_t* pk, const uint8_t* pv, const
  * to hold them: append first), out likewise out_stride apart. A row that sees
  * no token is zero; sums are held in fp32 until they are divided, so scores or
  * sums of weighted values past its range give infinities and NaN in the rows
- * concerned. Hq / Hkv 1 to 16. out must not overlap q. ws: a workspace
+ * concerned. Queries and weights keep the 24 bits of fp32; in calls that give
+ * 128 rows to a workgroup (prompts: over 64 rows times heads a kv head and
+ * sequence, and many of them or a wide table) 22, and there weights below 2^-40
+ * of a row's largest are lost, and where scales leave the range of fp16 also
+ * what lies below 2^-37 of the largest: of a key's elements, and of the values
+ * that a workgroup's rows see. Hq / Hkv 1 to 16. out must not overlap q. ws: a workspace
  * of tenzo_hip_attn_kv4_ws_bytes(...) bytes, 16-byte aligned, of this call
  * alone until it has run (null where that is 0); has_cu: cu_q is not null. The
  * split of rows and tokens over workgroups follows from T, B, the heads and

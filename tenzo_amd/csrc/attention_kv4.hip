@@ -48,6 +48,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 union Frag {
     uint32_t w[4];
@@ -769,7 +770,7 @@ template <bool HALF>
 __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seqs sq) {
     // two tiles' keys and values (the first is the queries' on their way to registers before)
     __shared__ __align__(16) uint16_t tiles[2][2][kTile * kKv4Dim];
-    __shared__ float moved[2][kTile];  // 2^ the power of two that a token's keys are moved by
+    __shared__ __align__(16) int moved[2][kTile];  // the power of two that a token's keys are moved by
     __shared__ int flags[2][4], tops[4];
     __shared__ int pg[kMaxPages];
     const int per_unit = sq.Hkv * a.splits;
@@ -805,7 +806,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
     int64_t grow[2];
     int head[2];
     bool row_ok[2];
-    float unit[2];
+    int up[2];  // the power of two that a row's query is moved by
     Frag16 qf[2][2][4];
 #pragma unroll
     for (int ct = 0; ct < 2; ++ct) {
@@ -852,11 +853,10 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
 #pragma unroll
             for (int k = 0; k < 4; ++k) amax = fmaxf(amax, fabsf(x[e][k]));
         }
-        const int up = row_shift(max_quarters(amax));
-        unit[ct] = pow2(-up);
+        up[ct] = row_shift(max_quarters(amax));
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            x[e] *= pow2(up);
+            x[e] *= pow2(up[ct]);
 #pragma unroll
             for (int k = 0; k < 4; k += 2) {
                 const uint32_t hi = pack16(x[e][k], x[e][k + 1]);
@@ -928,7 +928,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
         if (!skip) vtop = max(vtop, vby);
         store(tiles[half][0], kr, kb);
         store(tiles[half][1], vr, vby - vshift);
-        if (j == 0) moved[half][16 * wave + col] = pow2(by);
+        if (j == 0) moved[half][16 * wave + col] = by;
         if (lane == 0) flags[half][wave] = flag;
     };
     int w0 = t0;
@@ -1001,13 +1001,18 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
                             s[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                                 kf[tt], qf[ct][p][st].v, s[ct][tt], 0, 0, 0);
             }
+            // (by both powers at once: a large key's and a small query's may be beyond fp32 alone)
             if (scaled)
 #pragma unroll
                 for (int tt = 0; tt < 4; ++tt) {
-                    const f32x4 f = *reinterpret_cast<const f32x4*>(moved[half] + 16 * tt + 4 * j);
-                    s[0][tt] *= f;
-                    s[1][tt] *= f;
+                    const i32x4 by = *reinterpret_cast<const i32x4*>(moved[half] + 16 * tt + 4 * j);
+#pragma unroll
+                    for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[ct][tt][i] = __builtin_ldexpf(s[ct][tt][i], by[i] - up[ct]);
                 }
+            const float unit[2] = {scaled ? 1.0f : pow2(-up[0]), scaled ? 1.0f : pow2(-up[1])};
             const bool mask = bad || t + kTile - 1 > low;
             float shift[2];
 #pragma unroll
@@ -1097,24 +1102,35 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
     }
 #pragma unroll
     for (int ct = 0; ct < 2; ++ct) {
-        const float L = sum_quarters(l[ct]);
+        float L = sum_quarters(l[ct]);
         if (!row_ok[ct]) continue;
-        if (vshift != 0)
+        // (by the sum of weights, and the 2^15 in both, before the values' power of two)
+        const auto times = [](f32x4 v, int e) {
 #pragma unroll
-            for (int d = 0; d < 8; ++d) acc[ct][d] *= pow2(vshift);
+            for (int i = 0; i < 4; ++i) v[i] = __builtin_ldexpf(v[i], e);
+            return v;
+        };
         if (pos[ct] < a.chunk || a.splits == 1) {
-            if (split == 0)
+            if (split > 0) continue;
+            if (vshift != 0 && L != 0.0f) {
 #pragma unroll
-                for (int d = 0; d < 8; ++d)
-                    store4<HALF>(a, grow[ct] * a.out_stride + (int64_t)head[ct] * kKv4Dim + 16 * d +
-                                        4 * j,
-                                 acc[ct][d], L);
-        } else {
-            const int64_t at = (grow[ct] * a.Hq + head[ct]) * a.splits + split;
+                for (int d = 0; d < 8; ++d) acc[ct][d] = times(acc[ct][d] * (1.0f / L), vshift);
+                L = 1.0f;
+            }
 #pragma unroll
             for (int d = 0; d < 8; ++d)
-                *reinterpret_cast<f32x4*>(a.part_o + at * kKv4Dim + 16 * d + 4 * j) = acc[ct][d];
-            if (j == 0) a.part_ml[at] = make_float2(m[ct], L);
+                store4<HALF>(a, grow[ct] * a.out_stride + (int64_t)head[ct] * kKv4Dim + 16 * d +
+                                    4 * j,
+                             acc[ct][d], L);
+        } else {
+            const int64_t at = (grow[ct] * a.Hq + head[ct]) * a.splits + split;
+            const int e = vshift - (int)kWeightBits;
+#pragma unroll
+            for (int d = 0; d < 8; ++d)
+                *reinterpret_cast<f32x4*>(a.part_o + at * kKv4Dim + 16 * d + 4 * j) =
+                    times(acc[ct][d], e);
+            if (j == 0)
+                a.part_ml[at] = make_float2(m[ct], __builtin_ldexpf(L, -(int)kWeightBits));
         }
     }
 }
