@@ -296,6 +296,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
                                             Kv4Smem<ROWS, RW>& sm) {
     constexpr int SLOTS = 16 / ROWS, NM = SLOTS == 1 ? kParts : 1, TW = 4 / RW, RT = ROWS * RW;
     static_assert(SLOTS == 1 || SLOTS > kParts, "a column for each part");
+    static_assert(TW > 1, "a row's sums meet from several waves");
     static_assert(32 * kKv4Dim * 2 >= 16 * kKv4Dim * 4, "the rows' sums fit a wave's values");
     uint16_t* smem = sm.main;
     int* pg = sm.pg;
@@ -311,11 +312,8 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
     const int t1 = min(min(t0 + g.len, c - n + last_i + 1), c);  // tokens that some row sees
 
     // the lane's row
-    const int slot = col / ROWS, r = row0 + rw * ROWS + col % ROWS;
-    const int qi = a.token(r), head = h * a.G + (r - qi * a.G);
-    const bool row_ok = qi < n;
-    const int pos = row_ok && c > 0 ? c - n + qi : -1;
-    const int64_t grow = (int64_t)first + qi;
+    const int slot = col / ROWS, qi = a.token(row0 + rw * ROWS + col % ROWS);
+    const int pos = qi < n && c > 0 ? c - n + qi : -1;
 
     // the page numbers of the first kMaxPages pages and the rows' queries, rotated and scaled, by
     // way of LDS (each wave needs all of a row)
@@ -616,65 +614,45 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
                 acc[d][i] = v;
             }
     }
-    // a row's sums: to `out` where no other piece has any of its tokens, else a record
-    auto direct = [&](int p) { return EVEN ? g.whole : p < a.chunk || a.splits == 1; };
-    auto record = [&](int rr, int64_t gr, int64_t hd) {
-        return EVEN ? g.rec + rr : (gr * a.Hq + hd) * a.splits + g.split;
-    };
-    if (TW > 1) {
-        // the waves' sums meet: every wave's rows in its own part of the value buffer
-        float* o = reinterpret_cast<float*>(vb);
-        if (slot == 0) {
+    // the waves' sums meet: every wave's rows in its own part of the value buffer
+    float* o = reinterpret_cast<float*>(vb);
+    if (slot == 0) {
 #pragma unroll
-            for (int d = 0; d < 8; ++d)
-                *reinterpret_cast<f32x4*>(o + col * kKv4Dim + 16 * d + 4 * j) = acc[d];
-            if (j == 0) sm.ml[wave][col] = make_float2(m, l);
+        for (int d = 0; d < 8; ++d)
+            *reinterpret_cast<f32x4*>(o + col * kKv4Dim + 16 * d + 4 * j) = acc[d];
+        if (j == 0) sm.ml[wave][col] = make_float2(m, l);
+    }
+    __syncthreads();
+    for (int it = tid; it < RT * 32; it += 256) {
+        const int rr = it >> 5, d4 = it & 31, grp = rr / ROWS, cc = rr % ROWS;
+        const int r2 = row0 + rr, i2 = a.token(r2);
+        if (i2 >= n) continue;
+        float M = -INFINITY, L = 0.0f;
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < TW; ++w) M = fmaxf(M, sm.ml[w * RW + grp][cc].x);
+        const float base = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+        for (int w = 0; w < TW; ++w) {
+            const float2 e = sm.ml[w * RW + grp][cc];
+            const float f = __builtin_amdgcn_exp2f(e.x - base);
+            L += e.y * f;
+            const float* from =
+                reinterpret_cast<const float*>(smem + (w * RW + grp) * (32 * kKv4Dim));
+            v += f * *reinterpret_cast<const f32x4*>(from + cc * kKv4Dim + 4 * d4);
         }
-        __syncthreads();
-        for (int it = tid; it < RT * 32; it += 256) {
-            const int rr = it >> 5, d4 = it & 31, grp = rr / ROWS, cc = rr % ROWS;
-            const int r2 = row0 + rr, i2 = a.token(r2);
-            if (i2 >= n) continue;
-            float M = -INFINITY, L = 0.0f;
-            f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int w = 0; w < TW; ++w) M = fmaxf(M, sm.ml[w * RW + grp][cc].x);
-            const float base = M == -INFINITY ? 0.0f : M;
-#pragma unroll
-            for (int w = 0; w < TW; ++w) {
-                const float2 e = sm.ml[w * RW + grp][cc];
-                const float f = __builtin_amdgcn_exp2f(e.x - base);
-                L += e.y * f;
-                const float* from =
-                    reinterpret_cast<const float*>(smem + (w * RW + grp) * (32 * kKv4Dim));
-                v += f * *reinterpret_cast<const f32x4*>(from + cc * kKv4Dim + 4 * d4);
-            }
-            const int64_t g2 = (int64_t)first + i2, hd = h * a.G + (r2 - i2 * a.G);
-            if (direct(c - n + i2)) {
-                if (EVEN || g.split == 0)
-                    store4<HALF>(a, g2 * a.out_stride + hd * kKv4Dim + 4 * d4, v, L);
-            } else {
-                const int64_t at = record(rr, g2, hd);
-                *reinterpret_cast<f32x4*>(a.part_o + at * kKv4Dim + 4 * d4) = v;
-                if (d4 == 0) a.part_ml[at] = make_float2(M, L);
-            }
-        }
-        if (EVEN) __syncthreads();
-    } else if (row_ok && slot == 0) {
-        if (direct(pos)) {
-            if (g.split == 0)
-#pragma unroll
-                for (int d = 0; d < 8; ++d)
-                    store4<HALF>(a, grow * a.out_stride + (int64_t)head * kKv4Dim + 16 * d + 4 * j,
-                                 acc[d], l);
+        const int64_t g2 = (int64_t)first + i2, hd = h * a.G + (r2 - i2 * a.G);
+        // to `out` where no other piece has any of the row's tokens, else a record
+        if (EVEN ? g.whole : c - n + i2 < a.chunk || a.splits == 1) {
+            if (EVEN || g.split == 0)
+                store4<HALF>(a, g2 * a.out_stride + hd * kKv4Dim + 4 * d4, v, L);
         } else {
-            const int64_t at = record(0, grow, head);
-#pragma unroll
-            for (int d = 0; d < 8; ++d)
-                *reinterpret_cast<f32x4*>(a.part_o + at * kKv4Dim + 16 * d + 4 * j) = acc[d];
-            if (j == 0) a.part_ml[at] = make_float2(m, l);
+            const int64_t at = EVEN ? g.rec + rr : (g2 * a.Hq + hd) * a.splits + g.split;
+            *reinterpret_cast<f32x4*>(a.part_o + at * kKv4Dim + 4 * d4) = v;
+            if (d4 == 0) a.part_ml[at] = make_float2(M, L);
         }
     }
+    if (EVEN) __syncthreads();
 }
 
 // A grid of (unit, split, kv head): every workgroup one piece.
