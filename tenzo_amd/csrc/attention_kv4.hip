@@ -35,6 +35,7 @@ struct Kv4Attn {
     uint32_t g_mul;  // 2^32 / G, rounded up (0: G is 1)
     int chunk, splits;  // tokens of a split
     int wgs;            // workgroups of a call whose steps are dealt evenly
+    int most;           // and the steps that it can have, where no two sequences share rows
     int vec_out;        // out allows accesses of 4 elements
 
     // r / G, exact for r < 2^28 and G up to 16 (a division is some 40 instructions).
@@ -218,26 +219,37 @@ struct SeqWork {
     }
 };
 
-// Sum of v over the threads before this one, and over all of them (64 * NW threads).
-template <int NW>
-__device__ __forceinline__ int block_scan(int v, int* wsum, int& all) {
+// Sums that stay at the largest number once they reach it: where ranges of cu_q lie over each other
+// the sequences' work adds up to anything.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) {
+    return __builtin_elementwise_add_sat(a, b);
+}
+
+// The work of this thread's sequences, b0 up to b1, that of the threads before (the return value)
+// and of all of them; no work at all where it is more than `most`.
+template <int ROWS>
+__device__ __forceinline__ int scan_work(const Kv4Attn& a, const Kv4Seqs& sq, int b0, int b1,
+                                         uint32_t* wsum, int& mine, int& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int incl = v;
+    uint32_t v = 0;
+    for (int b = b0; b < b1; ++b) v = add_sat(v, SeqWork(sq, b, a.G, ROWS).total(sq.Hkv));
+    uint32_t incl = v;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(incl, d);
-        if (lane >= d) incl += o;
+        const uint32_t o = __shfl_up(incl, d);
+        if (lane >= d) incl = add_sat(incl, o);
     }
     if (lane == 63) wsum[wave] = incl;
     __syncthreads();
-    int before = incl - v;
-    all = 0;
+    uint32_t before = incl - v, sum = 0;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
+    for (int w = 0; w < 4; ++w) {
         before += w < wave ? wsum[w] : 0;
-        all += wsum[w];
+        sum = add_sat(sum, wsum[w]);
     }
-    return before;
+    mine = (int)v;
+    all = sum <= (uint32_t)a.most ? (int)sum : 0;
+    return (int)before;
 }
 
 // A value that all lanes of the wave hold, for scalar registers.
@@ -748,7 +760,7 @@ template <bool HALF>
 __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seqs sq) {
     // two tiles' keys and values (the first is the queries' on their way to registers before)
     __shared__ __align__(16) uint16_t tiles[2][2][kTile * kKv4Dim];
-    __shared__ __align__(16) int moved[2][kTile];  // the power of two that a token's keys are moved by
+    __shared__ __align__(16) int moved[2][kTile];  // the power of two that tokens' keys are moved by
     __shared__ int flags[2][4], tops[4];
     __shared__ int pg[kMaxPages];
     const int per_unit = sq.Hkv * a.splits;
@@ -1122,13 +1134,12 @@ template <int ROWS, bool HALF>
 __global__ void __launch_bounds__(256, ROWS == 16 ? 2 : 3)
 kv4_attn_even_kernel(Kv4Attn a, Kv4Seqs sq) {
     __shared__ Kv4Smem<ROWS, 1> sm;
-    __shared__ int wsum[4], at_base, at_seq;
+    __shared__ uint32_t wsum[4];
+    __shared__ int at_base, at_seq;
     const int per = (sq.B + 255) / 256, b0 = threadIdx.x * per;
-    int mine = 0, total;
-    for (int b = b0; b < min(sq.B, b0 + per); ++b)
-        mine += SeqWork(sq, b, a.G, ROWS).total(sq.Hkv);
     if (threadIdx.x == 0) at_seq = sq.B;
-    int base = block_scan<4>(mine, wsum, total);
+    int mine, total;
+    int base = scan_work<ROWS>(a, sq, b0, min(sq.B, b0 + per), wsum, mine, total);
     total = uniform(total);
     const int begin = wg_start(blockIdx.x, total, a.wgs);
     const int end = wg_start(blockIdx.x + 1, total, a.wgs);
@@ -1263,23 +1274,24 @@ template <int ROWS, bool HALF, bool WIDE>
 __global__ void __launch_bounds__(256) kv4_join_even_kernel(Kv4Attn a, Kv4Seqs sq) {
     __shared__ f32x4 ov[WIDE ? 8 : 1][32];
     __shared__ float lv[8];
-    __shared__ int wsum[4], at_base, at_seq;
+    __shared__ uint32_t wsum[4];
+    __shared__ unsigned long long at;  // the row's sequence, plus 1, and the work before it
     const int row = blockIdx.x, tid = threadIdx.x, grp = tid >> 5;
-    const int per = (sq.B + 255) / 256, b0 = tid * per;
-    int mine = 0, total;
-    if (tid == 0) at_seq = -1;
-    for (int b = b0; b < min(sq.B, b0 + per); ++b)
-        mine += SeqWork(sq, b, a.G, ROWS).total(sq.Hkv);
-    int base = block_scan<4>(mine, wsum, total);
-    for (int b = b0; b < min(sq.B, b0 + per); ++b) {
+    const int per = (sq.B + 255) / 256, b0 = tid * per, b1 = min(sq.B, b0 + per);
+    if (tid == 0) at = 0;
+    int mine, total;
+    int base = scan_work<ROWS>(a, sq, b0, b1, wsum, mine, total);
+    for (int b = b0; b < b1; ++b) {
         const SeqWork w(sq, b, a.G, ROWS);
-        if (row >= w.first && row < w.first + w.n) at_seq = b, at_base = base;
+        if (row >= w.first && row < w.first + w.n)
+            atomicMax(&at, (unsigned long long)(b + 1) << 32 | (uint32_t)base);
         base += w.total(sq.Hkv);
     }
     __syncthreads();
-    const int seq = uniform(at_seq), head = WIDE ? (int)blockIdx.y : (int)blockIdx.y * 8 + grp;
+    const int seq = uniform((int)(at >> 32)) - 1;
+    const int head = WIDE ? (int)blockIdx.y : (int)blockIdx.y * 8 + grp;
     if (seq < 0 || head >= a.Hq) return;
-    base = uniform(at_base);
+    base = uniform((int)at);
     total = uniform(total);
     const SeqWork w(sq, seq, a.G, ROWS);
     const int64_t out_at = row * a.out_stride + (int64_t)head * kKv4Dim;
@@ -1288,6 +1300,7 @@ __global__ void __launch_bounds__(256) kv4_join_even_kernel(Kv4Attn a, Kv4Seqs s
             store4<HALF>(a, out_at + 4 * (tid & 31), f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0.0f);
         return;
     }
+    if (total == 0) return;
     const int h = head / a.G, r = (row - w.first) * a.G + head - h * a.G;
     const int start = base + (h * w.tiles + r / ROWS) * w.slots() + 1;
     const int w0 = wg_of(start, total, a.wgs), w1 = wg_of(start + w.steps - 1, total, a.wgs);
@@ -1301,6 +1314,7 @@ __global__ void __launch_bounds__(256) kv4_join_even_kernel(Kv4Attn a, Kv4Seqs s
 struct Kv4Plan {
     int rows, rw, splits, chunk;  // rw 8: the prompts' kernel
     bool even;
+    int most;  // steps dealt evenly, at most
     int64_t wgs;
     size_t records;
 };
@@ -1333,6 +1347,7 @@ Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu) {
     p.even = p.rw == 1 && B > 1 && units * Hkv < 2 * room && units * Hkv * steps > room &&
              most <= INT32_MAX;
     if (p.even) {
+        p.most = (int)most;
         p.wgs = most < room ? most : room;
         p.splits = 1;
         p.records = (size_t)p.wgs * 2 * p.rows;
@@ -1455,6 +1470,7 @@ TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,
     a.g_mul = G == 1 ? 0 : (uint32_t)((0x100000000ull + G - 1) / G);
     a.Hq = Hq;
     a.T = (int)T;
+    a.most = p.most;
     a.chunk = p.chunk;
     a.splits = p.splits;
     a.vec_out = (((uintptr_t)out | (uintptr_t)(out_stride * (dtype ? 2 : 4))) & 15) == 0;

@@ -23,7 +23,8 @@ constexpr int kKv4Scales = 4;  // scale bytes of a row
 // (cu null: row r is sequence r's only one) and stands at position ctx[s] - n + (r - cu[s]), n
 // the sequence's rows. What the device finds in these arrays is checked before it is used: a
 // length above `limit` (the table's width, the rotation's rows) counts as 0, a range outside the T
-// rows as empty, a page outside the pool as absent.
+// rows as empty, a page outside the pool as absent. Ranges that lie over each other (cu decreasing
+// somewhere) give rows no meaning, but nothing else is read or written for them.
 struct Kv4Seqs {
     const int32_t* tables;
     const int32_t* ctx;
@@ -79,8 +80,9 @@ __device__ __forceinline__ bool kv4_place(const Kv4Seqs& q, int r, int lane16, i
             pos = c - n + (r - first);
         }
     }
+    const int mine = seq;  // (of two sequences with ranges over each other the later one)
     seq = max_row16(seq);
-    pos = max_row16(pos);
+    pos = max_row16(mine == seq ? pos : -1);
     return pos >= 0;
 }
 
