@@ -350,7 +350,7 @@ def _rope_rows(rope_cs, dev):
     if rope_cs is None:
         return None, 0
     shape = rope_cs.shape
-    if len(shape) != 2 or shape[1] != 128:
+    if len(shape) != 2 or shape[1] != 128 or not shape[0]:  # (none at all would mean no rotation)
         raise ValueError(f"rope_cs: {tuple(shape)}, not [positions][128]")
     if rope_cs.dtype is _F32 and rope_cs.get_device() == dev and rope_cs.is_contiguous():
         return rope_cs.data_ptr(), shape[0]
@@ -424,13 +424,13 @@ def attn_kv4(q, pk, pv, pks, pvs, block_tables, ctx_lens, layer: int, rope_cs=No
         op, os = _row_args(out, cols, dev, dtype, "out")
     else:
         raise ValueError(f"out: {tuple(out.shape)}, q: {tuple(q.shape)}")
+    rope = _rope_rows(rope_cs, dev)
     if not T:
         return out
     Hq = cols // 128
     nbytes = _attn_kv4_ws(T, seqs[5], Hq, Hkv, seqs[2], cu_q is not None, dt)
     ws = pk.new_empty(nbytes) if nbytes else None  # (held until the launch)
-    rc = _lib.load().tenzo_hip_attn_kv4(qp, dt, qs, *pools, *where[:3], Hq, Hkv, *seqs,
-                                        *_rope_rows(rope_cs, dev), op, os,
+    rc = _lib.load().tenzo_hip_attn_kv4(qp, dt, qs, *pools, *where[:3], Hq, Hkv, *seqs, *rope, op, os,
                                         ws.data_ptr() if nbytes else None, nbytes, _stream())
     if rc:
         _lib.check(rc, "attn_kv4")
