@@ -215,9 +215,9 @@ TENZO_HIP_API int tenzo_hip_attn_paged_int8_decode(const float* q, const float* 
  * negative positions for none, a table entry outside 0 .. n_blocks - 1 for a
  * page of absent tokens. Where cu_q decreases so that ranges lie over each
  * other, what is written for their sequences is not defined, nor which rows of
- * the call attend. Rows of no sequence (from cu_q[B] on) are neither
- * read nor written, but for the zeros of kv4_read. Tables hold up to 2^26
- * pages.
+ * the call attend. Rows of no sequence (from cu_q[B] on) are not
+ * written, but for the zeros of kv4_read; kv4_append may read theirs. Tables
+ * hold up to 2^26 pages.
  * dtype of k, v, q, out: 0 = fp32, 1 = fp16; strides in elements. */
 
 /* Rotates k ([T] rows of Hkv heads of 128, k_stride apart), rounds k and v to

@@ -430,8 +430,8 @@ def attn_kv4(q, pk, pv, pks, pvs, block_tables, ctx_lens, layer: int, rope_cs=No
     Hq = cols // 128
     nbytes = _attn_kv4_ws(T, seqs[5], Hq, Hkv, seqs[2], cu_q is not None, dt)
     ws = pk.new_empty(nbytes) if nbytes else None  # (held until the launch)
-    rc = _lib.load().tenzo_hip_attn_kv4(qp, dt, qs, *pools, *where[:3], Hq, Hkv, *seqs, *rope, op, os,
-                                        ws.data_ptr() if nbytes else None, nbytes, _stream())
+    rc = _lib.load().tenzo_hip_attn_kv4(qp, dt, qs, *pools, *where[:3], Hq, Hkv, *seqs, *rope,
+                                        op, os, ws.data_ptr() if nbytes else None, nbytes, _stream())
     if rc:
         _lib.check(rc, "attn_kv4")
     return out
