@@ -289,7 +289,7 @@ struct Segment {
 // parts stand in columns side by side (column = part * ROWS + row) and one MFMA serves all of them.
 //
 // A step loads 136 bytes a token straight to registers, the next step's during the products.
-// 130000 tokens of one sequence, 20 / 5 heads: 23.4 us, 3.8 TB/s (and 3 for the join), bound by
+// 130000 tokens of one sequence, 20 / 5 heads: 23 us, 3.8 TB/s (and 3 for the join), bound by
 // the vector work on codes and weights beside the loads; up to 256 tokens 6 us, a chain of loads
 // (length, page number, codes), the products' latency and the waves' meeting.
 template <int ROWS, int RW>
@@ -1129,7 +1129,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
 // and an equal share of them to each of as many workgroups as the GPU holds at once, so that
 // lengths, which only the device knows, need not be alike. A share holds the end of a unit that
 // an earlier workgroup began, whole units and the beginning of one: two records at most. 48
-// sequences of up to 8190 tokens (223127 in all), 32 / 8 heads, fp16: 55 us, 4.4 TB/s.
+// sequences of up to 8190 tokens (223127 in all), 32 / 8 heads, fp16: 54 us, 4.5 TB/s.
 template <int ROWS, bool HALF>
 __global__ void __launch_bounds__(256, ROWS == 16 ? 2 : 3)
 kv4_attn_even_kernel(Kv4Attn a, Kv4Seqs sq) {

@@ -332,7 +332,7 @@ __device__ __forceinline__ bool before(const BeamCand& a, const BeamCand& b) {
 // log-sums leave their order open, theirs are summed in 64 bits from the logits (27 us a beam of
 // 128256) and all are ranked once more. Where candidates are many (equal scores, masked beams) all
 // beams' are, and the k best are taken one after the other. 48 x 8 beams, 32 slices, 16 candidates:
-// 8 us, latency from end to end.
+// 8.5 us, latency from end to end.
 __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
     __shared__ double lse[kBeamMax], own[kBeamMax], peak[kBeamMax], part[16];
     __shared__ double ls[kPickCand];

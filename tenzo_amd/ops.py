@@ -298,7 +298,7 @@ def kv4_pool(n_blocks: int, n_layers: int, n_kv_heads: int, device="cuda"):
 
 # (The calls on a cache check a dozen tensors, and the smallest run for 4 us on the GPU: each
 # property is asked for once and the words for what is wrong are looked for afterwards. Host side
-# of a call: append 9 us, attn 15, select 14 (two launches each), reorder 8; the sizes of
+# of a call: append 9 us, attn 15, select 13 (two launches each), reorder 8; the sizes of
 # workspaces, a function of the arguments, are asked for once.)
 _U8, _I32, _F32 = torch.uint8, torch.int32, torch.float32
 
