@@ -326,13 +326,12 @@ __device__ __forceinline__ bool before(const BeamCand& a, const BeamCand& b) {
 
 // Stage 2, a workgroup per request: the rows' log-sums, then the best k of the slices' lists. The
 // first few of every list (2k of a beam's or more, up to 1024 in all) are put in order (sorted by
-// waves, merged in pairs), and their k-th (in fp32, rounded
-// down), less what the log-sums may be off by, is a bound that the k best reach. Those that
-// do are ranked by counting. Where one of the k best has another beam's candidate so near that the
-// log-sums leave their order open, theirs are summed in 64 bits from the logits (27 us a beam of
-// 128256) and all are ranked once more. Where candidates are many (equal scores, masked beams) all
-// beams' are, and the k best are taken one after the other. 48 x 8 beams, 32 slices, 16 candidates:
-// 8.5 us, latency from end to end.
+// waves, merged in pairs), and their k-th (in fp32, rounded down), less what the log-sums may be
+// off by, is a bound that the k best reach. Those that do are ranked by counting; where they are
+// many (equal scores, masked beams or tokens) the k best are taken one after the other. Where one
+// of the k best has another beam's candidate so near that the log-sums leave their order open, the
+// beams' are summed in 64 bits from the logits (27 us a beam of 128256) and all are ranked once
+// more. 48 x 8 beams, 32 slices, 16 candidates: 8.5 us, latency from end to end.
 __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
     __shared__ double lse[kBeamMax], own[kBeamMax], peak[kBeamMax], part[16];
     __shared__ double ls[kPickCand];
@@ -446,6 +445,10 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
         }
         __syncthreads();
     };
+    const auto sum_near = [&]() {
+        for (int w = 0; w < a.W; ++w)
+            if (near[w >> 5] >> (w & 31) & 1) sum_exactly(w);
+    };
     const int n = cnt;
     if (n <= kPickCand && opened <= kPickCand) {
         for (bool first = a.W > 1;; first = false) {
@@ -476,8 +479,7 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
             }
             __syncthreads();
             if (!first || !(near[0] | near[1])) break;
-            for (int w = 0; w < a.W; ++w)
-                if (near[w >> 5] >> (w & 31) & 1) sum_exactly(w);
+            sum_near();
             for (int i = tid; i < n; i += 1024)
                 if (ls[i] > -INFINITY) ls[i] = ((double)lx[i] - lse[lw[i]]) + own[lw[i]];
             __syncthreads();
@@ -490,33 +492,47 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamSelect a) {
             }
         return;
     }
-    if (a.W > 1)
-        for (int w = 0; w < a.W; ++w) sum_exactly(w);
-    BeamCand last{INFINITY, INFINITY, -1, -1};
     const BeamCand none{-INFINITY, -INFINITY, INT_MAX, INT_MAX};
-    for (int j = 0; j < a.k; ++j) {
-        BeamCand m = none;
-        for (int c = tid; c < total; c += 1024) {
-            const BeamCand e = get(c, cand[c]);
-            if (e.t != INT_MAX && before(last, e) && before(e, m)) m = e;
+    for (bool first = a.W > 1;; first = false) {
+        BeamCand last{INFINITY, INFINITY, -1, -1};
+        uint64_t beams = 0;
+        // (once more than k times where the last one's neighbours are looked for)
+        for (int j = 0; j < a.k + (first ? 1 : 0); ++j) {
+            BeamCand m = none;
+            for (int c = tid; c < total; c += 1024) {
+                const BeamCand e = get(c, cand[c]);
+                if (e.t == INT_MAX) continue;
+                if (first && j > 0 && e.w != last.w && fabs(e.s - last.s) <= 2 * kLogSumError)
+                    beams |= 1ull << e.w | 1ull << last.w;
+                if (before(last, e) && before(e, m)) m = e;
+            }
+            if (j == a.k) break;
+            for (int d = 32; d > 0; d >>= 1) {
+                const BeamCand o{__shfl_xor(m.s, d), __shfl_xor(m.x, d), __shfl_xor(m.w, d),
+                                 __shfl_xor(m.t, d)};
+                if (before(o, m)) m = o;
+            }
+            if (lane == 0) best[wave] = m;
+            __syncthreads();
+            m = best[0];
+            for (int w = 1; w < 16; ++w)
+                if (before(best[w], m)) m = best[w];
+            __syncthreads();
+            last = m;
+            if (tid == 0) {
+                a.out_scores[b * a.k + j] = (float)m.s;
+                a.out_beams[b * a.k + j] = m.w;
+                a.out_tokens[b * a.k + j] = m.t;
+            }
         }
-        for (int d = 32; d > 0; d >>= 1) {
-            const BeamCand o{__shfl_xor(m.s, d), __shfl_xor(m.x, d), __shfl_xor(m.w, d),
-                             __shfl_xor(m.t, d)};
-            if (before(o, m)) m = o;
+        if (!first) return;
+        if (beams) {
+            atomicOr(&near[0], (uint32_t)beams);
+            atomicOr(&near[1], (uint32_t)(beams >> 32));
         }
-        if (lane == 0) best[wave] = m;
         __syncthreads();
-        m = best[0];
-        for (int w = 1; w < 16; ++w)
-            if (before(best[w], m)) m = best[w];
-        __syncthreads();
-        last = m;
-        if (tid == 0) {
-            a.out_scores[b * a.k + j] = (float)m.s;
-            a.out_beams[b * a.k + j] = m.w;
-            a.out_tokens[b * a.k + j] = m.t;
-        }
+        if (!(near[0] | near[1])) return;
+        sum_near();
     }
 }
 

@@ -37,8 +37,10 @@ def check(torch, ops, x, s, k):
     want = plain.beam_select(x, s, k)
     np.testing.assert_array_equal(got[1].cpu().numpy(), want[1])
     np.testing.assert_array_equal(got[2].cpu().numpy(), want[2])
-    off = np.abs(got[0].cpu().numpy() - want[0])
-    assert (off <= 2.0 ** -24 * np.abs(want[0]) + 1.25e-6).all(), off.max()
+    score, real = got[0].cpu().numpy(), np.isfinite(want[0])
+    np.testing.assert_array_equal(score[~real], want[0][~real])
+    off = np.abs(score[real] - want[0][real])
+    assert (off <= 2.0 ** -24 * np.abs(want[0][real]) + 1.25e-6).all(), off.max()
 
 
 @pytest.mark.parametrize("B,W,V,k", [(40, 2, 128256, 2), (60, 4, 5000, 8), (25, 8, 32000, 16),
@@ -85,3 +87,17 @@ def test_level_sums(torch_dev, ops, V, gap):
     x = np.full((3, 1, V), -gap, np.float32) + np.float32([0, 1.3, -70.1])[:, None, None]
     x[..., V // 2] += np.float32(gap)
     check(torch_dev, ops, x, even(x, 0.0), 4)
+
+
+@pytest.mark.parametrize("allowed", [1, 3, 12])
+@pytest.mark.parametrize("V", [3000, 40000])
+def test_near_beams_of_few_tokens(torch_dev, ops, V, allowed):
+    """All but a few tokens masked, so that -inf is among the k best, and beams as near as fp32 puts
+    their scores."""
+    rng = np.random.default_rng(V + allowed)
+    x = level(rng, 30, 8, V, 1)
+    keep = rng.permutation(V)[:allowed]
+    y = np.full_like(x, -np.inf)
+    y[..., keep] = np.sort(x[..., rng.permutation(V)[:allowed]], -1)
+    y[..., keep[0]] += np.float32(7)
+    check(torch_dev, ops, y, even(y, -3.0), 16)
