@@ -33,11 +33,21 @@ def even(x, at):
 
 
 def check(torch, ops, x, s, k):
+    """Beams and tokens as in 64 bits. Candidates that are mathematically equal may lie 2^-46 from
+    each other there, in any order: sums of exponentials are rounded to some 20 * 2^-53 of
+    themselves (in pairs), the log, its sum with the largest logit and the two differences to
+    2^-53 of numbers up to 20 each, in numpy and in the kernel."""
     got = ops.beam_select(torch.from_numpy(x).cuda(), torch.from_numpy(s).cuda(), k)
+    score, beam, token = (a.cpu().numpy() for a in got)
     want = plain.beam_select(x, s, k)
-    np.testing.assert_array_equal(got[1].cpu().numpy(), want[1])
-    np.testing.assert_array_equal(got[2].cpu().numpy(), want[2])
-    score, real = got[0].cpu().numpy(), np.isfinite(want[0])
+    if (beam != want[1]).any() or (token != want[2]).any():
+        at = (np.arange(len(x))[:, None], beam, token)
+        mine = x[at] - log_sums(x)[at[:2]] + s[at[:2]]
+        real = np.isfinite(want[0])
+        assert (np.abs(mine - want[0])[real] <= 2.0 ** -46).all()
+        np.testing.assert_array_equal(mine[~real], want[0][~real])
+        assert all(len(set(zip(*c))) == k for c in zip(beam, token))
+    real = np.isfinite(want[0])
     np.testing.assert_array_equal(score[~real], want[0][~real])
     off = np.abs(score[real] - want[0][real])
     assert (off <= 2.0 ** -24 * np.abs(want[0][real]) + 1.25e-6).all(), off.max()
