@@ -207,17 +207,16 @@ TENZO_HIP_API int tenzo_hip_attn_paged_int8_decode(const float* q, const float* 
  * included. Its rows are cu_q[b] .. cu_q[b + 1] - 1 (cu_q: B + 1 non-decreasing
  * row numbers; null: row b is sequence b's only one, T == B) and stand at its
  * last positions: row i of n at ctx_lens[b] - n + i. rope_cs: n_pos rows of
- * cos[64], sin[64], row p for position p (null: no rotation).
- * ctx_lens, cu_q and the tables are read on the device, so what is wrong there
- * is left out, not reported: a length of 0 or less or above
- * min(16 * table_width, n_pos) stands for a padding slot (no tokens), a range
- * of cu_q that is not one of the T rows for a sequence without rows, rows at
- * negative positions for none, a table entry outside 0 .. n_blocks - 1 for a
- * page of absent tokens. Where cu_q decreases so that ranges lie over each
- * other, what is written for their sequences is not defined, nor which rows of
- * the call attend. Rows of no sequence (from cu_q[B] on) are not
- * written, but for the zeros of kv4_read; kv4_append may read theirs. Tables
- * hold up to 2^26 pages.
+ * cos[64], sin[64], row p for position p (null: no rotation). ctx_lens, cu_q
+ * and the tables are read on the device, so what is wrong there is left out,
+ * not reported: a length of 0 or less or above min(16 * table_width, n_pos)
+ * stands for a padding slot (no tokens), a range of cu_q that is not one of the
+ * T rows for a sequence without rows, rows at negative positions for none, a
+ * table entry outside 0 .. n_blocks - 1 for a page of absent tokens. Where cu_q
+ * decreases so that ranges lie over each other, what is written for their
+ * sequences is not defined, nor which rows of the call attend. Rows of no
+ * sequence (from cu_q[B] on) are not written, but for the zeros of kv4_read;
+ * kv4_append may read theirs. Tables hold up to 2^26 pages.
  * dtype of k, v, q, out: 0 = fp32, 1 = fp16; strides in elements. */
 
 /* Rotates k ([T] rows of Hkv heads of 128, k_stride apart), rounds k and v to
@@ -255,12 +254,12 @@ TENZO_HIP_API int tenzo_hip_kv4_read(const uint8_t* pk, const uint8_t* pv, const
  * sequence, and many of them or a wide table) 22, and there weights below 2^-40
  * of a row's largest are lost, and where scales leave the range of fp16 also
  * what lies below 2^-37 of the largest: of a key's elements, and of the values
- * that a workgroup's rows see. Hq / Hkv 1 to 16. out must not overlap q. ws: a workspace
- * of tenzo_hip_attn_kv4_ws_bytes(...) bytes, 16-byte aligned, of this call
- * alone until it has run (null where that is 0); has_cu: cu_q is not null. The
- * split of rows and tokens over workgroups follows from T, B, the heads and
- * table_width (the longest context that the call can have), so a row's sums
- * may be rounded differently in another batch. */
+ * that a workgroup's rows see. Hq / Hkv 1 to 16. out must not overlap q. ws: a
+ * workspace of tenzo_hip_attn_kv4_ws_bytes(...) bytes, 16-byte aligned, of this
+ * call alone until it has run (null where that is 0); has_cu: cu_q is not null.
+ * The split of rows and tokens over workgroups follows from T, B, the heads and
+ * table_width (the longest context that the call can have), so a row's sums may
+ * be rounded differently in another batch. */
 TENZO_HIP_API size_t tenzo_hip_attn_kv4_ws_bytes(int64_t T, int B, int Hq, int Hkv,
                                                  int table_width, int has_cu, int dtype);
 TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,
@@ -372,10 +371,11 @@ TENZO_HIP_API int tenzo_hip_sample_top_k_top_p(const float* logits, int64_t V, i
  * (w) and out_tokens (t), each [B][k]. The order is that of scores in 64 bits
  * (log-sums come from exponentials in fp32, and anew from 64-bit ones where
  * beams' candidates are within 2.5e-6); among equal ones the lower beam comes
- * first, then the larger logit, then the lower token. A score written is off
- * by at most 1.25e-6 and its rounding to fp32. A logit or a score that is not below +inf (NaN too) counts as -inf;
- * -inf candidates come last. W and k up to 64, k <= W * V, V up to 2^30 and
- * W * V below 2^31. ws: as above, tenzo_hip_beam_select_ws_bytes(...) bytes. */
+ * first, then the larger logit, then the lower token. A score written is off by
+ * at most 1.25e-6 and its rounding to fp32. A logit or a score that is not
+ * below +inf (NaN too) counts as -inf; -inf candidates come last. W and k up to
+ * 64, k <= W * V, V up to 2^30 and W * V below 2^31. ws: as above,
+ * tenzo_hip_beam_select_ws_bytes(...) bytes. */
 TENZO_HIP_API size_t tenzo_hip_beam_select_ws_bytes(int B, int W, int64_t V, int k);
 TENZO_HIP_API int tenzo_hip_beam_select(const float* logits, int64_t row_stride,
                                         const float* scores, int B, int W, int64_t V, int k,
