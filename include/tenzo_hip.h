@@ -272,6 +272,89 @@ TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,
                                      int64_t out_stride, void* ws, size_t ws_bytes,
                                      void* stream);
 
+/* ---- trees of drafted tokens over a paged cache -------------------------- */
+
+/* No counterpart in the reference. A sequence's rows of a call (cu_q, ctx_lens
+ * as above) are the nodes of a tree: node i of n is row i of the sequence and
+ * stands in slot ctx_lens[b] - n + i of its cache, at position ctx_lens[b] - n
+ * plus its depth. parents[row] is the place of a node's parent among the
+ * sequence's nodes; a negative one, or one that does not come before the node
+ * itself, is none (depth 0). One step: tree_plan, then in each layer rope at the
+ * nodes' positions, kv4_append without a rotation and attn_tree_kv4, then
+ * tree_accept. */
+
+/* mask[row] (ceil(most / 64) words, bit j of word w: node 64 w + j) holds a
+ * node's ancestors and itself, positions[row] its position; both 0 in padding
+ * slots and for nodes whose slot is negative. most (1 to 4096): at least the
+ * nodes of any sequence; those from `most` on are not written, nor rows of no
+ * sequence. mask 8-byte aligned. */
+TENZO_HIP_API int tenzo_hip_tree_plan(const int32_t* parents, const int32_t* ctx_lens,
+                                      const int32_t* cu_q, int B, int64_t T, int most,
+                                      uint64_t* mask, int32_t* positions, void* stream);
+/* Attention of the nodes over the cache: tenzo_hip_attn_kv4 with the same
+ * arguments, accuracy and workspace rules, but that q is taken as it is (rotated
+ * before, by tenzo_hip_rope), and that node i sees the ctx_lens[b] - n tokens in
+ * front of the tree and the nodes j whose bit is set in its row of mask
+ * (mask_words words, mask_stride words apart, 8-byte aligned; any bits, its own
+ * too; nodes behind the last word are not seen). */
+TENZO_HIP_API size_t tenzo_hip_attn_tree_kv4_ws_bytes(int64_t T, int B, int Hq, int Hkv,
+                                                      int table_width, int has_cu, int dtype);
+TENZO_HIP_API int tenzo_hip_attn_tree_kv4(const void* q, int dtype, int64_t q_stride,
+                                          const uint64_t* mask, int64_t mask_stride,
+                                          int mask_words, const uint8_t* pk, const uint8_t* pv,
+                                          const uint8_t* pks, const uint8_t* pvs,
+                                          int64_t n_blocks, int n_layers, int layer, int Hq,
+                                          int Hkv, const int32_t* block_tables,
+                                          int64_t table_stride, int table_width,
+                                          const int32_t* ctx_lens, const int32_t* cu_q, int B,
+                                          int64_t T, void* out, int64_t out_stride, void* ws,
+                                          size_t ws_bytes, void* stream);
+/* The path of each sequence's tree that the model agrees with, and the cache
+ * after it. Node 0 is taken as it is (its token is known); from node u on the
+ * lowest child v of u with tokens[v] == target[u], the token that the model
+ * gives after u. path[b] ([B][most] int32): the nodes of the path, -1 behind
+ * them (a path ends at `most`, 1 to 4096); count[b]: how many; next[b]: target
+ * of the last one; lens[b]: ctx_lens[b] - n + count[b]. Sequences without rows,
+ * without tokens or with fewer tokens than rows: no path, -1, lens as before.
+ * The k-th node's cache rows, in every layer and head, are moved to slot
+ * ctx_lens[b] - n + k; slots from lens[b] on hold what is left there. Pools as
+ * tenzo_hip_beam_reorder_paged has them; a page that the pool does not hold
+ * takes and gives nothing. Slots of one page in two sequences race. */
+TENZO_HIP_API int tenzo_hip_tree_accept(const int32_t* parents, const int32_t* tokens,
+                                        const int32_t* target, void* pk, void* pv, void* pks,
+                                        void* pvs, int64_t n_blocks, int n_layers, int Hkv,
+                                        int row_bytes, const int32_t* block_tables,
+                                        int64_t table_stride, int table_width,
+                                        const int32_t* ctx_lens, const int32_t* cu_q, int B,
+                                        int64_t T, int most, int32_t* path, int32_t* count,
+                                        int32_t* next, int32_t* lens, void* stream);
+
+/* ---- rotary positions ----------------------------------------------------- */
+
+/* Turns T rows of H heads of head_dim (rows x_stride apart) by their positions:
+ * with t = positions[row] * freqs[i], i < rot_dim / 2, the pair (a, b) becomes
+ * mscale * (a cos t - b sin t, a sin t + b cos t). Pairs are dims i and
+ * i + rot_dim / 2 (interleaved 0) or 2i and 2i + 1 (1); dims from rot_dim on are
+ * kept. dtype of x and out: 0 = fp32, 1 = fp16, 2 = bf16; computed in fp32 and
+ * rounded once. Cosines and sines are within 2^-23 and 2^-51 of the angle, which
+ * is taken in 64 bits. Any strides and alignment of rows; out may be x (with
+ * its stride), else it must not overlap it. head_dim up to 1024, H * head_dim up
+ * to 32768. */
+TENZO_HIP_API int tenzo_hip_rope(const void* x, int dtype, int64_t x_stride,
+                                 const int32_t* positions, const double* freqs, int64_t T, int H,
+                                 int head_dim, int rot_dim, int interleaved, float mscale,
+                                 void* out, int64_t out_stride, void* stream);
+/* HOST function: the rot_dim / 2 frequencies (radians a position) and the factor
+ * of cosines and sines for tenzo_hip_rope: theta^(-2i / rot_dim), and for
+ * contexts `factor` times as long as the `trained` positions by scaling: 0 as they
+ * are; 1 divided by factor; 2 theta times factor^(rot_dim / (rot_dim - 2)); 3 by
+ * parts (YaRN, Peng et al. 2023): divided by factor below `slow` turns within the
+ * trained positions, kept above `fast`, in between a blend linear in the turns,
+ * with *mscale = 0.1 ln(factor) + 1 (1 otherwise). */
+TENZO_HIP_API int tenzo_hip_rope_freqs(int rot_dim, double theta, int scaling, double factor,
+                                       double trained, double fast, double slow,
+                                       double* freqs_host, float* mscale);
+
 /* HOST function: fills cs[pos - pos0][0..127] = cos/sin table rows for
  * positions pos0 .. pos0+n_pos-1 with the reference's RoPE angles
  * (TenzoEngine.cpp:465-469; theta is 10000 there and a parameter here). */
@@ -348,6 +431,23 @@ TENZO_HIP_API int tenzo_hip_lm_head_i8_codes(const int8_t* codes, const tenzo_hi
  * the first maximum, written to *out_idx (device int32). */
 TENZO_HIP_API int tenzo_hip_argmax(const float* logits, int64_t V, int32_t* out_idx,
                                    void* stream);
+/* The product of tenzo_hip_lm_head_i8_codes for M rows, no counterpart in the
+ * reference: y[m][n] = float(sum_k codes[m][k] * W[n][k]) * (q[m].inv_scale *
+ * scales[n]), the sums exact in int32 and a row's values bit for bit those of
+ * that call. codes: rows codes_stride apart (a multiple of 16), as
+ * tenzo_hip_rmsnorm_quant127 writes them (code_sum is not read); w_packed from
+ * tenzo_hip_i8_rows_repack of N x K weights of any projection; y: rows y_stride
+ * apart, dtype 0 = fp32, 1 = fp16, 2 = bf16. K % 16 == 0, up to 131056; M up to
+ * 2^20. When out_idx is non-null, also each row's column of the largest value
+ * (in fp32, before it is rounded to dtype; the lowest of equal ones; NaN counts as
+ * -inf), by way of ws: a workspace of tenzo_hip_gemm_i8_ws_bytes(...) bytes,
+ * 8-byte aligned, of this call alone until it has run. */
+TENZO_HIP_API size_t tenzo_hip_gemm_i8_ws_bytes(int64_t M, int64_t N, int64_t K, int want_idx);
+TENZO_HIP_API int tenzo_hip_gemm_i8(const int8_t* codes, int64_t codes_stride,
+                                    const tenzo_hip_actq_t* q, const void* w_packed,
+                                    const float* scales, int64_t M, int64_t N, int64_t K, void* y,
+                                    int dtype, int64_t y_stride, int32_t* out_idx, void* ws,
+                                    size_t ws_bytes, void* stream);
 /* The model loader's int8 LM-head quantization (load_model_from_files,
  * TenzoEngine.cpp:1925-1941) of V fp32 rows of H, as the reference is built
  * (-ffast-math): scales[v] = amax * (1/127) (amax floored at 1e-8), codes =

@@ -15,6 +15,7 @@ _I64 = ctypes.c_int64
 _F = ctypes.c_float
 _SZ = ctypes.c_size_t
 _S = ctypes.c_char_p
+_D = ctypes.c_double
 
 # name: (restype, argtypes)
 SIGNATURES = {
@@ -51,6 +52,17 @@ SIGNATURES = {
     "tenzo_hip_beam_select": (_I, [_P, _I64, _P, _I, _I, _I64, _I, _P, _P, _P, _P, _SZ, _P]),
     "tenzo_hip_beam_reorder_paged": (_I, [_P, _I64, _P, _I64, _I, _P, _I, _I, _P, _P, _P, _P,
                                           _I64, _I, _I, _I, _P]),
+    "tenzo_hip_tree_plan": (_I, [_P, _P, _P, _I, _I64, _I, _P, _P, _P]),
+    "tenzo_hip_attn_tree_kv4_ws_bytes": (_SZ, [_I64, _I, _I, _I, _I, _I, _I]),
+    "tenzo_hip_attn_tree_kv4": (_I, [_P, _I, _I64, _P, _I64, _I, _P, _P, _P, _P, _I64, _I, _I, _I,
+                                     _I, _P, _I64, _I, _P, _P, _I, _I64, _P, _I64, _P, _SZ, _P]),
+    "tenzo_hip_tree_accept": (_I, [_P, _P, _P, _P, _P, _P, _P, _I64, _I, _I, _I, _P, _I64, _I, _P,
+                                   _P, _I, _I64, _I, _P, _P, _P, _P, _P]),
+    "tenzo_hip_rope": (_I, [_P, _I, _I64, _P, _P, _I64, _I, _I, _I, _I, _F, _P, _I64, _P]),
+    "tenzo_hip_rope_freqs": (_I, [_I, _D, _I, _D, _D, _D, _D, _P, _P]),
+    "tenzo_hip_gemm_i8_ws_bytes": (_SZ, [_I64, _I64, _I64, _I]),
+    "tenzo_hip_gemm_i8": (_I, [_P, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _I, _I64, _P, _P, _SZ,
+                               _P]),
     "tenzo_hip_rope_table": (None, [_F, _I, _I, _I, _P]),
     "tenzo_hip_gemv_q4_0": (_I, [_P, _I, _P, _P, _I, _I, _I, _P]),
     "tenzo_hip_gemv_q8_0": (_I, [_P, _I, _P, _P, _I, _I, _I, _P]),

@@ -29,6 +29,9 @@ struct Kv4Attn {
     const uint8_t* pks;
     const uint8_t* pvs;
     const float* rope;
+    const uint64_t* mask;  // trees: the nodes that a row sees, `words` of 64 bits a row
+    int64_t mask_stride;
+    int words;
     float* part_o;    // records of rows' unfinished sums: 128 sums,
     float2* part_ml;  // maximum (base 2) and sum of weights
     int G, Hq, T;
@@ -167,6 +170,19 @@ __device__ __forceinline__ void store4(const Kv4Attn& a, int64_t at, f32x4 v, fl
     }
 }
 
+// Trees of drafted tokens: a sequence's rows are the nodes in its last n slots, and a row sees the
+// c - n tokens before them and the nodes that its mask has. Of the 64 tokens from t on, one bit
+// each: whether row `row` (of all T) of a tree whose first node is in slot `base` sees them.
+__device__ __forceinline__ uint64_t seen64(const Kv4Attn& a, int64_t row, int t, int base, int c) {
+    const uint64_t* m = a.mask + row * a.mask_stride;
+    const int o = t - base, w = o >> 6, sh = o & 63;  // (w -1: the step has tokens before the tree)
+    const uint64_t lo = w >= 0 && w < a.words ? m[w] : w < 0 ? ~0ull : 0;
+    const uint64_t hi = w >= -1 && w + 1 < a.words ? m[w + 1] : w < -1 ? ~0ull : 0;
+    uint64_t bits = sh ? lo >> sh | hi << (64 - sh) : lo;
+    if (c - t < 64) bits &= (1ull << max(c - t, 0)) - 1;
+    return bits;
+}
+
 // Sequence and row tile of a work unit: the unit-th tile when every sequence has
 // ceil(rows * G / RT) of them. False past the last.
 __device__ __forceinline__ bool find_unit(const Kv4Seqs& sq, int unit, int G, int RT, int& seq,
@@ -303,7 +319,7 @@ struct Kv4Smem {
     int pg[kMaxPages];
 };
 
-template <int ROWS, int RW, bool HALF, bool EVEN>
+template <int ROWS, int RW, bool HALF, bool EVEN, bool TREE>
 __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq, const Segment& g,
                                             Kv4Smem<ROWS, RW>& sm) {
     constexpr int SLOTS = 16 / ROWS, NM = SLOTS == 1 ? kParts : 1, TW = 4 / RW, RT = ROWS * RW;
@@ -321,7 +337,8 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
     const int n = g.n, first = g.first, c = g.c, h = g.h, t0 = g.t0;
     const int row0 = g.tile * RT;  // of the sequence's n * G
     const int last_i = min(n - 1, a.token(row0 + RT - 1));
-    const int t1 = min(min(t0 + g.len, c - n + last_i + 1), c);  // tokens that some row sees
+    // tokens that some row sees
+    const int t1 = TREE ? min(t0 + g.len, c) : min(min(t0 + g.len, c - n + last_i + 1), c);
 
     // the lane's row
     const int slot = col / ROWS, qi = a.token(row0 + rw * ROWS + col % ROWS);
@@ -508,12 +525,16 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
                     s[tt][i] = v;
                 }
             // a step that a row may not see whole: past its position, or absent pages
-            if (bad || t + kTile - 1 > c - n + a.token(row0)) {
+            if (bad || t + kTile - 1 > (TREE ? c - n - 1 : c - n + a.token(row0))) {
+                const uint64_t bits =
+                    TREE && pos >= 0 ? seen64(a, first + qi, t, c - n, c) >> (4 * j) : 0;
 #pragma unroll
                 for (int tt = 0; tt < kSub; ++tt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (id_now[tt] < 0 || t + 16 * tt + 4 * j + i > pos) s[tt][i] = -INFINITY;
+                        if (id_now[tt] < 0 || (TREE ? !(bits >> (16 * tt + i) & 1)
+                                                    : t + 16 * tt + 4 * j + i > pos))
+                            s[tt][i] = -INFINITY;
             }
 #pragma unroll
             for (int tt = 0; tt < kSub; ++tt)
@@ -655,7 +676,8 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
         }
         const int64_t g2 = (int64_t)first + i2, hd = h * a.G + (r2 - i2 * a.G);
         // to `out` where no other piece has any of the row's tokens, else a record
-        if (EVEN ? g.whole : c - n + i2 < a.chunk || a.splits == 1) {
+        const int last = TREE && c - n + i2 >= 0 ? c - 1 : c - n + i2;  // token that the row sees
+        if (EVEN ? g.whole : last < a.chunk || a.splits == 1) {
             if (EVEN || g.split == 0)
                 store4<HALF>(a, g2 * a.out_stride + hd * kKv4Dim + 4 * d4, v, L);
         } else {
@@ -668,7 +690,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& a, const Kv4Seqs& sq,
 }
 
 // A grid of (unit, split, kv head): every workgroup one piece.
-template <int ROWS, int RW, bool HALF>
+template <int ROWS, int RW, bool HALF, bool TREE>
 __global__ void __launch_bounds__(256, ROWS == 16 ? 2 : 3)
 kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
     __shared__ Kv4Smem<ROWS, RW> sm;
@@ -685,8 +707,8 @@ kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
     g.t0 = g.split * a.chunk;
     g.len = a.chunk;
     const int last_i = min(g.n - 1, a.token(g.tile * ROWS * RW + ROWS * RW - 1));
-    if (g.split > 0 && g.t0 >= min(g.c - g.n + last_i + 1, g.c)) return;
-    kv4_segment<ROWS, RW, HALF, false>(a, sq, g, sm);
+    if (g.split > 0 && g.t0 >= (TREE ? g.c : min(g.c - g.n + last_i + 1, g.c))) return;
+    kv4_segment<ROWS, RW, HALF, false, TREE>(a, sq, g, sm);
 }
 
 constexpr int kRowsRT = 128;
@@ -756,7 +778,7 @@ __device__ __forceinline__ bool find_unit_latest(const Kv4Seqs& sq, int unit, in
 // that with the parts). The matrix units are busy for a third of it and the vector units nearly as
 // long, and two waves a SIMD, all that the registers allow, overlap them only in part; 16 us go
 // into a workgroup's queries and outputs.
-template <bool HALF>
+template <bool HALF, bool TREE>
 __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seqs sq) {
     // two tiles' keys and values (the first is the queries' on their way to registers before)
     __shared__ __align__(16) uint16_t tiles[2][2][kTile * kKv4Dim];
@@ -773,7 +795,8 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
     const int c = sq.length(seq);
     const int t0 = split * a.chunk, row0 = tile * kRowsRT;
     const int last_i = min(n - 1, a.token(row0 + kRowsRT - 1));
-    const int t1 = min(min(t0 + a.chunk, c - n + last_i + 1), c);  // tokens that some row sees
+    // tokens that some row sees
+    const int t1 = TREE ? min(t0 + a.chunk, c) : min(min(t0 + a.chunk, c - n + last_i + 1), c);
     if (split > 0 && t0 >= t1) return;
 
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, j = lane >> 4;
@@ -898,8 +921,9 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
             *reinterpret_cast<uint4*>(dst + wave * 16 * kKv4Dim + wr[st]) =
                 fp4_to_half8(w[st], sc);
     };
-    const int low = c - n + a.token(wrow);                      // the wave's first position
-    const int high = c - n + min(n - 1, a.token(wrow + 31));  // and its last
+    // the last token that all of the wave's rows see, and that any does
+    const int low = TREE ? c - n - 1 : c - n + a.token(wrow);
+    const int high = TREE ? c - 1 : c - n + min(n - 1, a.token(wrow + 31));
     // A tile into its half of LDS. What fp16 does not hold as it is: keys are moved token by token;
     // values all together, which waits for the tile's turn (the values then go in again).
     int vby = 0;
@@ -1007,13 +1031,17 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
             float shift[2];
 #pragma unroll
             for (int ct = 0; ct < 2; ++ct) {
-                if (mask)
+                if (mask) {
+                    const uint64_t bits =
+                        TREE && pos[ct] >= 0 ? seen64(a, grow[ct], t, c - n, c) >> (4 * j) : 0;
 #pragma unroll
                     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (ids[tt] < 0 || t + 16 * tt + 4 * j + i > pos[ct])
+                            if (ids[tt] < 0 || (TREE ? !(bits >> (16 * tt + i) & 1)
+                                                     : t + 16 * tt + 4 * j + i > pos[ct]))
                                 s[ct][tt][i] = -INFINITY;
+                }
                 float top[4];
 #pragma unroll
                 for (int tt = 0; tt < 4; ++tt)
@@ -1100,7 +1128,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
             for (int i = 0; i < 4; ++i) v[i] = __builtin_ldexpf(v[i], e);
             return v;
         };
-        if (pos[ct] < a.chunk || a.splits == 1) {
+        if ((TREE && pos[ct] >= 0 ? c - 1 : pos[ct]) < a.chunk || a.splits == 1) {
             if (split > 0) continue;
             if (vshift != 0 && L != 0.0f) {
 #pragma unroll
@@ -1130,7 +1158,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
 // lengths, which only the device knows, need not be alike. A share holds the end of a unit that
 // an earlier workgroup began, whole units and the beginning of one: two records at most. 48
 // sequences of up to 8190 tokens (223127 in all), 32 / 8 heads, fp16: 54 us, 4.5 TB/s.
-template <int ROWS, bool HALF>
+template <int ROWS, bool HALF, bool TREE>
 __global__ void __launch_bounds__(256, ROWS == 16 ? 2 : 3)
 kv4_attn_even_kernel(Kv4Attn a, Kv4Seqs sq) {
     __shared__ Kv4Smem<ROWS, 1> sm;
@@ -1183,7 +1211,7 @@ kv4_attn_even_kernel(Kv4Attn a, Kv4Seqs sq) {
         g.whole = to - from == w.steps;
         g.rec = ((int64_t)blockIdx.x * 2 + (from == 0 ? 1 : 0)) * ROWS;
         g.split = 0;
-        kv4_segment<ROWS, 1, HALF, true>(a, sq, g, sm);
+        kv4_segment<ROWS, 1, HALF, true, TREE>(a, sq, g, sm);
     }
 }
 
@@ -1253,13 +1281,15 @@ constexpr int kWideJoin = 1024;
 
 // Joins the splits of a grid: a workgroup has a row's head (WIDE: few rows, many records a head,
 // shared by 16 groups of lanes) or 16 of its heads.
-template <bool HALF, bool WIDE>
+template <bool HALF, bool WIDE, bool TREE>
 __global__ void __launch_bounds__(512) kv4_join_kernel(Kv4Attn a, Kv4Seqs sq) {
     __shared__ f32x4 ov[WIDE ? 16 : 1][32];
     __shared__ float lv[16];
     const int row = blockIdx.x, tid = threadIdx.x, grp = tid >> 5;
     int seq, pos;
-    if (!kv4_place(sq, row, tid & 15, seq, pos) || pos < a.chunk) return;
+    if (!kv4_place(sq, row, tid & 15, seq, pos)) return;
+    if (TREE) pos = sq.length(seq) - 1;  // (the last token that the row sees)
+    if (pos < a.chunk) return;
     const int head = WIDE ? (int)blockIdx.y : (int)blockIdx.y * 16 + grp;
     if (head >= a.Hq) return;
     const Records rc{((int64_t)row * a.Hq + head) * a.splits, 1, 0, pos / a.chunk + 1};
@@ -1367,13 +1397,15 @@ Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu) {
     return p;
 }
 
-template <int ROWS, int RW, bool HALF>
+template <int ROWS, int RW, bool HALF, bool TREE>
 void launch_kv4(const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
-    hipLaunchKernelGGL((kv4_attn_kernel<ROWS, RW, HALF>), dim3(a.wgs), dim3(256), 0, st, a, s);
+    hipLaunchKernelGGL((kv4_attn_kernel<ROWS, RW, HALF, TREE>), dim3(a.wgs), dim3(256), 0, st, a,
+                       s);
 }
-template <int ROWS, bool HALF>
+template <int ROWS, bool HALF, bool TREE>
 int launch_kv4_even(const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
-    hipLaunchKernelGGL((kv4_attn_even_kernel<ROWS, HALF>), dim3(a.wgs), dim3(256), 0, st, a, s);
+    hipLaunchKernelGGL((kv4_attn_even_kernel<ROWS, HALF, TREE>), dim3(a.wgs), dim3(256), 0, st, a,
+                       s);
     const int rc = launch_status("kv4_attn_even_kernel");
     if (rc) return rc;
     // few rows: a head to a workgroup, its records to 8 groups of lanes
@@ -1385,27 +1417,65 @@ int launch_kv4_even(const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
                            dim3(a.T, (a.Hq + 7) / 8), dim3(256), 0, st, a, s);
     return launch_status("kv4_join_even_kernel");
 }
-template <bool HALF>
+template <bool HALF, bool TREE>
 int launch_kv4_plan(const Kv4Plan& p, const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
     if (p.even)
-        return p.rows == 4 ? launch_kv4_even<4, HALF>(a, s, st)
-                           : launch_kv4_even<16, HALF>(a, s, st);
+        return p.rows == 4 ? launch_kv4_even<4, HALF, TREE>(a, s, st)
+                           : launch_kv4_even<16, HALF, TREE>(a, s, st);
     if (p.rows == 4)
-        launch_kv4<4, 1, HALF>(a, s, st);
+        launch_kv4<4, 1, HALF, TREE>(a, s, st);
     else if (p.rw == 1)
-        launch_kv4<16, 1, HALF>(a, s, st);
+        launch_kv4<16, 1, HALF, TREE>(a, s, st);
     else if (p.rw == 2)
-        launch_kv4<16, 2, HALF>(a, s, st);
+        launch_kv4<16, 2, HALF, TREE>(a, s, st);
     else
-        hipLaunchKernelGGL(kv4_attn_rows_kernel<HALF>, dim3(a.wgs), dim3(256), 0, st, a, s);
+        hipLaunchKernelGGL((kv4_attn_rows_kernel<HALF, TREE>), dim3(a.wgs), dim3(256), 0, st, a,
+                           s);
     const int rc = launch_status("kv4_attn_kernel");
     if (rc || p.splits == 1) return rc;
     if ((int64_t)a.T * a.Hq <= kWideJoin)
-        hipLaunchKernelGGL((kv4_join_kernel<HALF, true>), dim3(a.T, a.Hq), dim3(512), 0, st, a, s);
+        hipLaunchKernelGGL((kv4_join_kernel<HALF, true, TREE>), dim3(a.T, a.Hq), dim3(512), 0, st,
+                           a, s);
     else
-        hipLaunchKernelGGL((kv4_join_kernel<HALF, false>), dim3(a.T, (a.Hq + 15) / 16), dim3(512),
-                           0, st, a, s);
+        hipLaunchKernelGGL((kv4_join_kernel<HALF, false, TREE>), dim3(a.T, (a.Hq + 15) / 16),
+                           dim3(512), 0, st, a, s);
     return launch_status("kv4_join_kernel");
+}
+
+// What both entry points check and launch: a.mask is null without a tree.
+int attn_kv4(const char* what, Kv4Attn& a, Kv4Seqs& s, int dtype, int table_width, size_t need,
+             void* ws, size_t ws_bytes, hipStream_t st) {
+    TZ_CHECK(dtype == 0 || dtype == 1, "%s: dtype %d", what, dtype);
+    TZ_CHECK(a.Hq > 0 && a.Hq % s.Hkv == 0 && a.Hq / s.Hkv <= 16,
+             "%s: 1 to 16 query heads a kv head (Hq=%d Hkv=%d)", what, a.Hq, s.Hkv);
+    if (s.T == 0 || s.B == 0) return TENZO_SUCCESS;
+    TZ_CHECK(a.q && a.out, "%s: null pointer", what);
+    TZ_CHECK(s.T == 1 || (a.q_stride >= (int64_t)a.Hq * kKv4Dim &&
+                          a.out_stride >= (int64_t)a.Hq * kKv4Dim),
+             "%s: row strides %lld, %lld below %d heads", what, (long long)a.q_stride,
+             (long long)a.out_stride, a.Hq);
+    TZ_CHECK(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0),
+             "%s: %zu bytes of workspace needed, 16-byte aligned, %zu given", what, need,
+             ws ? ws_bytes : 0);
+    const int G = a.Hq / s.Hkv;
+    const Kv4Plan p = kv4_plan(s.T, s.B, G, s.Hkv, table_width, s.cu != nullptr);
+    TZ_CHECK(p.wgs <= 0xffffff && s.T <= 0x7fffff && a.Hq <= 65535, "%s: %d rows of %d heads",
+             what, s.T, a.Hq);
+    a.part_o = (float*)ws;
+    a.part_ml = (float2*)((char*)ws + p.records * kKv4Dim * 4);
+    a.wgs = (int)p.wgs;
+    a.G = G;
+    a.g_mul = G == 1 ? 0 : (uint32_t)((0x100000000ull + G - 1) / G);
+    a.T = s.T;
+    a.most = p.most;
+    a.chunk = p.chunk;
+    a.splits = p.splits;
+    a.vec_out = (((uintptr_t)a.out | (uintptr_t)(a.out_stride * (dtype ? 2 : 4))) & 15) == 0;
+    if (a.mask)
+        return dtype ? launch_kv4_plan<true, true>(p, a, s, st)
+                     : launch_kv4_plan<false, true>(p, a, s, st);
+    return dtype ? launch_kv4_plan<true, false>(p, a, s, st)
+                 : launch_kv4_plan<false, false>(p, a, s, st);
 }
 
 }  // namespace
@@ -1436,23 +1506,6 @@ TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,
                              block_tables, table_stride, table_width, ctx_lens, cu_q, B, T,
                              rope_cs, n_pos, s);
     if (rc) return rc;
-    TZ_CHECK(dtype == 0 || dtype == 1, "attn_kv4: dtype %d", dtype);
-    TZ_CHECK(Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= 16,
-             "attn_kv4: 1 to 16 query heads a kv head (Hq=%d Hkv=%d)", Hq, Hkv);
-    if (T == 0 || B == 0) return TENZO_SUCCESS;
-    TZ_CHECK(q && out, "attn_kv4: null pointer");
-    TZ_CHECK(T == 1 || (q_stride >= (int64_t)Hq * kKv4Dim && out_stride >= (int64_t)Hq * kKv4Dim),
-             "attn_kv4: row strides %lld, %lld below %d heads", (long long)q_stride,
-             (long long)out_stride, Hq);
-    const size_t need = tenzo_hip_attn_kv4_ws_bytes(T, B, Hq, Hkv, table_width, cu_q != nullptr,
-                                                    dtype);
-    TZ_CHECK(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0),
-             "attn_kv4: %zu bytes of workspace needed, 16-byte aligned, %zu given", need,
-             ws ? ws_bytes : 0);
-    const int G = Hq / Hkv;
-    const Kv4Plan p = kv4_plan(T, B, G, Hkv, table_width, cu_q != nullptr);
-    TZ_CHECK(p.wgs <= 0xffffff && T <= 0x7fffff && Hq <= 65535, "attn_kv4: %lld rows of %d heads",
-             (long long)T, Hq);
     Kv4Attn a{};
     a.q = q;
     a.out = out;
@@ -1463,19 +1516,53 @@ TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,
     a.pks = pks;
     a.pvs = pvs;
     a.rope = rope_cs;
-    a.part_o = (float*)ws;
-    a.part_ml = (float2*)((char*)ws + p.records * kKv4Dim * 4);
-    a.wgs = (int)p.wgs;
-    a.G = G;
-    a.g_mul = G == 1 ? 0 : (uint32_t)((0x100000000ull + G - 1) / G);
     a.Hq = Hq;
-    a.T = (int)T;
-    a.most = p.most;
-    a.chunk = p.chunk;
-    a.splits = p.splits;
-    a.vec_out = (((uintptr_t)out | (uintptr_t)(out_stride * (dtype ? 2 : 4))) & 15) == 0;
-    return dtype ? launch_kv4_plan<true>(p, a, s, (hipStream_t)stream)
-                 : launch_kv4_plan<false>(p, a, s, (hipStream_t)stream);
+    return attn_kv4("attn_kv4", a, s, dtype, table_width,
+                    tenzo_hip_attn_kv4_ws_bytes(T, B, Hq, Hkv, table_width, cu_q != nullptr, dtype),
+                    ws, ws_bytes, (hipStream_t)stream);
+}
+
+TENZO_HIP_API size_t tenzo_hip_attn_tree_kv4_ws_bytes(int64_t T, int B, int Hq, int Hkv,
+                                                      int table_width, int has_cu, int dtype) {
+    return tenzo_hip_attn_kv4_ws_bytes(T, B, Hq, Hkv, table_width, has_cu, dtype);
+}
+
+TENZO_HIP_API int tenzo_hip_attn_tree_kv4(const void* q, int dtype, int64_t q_stride,
+                                          const uint64_t* mask, int64_t mask_stride,
+                                          int mask_words, const uint8_t* pk, const uint8_t* pv,
+                                          const uint8_t* pks, const uint8_t* pvs,
+                                          int64_t n_blocks, int n_layers, int layer, int Hq,
+                                          int Hkv, const int32_t* block_tables,
+                                          int64_t table_stride, int table_width,
+                                          const int32_t* ctx_lens, const int32_t* cu_q, int B,
+                                          int64_t T, void* out, int64_t out_stride, void* ws,
+                                          size_t ws_bytes, void* stream) {
+    Kv4Seqs s{};
+    const int rc = kv4_check("attn_tree_kv4", pk, pv, pks, pvs, n_blocks, n_layers, layer, Hkv,
+                             block_tables, table_stride, table_width, ctx_lens, cu_q, B, T,
+                             nullptr, 0, s);
+    if (rc) return rc;
+    TZ_CHECK(mask_words >= 1 && mask_words <= 1024 && (T <= 1 || mask_stride >= mask_words),
+             "attn_tree_kv4: masks of %d words, %lld apart", mask_words, (long long)mask_stride);
+    TZ_CHECK((mask && ((uintptr_t)mask & 7) == 0) || T == 0 || B == 0,
+             "attn_tree_kv4: masks must be 8-byte aligned");
+    Kv4Attn a{};
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.pk = pk;
+    a.pv = pv;
+    a.pks = pks;
+    a.pvs = pvs;
+    a.mask = mask;
+    a.mask_stride = mask_stride;
+    a.words = mask_words;
+    a.Hq = Hq;
+    return attn_kv4(
+        "attn_tree_kv4", a, s, dtype, table_width,
+        tenzo_hip_attn_tree_kv4_ws_bytes(T, B, Hq, Hkv, table_width, cu_q != nullptr, dtype), ws,
+        ws_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -6,8 +6,9 @@ free GEMV functions ``compute_linear_gguf_q4_0`` / ``_gptq`` / ``_awq``
 (``TenzoEngine.cpp:1022-1175``), ``FusedKVCache::forward_attention_raw``
 (``TenzoEngine.cpp:447-919``) and ``compute_logits`` (``:1634-1720``) - with
 the same argument meaning; and, without a counterpart there, the operators of
-batched beam decoding over a paged cache in 4 bits. Every call goes through
-libtenzo_hip.so on the current torch stream; tensors must live on the GPU.
+batched beam decoding over a paged cache in 4 bits, and those that check trees of
+drafted tokens over it. Every call goes through libtenzo_hip.so on the current
+torch stream; tensors must live on the GPU.
 """
 from __future__ import annotations
 
@@ -19,7 +20,7 @@ import torch
 
 from . import _lib
 
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2
 
 
 def _ptr(t: torch.Tensor | None):
@@ -437,6 +438,204 @@ def attn_kv4(q, pk, pv, pks, pvs, block_tables, ctx_lens, layer: int, rope_cs=No
     return out
 
 
+# -------------------------------------------------- trees of drafted tokens ----
+
+def _tree_rows(parents, ctx_lens, cu_q, dev):
+    """(parents, lengths, cu_q, B, T) of a call, checked."""
+    if parents.dim() != 1 or ctx_lens.dim() != 1:
+        raise ValueError(f"parents, ctx_lens: {tuple(parents.shape)}, {tuple(ctx_lens.shape)}, "
+                         "not a number for each row and each sequence")
+    B, T = ctx_lens.shape[0], parents.shape[0]
+    if cu_q is None:
+        if T != B:
+            raise ValueError(f"{T} rows for {B} sequences of one node: pass cu_q")
+    elif cu_q.shape != (B + 1,):
+        raise ValueError(f"cu_q: {tuple(cu_q.shape)}, not ({B + 1},)")
+    return (_whole(parents, dev, _I32, "parents"), _whole(ctx_lens, dev, _I32, "ctx_lens"),
+            None if cu_q is None else _whole(cu_q, dev, _I32, "cu_q"), B, T)
+
+
+def tree_plan(parents, ctx_lens, most: int, cu_q=None):
+    """What the nodes of trees of drafted tokens see and where they stand: (mask [T][ceil(most /
+    64)] int64, positions [T] int32).
+
+    A sequence's rows (cu_q, ctx_lens as for attn_kv4, the nodes included in the lengths) are its
+    tree's nodes; parents int32 [T]: the place of a node's parent among them, which comes before
+    the node (a negative one: none). most: at least the nodes of any sequence, up to 4096. Bit j
+    % 64 of word j // 64 is set where node j is an ancestor or the node itself; a position is the
+    number of tokens in front of the tree plus the node's depth. Padding slots' rows are zeros;
+    rows behind the last sequence are not initialised."""
+    dev = _dev()
+    pp, cp, up, B, T = _tree_rows(parents, ctx_lens, cu_q, dev)
+    mask = parents.new_empty((T, max(-(-most // 64), 1)), dtype=torch.int64)
+    at = torch.empty_like(parents)
+    rc = _lib.load().tenzo_hip_tree_plan(pp, cp, up, B, T, most, mask.data_ptr(), at.data_ptr(),
+                                         _stream())
+    if rc:
+        _lib.check(rc, "tree_plan")
+    return mask, at
+
+
+@functools.lru_cache(4096)
+def _attn_tree_kv4_ws(*args: int) -> int:
+    return _lib.load().tenzo_hip_attn_tree_kv4_ws_bytes(*args)
+
+
+def attn_tree_kv4(q, mask, pk, pv, pks, pvs, block_tables, ctx_lens, layer: int, cu_q=None,
+                  out=None):
+    """Attention of trees of drafted tokens over a paged cache in 4 bits, which holds the nodes'
+    keys and values in the last slots of their sequences (kv4_append without rope_cs): a node sees
+    the tokens in front of its tree and the nodes that its row of mask has. q [T][Hq*128] (or
+    [T][Hq][128]) fp32 or fp16, already rotated (rope); mask int64 [T][words] as of tree_plan, or
+    any other bits; the rest as attn_kv4. Rows that see no token are zeros."""
+    dev = _dev()
+    T = q.shape[0]
+    pools, where, seqs = _kv4_cache(pk, pv, pks, pvs, block_tables, ctx_lens, cu_q, layer, T, dev)
+    cols = q.shape[1] if q.dim() == 2 else math.prod(q.shape[1:])
+    Hkv = where[3]
+    if Hkv < 1 or cols % 128 or (cols // 128) % Hkv:
+        raise ValueError(f"q: {tuple(q.shape)}, not rows of heads of 128 over {Hkv} kv heads")
+    dt, dtype = _dtype_code(q), q.dtype
+    qp, qs = _row_args(q, cols, dev, dtype, "q")
+    if mask.dim() != 2 or mask.shape[0] != T or not mask.shape[1]:
+        raise ValueError(f"mask: {tuple(mask.shape)}, not words for each of {T} rows")
+    words = mask.shape[1]
+    mp, ms = _row_args(mask, words, dev, torch.int64, "mask")
+    if out is None:
+        out = q.new_empty(q.shape)
+        op, os = out.data_ptr(), cols
+    elif out.shape == q.shape:
+        op, os = _row_args(out, cols, dev, dtype, "out")
+    else:
+        raise ValueError(f"out: {tuple(out.shape)}, q: {tuple(q.shape)}")
+    if not T:
+        return out
+    Hq = cols // 128
+    nbytes = _attn_tree_kv4_ws(T, seqs[5], Hq, Hkv, seqs[2], cu_q is not None, dt)
+    ws = pk.new_empty(nbytes) if nbytes else None  # (held until the launch)
+    rc = _lib.load().tenzo_hip_attn_tree_kv4(qp, dt, qs, mp, ms, words, *pools, *where[:3], Hq,
+                                             Hkv, *seqs, op, os, ws.data_ptr() if nbytes else None,
+                                             nbytes, _stream())
+    if rc:
+        _lib.check(rc, "attn_tree_kv4")
+    return out
+
+
+def _paged_pools(pk, pv, pks, pvs, dev):
+    """Pools of kv4_pool or of the int8 paged cache, checked: addresses, (n_blocks, n_layers,
+    Hkv, bytes of a row's codes)."""
+    shape = tuple(pk.shape)
+    kv4 = pk.dtype == torch.uint8
+    code, scale = (torch.uint8, torch.uint8) if kv4 else (torch.int8, torch.float32)
+    if len(shape) != 5 or shape[3:] != (KV4_PAGE, 64 if kv4 else 128) or pv.shape != shape:
+        raise ValueError(f"pk, pv: {shape}, {tuple(pv.shape)}")
+    want = shape[:4] + ((4,) if kv4 else ())
+    if pks.shape != want or pvs.shape != want:
+        raise ValueError(f"pks, pvs: {tuple(pks.shape)}, {tuple(pvs.shape)}, not {want}")
+    return ((_whole(pk, dev, code, "pk"), _whole(pv, dev, code, "pv"),
+             _whole(pks, dev, scale, "pks"), _whole(pvs, dev, scale, "pvs")),
+            (shape[0], shape[1], shape[2], 64 if kv4 else 128))
+
+
+def tree_accept(parents, tokens, target, pk, pv, pks, pvs, block_tables, ctx_lens, most: int,
+                cu_q=None):
+    """The path of each tree that the model agrees with, its cache rows moved, in all layers and
+    heads, to where the context goes on: (path [B][most], count [B], next [B], lens [B]), int32.
+
+    parents int32 [T] as for tree_plan; tokens int32 [T]: the nodes' tokens; target int32 [T]: the
+    token that the model gives after each node. Node 0 is taken as it is, then the lowest child
+    whose token is the target of the node before, and so on. path: the nodes, -1 behind them (it
+    ends at most); next: the target of the last one; lens: the lengths afterwards (ctx_lens stays
+    as it is). Padding slots, and sequences with fewer tokens than nodes: no path, -1, their
+    length. Pools of kv4_pool or of the int8 paged cache; a page belongs to one sequence's nodes."""
+    dev = _dev()
+    pp, cp, up, B, T = _tree_rows(parents, ctx_lens, cu_q, dev)
+    if tokens.shape != (T,) or target.shape != (T,):
+        raise ValueError(f"tokens, target: {tuple(tokens.shape)}, {tuple(target.shape)}, not "
+                         f"({T},)")
+    if block_tables.dim() != 2 or block_tables.shape[0] != B or (
+            block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+        raise ValueError(f"block_tables: {tuple(block_tables.shape)}, not a row of page numbers "
+                         f"for each of {B} sequences")
+    pools, sizes = _paged_pools(pk, pv, pks, pvs, dev)
+    width = block_tables.shape[1]
+    path = parents.new_empty((B, max(most, 0)))
+    per = parents.new_empty((3, B))
+    count, last, lens = per
+    rc = _lib.load().tenzo_hip_tree_accept(
+        pp, _whole(tokens, dev, _I32, "tokens"), _whole(target, dev, _I32, "target"), *pools,
+        *sizes, _on(block_tables, dev, _I32, "block_tables"),
+        block_tables.stride(0) if B > 1 else width, width, cp, up, B, T, most, path.data_ptr(),
+        count.data_ptr(), last.data_ptr(), lens.data_ptr(), _stream())
+    if rc:
+        _lib.check(rc, "tree_accept")
+    return path, count, last, lens
+
+
+# ------------------------------------------------------- rotary positions ----
+
+ROPE_SCALINGS = {None: 0, "linear": 1, "base": 2, "parts": 3}
+
+
+def rope_freqs(rot_dim: int, theta: float = 10000.0, scaling: str | None = None,
+               factor: float = 1.0, trained: float = 4096, fast: float = 32.0,
+               slow: float = 1.0):
+    """The frequencies of rope and its factor of cosines and sines: (freqs [rot_dim / 2] float64
+    on the CPU, mscale). scaling, for contexts `factor` times as long as the `trained` positions:
+    "linear" divides them by factor, "base" raises theta instead, "parts" (YaRN) divides those of
+    fewer than `slow` turns within the trained positions, keeps those of more than `fast`, blends
+    in between, and has an mscale of 0.1 ln(factor) + 1."""
+    f = torch.empty(max(rot_dim // 2, 1), dtype=torch.float64)
+    m = ctypes.c_float()
+    if scaling not in ROPE_SCALINGS:
+        raise ValueError(f"scaling {scaling!r}, not one of {list(ROPE_SCALINGS)}")
+    _lib.check(_lib.load().tenzo_hip_rope_freqs(rot_dim, theta, ROPE_SCALINGS[scaling], factor,
+                                                trained, fast, slow, f.data_ptr(),
+                                                ctypes.byref(m)), "rope_freqs")
+    return f, m.value
+
+
+_DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+
+
+def rope(x, positions, freqs, head_dim: int = 128, interleaved: bool = False, mscale: float = 1.0,
+         out=None):
+    """Rows of heads turned by their positions: x [T][H*head_dim] (or [T][H][head_dim]) fp32, fp16
+    or bf16, rows any stride apart (the q | k part of a fused projection does, both at once);
+    positions int32 [T], any values (a negative one turns back); freqs float64 [R / 2], radians a
+    position (rope_freqs). The first R dims of a head are turned, the others kept: pairs are dims
+    i and i + R / 2, or 2i and 2i + 1 when interleaved. Angles are taken in 64 bits, so far
+    positions lose nothing. Returns out like x; out may be x, else it must not overlap it."""
+    dev = _dev()
+    T = x.shape[0]
+    if x.dim() == 3:
+        head_dim = x.shape[2]
+    cols = math.prod(x.shape[1:])
+    dt = _DTYPES.get(x.dtype)
+    if dt is None:
+        raise ValueError(f"unsupported dtype {x.dtype}")
+    if x.dim() < 2 or head_dim < 1 or cols % head_dim or not cols:
+        raise ValueError(f"x: {tuple(x.shape)}, not rows of heads of {head_dim}")
+    if positions.shape != (T,) or freqs.dim() != 1:
+        raise ValueError(f"positions, freqs: {tuple(positions.shape)}, {tuple(freqs.shape)}, not "
+                         f"({T},) and a frequency for each pair")
+    xp, xs = _row_args(x, cols, dev, x.dtype, "x")
+    pp = _whole(positions, dev, _I32, "positions")
+    fp = _whole(freqs, dev, torch.float64, "freqs")
+    if out is None:
+        out = x.new_empty(x.shape)
+        op, os = out.data_ptr(), cols
+    elif out.shape == x.shape:
+        op, os = _row_args(out, cols, dev, x.dtype, "out")
+    else:
+        raise ValueError(f"out: {tuple(out.shape)}, x: {tuple(x.shape)}")
+    rc = _lib.load().tenzo_hip_rope(xp, dt, xs, pp, fp, T, cols // head_dim, head_dim,
+                                    2 * freqs.shape[0], interleaved, mscale, op, os, _stream())
+    if rc:
+        _lib.check(rc, "rope")
+    return out
+
+
 # -------------------------------------------------------- quantized GEMV ---
 
 def gemv_q4_0(act: torch.Tensor, w: torch.Tensor, K: int, N: int) -> torch.Tensor:
@@ -530,6 +729,54 @@ def lm_head_i8_codes_into(codes, q, w_packed, scales, V: int, H: int, logits,
     return logits
 
 
+@functools.lru_cache(4096)
+def _gemm_i8_ws(*args: int) -> int:
+    return _lib.load().tenzo_hip_gemm_i8_ws_bytes(*args)
+
+
+def gemm_i8(codes, q, w_packed, scales, N: int, K: int, dtype=torch.float32,
+            want_idx: bool = False, out=None):
+    """The product of 8-bit integers with a scale for each token and each channel: codes [M][K]
+    int8 and q [M][2] of actquant127 (rows of codes any multiple of 16 apart), w_packed of
+    i8_rows_repack, scales [N] fp32. Returns y [M][N] of dtype (fp32, fp16 or bf16; or into out,
+    whose type it then has), each value float(sum) * (token's scale * channel's), the sums exact;
+    with want_idx (y, idx [M] int32), each row's first column of the largest value (in fp32;
+    NaN counts as -inf). lm_head_i8_codes_into for M rows, with its values bit for bit."""
+    dev = _dev()
+    if codes.dim() != 2 or codes.shape[1] != K or q.shape != (codes.shape[0], 2):
+        raise ValueError(f"codes, q: {tuple(codes.shape)}, {tuple(q.shape)}, not [M][{K}] and "
+                         "[M][2]")
+    M = codes.shape[0]
+    cp, cs = _row_args(codes, K, dev, torch.int8, "codes")
+    if scales.shape != (N,) or w_packed.numel() < (N + 63) // 64 * (K // 16) * 1024:
+        raise ValueError(f"scales, w_packed: {tuple(scales.shape)}, {tuple(w_packed.shape)}, not "
+                         f"those of {N} channels of {K}")
+    if out is None:
+        out = codes.new_empty((M, N), dtype=dtype)
+        op, os = out.data_ptr(), N
+    elif out.shape == (M, N):
+        op, os = _row_args(out, N, dev, out.dtype, "out")
+    else:
+        raise ValueError(f"out: {tuple(out.shape)}, not ({M}, {N})")
+    dt = _DTYPES.get(out.dtype)
+    if dt is None:
+        raise ValueError(f"unsupported dtype {out.dtype}")
+    idx = ws = None
+    nbytes = 0
+    if want_idx:
+        idx = q.new_empty(M)
+        nbytes = _gemm_i8_ws(M, N, K, 1)
+        ws = q.new_empty(nbytes // 4)  # (held until the launch)
+    rc = _lib.load().tenzo_hip_gemm_i8(
+        cp, cs, _whole(q, dev, _I32, "q"), _whole(w_packed, dev, _U8, "w_packed"),
+        _whole(scales, dev, _F32, "scales"), M, N, K, op, dt, os,
+        idx.data_ptr() if want_idx else None, ws.data_ptr() if want_idx else None, nbytes,
+        _stream())
+    if rc:
+        _lib.check(rc, "gemm_i8")
+    return (out, idx) if want_idx else out
+
+
 def argmax(logits: torch.Tensor) -> torch.Tensor:
     out = torch.empty(1, dtype=torch.int32, device=logits.device)
     _lib.check(_lib.load().tenzo_hip_argmax(_ptr(logits), logits.numel(), _ptr(out), _stream()),
@@ -596,23 +843,14 @@ def beam_reorder_paged(parents, block_tables, ctx_lens, pk, pv, pks, pvs) -> Non
                          f"for each of {B} x {W} beams")
     if ctx_lens.shape != (B * W,):
         raise ValueError(f"ctx_lens: {tuple(ctx_lens.shape)}, not ({B * W},)")
-    shape = tuple(pk.shape)
-    kv4 = pk.dtype == torch.uint8
-    code, scale = (torch.uint8, torch.uint8) if kv4 else (torch.int8, torch.float32)
-    if len(shape) != 5 or shape[3:] != (KV4_PAGE, 64 if kv4 else 128) or pv.shape != shape:
-        raise ValueError(f"pk, pv: {shape}, {tuple(pv.shape)}")
-    want = shape[:4] + ((4,) if kv4 else ())
-    if pks.shape != want or pvs.shape != want:
-        raise ValueError(f"pks, pvs: {tuple(pks.shape)}, {tuple(pvs.shape)}, not {want}")
+    pools, sizes = _paged_pools(pk, pv, pks, pvs, dev)
     width = block_tables.shape[1]
     _lib.check(_lib.load().tenzo_hip_beam_reorder_paged(
         _on(parents, dev, torch.int32, "parents"), parents.stride(0) if B > 1 else W,
         _on(block_tables, dev, torch.int32, "block_tables"),
         block_tables.stride(0) if B * W > 1 else width, width,
-        _whole(ctx_lens, dev, torch.int32, "ctx_lens"), B, W, _whole(pk, dev, code, "pk"),
-        _whole(pv, dev, code, "pv"), _whole(pks, dev, scale, "pks"),
-        _whole(pvs, dev, scale, "pvs"), shape[0], shape[1], shape[2], 64 if kv4 else 128,
-        _stream()), "beam_reorder_paged")
+        _whole(ctx_lens, dev, torch.int32, "ctx_lens"), B, W, *pools, *sizes, _stream()),
+        "beam_reorder_paged")
 
 
 def embed_i8(w_packed, scales, token: torch.Tensor, V: int, H: int) -> torch.Tensor:
