@@ -434,7 +434,7 @@ TENZO_HIP_API int tenzo_hip_argmax(const float* logits, int64_t V, int32_t* out_
 /* The product of tenzo_hip_lm_head_i8_codes for M rows, no counterpart in the
  * reference: y[m][n] = float(sum_k codes[m][k] * W[n][k]) * (q[m].inv_scale *
  * scales[n]), the sums exact in int32 and a row's values bit for bit those of
- * that call. codes: rows codes_stride apart (a multiple of 16), as
+ * that call. codes: rows codes_stride apart (a multiple of 16, up to 2^22), as
  * tenzo_hip_rmsnorm_quant127 writes them (code_sum is not read); w_packed from
  * tenzo_hip_i8_rows_repack of N x K weights of any projection; y: rows y_stride
  * apart, dtype 0 = fp32, 1 = fp16, 2 = bf16. K % 16 == 0, up to 131056; M up to

@@ -2,12 +2,13 @@
 // y[m][n] = float(sum_k codes[m][k] W[n][k]) * (q[m].inv_scale * scales[n]), sums exact in int32,
 // over weights in the LM head's layout (blocks of 64 rows x 16 k, 1 KiB each, a row's blocks side
 // by side).
-#include "common.h"
+#include "lds_ring.h"
 
 namespace tz {
 namespace {
 
 typedef int i4v __attribute__((ext_vector_type(4)));
+typedef int i16v __attribute__((ext_vector_type(16)));
 
 struct GemmI8 {
     const int8_t* codes;
@@ -121,6 +122,210 @@ __global__ void __launch_bounds__(64 * KW) gemm_i8_few_kernel(GemmI8 a) {
     }
 }
 
+// Many tokens: a workgroup of WR x WT x KW waves has 32 RT WR weight rows x 32 CT WT tokens, a wave
+// 32 RT x 32 CT of them, and its KW groups of waves take turns of 64 k; their sums meet in LDS at
+// the end. A step is a turn of every group. Its slot of the ring in LDS holds for each group
+//   weights: blocks of 64 rows x 16 k as they are in memory (row r's 16 bytes at 16 r);
+//   codes:   rows of 64 bytes, the 16-byte piece p of row r at place p ^ (r / 4 % 4) of it.
+// Both are filled by loads straight into LDS, S - 1 steps ahead; a fragment of either is read
+// with the 16 lanes that LDS serves together in different banks. The codes are the first operand,
+// so that a register of the result holds 32 neighbouring channels of a token in 32 lanes.
+// Each half of a step's fragments (32 k) is read while the half before it is multiplied.
+template <int WR, int WT, int KW, int RT, int CT, int S>
+__global__ void __launch_bounds__(64 * WR * WT * KW, WR * WT * KW >= 8 ? 1 : 2)
+gemm_i8_tile_kernel(GemmI8 a) {
+    constexpr int W = WR * WT * KW, BN = 32 * RT * WR, BM = 32 * CT * WT;
+    static_assert(BN % 64 == 0, "whole blocks of rows");
+    constexpr int kWLoads = BN / 16, kGroup = kWLoads + BM / 16;  // loads of 1 KiB per group
+    constexpr int kSlot = KW * kGroup * 1024, X = KW * kGroup / W;
+    static_assert(X * W == KW * kGroup, "as many loads a step for each wave");
+    static_assert(S >= 3 && (S - 1) * X <= 63, "vmcnt counts at most 63 loads");
+    constexpr int kRed = (KW - 1) * WR * WT * RT * CT * 4096, kRing = S * kSlot;
+    __shared__ __attribute__((aligned(16))) char ring[kRing > kRed ? kRing : kRed];
+    __shared__ float inv[BM];
+
+    const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wave % WR, wt = wave / WR % WT, kg = wave / (WR * WT);
+    // Consecutive tiles to one XCD, as bands of 4 tiles of weight rows, so that what its
+    // workgroups read at a time is few tiles of either operand.
+    const int G = gridDim.x, id = blockIdx.x;
+    const int tid = (G & 7) == 0 ? (id & 7) * (G >> 3) + (id >> 3) : id;
+    const int nt = (int)((a.N + BN - 1) / BN), mt = (a.M + BM - 1) / BM;
+    if (tid >= nt * mt) return;
+    const int band = tid / (4 * mt), wide = min(4, nt - 4 * band), in_band = tid - band * 4 * mt;
+    const int bn = 4 * band + in_band % wide, m0 = in_band / wide * BM;
+    const int64_t n0 = (int64_t)bn * BN;
+    const int rows = min(BM, a.M - m0), blocks = min(BN / 64, (int)((a.N + 63) / 64 - n0 / 64));
+    const int K = a.KB * 16, steps = (a.KB + 4 * KW - 1) / (4 * KW);
+    for (int m = threadIdx.x; m < BM; m += 64 * W) inv[m] = a.q[m0 + min(m, rows - 1)].inv_scale;
+
+    const u4v rw = buf_words(a.w + (n0 >> 6) * ((int64_t)K * 64), (uint32_t)blocks * (uint32_t)K * 64u);
+    const u4v rc = buf_words(a.codes + (int64_t)m0 * a.ldc, (uint32_t)((rows - 1) * a.ldc + K));
+    // This wave's loads of a step: byte offsets, advanced from step to step. What lies past a row's
+    // K (which the next row's codes may follow) is taken from past the resource, as zeros; weights
+    // there count nothing then.
+    uint32_t off[X];
+    int left[X];  // K still in front of a lane's piece
+#pragma unroll
+    for (int x = 0; x < X; ++x) {
+        const int l = (wave + W * x) % kGroup, k = (wave + W * x) / kGroup;
+        const int row = 16 * (l - kWLoads) + (lane >> 2);
+        const int piece = (lane & 3) ^ (row >> 2 & 3);
+        off[x] = l < kWLoads ? (uint32_t)(l >> 2) * (uint32_t)K * 64u +
+                                   (uint32_t)(4 * k + (l & 3)) * 1024u + (uint32_t)lane * 16u
+                             : (uint32_t)(row * a.ldc) + (uint32_t)(64 * k + piece * 16);
+        left[x] = l < kWLoads ? INT32_MAX : K - 64 * k - piece * 16;
+    }
+    auto load = [&](uint32_t slot, int x) {
+        const int l = wave + W * x;
+        const bool isw = l % kGroup < kWLoads;
+        to_lds16_asm(isw ? rw : rc, slot + (uint32_t)l * 1024u, left[x] > 0 ? off[x] : 0x80000000u);
+        off[x] += isw ? 4096u * KW : 64u * KW;
+        left[x] -= isw ? 0 : 64 * KW;
+    };
+
+    i16v acc[RT][CT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int u = 0; u < CT; ++u) acc[t][u] = i16v{};
+    struct Frag {
+        i4v a[RT], b[CT];
+    };
+    const uint32_t wrow = (uint32_t)(kg * kGroup * 1024 + g * 1024 + i * 16);
+    const uint32_t crow = (uint32_t)((kg * kGroup + kWLoads) * 1024 + (wt * CT * 32 + i) * 64);
+    const uint32_t swz = (uint32_t)((g ^ (i >> 2 & 3)) * 16);
+    auto read = [&](const char* slot, int h, Frag& f) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const int rt = wr * RT + t;
+            f.a[t] = *reinterpret_cast<const i4v*>(slot + wrow + (rt >> 1) * 4096 + h * 2048 +
+                                                   (rt & 1) * 512);
+        }
+#pragma unroll
+        for (int u = 0; u < CT; ++u)
+            f.b[u] = *reinterpret_cast<const i4v*>(slot + crow + u * 2048 +
+                                                   (swz ^ (uint32_t)(h * 32)));
+    };
+    auto mma = [&](const Frag& f, uint32_t slot, bool loads) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+#pragma unroll
+            for (int u = 0; u < CT; ++u)
+                acc[t][u] =
+                    __builtin_amdgcn_mfma_i32_32x32x32_i8(f.b[u], f.a[t], acc[t][u], 0, 0, 0);
+            if (loads)  // (a later step's go out between the products)
+#pragma unroll
+                for (int x = 0; x < X; ++x)
+                    if (x * RT / X == t) load(slot, x);
+        }
+    };
+
+    const uint32_t ring0 = lds_addr(ring);
+    uint32_t in = ring0;  // the slot to load into next
+#pragma unroll
+    for (int j = 0; j < S - 1; ++j) {
+#pragma unroll
+        for (int x = 0; x < X; ++x) load(in, x);
+        in += kSlot;
+    }
+    const char* cur = ring;
+    const char* nxt = ring + kSlot;
+    Frag f0, f1;
+    wait_vm_asm<(S - 2) * X>();
+    block_barrier();
+    read(cur, 0, f0);
+    for (int s = 0; s < steps; ++s) {
+        wait_vm_asm<(S - 3) * X>();  // the next step's loads have landed
+        __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));  // lgkmcnt(0)
+        block_barrier();  // everyone's, and everyone has read the step before
+        read(cur, 1, f1);
+        issue_point();
+        mma(f0, in, true);
+        issue_point();
+        in = in == ring0 + (S - 1) * kSlot ? ring0 : in + kSlot;
+        read(nxt, 0, f0);
+        issue_point();
+        mma(f1, 0, false);
+        cur = nxt;
+        nxt = nxt == ring + (S - 1) * kSlot ? ring : nxt + kSlot;
+        __builtin_amdgcn_sched_barrier(0);  // the step's products stay ahead of the next barrier
+    }
+    wait_vm_asm<0>();  // the loads past the end still write the ring
+    __syncthreads();
+
+    if (KW > 1) {  // groups 1 .. hand their sums to group 0
+        i16v* red = reinterpret_cast<i16v*>(ring);
+        const int wv = wave % (WR * WT);
+        if (kg > 0) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int u = 0; u < CT; ++u)
+                    red[((((kg - 1) * WR * WT + wv) * RT + t) * CT + u) * 64 + lane] = acc[t][u];
+        }
+        __syncthreads();
+        if (kg > 0) return;
+#pragma unroll
+        for (int k = 0; k < KW - 1; ++k)
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int u = 0; u < CT; ++u)
+                    acc[t][u] += red[(((k * WR * WT + wv) * RT + t) * CT + u) * 64 + lane];
+    }
+
+    // register 4 q + e of acc[t][u]: channel 32 t + i, token 32 u + 8 q + 4 g + e
+    const int64_t nw = n0 + wr * RT * 32 + i;
+    float sc[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) sc[t] = nw + 32 * t < a.N ? a.scales[nw + 32 * t] : 0.0f;
+#pragma unroll
+    for (int u = 0; u < CT; ++u) {
+        float bv[16];
+        int bi[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int ml = (wt * CT + u) * 32 + 8 * (r >> 2) + 4 * g + (r & 3), m = m0 + ml;
+            const float iv = inv[ml];
+            bv[r] = -INFINITY;
+            bi[r] = (int)nw;
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                const float y = (float)acc[t][u][r] * __fmul_rn(iv, sc[t]);
+                const bool there = nw + 32 * t < a.N;
+                if (there && m < a.M) store_y(a, m * a.ldy + nw + 32 * t, y);
+                if (there && y > bv[r]) {
+                    bv[r] = y;
+                    bi[r] = (int)nw + 32 * t;
+                }
+            }
+        }
+        if (a.best) {
+            // 16 tokens' best of 32 lanes: half of the tokens go to the other half of the lanes
+            // each time, and the last of the five has one token in two lanes
+#pragma unroll
+            for (int d = 8; d >= 1; d >>= 1)
+#pragma unroll
+                for (int k = 0; k < d; ++k) {
+                    const bool up = i & (d << 1);
+                    float v = up ? bv[k + d] : bv[k];
+                    int n = up ? bi[k + d] : bi[k];
+                    take_best(v, n, __shfl_xor(up ? bv[k] : bv[k + d], d << 1),
+                              __shfl_xor(up ? bi[k] : bi[k + d], d << 1));
+                    bv[k] = v;
+                    bi[k] = n;
+                }
+            take_best(bv[0], bi[0], __shfl_xor(bv[0], 1), __shfl_xor(bi[0], 1));
+            const int r = i >> 1;  // (bits 4 .. 1 of the lane are bits 3 .. 0 of the token)
+            const int m = m0 + (wt * CT + u) * 32 + 8 * (r >> 2) + 4 * g + (r & 3);
+            if ((i & 1) == 0 && m < a.M)
+                a.best[(int64_t)m * a.parts + bn * WR + wr] = make_float2(bv[0], __int_as_float(bi[0]));
+        }
+    }
+}
+
 __global__ void __launch_bounds__(256) gemm_i8_best_kernel(const float2* best, int parts,
                                                            int32_t* out) {
     __shared__ float rv[4];
@@ -145,24 +350,46 @@ __global__ void __launch_bounds__(256) gemm_i8_best_kernel(const float2* best, i
     }
 }
 
-// Tokens and weight rows of a workgroup.
+// The kernel for M tokens and N channels, and the parts that a row's largest value comes in.
+enum GemmShape { kFewNarrow, kFewWide, kTile64, kTile128, kTile256 };
 struct GemmPlan {
-    int bm, bn;
+    GemmShape shape;
+    int bm;     // tokens of a workgroup, few tokens
+    int parts;  // columns: as many as the rows' bests
 };
 GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K) {
     GemmPlan p;
     p.bm = M <= 16 ? 16 : M <= 32 ? 32 : 64;
-    p.bn = ceil_div(N, 64) * ceil_div(M, p.bm) >= 512 ? 64 : 16;
+    if (M <= 64) {
+        p.shape = ceil_div(N, 64) >= 512 ? kFewWide : kFewNarrow;
+        p.parts = (int)ceil_div(N, p.shape == kFewWide ? 64 : 16);
+        return p;
+    }
+    if (ceil_div(M, 256) * ceil_div(N, 256) >= 160)
+        p.shape = kTile256;
+    else if (ceil_div(M, 128) * ceil_div(N, 128) >= 160)
+        p.shape = kTile128;
+    else
+        p.shape = kTile64;
+    p.parts = (int)(p.shape == kTile256 ? 2 * ceil_div(N, 256)
+                    : p.shape == kTile128 ? 2 * ceil_div(N, 128) : 2 * ceil_div(N, 64));
     return p;
 }
 
 template <int MT>
 void launch_few(const GemmPlan& p, const GemmI8& a, hipStream_t st) {
-    const dim3 grid((unsigned)ceil_div(a.N, p.bn), (unsigned)ceil_div(a.M, p.bm));
-    if (p.bn == 64)
+    const dim3 grid((unsigned)a.parts, (unsigned)ceil_div(a.M, p.bm));
+    if (p.shape == kFewWide)
         hipLaunchKernelGGL((gemm_i8_few_kernel<MT, 4, 4, 4>), grid, dim3(256), 0, st, a);
     else
         hipLaunchKernelGGL((gemm_i8_few_kernel<MT, 1, 8, 4>), grid, dim3(512), 0, st, a);
+}
+template <int WR, int WT, int KW, int RT, int CT, int S>
+void launch_tile(const GemmI8& a, hipStream_t st) {
+    // (a number of workgroups that is shared out among the XCDs evenly: the last have no tile)
+    const int64_t nt = ceil_div(a.N, 32 * RT * WR), mt = ceil_div(a.M, 32 * CT * WT);
+    hipLaunchKernelGGL((gemm_i8_tile_kernel<WR, WT, KW, RT, CT, S>),
+                       dim3((unsigned)(ceil_div(nt * mt, 8) * 8)), dim3(64 * WR * WT * KW), 0, st, a);
 }
 
 }  // namespace
@@ -174,7 +401,7 @@ extern "C" {
 
 TENZO_HIP_API size_t tenzo_hip_gemm_i8_ws_bytes(int64_t M, int64_t N, int64_t K, int want_idx) {
     if (M <= 0 || N <= 0 || K <= 0 || !want_idx) return 0;
-    return (size_t)(M * ceil_div(N, gemm_plan(M, N, K).bn)) * sizeof(float2);
+    return (size_t)(M * gemm_plan(M, N, K).parts) * sizeof(float2);
 }
 
 TENZO_HIP_API int tenzo_hip_gemm_i8(const int8_t* codes, int64_t codes_stride,
@@ -190,7 +417,8 @@ TENZO_HIP_API int tenzo_hip_gemm_i8(const int8_t* codes, int64_t codes_stride,
              "131056", (long long)K);
     if (M == 0) return TENZO_SUCCESS;
     TZ_CHECK(codes && q && w_packed && scales && y, "gemm_i8: null pointer");
-    TZ_CHECK(M == 1 || (codes_stride >= K && codes_stride % 16 == 0 && y_stride >= N),
+    TZ_CHECK(M == 1 || (codes_stride >= K && codes_stride % 16 == 0 && codes_stride <= 1 << 22 &&
+                        y_stride >= N),
              "gemm_i8: row strides %lld, %lld of %lld codes, %lld outputs",
              (long long)codes_stride, (long long)y_stride, (long long)K, (long long)N);
     TZ_CHECK((((uintptr_t)codes | (uintptr_t)w_packed) & 15) == 0 &&
@@ -203,16 +431,21 @@ TENZO_HIP_API int tenzo_hip_gemm_i8(const int8_t* codes, int64_t codes_stride,
              ws ? ws_bytes : 0);
     const GemmPlan p = gemm_plan(M, N, K);
     const hipStream_t st = (hipStream_t)stream;
-    GemmI8 a{codes, codes_stride, q, (const uint8_t*)w_packed, scales, y, y_stride,
-             out_idx ? (float2*)ws : nullptr, N, (int)M, (int)(K / 16), (int)ceil_div(N, p.bn),
-             dtype};
-    if (p.bm == 16)
+    GemmI8 a{codes, M == 1 ? K : codes_stride, q, (const uint8_t*)w_packed, scales, y, y_stride,
+             out_idx ? (float2*)ws : nullptr, N, (int)M, (int)(K / 16), p.parts, dtype};
+    if (p.shape == kTile256)
+        launch_tile<2, 4, 1, 4, 2, 4>(a, st);
+    else if (p.shape == kTile128)
+        launch_tile<2, 2, 1, 2, 2, 4>(a, st);
+    else if (p.shape == kTile64)
+        launch_tile<2, 2, 2, 1, 1, 4>(a, st);
+    else if (p.bm == 16)
         launch_few<1>(p, a, st);
     else if (p.bm == 32)
         launch_few<2>(p, a, st);
     else
         launch_few<4>(p, a, st);
-    const int rc = launch_status("gemm_i8_few_kernel");
+    const int rc = launch_status("gemm_i8 kernel");
     if (rc || !out_idx) return rc;
     hipLaunchKernelGGL(gemm_i8_best_kernel, dim3((unsigned)M), dim3(256), 0, st, a.best, a.parts,
                        out_idx);
