@@ -34,6 +34,34 @@ __device__ __forceinline__ void store_y(const GemmI8& a, int64_t at, float v) {
         reinterpret_cast<__bf16*>(a.y)[at] = (__bf16)v;
 }
 
+// Two outputs of 16 bits, each rounded from its fp32 value.
+template <int TYPE>
+__device__ __forceinline__ uint32_t pack_y(float a, float b) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    if (TYPE == 1) return float_to_half_bits(a) | (uint32_t)float_to_half_bits(b) << 16;
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+// 16 bytes of outputs, and as they are stored: at any element's address.
+template <int TYPE>
+struct Out {
+    typedef float type;
+    struct __attribute__((packed, aligned(4))) any {
+        float v __attribute__((ext_vector_type(4)));
+    };
+    any v;
+};
+template <>
+struct Out<1> {
+    typedef uint16_t type;
+    struct __attribute__((packed, aligned(2))) any {
+        uint16_t v __attribute__((ext_vector_type(8)));
+    };
+    any v;
+};
+template <>
+struct Out<2> : Out<1> {};
+
 // The larger value, of equal ones the lower column; NaN counts as -inf.
 __device__ __forceinline__ void take_best(float& v, int& n, float ov, int on) {
     if (ov > v || (ov == v && on < n)) {
@@ -131,7 +159,7 @@ __global__ void __launch_bounds__(64 * KW) gemm_i8_few_kernel(GemmI8 a) {
 // with the 16 lanes that LDS serves together in different banks. The codes are the first operand,
 // so that a register of the result holds 32 neighbouring channels of a token in 32 lanes.
 // Each half of a step's fragments (32 k) is read while the half before it is multiplied.
-template <int WR, int WT, int KW, int RT, int CT, int S>
+template <int TYPE, int WR, int WT, int KW, int RT, int CT, int S>
 __global__ void __launch_bounds__(64 * WR * WT * KW, WR * WT * KW >= 8 ? 1 : 2)
 gemm_i8_tile_kernel(GemmI8 a) {
     constexpr int W = WR * WT * KW, BN = 32 * RT * WR, BM = 32 * CT * WT;
@@ -141,7 +169,8 @@ gemm_i8_tile_kernel(GemmI8 a) {
     static_assert(X * W == KW * kGroup, "as many loads a step for each wave");
     static_assert(S >= 3 && (S - 1) * X <= 63, "vmcnt counts at most 63 loads");
     constexpr int kRed = (KW - 1) * WR * WT * RT * CT * 4096, kRing = S * kSlot;
-    __shared__ __attribute__((aligned(16))) char ring[kRing > kRed ? kRing : kRed];
+    static_assert(kRed + WR * WT * RT * 4096 <= kRing, "sums and outputs go out by way of the ring");
+    __shared__ __attribute__((aligned(16))) char ring[kRing];
     __shared__ float inv[BM];
 
     const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5;
@@ -276,32 +305,74 @@ gemm_i8_tile_kernel(GemmI8 a) {
                     acc[t][u] += red[(((k * WR * WT + wv) * RT + t) * CT + u) * 64 + lane];
     }
 
-    // register 4 q + e of acc[t][u]: channel 32 t + i, token 32 u + 8 q + 4 g + e
-    const int64_t nw = n0 + wr * RT * 32 + i;
+    // Register 4 q + e of acc[t][u]: channel 32 t + i, token 32 u + 8 q + 4 g + e. 32 tokens at a
+    // time go through the wave's part of the ring, so that a lane stores 16 bytes of a token:
+    // pieces of 16 bytes, in an order of the token's own that brings what is written at a time
+    // into all banks. Two bytes of one or four to a store: 14 us of 256 x 256 outputs, 3 so.
+    constexpr int E = TYPE ? 8 : 4, P = 32 * RT / E;  // outputs of a piece, pieces of a token
+    auto place = [](int row) { return ((TYPE ? (row & 1) * 4 : 0) ^ (row >> 2 & 1) * 8) & (P - 1); };
+    char* out = ring + kRed + wave % (WR * WT) * (RT * 4096);
+    const int64_t nw = n0 + wr * RT * 32;
     float sc[RT];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) sc[t] = nw + 32 * t < a.N ? a.scales[nw + 32 * t] : 0.0f;
+    for (int t = 0; t < RT; ++t) sc[t] = nw + i + 32 * t < a.N ? a.scales[nw + i + 32 * t] : 0.0f;
 #pragma unroll
     for (int u = 0; u < CT; ++u) {
+        const int mu = (wt * CT + u) * 32;
         float bv[16];
         int bi[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int ml = (wt * CT + u) * 32 + 8 * (r >> 2) + 4 * g + (r & 3), m = m0 + ml;
-            const float iv = inv[ml];
-            bv[r] = -INFINITY;
-            bi[r] = (int)nw;
+        for (int r = 0; r < 16; r += 2) {
+            const int row = 8 * (r >> 2) + 4 * g + (r & 3);
+            const float iv[2] = {inv[mu + row], inv[mu + row + 1]};
+            bv[r] = bv[r + 1] = -INFINITY;
+            bi[r] = bi[r + 1] = (int)nw + i;
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-                const float y = (float)acc[t][u][r] * __fmul_rn(iv, sc[t]);
-                const bool there = nw + 32 * t < a.N;
-                if (there && m < a.M) store_y(a, m * a.ldy + nw + 32 * t, y);
-                if (there && y > bv[r]) {
-                    bv[r] = y;
-                    bi[r] = (int)nw + 32 * t;
+                float y[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    y[k] = (float)acc[t][u][r + k] * __fmul_rn(iv[k], sc[t]);
+                    if (a.best && nw + i + 32 * t < a.N && y[k] > bv[r + k]) {
+                        bv[r + k] = y[k];
+                        bi[r + k] = (int)nw + i + 32 * t;
+                    }
+                }
+                const int n = 32 * t + i;
+                if (TYPE == 0) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        *reinterpret_cast<float*>(out + (row + k) * (P * 16) +
+                                                  (n / 4 ^ place(row + k)) * 16 + n % 4 * 4) = y[k];
+                } else {
+                    // (lanes of two neighbouring channels: one has both of a token, one of the next)
+                    const int odd = i & 1;
+                    const float other = dpp_f<kDppXor1>(odd ? y[0] : y[1]);
+                    const uint32_t w = pack_y<TYPE>(odd ? other : y[0], odd ? y[1] : other);
+                    *reinterpret_cast<uint32_t*>(out + (row + odd) * (P * 16) +
+                                                 (n / 8 ^ place(row + odd)) * 16 + n % 8 / 2 * 4) =
+                        w;
                 }
             }
         }
+        asm volatile("" ::: "memory");  // (a wave's accesses to LDS are made in order)
+#pragma unroll
+        for (int k = 0; k < P / 2; ++k) {
+            const int at = lane + 64 * k, row = at / P, m = m0 + mu + row;
+            const int64_t n = nw + (at % P ^ place(row)) * E;
+            const Out<TYPE> v = *reinterpret_cast<const Out<TYPE>*>(out + at * 16);
+            if (m >= a.M) continue;
+            typename Out<TYPE>::type* y =
+                reinterpret_cast<typename Out<TYPE>::type*>(a.y) + m * a.ldy + n;
+            if (n + E <= a.N) {
+                *reinterpret_cast<typename Out<TYPE>::any*>(y) = v.v;
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (n + e < a.N) y[e] = v.v.v[e];
+            }
+        }
+        asm volatile("" ::: "memory");
         if (a.best) {
             // 16 tokens' best of 32 lanes: half of the tokens go to the other half of the lanes
             // each time, and the last of the five has one token in two lanes
@@ -319,7 +390,7 @@ gemm_i8_tile_kernel(GemmI8 a) {
                 }
             take_best(bv[0], bi[0], __shfl_xor(bv[0], 1), __shfl_xor(bi[0], 1));
             const int r = i >> 1;  // (bits 4 .. 1 of the lane are bits 3 .. 0 of the token)
-            const int m = m0 + (wt * CT + u) * 32 + 8 * (r >> 2) + 4 * g + (r & 3);
+            const int m = m0 + mu + 8 * (r >> 2) + 4 * g + (r & 3);
             if ((i & 1) == 0 && m < a.M)
                 a.best[(int64_t)m * a.parts + bn * WR + wr] = make_float2(bv[0], __int_as_float(bi[0]));
         }
@@ -384,12 +455,22 @@ void launch_few(const GemmPlan& p, const GemmI8& a, hipStream_t st) {
     else
         hipLaunchKernelGGL((gemm_i8_few_kernel<MT, 1, 8, 4>), grid, dim3(512), 0, st, a);
 }
-template <int WR, int WT, int KW, int RT, int CT, int S>
+template <int TYPE, int WR, int WT, int KW, int RT, int CT, int S>
 void launch_tile(const GemmI8& a, hipStream_t st) {
     // (a number of workgroups that is shared out among the XCDs evenly: the last have no tile)
     const int64_t nt = ceil_div(a.N, 32 * RT * WR), mt = ceil_div(a.M, 32 * CT * WT);
-    hipLaunchKernelGGL((gemm_i8_tile_kernel<WR, WT, KW, RT, CT, S>),
+    hipLaunchKernelGGL((gemm_i8_tile_kernel<TYPE, WR, WT, KW, RT, CT, S>),
                        dim3((unsigned)(ceil_div(nt * mt, 8) * 8)), dim3(64 * WR * WT * KW), 0, st, a);
+}
+
+template <int TYPE>
+void launch_shape(GemmShape shape, const GemmI8& a, hipStream_t st) {
+    if (shape == kTile256)
+        launch_tile<TYPE, 2, 4, 1, 4, 2, 4>(a, st);
+    else if (shape == kTile128)
+        launch_tile<TYPE, 2, 2, 1, 2, 2, 4>(a, st);
+    else
+        launch_tile<TYPE, 2, 2, 2, 1, 1, 4>(a, st);
 }
 
 }  // namespace
@@ -433,13 +514,14 @@ TENZO_HIP_API int tenzo_hip_gemm_i8(const int8_t* codes, int64_t codes_stride,
     const hipStream_t st = (hipStream_t)stream;
     GemmI8 a{codes, M == 1 ? K : codes_stride, q, (const uint8_t*)w_packed, scales, y, y_stride,
              out_idx ? (float2*)ws : nullptr, N, (int)M, (int)(K / 16), p.parts, dtype};
-    if (p.shape == kTile256)
-        launch_tile<2, 4, 1, 4, 2, 4>(a, st);
-    else if (p.shape == kTile128)
-        launch_tile<2, 2, 1, 2, 2, 4>(a, st);
-    else if (p.shape == kTile64)
-        launch_tile<2, 2, 2, 1, 1, 4>(a, st);
-    else if (p.bm == 16)
+    if (p.shape >= kTile64) {
+        if (dtype == 0)
+            launch_shape<0>(p.shape, a, st);
+        else if (dtype == 1)
+            launch_shape<1>(p.shape, a, st);
+        else
+            launch_shape<2>(p.shape, a, st);
+    } else if (p.bm == 16)
         launch_few<1>(p, a, st);
     else if (p.bm == 32)
         launch_few<2>(p, a, st);
