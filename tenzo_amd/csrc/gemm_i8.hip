@@ -70,6 +70,32 @@ __device__ __forceinline__ void take_best(float& v, int& n, float ov, int on) {
     }
 }
 
+// A token of 16 from either half of a wave's rows of 16 lanes: lanes with bit 4 keep the upper 8.
+__device__ __forceinline__ void best_swap16(float (&v)[16], int (&n)[16]) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[k]),
+                                                        __float_as_uint(v[k + 8]), false, false);
+        const auto b = __builtin_amdgcn_permlane16_swap((uint32_t)n[k], (uint32_t)n[k + 8], false,
+                                                        false);
+        v[k] = __uint_as_float(a[0]);
+        n[k] = (int)b[0];
+        take_best(v[k], n[k], __uint_as_float(a[1]), (int)b[1]);
+    }
+}
+// And of 2 D tokens: lanes that are `up` keep the upper D, their partners by CTRL the others.
+template <int D, int CTRL>
+__device__ __forceinline__ void best_halve(float (&v)[16], int (&n)[16], bool up) {
+#pragma unroll
+    for (int k = 0; k < D; ++k) {
+        const float give = up ? v[k] : v[k + D];
+        const int give_n = up ? n[k] : n[k + D];
+        v[k] = up ? v[k + D] : v[k];
+        n[k] = up ? n[k + D] : n[k];
+        take_best(v[k], n[k], dpp_f<CTRL>(give), dpp_i<CTRL>(give_n));
+    }
+}
+
 // Few tokens: 16 NT rows of weights to a workgroup, whose KW waves share K: a wave has every KW-th
 // 64 of it, straight from memory to the matrix cores' operands, DEPTH steps ahead. The codes of the
 // 16 MT tokens come the same way, out of the L2. At the end the waves' sums meet in LDS.
@@ -81,7 +107,11 @@ __global__ void __launch_bounds__(64 * KW) gemm_i8_few_kernel(GemmI8 a) {
     const int64_t n0 = (int64_t)blockIdx.x * (16 * NT);
     const int m0 = blockIdx.y * (16 * MT);
     const int steps = (a.KB + 3) >> 2, mine = steps > wave ? (steps - wave + KW - 1) / KW : 0;
-    const uint8_t* wb = a.w + (n0 >> 6) * ((int64_t)a.KB << 10) + ((n0 & 63) + col) * 16;
+    const int64_t blocks = (a.N + 63) >> 6, block = (int64_t)a.KB << 10;
+    const uint8_t* wb[NT > 4 ? NT / 4 : 1];  // (past the last block of rows: that one again)
+#pragma unroll
+    for (int b = 0; b < (NT > 4 ? NT / 4 : 1); ++b)
+        wb[b] = a.w + min((n0 >> 6) + b, blocks - 1) * block + ((n0 & 63) + col) * 16;
     const int8_t* ab[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) ab[t] = a.codes + (int64_t)min(m0 + 16 * t + col, a.M - 1) * a.ldc;
@@ -92,7 +122,7 @@ __global__ void __launch_bounds__(64 * KW) gemm_i8_few_kernel(GemmI8 a) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
             wv[u][t] = __builtin_nontemporal_load(
-                reinterpret_cast<const i4v*>(wb + ((int64_t)kb << 10) + t * 256));
+                reinterpret_cast<const i4v*>(wb[t >> 2] + ((int64_t)kb << 10) + (t & 3) * 256));
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             av[u][t] = *reinterpret_cast<const i4v*>(ab[t] + kb * 16);
@@ -141,8 +171,12 @@ __global__ void __launch_bounds__(64 * KW) gemm_i8_few_kernel(GemmI8 a) {
         }
         if (a.best) {
             int at = (int)n;
+            take_best(v, at, dpp_f<kDppXor1>(v), dpp_i<kDppXor1>(at));
+            take_best(v, at, dpp_f<kDppXor2>(v), dpp_i<kDppXor2>(at));
+            take_best(v, at, dpp_f<kDppHalfMirror>(v), dpp_i<kDppHalfMirror>(at));
+            take_best(v, at, dpp_f<kDppMirror>(v), dpp_i<kDppMirror>(at));
 #pragma unroll
-            for (int d = 1; d < 16 * NT; d <<= 1)
+            for (int d = 16; d < 16 * NT; d <<= 1)
                 take_best(v, at, __shfl_xor(v, d), __shfl_xor(at, d));
             if (nn == 0 && m < a.M)
                 a.best[(int64_t)m * a.parts + blockIdx.x] = make_float2(v, __int_as_float(at));
@@ -159,8 +193,8 @@ __global__ void __launch_bounds__(64 * KW) gemm_i8_few_kernel(GemmI8 a) {
 // with the 16 lanes that LDS serves together in different banks. The codes are the first operand,
 // so that a register of the result holds 32 neighbouring channels of a token in 32 lanes.
 // Each half of a step's fragments (32 k) is read while the half before it is multiplied.
-template <int TYPE, int WR, int WT, int KW, int RT, int CT, int S>
-__global__ void __launch_bounds__(64 * WR * WT * KW, WR * WT * KW >= 8 ? 1 : 2)
+template <int TYPE, bool BEST, int WR, int WT, int KW, int RT, int CT, int S>
+__global__ void __launch_bounds__(64 * WR * WT * KW, RT * CT > 4 || KW > 1 ? 2 : WR * WT / 2)
 gemm_i8_tile_kernel(GemmI8 a) {
     constexpr int W = WR * WT * KW, BN = 32 * RT * WR, BM = 32 * CT * WT;
     static_assert(BN % 64 == 0, "whole blocks of rows");
@@ -319,6 +353,7 @@ gemm_i8_tile_kernel(GemmI8 a) {
 #pragma unroll
     for (int u = 0; u < CT; ++u) {
         const int mu = (wt * CT + u) * 32;
+        if (m0 + mu >= a.M) break;
         float bv[16];
         int bi[16];
 #pragma unroll
@@ -333,7 +368,7 @@ gemm_i8_tile_kernel(GemmI8 a) {
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     y[k] = (float)acc[t][u][r + k] * __fmul_rn(iv[k], sc[t]);
-                    if (a.best && nw + i + 32 * t < a.N && y[k] > bv[r + k]) {
+                    if (BEST && nw + i + 32 * t < a.N && y[k] > bv[r + k]) {
                         bv[r + k] = y[k];
                         bi[r + k] = (int)nw + i + 32 * t;
                     }
@@ -373,104 +408,137 @@ gemm_i8_tile_kernel(GemmI8 a) {
             }
         }
         asm volatile("" ::: "memory");
-        if (a.best) {
+        if (BEST) {
             // 16 tokens' best of 32 lanes: half of the tokens go to the other half of the lanes
-            // each time, and the last of the five has one token in two lanes
-#pragma unroll
-            for (int d = 8; d >= 1; d >>= 1)
-#pragma unroll
-                for (int k = 0; k < d; ++k) {
-                    const bool up = i & (d << 1);
-                    float v = up ? bv[k + d] : bv[k];
-                    int n = up ? bi[k + d] : bi[k];
-                    take_best(v, n, __shfl_xor(up ? bv[k] : bv[k + d], d << 1),
-                              __shfl_xor(up ? bi[k] : bi[k + d], d << 1));
-                    bv[k] = v;
-                    bi[k] = n;
-                }
-            take_best(bv[0], bi[0], __shfl_xor(bv[0], 1), __shfl_xor(bi[0], 1));
-            const int r = i >> 1;  // (bits 4 .. 1 of the lane are bits 3 .. 0 of the token)
-            const int m = m0 + mu + 8 * (r >> 2) + 4 * g + (r & 3);
+            // each time (lane bits 4 .. 1 become token bits 3 .. 0), the last time a token has two
+            best_swap16(bv, bi);
+            best_halve<4, kDppMirror>(bv, bi, i & 8);
+            best_halve<2, kDppHalfMirror>(bv, bi, i & 4);
+            best_halve<1, kDppXor2>(bv, bi, i & 2);
+            take_best(bv[0], bi[0], dpp_f<kDppXor1>(bv[0]), dpp_i<kDppXor1>(bi[0]));
+            const int r = i >> 1, m = m0 + mu + 8 * (r >> 2) + 4 * g + (r & 3);
             if ((i & 1) == 0 && m < a.M)
-                a.best[(int64_t)m * a.parts + bn * WR + wr] = make_float2(bv[0], __int_as_float(bi[0]));
+                a.best[(int64_t)m * a.parts + bn * WR + wr] =
+                    make_float2(bv[0], __int_as_float(bi[0]));
         }
     }
 }
 
-__global__ void __launch_bounds__(256) gemm_i8_best_kernel(const float2* best, int parts,
-                                                           int32_t* out) {
-    __shared__ float rv[4];
-    __shared__ int ri[4];
-    const float2* row = best + (int64_t)blockIdx.x * parts;
+// Joins the parts of a row's largest value, W waves to a row.
+template <int W>
+__global__ void __launch_bounds__(W > 1 ? 64 * W : 256)
+gemm_i8_best_kernel(const float2* best, int parts, int M, int32_t* out) {
+    __shared__ float rv[W];
+    __shared__ int ri[W];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int m = W > 1 ? blockIdx.x : blockIdx.x * 4 + wave;
+    if (m >= M) return;
+    const float2* row = best + (int64_t)m * parts;
     float v = -INFINITY;
     int n = INT32_MAX;
-    for (int i = threadIdx.x; i < parts; i += 256) {
+#pragma unroll 4
+    for (int i = W > 1 ? threadIdx.x : lane; i < parts; i += 64 * W) {
         const float2 e = row[i];
         take_best(v, n, e.x, __float_as_int(e.y));
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) take_best(v, n, __shfl_xor(v, d), __shfl_xor(n, d));
-    if ((threadIdx.x & 63) == 0) {
-        rv[threadIdx.x >> 6] = v;
-        ri[threadIdx.x >> 6] = n;
+    if (W > 1) {
+        if (lane == 0) {
+            rv[wave] = v;
+            ri[wave] = n;
+        }
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int w = 1; w < W; ++w) take_best(v, n, rv[w], ri[w]);
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 4; ++w) take_best(v, n, rv[w], ri[w]);
-        out[blockIdx.x] = n;
-    }
+    if (lane == 0) out[m] = n;
 }
 
-// The kernel for M tokens and N channels, and the parts that a row's largest value comes in.
-enum GemmShape { kFewNarrow, kFewWide, kTile64, kTile128, kTile256 };
+// The kernel of a call, and the parts that a row's largest value comes in.
+enum GemmShape { kFew16x16, kFew32x16, kFew32x32, kFew64x32, kTile64x32, kTile64x64, kTile128x64,
+                 kTile128x128, kTile256x128, kTile256x256 };  // channels x tokens
 struct GemmPlan {
     GemmShape shape;
-    int bm;     // tokens of a workgroup, few tokens
-    int parts;  // columns: as many as the rows' bests
+    int parts;
 };
+// Larger workgroups read less for a product, smaller ones are more, and a step of a tile takes 0.16
+// to 0.6 us whatever its size: the largest shape of which there are enough to fill the GPU. Measured,
+// us (fp16 outputs, weights not in the caches), by the columns of kShapes below:
+//                       16x16 32x16 32x32 64x32 | 64x32 64x64 128x64 128x128 256x128 256x256
+//     1 x   2560 x 2560   4.5   5.1   6.8  12.4 |   6.6   8.6     11      20      25      31
+//    32 x   2560 x 2560   8.7   6.8   8.7    11 |   7.7   8.5     12      20      25      31
+//   128 x   2560 x 6912    33    20    26    18 |  16.6  20.3     32      62      88      70
+//   300 x   2560 x 6912                         |  25.5  18.9     28      61      88      87
+//    16 x   6912 x 2560   9.5   7.5   8.1    13 |   9.2   9.0     12      22      29      32
+//    32 x   6912 x 2560    18  11.9   9.4  11.5 |  10.1   9.3     13      22      29      32
+//   200 x   6912 x 2560                         |  19.9  13.6   12.6    19.1      29      34
+//   512 x   6912 x 2560                         |  45.6  26.7   22.1    20.9      38      42
+//  1024 x   6912 x 2560                         |  84.3  44.2   37.3    29.9    37.0    41.2
+//  2048 x   6912 x 2560                         |        76.6   61.1    53.1    42.3    42.8
+//  4001 x   2560 x 6912                         |                        101      91      80
+//     1 x 128256 x 2560    83    65    61    58 |    75    63     62      65      65      78
+//    32 x 128256 x 2560               110    79 |    87    74     70      72      70      85
+//   300 x 128256 x 2560                         |                191     179     142     192
+// (channels and tokens of a workgroup, channels of a part)
+constexpr int kShapes[][3] = {{16, 16, 16},  {32, 16, 32},   {32, 32, 32},   {64, 32, 64},
+                              {64, 32, 32},  {64, 64, 32},   {128, 64, 64},  {128, 128, 32},
+                              {256, 128, 64}, {256, 256, 128}};
 GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K) {
-    GemmPlan p;
-    p.bm = M <= 16 ? 16 : M <= 32 ? 32 : 64;
-    if (M <= 64) {
-        p.shape = ceil_div(N, 64) >= 512 ? kFewWide : kFewNarrow;
-        p.parts = (int)ceil_div(N, p.shape == kFewWide ? 64 : 16);
-        return p;
-    }
-    if (ceil_div(M, 256) * ceil_div(N, 256) >= 160)
-        p.shape = kTile256;
-    else if (ceil_div(M, 128) * ceil_div(N, 128) >= 160)
-        p.shape = kTile128;
-    else
-        p.shape = kTile64;
-    p.parts = (int)(p.shape == kTile256 ? 2 * ceil_div(N, 256)
-                    : p.shape == kTile128 ? 2 * ceil_div(N, 128) : 2 * ceil_div(N, 64));
-    return p;
+    const auto count = [&](GemmShape s) {
+        return ceil_div(N, kShapes[s][0]) * ceil_div(M, kShapes[s][1]);
+    };
+    GemmShape s = kTile64x32;
+    if (count(kFew16x16) <= 256)
+        s = kFew16x16;
+    else if (M <= 64 && count(kFew32x16) <= 256)
+        s = kFew32x16;
+    else if (M <= 32 && count(kFew32x32) <= 256)
+        s = kFew32x32;
+    else if (M <= 16 && count(kFew64x32) >= 900)
+        s = kFew64x32;
+    else if (count(kTile256x256) >= 150 && count(kTile256x256) <= 192 &&
+             2 * ceil_div(M, 256) == ceil_div(M, 128))
+        s = kTile256x256;  // (one to a CU: of 256 x 128 some CUs would have two)
+    else if (count(kTile256x128) >= 300)
+        s = kTile256x128;
+    else if (count(kTile128x128) >= 200)
+        s = kTile128x128;
+    else if (count(kTile128x64) >= (K < 4096 ? 150 : 200))
+        s = kTile128x64;
+    else if (count(kTile64x64) >= 150)
+        s = kTile64x64;
+    return {s, (int)(ceil_div(N, kShapes[s][0]) * (kShapes[s][0] / kShapes[s][2]))};
 }
 
-template <int MT>
-void launch_few(const GemmPlan& p, const GemmI8& a, hipStream_t st) {
-    const dim3 grid((unsigned)a.parts, (unsigned)ceil_div(a.M, p.bm));
-    if (p.shape == kFewWide)
-        hipLaunchKernelGGL((gemm_i8_few_kernel<MT, 4, 4, 4>), grid, dim3(256), 0, st, a);
-    else
-        hipLaunchKernelGGL((gemm_i8_few_kernel<MT, 1, 8, 4>), grid, dim3(512), 0, st, a);
+template <int MT, int NT, int KW, int DEPTH>
+void launch_few(const GemmI8& a, hipStream_t st) {
+    hipLaunchKernelGGL((gemm_i8_few_kernel<MT, NT, KW, DEPTH>),
+                       dim3((unsigned)ceil_div(a.N, 16 * NT), (unsigned)ceil_div(a.M, 16 * MT)),
+                       dim3(64 * KW), 0, st, a);
 }
-template <int TYPE, int WR, int WT, int KW, int RT, int CT, int S>
+template <int TYPE, bool BEST, int WR, int WT, int KW, int RT, int CT, int S>
 void launch_tile(const GemmI8& a, hipStream_t st) {
     // (a number of workgroups that is shared out among the XCDs evenly: the last have no tile)
     const int64_t nt = ceil_div(a.N, 32 * RT * WR), mt = ceil_div(a.M, 32 * CT * WT);
-    hipLaunchKernelGGL((gemm_i8_tile_kernel<TYPE, WR, WT, KW, RT, CT, S>),
+    hipLaunchKernelGGL((gemm_i8_tile_kernel<TYPE, BEST, WR, WT, KW, RT, CT, S>),
                        dim3((unsigned)(ceil_div(nt * mt, 8) * 8)), dim3(64 * WR * WT * KW), 0, st, a);
 }
-
-template <int TYPE>
+template <int TYPE, bool BEST>
 void launch_shape(GemmShape shape, const GemmI8& a, hipStream_t st) {
-    if (shape == kTile256)
-        launch_tile<TYPE, 2, 4, 1, 4, 2, 4>(a, st);
-    else if (shape == kTile128)
-        launch_tile<TYPE, 2, 2, 1, 2, 2, 4>(a, st);
-    else
-        launch_tile<TYPE, 2, 2, 2, 1, 1, 4>(a, st);
+    switch (shape) {
+        case kFew16x16: return launch_few<1, 1, 16, 2>(a, st);
+        case kFew32x16: return launch_few<1, 2, 16, 2>(a, st);
+        case kFew32x32: return launch_few<2, 2, 8, 2>(a, st);
+        case kFew64x32: return launch_few<2, 4, 4, 3>(a, st);
+        case kTile64x32: return launch_tile<TYPE, BEST, 2, 1, 4, 1, 1, 4>(a, st);
+        case kTile64x64: return launch_tile<TYPE, BEST, 2, 2, 1, 1, 1, 9>(a, st);
+        case kTile128x64: return launch_tile<TYPE, BEST, 2, 2, 1, 2, 1, 6>(a, st);
+        case kTile128x128: return launch_tile<TYPE, BEST, 4, 2, 1, 1, 2, 4>(a, st);
+        case kTile256x128: return launch_tile<TYPE, BEST, 4, 2, 1, 2, 2, 3>(a, st);
+        case kTile256x256: return launch_tile<TYPE, BEST, 2, 4, 1, 4, 2, 4>(a, st);
+    }
 }
 
 }  // namespace
@@ -514,23 +582,20 @@ TENZO_HIP_API int tenzo_hip_gemm_i8(const int8_t* codes, int64_t codes_stride,
     const hipStream_t st = (hipStream_t)stream;
     GemmI8 a{codes, M == 1 ? K : codes_stride, q, (const uint8_t*)w_packed, scales, y, y_stride,
              out_idx ? (float2*)ws : nullptr, N, (int)M, (int)(K / 16), p.parts, dtype};
-    if (p.shape >= kTile64) {
-        if (dtype == 0)
-            launch_shape<0>(p.shape, a, st);
-        else if (dtype == 1)
-            launch_shape<1>(p.shape, a, st);
-        else
-            launch_shape<2>(p.shape, a, st);
-    } else if (p.bm == 16)
-        launch_few<1>(p, a, st);
-    else if (p.bm == 32)
-        launch_few<2>(p, a, st);
+    if (dtype == 0)
+        out_idx ? launch_shape<0, true>(p.shape, a, st) : launch_shape<0, false>(p.shape, a, st);
+    else if (dtype == 1)
+        out_idx ? launch_shape<1, true>(p.shape, a, st) : launch_shape<1, false>(p.shape, a, st);
     else
-        launch_few<4>(p, a, st);
+        out_idx ? launch_shape<2, true>(p.shape, a, st) : launch_shape<2, false>(p.shape, a, st);
     const int rc = launch_status("gemm_i8 kernel");
     if (rc || !out_idx) return rc;
-    hipLaunchKernelGGL(gemm_i8_best_kernel, dim3((unsigned)M), dim3(256), 0, st, a.best, a.parts,
-                       out_idx);
+    if (a.parts > 256)
+        hipLaunchKernelGGL(gemm_i8_best_kernel<8>, dim3((unsigned)M), dim3(512), 0, st, a.best,
+                           a.parts, a.M, out_idx);
+    else
+        hipLaunchKernelGGL(gemm_i8_best_kernel<1>, dim3((unsigned)ceil_div(M, 4)), dim3(256), 0,
+                           st, a.best, a.parts, a.M, out_idx);
     return launch_status("gemm_i8_best_kernel");
 }
 
