@@ -1,7 +1,10 @@
 // Attention over the paged cache held in 4 bits (layout: kv4.h): every row of queries at its own
 // position of its own sequence, o = sum_t softmax_t(q.k_t / sqrt(128)) v_t over the positions up
 // to its own; a row that sees no position is zero.
+#include <type_traits>
+
 #include "kv4.h"
+#include "lds_ring.h"
 
 namespace tz {
 namespace {
@@ -220,16 +223,20 @@ __device__ __forceinline__ bool find_unit(const Kv4Seqs& sq, int unit, int G, in
 // Work of a sequence where steps are dealt evenly: each of its (kv head, row tile) units takes
 // ceil(length / 256) steps, whatever of them a row sees, and counts one more for what a unit costs
 // besides (its queries, the first tokens' way, the sums' meeting: about 4 us, a step 3 to 5).
-constexpr int kStep = 4 * kTile;
+// (128 rows: steps of 64 tokens, and four more for a unit's queries and sums.)
+constexpr int kRowsRT = 128;
+template <int ROWS>
 struct SeqWork {
+    static constexpr int kStep = ROWS == kRowsRT ? kTile : 4 * kTile;
+    static constexpr int kExtra = ROWS == kRowsRT ? 4 : 1;
     int first, n, c, steps, tiles;
-    __device__ __forceinline__ SeqWork(const Kv4Seqs& sq, int b, int G, int RT) {
+    __device__ __forceinline__ SeqWork(const Kv4Seqs& sq, int b, int G) {
         n = sq.rows(b, first);
         c = sq.length(b);
         steps = (c + kStep - 1) / kStep;
-        tiles = (n * G + RT - 1) / RT;
+        tiles = (n * G + ROWS - 1) / ROWS;
     }
-    __device__ __forceinline__ int slots() const { return steps + 1; }  // of a unit
+    __device__ __forceinline__ int slots() const { return steps + kExtra; }  // of a unit
     __device__ __forceinline__ int total(int Hkv) const {
         return c > 0 ? slots() * tiles * Hkv : 0;
     }
@@ -248,7 +255,7 @@ __device__ __forceinline__ int scan_work(const Kv4Attn& a, const Kv4Seqs& sq, in
                                          uint32_t* wsum, int& mine, int& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t v = 0;
-    for (int b = b0; b < b1; ++b) v = add_sat(v, SeqWork(sq, b, a.G, ROWS).total(sq.Hkv));
+    for (int b = b0; b < b1; ++b) v = add_sat(v, SeqWork<ROWS>(sq, b, a.G).total(sq.Hkv));
     uint32_t incl = v;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -711,8 +718,6 @@ kv4_attn_kernel(Kv4Attn a, Kv4Seqs sq) {
     kv4_segment<ROWS, RW, HALF, false, TREE>(a, sq, g, sm);
 }
 
-constexpr int kRowsRT = 128;
-
 // Sequence and row tile of a work unit of the prompts' kernel, those that see the most tokens first
 // whatever their sequence: tile k of a sequence starts at position length - rows + 128 k / G, and
 // the unit-th largest start, in 64 tokens, is found by bisection (a lane a sequence; one sequence,
@@ -778,7 +783,7 @@ __device__ __forceinline__ bool find_unit_latest(const Kv4Seqs& sq, int unit, in
 // that with the parts). The matrix units are busy for a third of it and the vector units nearly as
 // long, and two waves a SIMD, all that the registers allow, overlap them only in part; 16 us go
 // into a workgroup's queries and outputs.
-template <bool HALF, bool TREE>
+template <bool HALF>
 __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seqs sq) {
     // two tiles' keys and values (the first is the queries' on their way to registers before)
     __shared__ __align__(16) uint16_t tiles[2][2][kTile * kKv4Dim];
@@ -795,8 +800,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
     const int c = sq.length(seq);
     const int t0 = split * a.chunk, row0 = tile * kRowsRT;
     const int last_i = min(n - 1, a.token(row0 + kRowsRT - 1));
-    // tokens that some row sees
-    const int t1 = TREE ? min(t0 + a.chunk, c) : min(min(t0 + a.chunk, c - n + last_i + 1), c);
+    const int t1 = min(min(t0 + a.chunk, c - n + last_i + 1), c);  // tokens that some row sees
     if (split > 0 && t0 >= t1) return;
 
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, j = lane >> 4;
@@ -921,9 +925,8 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
             *reinterpret_cast<uint4*>(dst + wave * 16 * kKv4Dim + wr[st]) =
                 fp4_to_half8(w[st], sc);
     };
-    // the last token that all of the wave's rows see, and that any does
-    const int low = TREE ? c - n - 1 : c - n + a.token(wrow);
-    const int high = TREE ? c - 1 : c - n + min(n - 1, a.token(wrow + 31));
+    const int low = c - n + a.token(wrow);                      // the wave's first position
+    const int high = c - n + min(n - 1, a.token(wrow + 31));  // and its last
     // A tile into its half of LDS. What fp16 does not hold as it is: keys are moved token by token;
     // values all together, which waits for the tile's turn (the values then go in again).
     int vby = 0;
@@ -1031,17 +1034,13 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
             float shift[2];
 #pragma unroll
             for (int ct = 0; ct < 2; ++ct) {
-                if (mask) {
-                    const uint64_t bits =
-                        TREE && pos[ct] >= 0 ? seen64(a, grow[ct], t, c - n, c) >> (4 * j) : 0;
+                if (mask)
 #pragma unroll
                     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (ids[tt] < 0 || (TREE ? !(bits >> (16 * tt + i) & 1)
-                                                     : t + 16 * tt + 4 * j + i > pos[ct]))
+                            if (ids[tt] < 0 || t + 16 * tt + 4 * j + i > pos[ct])
                                 s[ct][tt][i] = -INFINITY;
-                }
                 float top[4];
 #pragma unroll
                 for (int tt = 0; tt < 4; ++tt)
@@ -1128,7 +1127,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
             for (int i = 0; i < 4; ++i) v[i] = __builtin_ldexpf(v[i], e);
             return v;
         };
-        if ((TREE && pos[ct] >= 0 ? c - 1 : pos[ct]) < a.chunk || a.splits == 1) {
+        if (pos[ct] < a.chunk || a.splits == 1) {
             if (split > 0) continue;
             if (vshift != 0 && L != 0.0f) {
 #pragma unroll
@@ -1153,15 +1152,35 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
     }
 }
 
+#include "attention_kv4_tree.h"
+
 // Several sequences of a few rows: all their steps in a row (sequence by sequence, unit by unit)
 // and an equal share of them to each of as many workgroups as the GPU holds at once, so that
 // lengths, which only the device knows, need not be alike. A share holds the end of a unit that
 // an earlier workgroup began, whole units and the beginning of one: two records at most. 48
 // sequences of up to 8190 tokens (223127 in all), 32 / 8 heads, fp16: 54 us, 4.5 TB/s.
 template <int ROWS, bool HALF, bool TREE>
-__global__ void __launch_bounds__(256, ROWS == 16 ? 2 : 3)
+struct EvenSegment {
+    typedef Kv4Smem<ROWS, 1> Smem;
+    static __device__ __forceinline__ void run(const Kv4Attn& a, const Kv4Seqs& sq,
+                                               const Segment& g, Smem& sm) {
+        kv4_segment<ROWS, 1, HALF, true, TREE>(a, sq, g, sm);
+    }
+};
+template <bool HALF>
+struct EvenSegment<kRowsRT, HALF, true> {
+    typedef Kv4TreeSmem Smem;
+    static __device__ __forceinline__ void run(const Kv4Attn& a, const Kv4Seqs& sq,
+                                               const Segment& g, Smem& sm) {
+        kv4_tree_segment<HALF>(a, sq, g, sm);
+    }
+};
+template <int ROWS, bool HALF, bool TREE>
+__global__ void __launch_bounds__(256, ROWS >= 16 ? 2 : 3)
 kv4_attn_even_kernel(Kv4Attn a, Kv4Seqs sq) {
-    __shared__ Kv4Smem<ROWS, 1> sm;
+    typedef EvenSegment<ROWS, HALF, TREE> Piece;
+    typedef SeqWork<ROWS> Work;
+    __shared__ typename Piece::Smem sm;
     __shared__ uint32_t wsum[4];
     __shared__ int at_base, at_seq;
     const int per = (sq.B + 255) / 256, b0 = threadIdx.x * per;
@@ -1175,7 +1194,7 @@ kv4_attn_even_kernel(Kv4Attn a, Kv4Seqs sq) {
     if (begin >= base && begin < base + mine) {
         int b = b0;
         for (;; ++b) {
-            const int w = SeqWork(sq, b, a.G, ROWS).total(sq.Hkv);
+            const int w = Work(sq, b, a.G).total(sq.Hkv);
             if (begin < base + w) break;
             base += w;
         }
@@ -1186,7 +1205,7 @@ kv4_attn_even_kernel(Kv4Attn a, Kv4Seqs sq) {
     int b = uniform(at_seq);
     base = uniform(at_base);
     for (int at = begin; at < end && b < sq.B;) {
-        const SeqWork w(sq, b, a.G, ROWS);
+        const Work w(sq, b, a.G);
         const int past = at - base;
         if (past >= w.total(sq.Hkv)) {
             base += w.total(sq.Hkv);
@@ -1196,9 +1215,9 @@ kv4_attn_even_kernel(Kv4Attn a, Kv4Seqs sq) {
         const int unit = past / w.slots(), s0 = past - unit * w.slots();
         const int len = min(w.slots() - s0, end - at);
         at += len;
-        // (slot 0 is the one without tokens)
-        const int from = max(s0 - 1, 0), to = s0 + len - 1;
-        if (to == from) continue;
+        // (the first slots are those without tokens)
+        const int from = max(s0 - Work::kExtra, 0), to = s0 + len - Work::kExtra;
+        if (to <= from) continue;
         Segment g;
         g.seq = b;
         g.first = w.first;
@@ -1206,12 +1225,12 @@ kv4_attn_even_kernel(Kv4Attn a, Kv4Seqs sq) {
         g.c = w.c;
         g.h = unit / w.tiles;
         g.tile = unit - g.h * w.tiles;
-        g.t0 = from * kStep;
-        g.len = (to - from) * kStep;
+        g.t0 = from * Work::kStep;
+        g.len = (to - from) * Work::kStep;
         g.whole = to - from == w.steps;
         g.rec = ((int64_t)blockIdx.x * 2 + (from == 0 ? 1 : 0)) * ROWS;
         g.split = 0;
-        kv4_segment<ROWS, 1, HALF, true, TREE>(a, sq, g, sm);
+        Piece::run(a, sq, g, sm);
     }
 }
 
@@ -1312,7 +1331,7 @@ __global__ void __launch_bounds__(256) kv4_join_even_kernel(Kv4Attn a, Kv4Seqs s
     int mine, total;
     int base = scan_work<ROWS>(a, sq, b0, b1, wsum, mine, total);
     for (int b = b0; b < b1; ++b) {
-        const SeqWork w(sq, b, a.G, ROWS);
+        const SeqWork<ROWS> w(sq, b, a.G);
         if (row >= w.first && row < w.first + w.n)
             atomicMax(&at, (unsigned long long)(b + 1) << 32 | (uint32_t)base);
         base += w.total(sq.Hkv);
@@ -1323,7 +1342,7 @@ __global__ void __launch_bounds__(256) kv4_join_even_kernel(Kv4Attn a, Kv4Seqs s
     if (seq < 0 || head >= a.Hq) return;
     base = uniform((int)at);
     total = uniform(total);
-    const SeqWork w(sq, seq, a.G, ROWS);
+    const SeqWork<ROWS> w(sq, seq, a.G);
     const int64_t out_at = row * a.out_stride + (int64_t)head * kKv4Dim;
     if (w.c == 0) {
         if (!WIDE || grp == 0)
@@ -1332,7 +1351,7 @@ __global__ void __launch_bounds__(256) kv4_join_even_kernel(Kv4Attn a, Kv4Seqs s
     }
     if (total == 0) return;
     const int h = head / a.G, r = (row - w.first) * a.G + head - h * a.G;
-    const int start = base + (h * w.tiles + r / ROWS) * w.slots() + 1;
+    const int start = base + (h * w.tiles + r / ROWS) * w.slots() + SeqWork<ROWS>::kExtra;
     const int w0 = wg_of(start, total, a.wgs), w1 = wg_of(start + w.steps - 1, total, a.wgs);
     if (w0 == w1) return;
     // workgroup w0 has the unit's beginning (its second record), those after it continue it
@@ -1348,11 +1367,34 @@ struct Kv4Plan {
     int64_t wgs;
     size_t records;
 };
-Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu) {
+// kind: 0 no tree, 1 trees of fp32 rows, 2 of fp16 rows.
+enum { kNoTree, kTreeFloat, kTreeHalf };
+Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, int kind) {
     Kv4Plan p{};
     const int64_t per = cu ? ceil_div(T * G, B) : G;  // rows of an average sequence
     p.rows = per <= 4 ? 4 : 16;
     const int64_t ctx = (int64_t)table_width * kKv4Page;
+    // Trees, by rows x heads x tokens: 128 rows a workgroup and the steps dealt evenly cost 22 us
+    // before their first step (queries split into parts, the records of 512 shares), then two
+    // thirds of the time of 16 rows a workgroup. us, 16 rows | 128, B x nodes after tokens, 32 / 8
+    // heads: fp16 4 x 64 after 2000 (16M) 36 | 44, 16 x 32 after 2000 (33M) 44 | 36, 16 x 64 after
+    // 4000 (134M) 126 | 69; fp32 37 | 50, 45 | 42, 127 | 85.
+    const double pairs = (double)T * G * Hkv * ctx;
+    if (kind != kNoTree && per > 64 && ctx > 1024 && pairs > (kind == kTreeHalf ? 18e6 : 40e6)) {
+        const int64_t units = T * G / kRowsRT + B;
+        const int64_t most = units * Hkv * (ceil_div(ctx, kTile) + SeqWork<kRowsRT>::kExtra);
+        if (most <= INT32_MAX) {
+            p.rows = kRowsRT;
+            p.rw = 1;
+            p.even = true;
+            p.most = (int)most;
+            // (at least four steps to each: a share's sums are 64 KB to write and to read)
+            p.wgs = most < 2048 ? ceil_div(most, 4) : 512;
+            p.splits = 1;
+            p.records = (size_t)p.wgs * 2 * kRowsRT;
+            return p;
+        }
+    }
     // Rows of a workgroup: 16 against 256 tokens at a time spread few rows over the GPU; the
     // prompts' kernel, once it has work for a while (16 us go into its queries and outputs), reads
     // and converts a token once for 128; between, many rows of few tokens, 32. Measured in us, 20 /
@@ -1361,7 +1403,7 @@ Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu) {
     // 56, 512 after 8000 160 | 200 | 102.
     const double units128 = (double)T * G * Hkv / kRowsRT;
     p.rw = 1;
-    if (per > 64 && (units128 > 320 || units128 * ctx > 3500 * kTile))
+    if (kind == kNoTree && per > 64 && (units128 > 320 || units128 * ctx > 3500 * kTile))
         p.rw = 8;
     else if (per > 16 && T * G / 16 * Hkv > 512 && ctx <= 1024)
         p.rw = 2;
@@ -1408,8 +1450,9 @@ int launch_kv4_even(const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
                        s);
     const int rc = launch_status("kv4_attn_even_kernel");
     if (rc) return rc;
-    // few rows: a head to a workgroup, its records to 8 groups of lanes
-    if ((int64_t)a.T * a.Hq <= kWideJoin)
+    // few rows, or many records of each: a head to a workgroup, its records to 8 groups of lanes
+    const int64_t units = ((int64_t)a.T * a.G / ROWS + s.B) * s.Hkv;
+    if ((int64_t)a.T * a.Hq <= kWideJoin || (ROWS == kRowsRT && a.wgs > 4 * units))
         hipLaunchKernelGGL((kv4_join_even_kernel<ROWS, HALF, true>), dim3(a.T, a.Hq), dim3(256), 0,
                            st, a, s);
     else
@@ -1419,6 +1462,8 @@ int launch_kv4_even(const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
 }
 template <bool HALF, bool TREE>
 int launch_kv4_plan(const Kv4Plan& p, const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
+    if constexpr (TREE)
+        if (p.rows == kRowsRT) return launch_kv4_even<kRowsRT, HALF, true>(a, s, st);
     if (p.even)
         return p.rows == 4 ? launch_kv4_even<4, HALF, TREE>(a, s, st)
                            : launch_kv4_even<16, HALF, TREE>(a, s, st);
@@ -1429,8 +1474,7 @@ int launch_kv4_plan(const Kv4Plan& p, const Kv4Attn& a, const Kv4Seqs& s, hipStr
     else if (p.rw == 2)
         launch_kv4<16, 2, HALF, TREE>(a, s, st);
     else
-        hipLaunchKernelGGL((kv4_attn_rows_kernel<HALF, TREE>), dim3(a.wgs), dim3(256), 0, st, a,
-                           s);
+        hipLaunchKernelGGL(kv4_attn_rows_kernel<HALF>, dim3(a.wgs), dim3(256), 0, st, a, s);
     const int rc = launch_status("kv4_attn_kernel");
     if (rc || p.splits == 1) return rc;
     if ((int64_t)a.T * a.Hq <= kWideJoin)
@@ -1458,7 +1502,8 @@ int attn_kv4(const char* what, Kv4Attn& a, Kv4Seqs& s, int dtype, int table_widt
              "%s: %zu bytes of workspace needed, 16-byte aligned, %zu given", what, need,
              ws ? ws_bytes : 0);
     const int G = a.Hq / s.Hkv;
-    const Kv4Plan p = kv4_plan(s.T, s.B, G, s.Hkv, table_width, s.cu != nullptr);
+    const Kv4Plan p = kv4_plan(s.T, s.B, G, s.Hkv, table_width, s.cu != nullptr,
+                               !a.mask ? kNoTree : dtype ? kTreeHalf : kTreeFloat);
     TZ_CHECK(p.wgs <= 0xffffff && s.T <= 0x7fffff && a.Hq <= 65535, "%s: %d rows of %d heads",
              what, s.T, a.Hq);
     a.part_o = (float*)ws;
@@ -1488,7 +1533,7 @@ extern "C" {
 TENZO_HIP_API size_t tenzo_hip_attn_kv4_ws_bytes(int64_t T, int B, int Hq, int Hkv,
                                                  int table_width, int has_cu, int /*dtype*/) {
     if (T <= 0 || B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || table_width < 0) return 0;
-    const Kv4Plan p = kv4_plan(T, B, Hq / Hkv, Hkv, table_width, has_cu != 0);
+    const Kv4Plan p = kv4_plan(T, B, Hq / Hkv, Hkv, table_width, has_cu != 0, kNoTree);
     return p.records * (kKv4Dim * 4 + 8);
 }
 
@@ -1524,7 +1569,10 @@ TENZO_HIP_API int tenzo_hip_attn_kv4(const void* q, int dtype, int64_t q_stride,
 
 TENZO_HIP_API size_t tenzo_hip_attn_tree_kv4_ws_bytes(int64_t T, int B, int Hq, int Hkv,
                                                       int table_width, int has_cu, int dtype) {
-    return tenzo_hip_attn_kv4_ws_bytes(T, B, Hq, Hkv, table_width, has_cu, dtype);
+    if (T <= 0 || B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || table_width < 0) return 0;
+    const Kv4Plan p = kv4_plan(T, B, Hq / Hkv, Hkv, table_width, has_cu != 0,
+                               dtype ? kTreeHalf : kTreeFloat);
+    return p.records * (kKv4Dim * 4 + 8);
 }
 
 TENZO_HIP_API int tenzo_hip_attn_tree_kv4(const void* q, int dtype, int64_t q_stride,

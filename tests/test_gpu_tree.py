@@ -4,8 +4,8 @@ import numpy as np
 import pytest
 
 from tests import tree_plain as plain
-from tests.kv4_plan import plan
 from tests.test_gpu_kv4 import D, PAGE, Setup, ops, torch_dev  # noqa: F401
+from tests.tree_kernels import plan
 
 pytestmark = pytest.mark.gpu
 
@@ -64,6 +64,9 @@ def test_plan_of_single_nodes(torch_dev, ops):
 
 # --------------------------------------------------------------- attention ----
 
+WIDE = 20000  # pages of a table: the plan takes its width for the context
+
+
 class Trees(Setup):
     def __init__(self, seqs, Hq, Hkv, way="tree", words=None, **more):
         super().__init__(seqs, Hq, Hkv, rope=False, **more)
@@ -93,8 +96,12 @@ class Trees(Setup):
 
     def check(self, out, start=None):
         want = np.zeros((self.T, self.Hq, D)) if start is None else start.astype(np.float64)
+        # queries and weights are held to 22 bits or more in fp32 calls (2^-21 for the two), in
+        # fp16 calls of 128 rows weights to 11 (half a step: 2^-11), elsewhere every bit
+        half = self.dtype == np.float16 and self.kernel() == "128 even"
         want, tol = plain.attention(self.q, self.mask, self.pools, self.tables, self.ctx,
-                                    self.layer, self.cu, want, 2.0 ** -21)
+                                    self.layer, self.cu, want, 2.0 ** -21,
+                                    2.0 ** -11 if half else 2.0 ** -21)
         got = out.cpu().numpy().reshape(want.shape).astype(np.float64)
         step = np.finfo(self.dtype)
         tol = tol + float(step.eps) / 2 * (np.abs(want) + tol) + float(step.smallest_subnormal) / 2
@@ -103,7 +110,7 @@ class Trees(Setup):
 
     def kernel(self):
         return plan(self.T, len(self.seqs), self.Hq, self.Hkv, self.tables.shape[1],
-                    self.cu is not None)[0]
+                    self.cu is not None, self.dtype == np.float16)[0]
 
 
 @pytest.mark.parametrize("way", ["tree", "bits"])
@@ -111,15 +118,18 @@ class Trees(Setup):
 @pytest.mark.parametrize("seqs,Hq,Hkv,kernel,width", [
     ([(1, 1)], 1, 1, "4", None), ([(2, 3000)], 2, 2, "4", None),
     ([(3, 3), (0, 40), (2, 0), (1, 17)], 2, 2, "4", None),
-    ([(9, 9)], 10, 5, "16", None), ([(26, 777)], 20, 5, "16", None),
-    ([(33, 40), (5, 5), (64, 130), (7, 0), (1, 65)], 16, 2, "16", None),
-    ([(70, 600), (65, 65)], 4, 4, "16", None), ([(12, 5000)], 8, 8, "16", None),
+    ([(9, 9)], 10, 5, "16", None), ([(12, 777)], 20, 5, "16", None),
+    ([(3, 40), (5, 5), (6, 130), (7, 0), (1, 65)], 16, 2, "16", None),
+    ([(60, 600), (55, 65)], 4, 4, "16", None), ([(12, 5000)], 8, 8, "16", None),
     ([(6, 700 + 97 * i) for i in range(9)], 8, 8, "16 even", None),
     ([(1 + i % 2, 500 + 211 * i) for i in range(12)], 16, 16, "4 even", None),
     ([(2, 300)] * 5 + [(4, 4000)], 8, 8, "4 even", 400),
-    ([(20, 60 + i) for i in range(24)], 32, 8, "32", None),
-    ([(130, 170), (100, 1000), (64, 64)], 16, 1, "128", 2100),
-    ([(64, 200), (61, 5000), (40, 0), (30, 30)], 16, 1, "128", 2100)])
+    ([(10, 60 + i) for i in range(48)], 32, 8, "32", None),
+    ([(26, 777)], 20, 5, "128 even", WIDE), ([(130, 131)], 1, 1, "128 even", WIDE),
+    ([(33, 40), (5, 5), (64, 130), (7, 0), (1, 65)], 16, 2, "128 even", WIDE),
+    ([(130, 170), (100, 1000), (64, 64)], 16, 1, "128 even", WIDE),
+    ([(64, 200), (61, 5000), (40, 0), (30, 30)], 16, 1, "128 even", WIDE),
+    ([(40 + i, 300 + 50 * i) for i in range(9)], 8, 4, "128 even", WIDE)])
 def test_attention(torch_dev, ops, seqs, Hq, Hkv, kernel, width, dtype, way):
     s = Trees(seqs, Hq, Hkv, way, dtype=dtype, width=width, tail=2, seed=len(seqs)).dev(torch_dev)
     print("tree", seqs[:4], Hq, Hkv, dtype.__name__, way, s.kernel(), flush=True)
@@ -130,23 +140,32 @@ def test_attention(torch_dev, ops, seqs, Hq, Hkv, kernel, width, dtype, way):
     s.check(out, np.full((s.T, Hq, D), 7.0))  # (rows behind the last sequence as they were)
 
 
+BOTH = pytest.mark.parametrize("width", [None, WIDE])  # 16 rows a workgroup, 128
+
+
+@BOTH
 @pytest.mark.parametrize("way", ["chain", "flat", "odd"])
-def test_attention_shapes_of_trees(torch_dev, ops, way):
-    s = Trees([(40, 100), (64, 64), (129, 400)], 8, 2, way).dev(torch_dev)
+def test_attention_shapes_of_trees(torch_dev, ops, way, width):
+    s = Trees([(40, 100), (64, 64), (129, 400)], 8, 2, way, width=width).dev(torch_dev)
+    assert (s.kernel() == "128 even") == (width == WIDE)
     s.check(s.run(ops))
 
 
+@BOTH
 @pytest.mark.parametrize("prior", list(range(0, 70, 3)))
-def test_attention_where_the_tree_begins(torch_dev, ops, prior):
+def test_attention_where_the_tree_begins(torch_dev, ops, prior, width):
     """Trees that begin anywhere within a tile of 64 tokens and go over its end."""
-    s = Trees([(67, prior + 67), (5, prior + 5)], 4, 2, "bits", seed=prior).dev(torch_dev)
+    s = Trees([(67, prior + 67), (5, prior + 5)], 4, 2, "bits", seed=prior,
+              width=width).dev(torch_dev)
+    assert (s.kernel() == "128 even") == (width == WIDE)
     s.check(s.run(ops))
 
 
-def test_attention_chain_is_causal(torch_dev, ops):
+@BOTH
+def test_attention_chain_is_causal(torch_dev, ops, width):
     """A tree that is a chain gives what attn_kv4 gives for the same rows."""
     torch = torch_dev
-    s = Trees([(30, 333), (7, 64)], 8, 2, "chain").dev(torch)
+    s = Trees([(30, 333), (27, 64)], 8, 2, "chain", width=width).dev(torch)
     a = s.run(ops).cpu().numpy()
     b = ops.attn_kv4(s.d["q"], *s.args(), cu_q=s.d["cu"]).cpu().numpy()
     np.testing.assert_allclose(a, b, rtol=0, atol=2e-5 * np.abs(b).max())
@@ -157,17 +176,19 @@ def test_attention_without_cu(torch_dev, ops):
     s.check(s.run(ops))
 
 
-def test_attention_more_rows_than_tokens(torch_dev, ops):
-    s = Trees([(20, 12), (70, 3), (8, 8), (90, 66)], 8, 2, "bits").dev(torch_dev)
+@BOTH
+def test_attention_more_rows_than_tokens(torch_dev, ops, width):
+    s = Trees([(20, 12), (70, 3), (8, 8), (90, 66)], 8, 2, "bits", width=width).dev(torch_dev)
     s.check(s.run(ops))
 
 
-def test_attention_fewer_words_than_nodes(torch_dev, ops):
-    s = Trees([(140, 300), (3, 10)], 4, 2, "bits", words=1).dev(torch_dev)
+@BOTH
+def test_attention_fewer_words_than_nodes(torch_dev, ops, width):
+    s = Trees([(140, 300), (3, 10)], 4, 2, "bits", words=1, width=width).dev(torch_dev)
     s.check(s.run(ops))
 
 
-@pytest.mark.parametrize("width", [None, 1500])
+@BOTH
 def test_attention_absent_pages(torch_dev, ops, width):
     """Pages outside the pool, in front of the tree, within it, and all of a sequence's."""
     s = Trees([(40, 300), (33, 100), (16, 90), (66, 500)], 16, 1, "bits", width=width)
@@ -193,10 +214,11 @@ def test_attention_strides(torch_dev, ops):
     assert (out[1::2] == 3).all()
 
 
-def test_attention_large_scales(torch_dev, ops):
+@BOTH
+def test_attention_large_scales(torch_dev, ops, width):
     """Rows of the cache whose scales are the largest and the smallest ones stand where the mask
     does not look."""
-    s = Trees([(40, 200), (64, 64)], 8, 1, "bits")
+    s = Trees([(40, 200), (64, 64)], 8, 1, "bits", width=width)
     for b, (n, c) in enumerate(s.seqs):
         rows = s.mask[s.cu[b]:s.cu[b + 1]]
         rows &= ~np.uint64(0b101000)  # nodes 3 and 5
@@ -206,6 +228,73 @@ def test_attention_large_scales(torch_dev, ops):
                 a[s.tables[b, t // PAGE], :, :, t % PAGE] = v
     s.dev(torch_dev)
     s.check(s.run(ops))
+
+
+@pytest.mark.parametrize("order", ["rising", "falling", "any"])
+def test_attention_values_of_every_size(torch_dev, ops, order):
+    """Scales of values from the smallest to the largest, fp32, 128 rows a workgroup: what fp16 does
+    not hold as it is moves by a power of two."""
+    s = Trees([(40, 300), (33, 100), (9, 700)], 8, 1, "bits", width=WIDE)
+    assert s.kernel() == "128 even"
+    for b, (n, c) in enumerate(s.seqs):
+        e = s.rng.integers(1, 250, c)
+        e = np.sort(e) if order == "rising" else -np.sort(-e) if order == "falling" else e
+        for t in range(c):
+            at = (s.tables[b, t // PAGE], slice(None), slice(None), t % PAGE)
+            s.pools[3][at] = e[t] - s.rng.integers(0, 2, 4)
+    s.dev(torch_dev)
+    s.check(s.run(ops))
+
+
+@pytest.mark.parametrize("scale", [20, 100, 150, 220])
+def test_attention_keys_of_every_size(torch_dev, ops, scale):
+    """Scales of keys far from 1, and queries that bring the scores back, fp32."""
+    s = Trees([(40, 300), (33, 100)], 8, 1, "bits", width=WIDE)
+    s.pools[2][:] = scale + s.rng.integers(-2, 3, s.pools[2].shape)
+    s.q = (s.q * 2.0 ** (126 - scale)).astype(np.float32)
+    s.dev(torch_dev)
+    s.check(s.run(ops))
+
+
+@BOTH
+def test_attention_queries_that_are_not_finite(torch_dev, ops, width):
+    """A row with an infinity or NaN in its query is NaN where it sees a token, and no other row is
+    touched."""
+    s = Trees([(40, 300), (64, 64)], 8, 1, "tree", width=width).dev(torch_dev)
+    want = s.run(ops).cpu().numpy()
+    bad = [(3, 0, 5, np.inf), (17, 7, 127, np.nan), (60, 2, 64, -np.inf)]
+    for r, h, d, v in bad:
+        s.d["q"][r, h, d] = v
+    got = s.run(ops).cpu().numpy()
+    for r, h, _, _ in bad:
+        assert np.isnan(got[r, h]).all(), (r, h)
+        got[r, h] = want[r, h]
+    np.testing.assert_array_equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_attention_over_many_pages(torch_dev, ops, dtype):
+    """Shares of more pages than a workgroup has page numbers at a time (1024); a few rows looked
+    at."""
+    s = Trees([(130, 64400)], 128, 8, "tree", dtype=dtype, layers=1).dev(torch_dev)
+    assert s.kernel() == "128 even"
+    n, c = s.seqs[0]
+    assert (n * 16 // 128 + 1) * 8 * (c // 64) // 512 > 1024 // 4
+    got = s.run(ops).cpu().numpy()
+    half = dtype == np.float16
+    t = np.arange(c)
+    at = (s.tables[0, t // PAGE], 0)
+    for r, h in ((0, 0), (63, 17), (64, 127), (129, 64), (100, 90)):
+        K, V = (plain.values(a[at[0], 0, h // 16, t % PAGE], b[at[0], 0, h // 16, t % PAGE])
+                for a, b in ((s.pools[0], s.pools[2]), (s.pools[1], s.pools[3])))
+        node = t - (c - n)
+        bit = (s.mask[r, np.clip(node // 64, 0, 2)] >> (node % 64).astype(np.uint64)) & np.uint64(1)
+        see = (node < 0) | (bit == 1)
+        want, tol = plain.attention_row(s.q[r, h].astype(np.float64) / np.sqrt(D), K[see], V[see],
+                                        np.abs(V).max(), 2.0 ** -21,
+                                        2.0 ** -11 if half else 2.0 ** -21)
+        tol = tol + float(np.finfo(dtype).eps) / 2 * (np.abs(want) + tol) + 2.0 ** -25 * half
+        assert (np.abs(got[r, h] - want) <= tol).all(), (r, h)
 
 
 # ------------------------------------------------------------------ accept ----

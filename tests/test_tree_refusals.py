@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from tenzo_amd import _lib, ops
+from tests import tree_kernels
 from tests.test_kv4_refusals import A, POOLS, SEQS, _cache, _swap, cpu  # noqa: F401
 
 CALLS = {
@@ -78,6 +79,19 @@ def test_workspaces():
     assert L.tenzo_hip_gemm_i8_ws_bytes(5, 128256, 2560, 1) >= 5 * 8
     assert L.tenzo_hip_attn_tree_kv4_ws_bytes(0, 3, 8, 2, 9, 1, 0) == 0
     assert L.tenzo_hip_attn_tree_kv4_ws_bytes(30, 1, 8, 3, 9, 1, 0) == 0
+
+
+def test_plan_of_trees():
+    L, rng = _lib.load(), np.random.default_rng(0)
+    for _ in range(3000):
+        Hkv = int(rng.choice([1, 2, 5, 8]))
+        Hq, B = Hkv * int(rng.choice([1, 2, 4, 8, 16])), int(rng.integers(1, 65))
+        T, width = int(rng.integers(B, 130 * B)), int(rng.integers(0, 4000) * rng.integers(0, 2))
+        cu = bool(rng.integers(0, 5))
+        T = T if cu else B
+        for half in (0, 1):
+            want = tree_kernels.plan(T, B, Hq, Hkv, width, cu, half)[2]
+            assert L.tenzo_hip_attn_tree_kv4_ws_bytes(T, B, Hq, Hkv, width, cu, half) == want
 
 
 def _i32(*shape):

@@ -61,13 +61,40 @@ def tree_accept(parents, tokens, target, pools, tables, ctx, cu, most):
     return path, count, last, lens
 
 
-def attention(q, mask, pools, tables, ctx, layer, cu, out, parts_eps):
+def attention_row(x, kk, vv, vmax, q_eps, w_eps):
+    """softmax(kk x) vv of one row and head (x over sqrt(128) already) over the tokens that it sees,
+    and how far fp32 sums may be from it; vmax: the largest value that any row sees."""
+    u = 2.0 ** -24
+    s = kk @ x
+    p = np.exp(s - s.max())
+    p /= p.sum()
+    out = p @ vv
+    # (of a query's dim also 2^-19 of the largest of its 32 dims in fp16 calls of 128 rows, which
+    # hold it in 4 parts of 6 bits, and 2^-24 in fp32 ones: 5 parts)
+    half = w_eps > 2.0 ** -12
+    big = np.abs(x).reshape(4, 32).max(1).repeat(32)
+    ds = ((3 * u + q_eps + 128 * u) * (np.abs(kk) @ np.abs(x)) +
+          (2.0 ** -19 if half else 2.0 ** -24) * (np.abs(kk) @ big) +
+          2.0 ** -37 * np.abs(kk).max(-1) * np.abs(x).sum()).max()
+    # (weights p (1 + e), |e| <= w_eps, over their own sum: sum p (1 + e) v / sum p (1 + e) - sum p v
+    # = sum p e (v - o) to first order, o the output, and sum p |e| |v - o| <= w_eps (sum p |v| + |o|)
+    # <= 2 w_eps sum p |v|)
+    dp = 2 * ds + (8 + 2 * (s.max() - s).max()) * u + 2 * w_eps
+    tol = (dp + 2 * (len(s) + 32) * u) * (p @ np.abs(vv))
+    tol += 2.0 ** -126 * (1 + np.abs(vv)).sum(0)
+    # weights below fp16's normal numbers have a constant step, 2^-24 of what 1 stands for: 2^-15 of
+    # the largest weight, in fp16 calls of 128 rows 2^-8; half of it
+    tol += (2.0 ** -33 if half else 2.0 ** -40) * p.max() * np.abs(vv).sum(0)
+    return out, tol + 2.0 ** -37 * vmax
+
+
+def attention(q, mask, pools, tables, ctx, layer, cu, out, q_eps, w_eps):
     """out [T][Hq][128] and how far fp32 sums may be from it (the roundings that
     kv4_plain.attention counts, without those of a rotation), both updated for the rows of
-    sequences. q [T][Hq][128]; parts_eps: what queries and weights are rounded to."""
+    sequences. q [T][Hq][128]; q_eps, w_eps: what queries and weights are rounded to."""
     pk, pv, pks, pvs = pools
     Hq, Hkv = q.shape[1], pk.shape[2]
-    G, u = Hq // Hkv, 2.0 ** -24
+    G = Hq // Hkv
     tol = np.zeros_like(out)
     for b, (first, n, c) in enumerate(sequences(len(q), ctx, cu, tables.shape[1] * PAGE)):
         t = np.arange(c)
@@ -88,18 +115,8 @@ def attention(q, mask, pools, tables, ctx, layer, cu, out, parts_eps):
                 continue
             x = np.asarray(q[r], np.float64) / np.sqrt(D)
             for h in range(Hq):
-                kk, vv = K[see, h // G], V[see, h // G]
-                s = kk @ x[h]
-                p = np.exp(s - s.max())
-                p /= p.sum()
-                out[r, h] = p @ vv
-                ds = ((3 * u + parts_eps + 128 * u) * (np.abs(kk) @ np.abs(x[h])) +
-                      2.0 ** -37 * np.abs(kk).max(-1) * np.abs(x[h]).sum()).max()
-                dp = 2 * ds + (8 + 2 * (s.max() - s).max()) * u + parts_eps
-                tol[r, h] = (dp + 2 * (len(s) + 32) * u) * (p @ np.abs(vv))
-                tol[r, h] += 2.0 ** -126 * (1 + np.abs(vv)).sum(0)
-                tol[r, h] += 2.0 ** -40 * p.max() * np.abs(vv).sum(0)
-                tol[r, h] += 2.0 ** -37 * vmax[h // G]
+                out[r, h], tol[r, h] = attention_row(x[h], K[see, h // G], V[see, h // G],
+                                                     vmax[h // G], q_eps, w_eps)
     return out, tol
 
 
