@@ -292,11 +292,16 @@ TENZO_HIP_API int tenzo_hip_tree_plan(const int32_t* parents, const int32_t* ctx
                                       const int32_t* cu_q, int B, int64_t T, int most,
                                       uint64_t* mask, int32_t* positions, void* stream);
 /* Attention of the nodes over the cache: tenzo_hip_attn_kv4 with the same
- * arguments, accuracy and workspace rules, but that q is taken as it is (rotated
- * before, by tenzo_hip_rope), and that node i sees the ctx_lens[b] - n tokens in
- * front of the tree and the nodes j whose bit is set in its row of mask
- * (mask_words words, mask_stride words apart, 8-byte aligned; any bits, its own
- * too; nodes behind the last word are not seen). */
+ * arguments and workspace rules, but that q is taken as it is (rotated before, by
+ * tenzo_hip_rope), and that node i sees the ctx_lens[b] - n tokens in front of the
+ * tree and the nodes j whose bit is set in its row of mask (mask_words words, up
+ * to 1024, mask_stride words apart, 8-byte aligned; any bits, its own too; nodes
+ * behind the last word are not seen). Accuracy as there but in calls that give 128
+ * rows to a workgroup (over 64 rows times heads a kv head and sequence, a table of
+ * over 1024 tokens, and enough of them): a query's element is held to 2^-24 of the
+ * largest of its group of 32 dims, in fp16 calls to 2^-19; weights to 2^-22, in
+ * fp16 calls rounded once to fp16 (2^-11, as outputs are; below 2^-33 of a row's
+ * largest they are lost). */
 TENZO_HIP_API size_t tenzo_hip_attn_tree_kv4_ws_bytes(int64_t T, int B, int Hq, int Hkv,
                                                       int table_width, int has_cu, int dtype);
 TENZO_HIP_API int tenzo_hip_attn_tree_kv4(const void* q, int dtype, int64_t q_stride,
@@ -319,7 +324,8 @@ TENZO_HIP_API int tenzo_hip_attn_tree_kv4(const void* q, int dtype, int64_t q_st
  * The k-th node's cache rows, in every layer and head, are moved to slot
  * ctx_lens[b] - n + k; slots from lens[b] on hold what is left there. Pools as
  * tenzo_hip_beam_reorder_paged has them; a page that the pool does not hold
- * takes and gives nothing. Slots of one page in two sequences race. */
+ * takes and gives nothing. Slots of one page in two sequences race. lens and the
+ * other outputs are buffers of their own: none of them may be ctx_lens. */
 TENZO_HIP_API int tenzo_hip_tree_accept(const int32_t* parents, const int32_t* tokens,
                                         const int32_t* target, void* pk, void* pv, void* pks,
                                         void* pvs, int64_t n_blocks, int n_layers, int Hkv,
@@ -339,7 +345,7 @@ TENZO_HIP_API int tenzo_hip_tree_accept(const int32_t* parents, const int32_t* t
  * rounded once. Cosines and sines are within 2^-23 and 2^-51 of the angle, which
  * is taken in 64 bits. Any strides and alignment of rows; out may be x (with
  * its stride), else it must not overlap it. head_dim up to 1024, H * head_dim up
- * to 32768. */
+ * to 32768, T below 2^24. */
 TENZO_HIP_API int tenzo_hip_rope(const void* x, int dtype, int64_t x_stride,
                                  const int32_t* positions, const double* freqs, int64_t T, int H,
                                  int head_dim, int rot_dim, int interleaved, float mscale,
@@ -441,7 +447,7 @@ TENZO_HIP_API int tenzo_hip_argmax(const float* logits, int64_t V, int32_t* out_
  * 2^20. When out_idx is non-null, also each row's column of the largest value
  * (in fp32, before it is rounded to dtype; the lowest of equal ones; NaN counts as
  * -inf), by way of ws: a workspace of tenzo_hip_gemm_i8_ws_bytes(...) bytes,
- * 8-byte aligned, of this call alone until it has run. */
+ * 8-byte aligned, of this call alone until it has run. N up to 2^29. */
 TENZO_HIP_API size_t tenzo_hip_gemm_i8_ws_bytes(int64_t M, int64_t N, int64_t K, int want_idx);
 TENZO_HIP_API int tenzo_hip_gemm_i8(const int8_t* codes, int64_t codes_stride,
                                     const tenzo_hip_actq_t* q, const void* w_packed,

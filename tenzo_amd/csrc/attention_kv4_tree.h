@@ -19,8 +19,8 @@
 // A row's scores come out of the products as logarithms of its weights: queries carry 1/sqrt(128)
 // and log2 e, and the sums begin at kBits less the row's maximum so far. Only where a score goes
 // beyond what the weights' type holds (fp16 calls: 2^7 above the maximum; fp32 calls: at all) are
-// maximum, weights and sums moved. In fp16 calls weights are rounded to fp16 once (2^-12 of a weight,
-// as much as outputs are rounded by; those below 2^-33 of the largest are lost), in fp32 calls held
+// maximum, weights and sums moved. In fp16 calls weights are rounded to fp16 once (2^-11 of a weight
+// at most, as outputs are; those below 2^-33 of the largest are lost), in fp32 calls held
 // in two parts, 22 bits (2^-40). Their sum comes from the products too, from the same rounded
 // weights against ones.
 #pragma once

@@ -559,7 +559,7 @@ TENZO_HIP_API int tenzo_hip_gemm_i8(const int8_t* codes, int64_t codes_stride,
                                     int dtype, int64_t y_stride, int32_t* out_idx, void* ws,
                                     size_t ws_bytes, void* stream) {
     TZ_CHECK(dtype >= 0 && dtype <= 2, "gemm_i8: dtype %d", dtype);
-    TZ_CHECK(M >= 0 && M <= (1 << 20) && N > 0 && N <= (1 << 30), "gemm_i8: M=%lld N=%lld",
+    TZ_CHECK(M >= 0 && M <= (1 << 20) && N > 0 && N <= (1 << 29), "gemm_i8: M=%lld N=%lld",
              (long long)M, (long long)N);
     // (sums of K products of at most 2^14 stay within int32)
     TZ_CHECK(K > 0 && K % 16 == 0 && K <= 131056, "gemm_i8: K=%lld, not a multiple of 16 up to "

@@ -229,6 +229,8 @@ TENZO_HIP_API int tenzo_hip_tree_accept(const int32_t* parents, const int32_t* t
     TZ_CHECK(n_layers <= 65535 && Hkv <= 65535 * kMoveHeads, "tree_accept: %d layers", n_layers);
     if (B == 0) return TENZO_SUCCESS;
     TZ_CHECK(ctx_lens && path && count && next && lens, "tree_accept: null pointer");
+    TZ_CHECK(lens != ctx_lens && count != ctx_lens && next != ctx_lens && path != ctx_lens,
+             "tree_accept: the lengths are read while outputs are written");
     TZ_CHECK(T == 0 || (parents && tokens && target), "tree_accept: null pointer");
     const TreeAccept a{parents, tokens, target, path, count, next, lens, (uint8_t*)pk,
                        (uint8_t*)pv, (uint8_t*)pks, (uint8_t*)pvs, most};

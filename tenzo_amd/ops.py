@@ -560,8 +560,8 @@ def tree_accept(parents, tokens, target, pk, pv, pks, pvs, block_tables, ctx_len
     pools, sizes = _paged_pools(pk, pv, pks, pvs, dev)
     width = block_tables.shape[1]
     path = parents.new_empty((B, max(most, 0)))
-    per = parents.new_empty((3, B))
-    count, last, lens = per
+    count, last, lens = (torch.empty_like(ctx_lens), torch.empty_like(ctx_lens),
+                         torch.empty_like(ctx_lens))
     rc = _lib.load().tenzo_hip_tree_accept(
         pp, _whole(tokens, dev, _I32, "tokens"), _whole(target, dev, _I32, "target"), *pools,
         *sizes, _on(block_tables, dev, _I32, "block_tables"),

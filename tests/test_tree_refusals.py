@@ -19,8 +19,8 @@ CALLS = {
                                              ws_bytes=1 << 40, stream=None)),
     "accept": ("tenzo_hip_tree_accept", dict(
         parents=A, tokens=A, target=A, pk=A, pv=A, pks=A, pvs=A, n_blocks=4, n_layers=2, Hkv=2,
-        row_bytes=64, tables=A, stride=8, width=8, ctx=A, cu=A, B=3, T=9, most=5, path=A, count=A,
-        next=A, lens=A, stream=None)),
+        row_bytes=64, tables=A, stride=8, width=8, ctx=A, cu=A, B=3, T=9, most=5, path=A + 4096,
+        count=A + 4160, next=A + 4176, lens=A + 4192, stream=None)),
     "rope": ("tenzo_hip_rope", dict(x=A, dtype=0, xs=1024, at=A, f=A, T=3, H=8, dim=128, rot=128,
                                     inter=0, m=1.0, out=A + 8192, os=1024, stream=None)),
     "gemm": ("tenzo_hip_gemm_i8", dict(codes=A, cs=64, q=A, w=A, s=A, M=3, N=70, K=64, y=A, dtype=0,
@@ -41,14 +41,15 @@ BAD = {
     "accept": CACHE_BAD + [dict(parents=None), dict(tokens=None), dict(target=None),
                            dict(path=None), dict(count=None), dict(next=None), dict(lens=None),
                            dict(row_bytes=32), dict(most=0), dict(most=4097), dict(cu=None),
-                           dict(n_layers=65536)],
-    "rope": [dict(x=None), dict(at=None), dict(f=None), dict(out=None), dict(dtype=3),
+                           dict(n_layers=65536), dict(lens=A), dict(count=A), dict(next=A),
+                           dict(path=A)],
+    "rope": [dict(T=1 << 24), dict(x=None), dict(at=None), dict(f=None), dict(out=None), dict(dtype=3),
              dict(dtype=-1), dict(T=-1), dict(H=0), dict(dim=1), dict(dim=1026), dict(rot=0),
              dict(rot=3), dict(rot=130), dict(xs=1023), dict(os=1000), dict(H=257), dict(x=A + 2),
              dict(f=A + 4), dict(at=A + 2), dict(out=A, os=2048)],
     "gemm": [dict(codes=None), dict(q=None), dict(w=None), dict(s=None), dict(y=None),
              dict(ws=None), dict(ws_bytes=8), dict(ws=A + 4), dict(dtype=3), dict(M=-1),
-             dict(M=(1 << 20) + 1), dict(N=0), dict(N=(1 << 30) + 1), dict(K=0), dict(K=40),
+             dict(M=(1 << 20) + 1), dict(N=0), dict(N=(1 << 29) + 1), dict(K=0), dict(K=40),
              dict(K=131072, cs=131072), dict(cs=48), dict(cs=72), dict(ys=69), dict(codes=A + 8),
              dict(w=A + 4), dict(s=A + 2), dict(y=A + 2)],
 }
