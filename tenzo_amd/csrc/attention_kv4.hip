@@ -1374,13 +1374,18 @@ Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, int
     const int64_t per = cu ? ceil_div(T * G, B) : G;  // rows of an average sequence
     p.rows = per <= 4 ? 4 : 16;
     const int64_t ctx = (int64_t)table_width * kKv4Page;
-    // Trees, by rows x heads x tokens: 128 rows a workgroup and the steps dealt evenly cost 22 us
-    // before their first step (queries split into parts, the records of 512 shares), then two
-    // thirds of the time of 16 rows a workgroup. us, 16 rows | 128, B x nodes after tokens, 32 / 8
-    // heads: fp16 4 x 64 after 2000 (16M) 36 | 44, 16 x 32 after 2000 (33M) 44 | 36, 16 x 64 after
-    // 4000 (134M) 126 | 69; fp32 37 | 50, 45 | 42, 127 | 85.
+    // Trees, by rows x heads x tokens: 128 rows a workgroup and the steps dealt evenly cost 20 us
+    // before their first step (queries split into parts, the records of 512 shares), then half to
+    // two thirds of the time of 16 rows a workgroup. us, 16 rows | 128, B x up to n nodes after up to
+    // that many tokens: fp16, 16 / 2 heads, 1 x 26 after 16000 (7M) 26 | 28, 8 x 32 after 4000 (14M)
+    // 35 | 36, 32 / 8 heads, 4 x 64 after 2000 (14M) 38 | 35, 8 x 64 after 2000 (26M) 48 | 38, 16 x
+    // 64 after 4000 (134M) 126 | 69; fp32, the same but the first, 35 | 41, 38 | 43, 47 | 46, 127 |
+    // 85, and 1 x 64 after 16000 (33M) 66 | 54. A sequence of few rows leaves most of 128 unused:
+    // of 37 rows (19M) fp16 39 | 44, of 47 (48M) 81 | 62, fp32 of 47 (30M) 56 | 59, of 60 (62M) 91 |
+    // 80.
     const double pairs = (double)T * G * Hkv * ctx;
-    if (kind != kNoTree && per > 64 && ctx > 1024 && pairs > (kind == kTreeHalf ? 18e6 : 40e6)) {
+    if ((kind == kTreeHalf && per > 40 && pairs > 14e6 && ctx > 1024) ||
+        (kind == kTreeFloat && per > 56 && pairs > 22e6 && ctx > 1024)) {
         const int64_t units = T * G / kRowsRT + B;
         const int64_t most = units * Hkv * (ceil_div(ctx, kTile) + SeqWork<kRowsRT>::kExtra);
         if (most <= INT32_MAX) {
@@ -1450,9 +1455,11 @@ int launch_kv4_even(const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
                        s);
     const int rc = launch_status("kv4_attn_even_kernel");
     if (rc) return rc;
-    // few rows, or many records of each: a head to a workgroup, its records to 8 groups of lanes
+    // Few rows, or many records of each: a head to a workgroup, its records to 8 groups of lanes.
+    // Shares of a unit in trees' calls, and us with 8 groups | one: 34 39 | 49, 19 34 | 43, 13 74 |
+    // 72, 8 44 | 40, 6 49 | 40.
     const int64_t units = ((int64_t)a.T * a.G / ROWS + s.B) * s.Hkv;
-    if ((int64_t)a.T * a.Hq <= kWideJoin || (ROWS == kRowsRT && a.wgs > 4 * units))
+    if ((int64_t)a.T * a.Hq <= kWideJoin || (ROWS == kRowsRT && a.wgs > 16 * units))
         hipLaunchKernelGGL((kv4_join_even_kernel<ROWS, HALF, true>), dim3(a.T, a.Hq), dim3(256), 0,
                            st, a, s);
     else

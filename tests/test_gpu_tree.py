@@ -256,6 +256,20 @@ def test_attention_keys_of_every_size(torch_dev, ops, scale):
     s.check(s.run(ops))
 
 
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("seqs,Hkv,shares", [([(140, 3000), (60, 2500)], 1, 36),
+                                             ([(140, 3000), (60, 2500)], 8, 21),
+                                             ([(100, 2000)] * 7, 2, 5)])
+def test_attention_joins(torch_dev, ops, seqs, Hkv, shares, dtype):
+    """128 rows a workgroup, over 1024 rows times heads: the records of a row's head come from one
+    group of lanes up to 16 shares a unit, from 8 beyond."""
+    Hq = 8 * Hkv if Hkv < 8 else Hkv
+    s = Trees(seqs, Hq, Hkv, "tree", dtype=dtype, width=WIDE).dev(torch_dev)
+    assert s.kernel() == "128 even" and s.T * Hq > 1024
+    assert 512 // ((s.T * Hq // Hkv // 128 + len(seqs)) * Hkv) == shares
+    s.check(s.run(ops))
+
+
 @BOTH
 def test_attention_queries_that_are_not_finite(torch_dev, ops, width):
     """A row with an infinity or NaN in its query is NaN where it sees a token, and no other row is

@@ -9,7 +9,7 @@ def plan(T, B, Hq, Hkv, width, cu, half):
     """(kernel, splits, bytes of workspace), as kv4_plan.plan has them."""
     G, ctx = Hq // Hkv, width * PAGE
     per = _up(T * G, B) if cu else G
-    if per > 64 and ctx > 1024 and T * Hq * ctx > (18e6 if half else 40e6):
+    if per > (40 if half else 56) and ctx > 1024 and T * Hq * ctx > (14e6 if half else 22e6):
         most = (T * G // 128 + B) * Hkv * (_up(ctx, TILE) + 4)
         return "128 even", 1, min(_up(most, 4), 512) * 2 * 128 * RECORD
     # (the prompts' kernel serves no trees)
