@@ -99,6 +99,8 @@ __device__ __forceinline__ void best_halve(float (&v)[16], int (&n)[16], bool up
 // Few tokens: 16 NT rows of weights to a workgroup, whose KW waves share K: a wave has every KW-th
 // 64 of it, straight from memory to the matrix cores' operands, DEPTH steps ahead. The codes of the
 // 16 MT tokens come the same way, out of the L2. At the end the waves' sums meet in LDS.
+// 1 x 2560 x 6912: 7.1 us, 26 x 2560 x 6912: 10.3, where the weights take 3.5: a launch, 4 to 7
+// dependent rounds of loads a wave, and the meeting.
 template <int MT, int NT, int KW, int DEPTH>
 __global__ void __launch_bounds__(64 * KW) gemm_i8_few_kernel(GemmI8 a) {
     __shared__ i4v red[KW][NT * MT][64];
@@ -193,6 +195,8 @@ __global__ void __launch_bounds__(64 * KW) gemm_i8_few_kernel(GemmI8 a) {
 // with the 16 lanes that LDS serves together in different banks. The codes are the first operand,
 // so that a register of the result holds 32 neighbouring channels of a token in 32 lanes.
 // Each half of a step's fragments (32 k) is read while the half before it is multiplied.
+// 4001 x 6912 x 2560, fp16: 78 us, 1.8 POP/s, bound by the matrix units and the clock that their
+// power leaves (zeros run faster); 26 x 128256 x 2560, fp32: 66 us, 5.1 TB/s, bound by the weights.
 template <int TYPE, bool BEST, int WR, int WT, int KW, int RT, int CT, int S>
 __global__ void __launch_bounds__(64 * WR * WT * KW, RT * CT > 4 || KW > 1 ? 2 : WR * WT / 2)
 gemm_i8_tile_kernel(GemmI8 a) {

@@ -19,7 +19,8 @@ struct TreePlan {
 // A wave to 64 nodes of a sequence. Up to 64 nodes in all a node's ancestors are gathered by
 // doubling: after k rounds a lane knows 2^k of them and the one after those. More nodes walk up
 // one by one, over parents in LDS; each is smaller than the one before, so the words of a mask
-// come from its last to its first.
+// come from its last to its first. 64 trees of up to 64 nodes: 2.5 us, a launch and two loads in a
+// row; 8 of up to 130: 3.4.
 __global__ void __launch_bounds__(64) tree_plan_kernel(TreePlan a, Kv4Seqs sq) {
     __shared__ int par[kMostNodes];
     const int b = blockIdx.x, lane = threadIdx.x, i = blockIdx.y * 64 + lane;
@@ -105,7 +106,9 @@ constexpr int kMoveRows = 16, kMoveHeads = 8;
 // A workgroup to a sequence, layer and 8 heads. Each walks the tree by itself (a second launch
 // would cost more); those of the first layer and heads write what came out. Rows are moved 16 at a
 // time, all read before one is written: a row's new slot is never above its old one, so slots that
-// are still to be read lie behind those that are written.
+// are still to be read lie behind those that are written. 64 trees of up to 64 nodes, 30 layers of 5
+// heads: 8.6 us, the walk's chain of loads (a target, then 64 parents and tokens, for each node of the
+// path); one tree of 26, 3.4.
 template <int PIECES>  // of 16 bytes, of a row's codes
 __global__ void __launch_bounds__(256) tree_accept_kernel(TreeAccept a, Kv4Seqs sq) {
     __shared__ int path[kMostNodes];
