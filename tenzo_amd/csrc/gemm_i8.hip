@@ -97,39 +97,41 @@ __device__ __forceinline__ void best_halve(float (&v)[16], int (&n)[16], bool up
 }
 
 // Few tokens: 16 NT rows of weights to a workgroup, whose KW waves share K: a wave has every KW-th
-// 64 of it, straight from memory to the matrix cores' operands, DEPTH steps ahead. The codes of the
-// 16 MT tokens come the same way, out of the L2. At the end the waves' sums meet in LDS.
-// 1 x 2560 x 6912: 7.1 us, 26 x 2560 x 6912: 10.3, where the weights take 3.5: a launch, 4 to 7
-// dependent rounds of loads a wave, and the meeting.
-template <int MT, int NT, int KW, int DEPTH>
+// 128 of it, straight from memory to the matrix cores' operands, both halves loaded a turn ahead
+// (loads three to seven steps ahead, or 16 waves where there are tokens, take longer; a line of codes,
+// 128 bytes of a row, belongs to one wave's turn). The codes of the 16 MT tokens come the same way,
+// out of the L2. At the end the waves' sums meet in LDS. 1 x 2560 x 6912: 5.7 us, 24 x 2560 x 6912:
+// 8.4, where the weights take 3.5: a launch, three or four dependent rounds of loads, and the meeting;
+// 1 x 128256 x 2560: 52 us, 6.3 TB/s (a part of it out of the last cache).
+constexpr uint32_t kNone = 0x80000000u;  // an offset past every resource
+constexpr int kNt = 2;                   // a load that leaves nothing in the caches
+template <int MT, int NT, int KW>
 __global__ void __launch_bounds__(64 * KW) gemm_i8_few_kernel(GemmI8 a) {
     __shared__ i4v red[KW][NT * MT][64];
     const int lane = threadIdx.x & 63, col = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t n0 = (int64_t)blockIdx.x * (16 * NT);
     const int m0 = blockIdx.y * (16 * MT);
-    const int steps = (a.KB + 3) >> 2, mine = steps > wave ? (steps - wave + KW - 1) / KW : 0;
-    const int64_t blocks = (a.N + 63) >> 6, block = (int64_t)a.KB << 10;
-    const uint8_t* wb[NT > 4 ? NT / 4 : 1];  // (past the last block of rows: that one again)
-#pragma unroll
-    for (int b = 0; b < (NT > 4 ? NT / 4 : 1); ++b)
-        wb[b] = a.w + min((n0 >> 6) + b, blocks - 1) * block + ((n0 & 63) + col) * 16;
-    const int8_t* ab[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) ab[t] = a.codes + (int64_t)min(m0 + 16 * t + col, a.M - 1) * a.ldc;
-    i4v wv[DEPTH][NT], av[DEPTH][MT];
-    auto load = [&](int u, int i) {  // (past the last: that one again)
-        const int st = min(wave + KW * max(min(i, mine - 1), 0), steps - 1);
-        const int kb = min(4 * st + j, a.KB - 1);
+    const int turns = ((a.KB + 7) / 8 - wave + KW - 1) / KW;
+    // (what lies past K, or past the last turn, is taken from past the resources: zeros, and nothing
+    // is read)
+    const int rows = min(16 * MT, a.M - m0);
+    const auto rw = buf(a.w + (n0 >> 6) * ((int64_t)a.KB << 10), (uint32_t)a.KB << 10);
+    const auto rc = buf(a.codes + (int64_t)m0 * a.ldc, (uint32_t)((rows - 1) * a.ldc + a.KB * 16));
+    const uint32_t w0 = (uint32_t)((n0 & 63) + col) * 16, c0 = (uint32_t)(col * a.ldc);
+    i4v wv[2][NT], av[2][MT];
+    auto load = [&](int u, int turn) {
+        const uint32_t kb = (uint32_t)(8 * (wave + KW * turn) + 4 * u + j);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
-            wv[u][t] = __builtin_nontemporal_load(
-                reinterpret_cast<const i4v*>(wb[t >> 2] + ((int64_t)kb << 10) + (t & 3) * 256));
+            wv[u][t] = __builtin_bit_cast(
+                i4v, __builtin_amdgcn_raw_buffer_load_b128(rw, w0 + (kb << 10) + t * 256, 0, kNt));
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            av[u][t] = *reinterpret_cast<const i4v*>(ab[t] + kb * 16);
-            if (4 * st + j >= a.KB) av[u][t] = i4v{0, 0, 0, 0};
-        }
+        for (int t = 0; t < MT; ++t)
+            av[u][t] = __builtin_bit_cast(
+                i4v, __builtin_amdgcn_raw_buffer_load_b128(
+                         rc, kb < (uint32_t)a.KB ? c0 + (uint32_t)(16 * t * a.ldc) + kb * 16 : kNone,
+                         0, 0));
     };
     i4v acc[NT][MT];
 #pragma unroll
@@ -137,19 +139,17 @@ __global__ void __launch_bounds__(64 * KW) gemm_i8_few_kernel(GemmI8 a) {
 #pragma unroll
         for (int s = 0; s < MT; ++s) acc[t][s] = i4v{0, 0, 0, 0};
 #pragma unroll
-    for (int u = 0; u < DEPTH; ++u) load(u, u);
-    for (int i = 0; i < mine; i += DEPTH) {
+    for (int u = 0; u < 2; ++u) load(u, 0);
+    for (int i = 0; i < turns; ++i) {
 #pragma unroll
-        for (int u = 0; u < DEPTH; ++u) {
-            if (i + u < mine) {
+        for (int u = 0; u < 2; ++u) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int s = 0; s < MT; ++s)
-                        acc[t][s] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av[u][s], wv[u][t],
-                                                                         acc[t][s], 0, 0, 0);
-            }
-            load(u, i + u + DEPTH);
+                for (int s = 0; s < MT; ++s)
+                    acc[t][s] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av[u][s], wv[u][t], acc[t][s],
+                                                                     0, 0, 0);
+            load(u, i + 1);
         }
     }
 #pragma unroll
@@ -461,64 +461,73 @@ gemm_i8_best_kernel(const float2* best, int parts, int M, int32_t* out) {
 }
 
 // The kernel of a call, and the parts that a row's largest value comes in.
-enum GemmShape { kFew16x16, kFew32x16, kFew32x32, kFew64x32, kTile64x32, kTile64x64, kTile128x64,
-                 kTile128x128, kTile256x128, kTile256x256 };  // channels x tokens
+enum GemmShape { kOne16x16, kFew16x16, kFew32x16, kFew32x32, kFew64x32, kTile64x32, kTile64x64,
+                 kTile128x64, kTile128x128, kTile256x128, kTile256x256 };  // channels x tokens
 struct GemmPlan {
     GemmShape shape;
     int parts;
 };
-// Larger workgroups read less for a product, smaller ones are more, and a step of a tile takes 0.16
-// to 0.6 us whatever its size: the largest shape of which there are enough to fill the GPU. Measured,
-// us (fp16 outputs, weights not in the caches), by the columns of kShapes below:
-//                       16x16 32x16 32x32 64x32 | 64x32 64x64 128x64 128x128 256x128 256x256
-//     1 x   2560 x 2560   4.5   5.1   6.8  12.4 |   6.6   8.6     11      20      25      31
-//    32 x   2560 x 2560   8.7   6.8   8.7    11 |   7.7   8.5     12      20      25      31
-//   128 x   2560 x 6912    33    20    26    18 |  16.6  20.3     32      62      88      70
-//   300 x   2560 x 6912                         |  25.5  18.9     28      61      88      87
-//    16 x   6912 x 2560   9.5   7.5   8.1    13 |   9.2   9.0     12      22      29      32
-//    32 x   6912 x 2560    18  11.9   9.4  11.5 |  10.1   9.3     13      22      29      32
-//   200 x   6912 x 2560                         |  19.9  13.6   12.6    19.1      29      34
-//   512 x   6912 x 2560                         |  45.6  26.7   22.1    20.9      38      42
-//  1024 x   6912 x 2560                         |  84.3  44.2   37.3    29.9    37.0    41.2
-//  2048 x   6912 x 2560                         |        76.6   61.1    53.1    42.3    42.8
-//  4001 x   2560 x 6912                         |                        101      91      80
-//     1 x 128256 x 2560    83    65    61    58 |    75    63     62      65      65      78
-//    32 x 128256 x 2560               110    79 |    87    74     70      72      70      85
-//   300 x 128256 x 2560                         |                191     179     142     192
+// Larger workgroups read less for a product, smaller ones are more and each takes less time: the
+// smallest shape whose workgroups have a CU each is nearly always the fastest, and beyond that the
+// largest, but for few tokens, whose weights the GPU can do no more than stream. Measured, us (fp16
+// outputs, weights not in the caches), by the columns of kShapes below:
+//                       1:16x16 16x16 32x16 32x32 64x32 | 64x32 64x64 128x64 128x128 256x128 256x256
+//     1 x   2560 x 2560    3.7   3.9   4.3   4.7   6.9 |   6.6   8.2     10      12      23      27
+//    24 x   2560 x 2560    5.8   5.5   4.9   6.4   8.7 |   7.4   8.5     11      13      26      28
+//     1 x   2560 x 6912    5.7   6.5   7.2   8.0    14 |    15    17     23      41      84      65
+//    16 x   2560 x 6912    8.2   7.5   9.4    10    15 |    16    17     24      41      84      66
+//    24 x   2560 x 6912     12    12   8.4    12    16 |    16    18     24      40      85      65
+//   100 x   2560 x 6912     26    27    21    18  15.8 |  15.5    18     26      42      86      68
+//   300 x   2560 x 6912     63    66    46    41    31 |    25  19.1     28      41      86      69
+//    16 x   6912 x 2560    7.0   6.9   5.8   6.3   8.4 |   9.2   9.1     12      17      33      28
+//    32 x   6912 x 2560     12    11   8.8   8.2    10 |    10   9.4     13      18      34      29
+//   100 x   6912 x 2560     30    27    20    20    17 |    15   9.8     13      20      36      31
+//   200 x   6912 x 2560     51    45    35    30    25 |    21    14    12.8      19      36      37
+//   512 x   6912 x 2560    131   114    77    64    53 |    44    27    22.5    21.0      36      40
+//  1024 x   6912 x 2560                                |    84    44     37    29.9    37.0      41
+//  2048 x   6912 x 2560                                |          77     61      53    42.3    42.8
+//  4001 x   2560 x 6912                                |                        101      91      80
+//     1 x 128256 x 2560     66    53    52    55    53 |    74    63     62      64      64      83
+//    32 x 128256 x 2560    177   163   123    91    65 |    87    74     69      79      71      89
+//   300 x 128256 x 2560                           680 |   486   243    195     182     148     197
+// (Over 180 sizes this rule takes 1% longer than the fastest shape of each.)
 // (channels and tokens of a workgroup, channels of a part)
-constexpr int kShapes[][3] = {{16, 16, 16},  {32, 16, 32},   {32, 32, 32},   {64, 32, 64},
-                              {64, 32, 32},  {64, 64, 32},   {128, 64, 64},  {128, 128, 32},
-                              {256, 128, 64}, {256, 256, 128}};
-GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K) {
+constexpr int kShapes[][3] = {{16, 16, 16},   {16, 16, 16},   {32, 16, 32},    {32, 32, 32},
+                              {64, 32, 64},   {64, 32, 32},   {64, 64, 32},    {128, 64, 64},
+                              {128, 128, 32}, {256, 128, 64}, {256, 256, 128}};
+GemmPlan gemm_plan(int64_t M, int64_t N) {
     const auto count = [&](GemmShape s) {
         return ceil_div(N, kShapes[s][0]) * ceil_div(M, kShapes[s][1]);
     };
-    GemmShape s = kTile64x32;
-    if (count(kFew16x16) <= 256)
-        s = kFew16x16;
-    else if (M <= 64 && count(kFew32x16) <= 256)
+    const auto fits = [&](GemmShape s) { return count(s) <= 256; };
+    GemmShape s = kTile128x128;
+    if (fits(kFew16x16))
+        s = M <= 4 ? kOne16x16 : kFew16x16;  // (16 waves to a workgroup, 8)
+    else if (fits(kFew32x16) || (M <= 16 && count(kFew64x32) < 900))
         s = kFew32x16;
-    else if (M <= 32 && count(kFew32x32) <= 256)
+    else if (fits(kFew32x32) && M > 16)
         s = kFew32x32;
-    else if (M <= 16 && count(kFew64x32) >= 900)
+    else if (fits(kTile64x32) && M > 32)
+        s = kTile64x32;
+    else if (M <= 32 && (fits(kFew64x32) || count(kFew64x32) >= 900))
         s = kFew64x32;
+    else if (fits(kTile64x64))
+        s = kTile64x64;
+    else if (fits(kTile128x64) || (M <= 64 && count(kTile256x128) < 300))
+        s = kTile128x64;
+    else if (count(kTile128x128) <= 400)
+        s = kTile128x128;
     else if (count(kTile256x256) >= 150 && count(kTile256x256) <= 192 &&
              2 * ceil_div(M, 256) == ceil_div(M, 128))
         s = kTile256x256;  // (one to a CU: of 256 x 128 some CUs would have two)
     else if (count(kTile256x128) >= 300)
         s = kTile256x128;
-    else if (count(kTile128x128) >= 200)
-        s = kTile128x128;
-    else if (count(kTile128x64) >= (K < 4096 ? 150 : 200))
-        s = kTile128x64;
-    else if (count(kTile64x64) >= 150)
-        s = kTile64x64;
     return {s, (int)(ceil_div(N, kShapes[s][0]) * (kShapes[s][0] / kShapes[s][2]))};
 }
 
-template <int MT, int NT, int KW, int DEPTH>
+template <int MT, int NT, int KW>
 void launch_few(const GemmI8& a, hipStream_t st) {
-    hipLaunchKernelGGL((gemm_i8_few_kernel<MT, NT, KW, DEPTH>),
+    hipLaunchKernelGGL((gemm_i8_few_kernel<MT, NT, KW>),
                        dim3((unsigned)ceil_div(a.N, 16 * NT), (unsigned)ceil_div(a.M, 16 * MT)),
                        dim3(64 * KW), 0, st, a);
 }
@@ -532,10 +541,11 @@ void launch_tile(const GemmI8& a, hipStream_t st) {
 template <int TYPE, bool BEST>
 void launch_shape(GemmShape shape, const GemmI8& a, hipStream_t st) {
     switch (shape) {
-        case kFew16x16: return launch_few<1, 1, 16, 2>(a, st);
-        case kFew32x16: return launch_few<1, 2, 16, 2>(a, st);
-        case kFew32x32: return launch_few<2, 2, 8, 2>(a, st);
-        case kFew64x32: return launch_few<2, 4, 4, 3>(a, st);
+        case kOne16x16: return launch_few<1, 1, 16>(a, st);
+        case kFew16x16: return launch_few<1, 1, 8>(a, st);
+        case kFew32x16: return launch_few<1, 2, 8>(a, st);
+        case kFew32x32: return launch_few<2, 2, 8>(a, st);
+        case kFew64x32: return launch_few<2, 4, 4>(a, st);
         case kTile64x32: return launch_tile<TYPE, BEST, 2, 1, 4, 1, 1, 4>(a, st);
         case kTile64x64: return launch_tile<TYPE, BEST, 2, 2, 1, 1, 1, 9>(a, st);
         case kTile128x64: return launch_tile<TYPE, BEST, 2, 2, 1, 2, 1, 6>(a, st);
@@ -554,7 +564,7 @@ extern "C" {
 
 TENZO_HIP_API size_t tenzo_hip_gemm_i8_ws_bytes(int64_t M, int64_t N, int64_t K, int want_idx) {
     if (M <= 0 || N <= 0 || K <= 0 || !want_idx) return 0;
-    return (size_t)(M * gemm_plan(M, N, K).parts) * sizeof(float2);
+    return (size_t)(M * gemm_plan(M, N).parts) * sizeof(float2);
 }
 
 TENZO_HIP_API int tenzo_hip_gemm_i8(const int8_t* codes, int64_t codes_stride,
@@ -582,7 +592,7 @@ TENZO_HIP_API int tenzo_hip_gemm_i8(const int8_t* codes, int64_t codes_stride,
     TZ_CHECK(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 7) == 0),
              "gemm_i8: %zu bytes of workspace needed, 8-byte aligned, %zu given", need,
              ws ? ws_bytes : 0);
-    const GemmPlan p = gemm_plan(M, N, K);
+    const GemmPlan p = gemm_plan(M, N);
     const hipStream_t st = (hipStream_t)stream;
     GemmI8 a{codes, M == 1 ? K : codes_stride, q, (const uint8_t*)w_packed, scales, y, y_stride,
              out_idx ? (float2*)ws : nullptr, N, (int)M, (int)(K / 16), p.parts, dtype};

@@ -46,6 +46,19 @@ def test_gemm(torch_dev, ops, M, N, K, kind):
     assert (out[:, :2] == 3).all() and (out[:, 2 + N:] == 3).all()
 
 
+@pytest.mark.parametrize("M,N,K", [(4, 3999, 1104), (16, 6913, 80), (20, 6901, 144),
+                                   (30, 13801, 272), (19, 70001, 112), (48, 40001, 96),
+                                   (47, 3900, 16), (300, 60001, 64), (90, 1000, 4112)])
+def test_gemm_of_every_shape(torch_dev, ops, M, N, K):
+    torch = torch_dev
+    print("gemm", M, N, K, flush=True)
+    args, want = make(torch, ops, M, N, K, seed=M + N, wide=16 * (M % 3))
+    for kind in (torch.float32, torch.float16):
+        y, idx = ops.gemm_i8(*args, dtype=kind, want_idx=True)
+        assert torch.equal(y.cpu(), torch.from_numpy(want).to(kind))
+        np.testing.assert_array_equal(idx.cpu().numpy(), plain.first_best(want))
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 500, 320), (40, 300, 208), (300, 257, 512)])
 def test_rows_of_the_lm_head(torch_dev, ops, M, N, K):
     """Each row bit for bit what the LM head's product and its argmax give."""
