@@ -70,13 +70,28 @@ __device__ __forceinline__ void take_best(float& v, int& n, float ov, int on) {
     }
 }
 
-// A token of 16 from either half of a wave's rows of 16 lanes: lanes with bit 4 keep the upper 8.
-__device__ __forceinline__ void best_swap16(float (&v)[16], int (&n)[16]) {
+// A token of 2 D from either half of a wave's rows of 16 lanes: lanes with bit 4 keep the upper D.
+template <int D, int N>
+__device__ __forceinline__ void best_swap16(float (&v)[N], int (&n)[N]) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < D; ++k) {
         const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[k]),
-                                                        __float_as_uint(v[k + 8]), false, false);
-        const auto b = __builtin_amdgcn_permlane16_swap((uint32_t)n[k], (uint32_t)n[k + 8], false,
+                                                        __float_as_uint(v[k + D]), false, false);
+        const auto b = __builtin_amdgcn_permlane16_swap((uint32_t)n[k], (uint32_t)n[k + D], false,
+                                                        false);
+        v[k] = __uint_as_float(a[0]);
+        n[k] = (int)b[0];
+        take_best(v[k], n[k], __uint_as_float(a[1]), (int)b[1]);
+    }
+}
+// From either half of the wave: the upper 32 lanes keep the upper D.
+template <int D, int N>
+__device__ __forceinline__ void best_swap32(float (&v)[N], int (&n)[N]) {
+#pragma unroll
+    for (int k = 0; k < D; ++k) {
+        const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[k]),
+                                                        __float_as_uint(v[k + D]), false, false);
+        const auto b = __builtin_amdgcn_permlane32_swap((uint32_t)n[k], (uint32_t)n[k + D], false,
                                                         false);
         v[k] = __uint_as_float(a[0]);
         n[k] = (int)b[0];
@@ -84,8 +99,8 @@ __device__ __forceinline__ void best_swap16(float (&v)[16], int (&n)[16]) {
     }
 }
 // And of 2 D tokens: lanes that are `up` keep the upper D, their partners by CTRL the others.
-template <int D, int CTRL>
-__device__ __forceinline__ void best_halve(float (&v)[16], int (&n)[16], bool up) {
+template <int D, int CTRL, int N>
+__device__ __forceinline__ void best_halve(float (&v)[N], int (&n)[N], bool up) {
 #pragma unroll
     for (int k = 0; k < D; ++k) {
         const float give = up ? v[k] : v[k + D];
@@ -158,30 +173,55 @@ __global__ void __launch_bounds__(64 * KW) gemm_i8_few_kernel(GemmI8 a) {
         for (int s = 0; s < MT; ++s) red[wave][t * MT + s][lane] = acc[t][s];
     __syncthreads();
     // thread: a row of the tile and a column, the columns side by side
-    for (int it = threadIdx.x; it < 16 * MT * 16 * NT; it += 64 * KW) {
+    constexpr int kOutputs = 16 * MT * 16 * NT, PER = (kOutputs + 64 * KW - 1) / (64 * KW);
+    float best[PER];
+    int at[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int it = threadIdx.x + 64 * KW * k;
+        if (it >= kOutputs) return;
         const int nn = it % (16 * NT), mm = it / (16 * NT), m = m0 + mm;
         const int64_t n = n0 + nn;
         const int tile = nn / 16 * MT + mm / 16, from = nn % 16 + 16 * (mm % 16 / 4);
         int sum = 0;
 #pragma unroll
         for (int w = 0; w < KW; ++w) sum += red[w][tile][from][mm % 4];
-        float v = -INFINITY;
+        best[k] = -INFINITY;
+        at[k] = (int)n;
         if (m < a.M && n < a.N) {
             const float y = (float)sum * __fmul_rn(a.q[m].inv_scale, a.scales[n]);
             store_y(a, m * a.ldy + n, y);
-            if (y > v) v = y;
+            if (y > best[k]) best[k] = y;
         }
-        if (a.best) {
-            int at = (int)n;
-            take_best(v, at, dpp_f<kDppXor1>(v), dpp_i<kDppXor1>(at));
-            take_best(v, at, dpp_f<kDppXor2>(v), dpp_i<kDppXor2>(at));
-            take_best(v, at, dpp_f<kDppHalfMirror>(v), dpp_i<kDppHalfMirror>(at));
-            take_best(v, at, dpp_f<kDppMirror>(v), dpp_i<kDppMirror>(at));
+    }
+    if (!a.best) return;
+    if constexpr (PER == 8 && NT == 4) {
+        // 8 tokens' best of 64 lanes: half of them go to the other half of the lanes each time (lane
+        // bits 5, 4, 3 become bits 2, 1, 0 of the token's number), then each has 8 lanes
+        best_swap32<4>(best, at);
+        best_swap16<2>(best, at);
+        best_halve<1, kDppMirror>(best, at, lane & 8);
+        take_best(best[0], at[0], dpp_f<kDppHalfMirror>(best[0]), dpp_i<kDppHalfMirror>(at[0]));
+        take_best(best[0], at[0], dpp_f<kDppXor2>(best[0]), dpp_i<kDppXor2>(at[0]));
+        take_best(best[0], at[0], dpp_f<kDppXor1>(best[0]), dpp_i<kDppXor1>(at[0]));
+        const int k = (lane >> 5) * 4 + (lane >> 4 & 1) * 2 + (lane >> 3 & 1), m = m0 + wave + KW * k;
+        if ((lane & 7) == 0 && m < a.M)
+            a.best[(int64_t)m * a.parts + blockIdx.x] = make_float2(best[0], __int_as_float(at[0]));
+    } else {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            float v = best[k];
+            int n = at[k];
+            take_best(v, n, dpp_f<kDppXor1>(v), dpp_i<kDppXor1>(n));
+            take_best(v, n, dpp_f<kDppXor2>(v), dpp_i<kDppXor2>(n));
+            take_best(v, n, dpp_f<kDppHalfMirror>(v), dpp_i<kDppHalfMirror>(n));
+            take_best(v, n, dpp_f<kDppMirror>(v), dpp_i<kDppMirror>(n));
 #pragma unroll
             for (int d = 16; d < 16 * NT; d <<= 1)
-                take_best(v, at, __shfl_xor(v, d), __shfl_xor(at, d));
-            if (nn == 0 && m < a.M)
-                a.best[(int64_t)m * a.parts + blockIdx.x] = make_float2(v, __int_as_float(at));
+                take_best(v, n, __shfl_xor(v, d), __shfl_xor(n, d));
+            const int it = threadIdx.x + 64 * KW * k, m = m0 + it / (16 * NT);
+            if (it % (16 * NT) == 0 && m < a.M)
+                a.best[(int64_t)m * a.parts + blockIdx.x] = make_float2(v, __int_as_float(n));
         }
     }
 }
@@ -415,7 +455,7 @@ gemm_i8_tile_kernel(GemmI8 a) {
         if (BEST) {
             // 16 tokens' best of 32 lanes: half of the tokens go to the other half of the lanes
             // each time (lane bits 4 .. 1 become token bits 3 .. 0), the last time a token has two
-            best_swap16(bv, bi);
+            best_swap16<8>(bv, bi);
             best_halve<4, kDppMirror>(bv, bi, i & 8);
             best_halve<2, kDppHalfMirror>(bv, bi, i & 4);
             best_halve<1, kDppXor2>(bv, bi, i & 2);
