@@ -116,8 +116,8 @@ __device__ __forceinline__ void best_halve(float (&v)[N], int (&n)[N], bool up) 
 // (loads three to seven steps ahead, or 16 waves where there are tokens, take longer; a line of codes,
 // 128 bytes of a row, belongs to one wave's turn). The codes of the 16 MT tokens come the same way,
 // out of the L2. At the end the waves' sums meet in LDS. 1 x 2560 x 6912: 5.7 us, 24 x 2560 x 6912:
-// 8.4, where the weights take 3.5: a launch, three or four dependent rounds of loads, and the meeting;
-// 1 x 128256 x 2560: 52 us, 6.3 TB/s (a part of it out of the last cache).
+// 8.4, where the weights take 3.5: a launch, 7 dependent rounds of loads, and the meeting;
+// 26 x 128256 x 2560: 64 to 67 us, 5.1 TB/s, bound by the weights.
 constexpr uint32_t kNone = 0x80000000u;  // an offset past every resource
 constexpr int kNt = 2;                   // a load that leaves nothing in the caches
 template <int MT, int NT, int KW>
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(64 * KW) gemm_i8_few_kernel(GemmI8 a) {
 // so that a register of the result holds 32 neighbouring channels of a token in 32 lanes.
 // Each half of a step's fragments (32 k) is read while the half before it is multiplied.
 // 4001 x 6912 x 2560, fp16: 78 us, 1.8 POP/s, bound by the matrix units and the clock that their
-// power leaves (zeros run faster); 26 x 128256 x 2560, fp32: 66 us, 5.1 TB/s, bound by the weights.
+// power leaves (zeros run faster); 300 x 128256 x 2560, fp16: 148 us.
 template <int TYPE, bool BEST, int WR, int WT, int KW, int RT, int CT, int S>
 __global__ void __launch_bounds__(64 * WR * WT * KW, RT * CT > 4 || KW > 1 ? 2 : WR * WT / 2)
 gemm_i8_tile_kernel(GemmI8 a) {
