@@ -23,6 +23,7 @@ struct GemmI8 {
     int M, KB;  // KB: K / 16
     int parts;
     int dtype;
+    int full;  // (tiles: the first that comes as halves)
 };
 
 __device__ __forceinline__ void store_y(const GemmI8& a, int64_t at, float v) {
@@ -237,32 +238,31 @@ __global__ void __launch_bounds__(64 * KW) gemm_i8_few_kernel(GemmI8 a) {
 // Each half of a step's fragments (32 k) is read while the half before it is multiplied.
 // 4001 x 6912 x 2560, fp16: 78 us, 1.8 POP/s, bound by the matrix units and the clock that their
 // power leaves (zeros run faster); 300 x 128256 x 2560, fp16: 148 us.
-template <int TYPE, bool BEST, int WR, int WT, int KW, int RT, int CT, int S>
-__global__ void __launch_bounds__(64 * WR * WT * KW, RT * CT > 4 || KW > 1 ? 2 : WR * WT / 2)
-gemm_i8_tile_kernel(GemmI8 a) {
-    constexpr int W = WR * WT * KW, BN = 32 * RT * WR, BM = 32 * CT * WT;
+template <int WR, int WT, int KW, int RT, int CT, int S>
+struct GemmTile {
+    static constexpr int W = WR * WT * KW, BN = 32 * RT * WR, BM = 32 * CT * WT;
     static_assert(BN % 64 == 0, "whole blocks of rows");
-    constexpr int kWLoads = BN / 16, kGroup = kWLoads + BM / 16;  // loads of 1 KiB per group
-    constexpr int kSlot = KW * kGroup * 1024, X = KW * kGroup / W;
+    static constexpr int kWLoads = BN / 16, kGroup = kWLoads + BM / 16;  // loads of 1 KiB per group
+    static constexpr int kSlot = KW * kGroup * 1024, X = KW * kGroup / W;
     static_assert(X * W == KW * kGroup, "as many loads a step for each wave");
     static_assert(S >= 3 && (S - 1) * X <= 63, "vmcnt counts at most 63 loads");
-    constexpr int kRed = (KW - 1) * WR * WT * RT * CT * 4096, kRing = S * kSlot;
+    static constexpr int kRed = (KW - 1) * WR * WT * RT * CT * 4096, kRing = S * kSlot;
     static_assert(kRed + WR * WT * RT * 4096 <= kRing, "sums and outputs go out by way of the ring");
-    __shared__ __attribute__((aligned(16))) char ring[kRing];
-    __shared__ float inv[BM];
 
+    // The tile of channels from n0 (its number among those: bn) and tokens from m0.
+    template <int TYPE, bool BEST>
+    static __device__ __forceinline__ void run(const GemmI8& a, int64_t n0, int bn, int m0,
+                                               char* ring, float* inv);
+};
+
+template <int WR, int WT, int KW, int RT, int CT, int S>
+template <int TYPE, bool BEST>
+__device__ __forceinline__ void GemmTile<WR, WT, KW, RT, CT, S>::run(const GemmI8& a, int64_t n0,
+                                                                     int bn, int m0, char* ring,
+                                                                     float* inv) {
     const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave % WR, wt = wave / WR % WT, kg = wave / (WR * WT);
-    // Consecutive tiles to one XCD, as bands of 4 tiles of weight rows, so that what its
-    // workgroups read at a time is few tiles of either operand.
-    const int G = gridDim.x, id = blockIdx.x;
-    const int tid = (G & 7) == 0 ? (id & 7) * (G >> 3) + (id >> 3) : id;
-    const int nt = (int)((a.N + BN - 1) / BN), mt = (a.M + BM - 1) / BM;
-    if (tid >= nt * mt) return;
-    const int band = tid / (4 * mt), wide = min(4, nt - 4 * band), in_band = tid - band * 4 * mt;
-    const int bn = 4 * band + in_band % wide, m0 = in_band / wide * BM;
-    const int64_t n0 = (int64_t)bn * BN;
     const int rows = min(BM, a.M - m0), blocks = min(BN / 64, (int)((a.N + 63) / 64 - n0 / 64));
     const int K = a.KB * 16, steps = (a.KB + 4 * KW - 1) / (4 * KW);
     for (int m = threadIdx.x; m < BM; m += 64 * W) inv[m] = a.q[m0 + min(m, rows - 1)].inv_scale;
@@ -468,6 +468,36 @@ gemm_i8_tile_kernel(GemmI8 a) {
     }
 }
 
+// HALVES: tiles from a.full on come as two halves of their channels, where up to 128 tiles are left
+// over from a multiple of 256: a CU with one tile more than the others makes all wait for it, a half
+// takes less. us, whole | halves: 1024 x 20480 x 2560 (640 tiles) 70 | 62, 2500 x 6912 x 2560 (540) 68 |
+// 60, 8000 x 2560 x 2560 (630) 69 | 65; no change where the multiple is odd (864 tiles: 81), since
+// two tiles of a CU take little longer than one.
+template <int TYPE, bool BEST, int WR, int WT, int KW, int RT, int CT, int S, bool HALVES>
+__global__ void __launch_bounds__(64 * WR * WT * KW, RT * CT > 4 || KW > 1 ? 2 : WR * WT / 2)
+gemm_i8_tile_kernel(GemmI8 a) {
+    typedef GemmTile<WR, WT, KW, RT, CT, S> Tile;
+    typedef GemmTile<WR, WT, KW, HALVES ? RT / 2 : RT, CT, HALVES ? S + 1 : S> Half;
+    __shared__ __attribute__((aligned(16))) char ring[Tile::kRing > Half::kRing ? Tile::kRing
+                                                                                : Half::kRing];
+    __shared__ float inv[Tile::BM];
+    const int nt = (int)((a.N + Tile::BN - 1) / Tile::BN), mt = (a.M + Tile::BM - 1) / Tile::BM;
+    // Consecutive tiles to one XCD, as bands of 4 tiles of weight rows, so that what its
+    // workgroups read at a time is few tiles of either operand.
+    const int G = HALVES ? a.full : gridDim.x, id = blockIdx.x, past = id - G;
+    const int tid = past >= 0 ? G + (past >> 1) : (id & 7) * (G >> 3) + (id >> 3);
+    if (tid >= nt * mt) return;
+    const int band = tid / (4 * mt), wide = min(4, nt - 4 * band), in_band = tid - band * 4 * mt;
+    const int bn = 4 * band + in_band % wide, m0 = in_band / wide * Tile::BM;
+    const int64_t n0 = (int64_t)bn * Tile::BN;
+    if (HALVES && past >= 0) {
+        const int64_t h0 = n0 + (past & 1) * Half::BN;
+        if (h0 < a.N) Half::template run<TYPE, BEST>(a, h0, 2 * bn + (past & 1), m0, ring, inv);
+    } else {
+        Tile::template run<TYPE, BEST>(a, n0, bn, m0, ring, inv);
+    }
+}
+
 // Joins the parts of a row's largest value, W waves to a row.
 template <int W>
 __global__ void __launch_bounds__(W > 1 ? 64 * W : 256)
@@ -571,12 +601,18 @@ void launch_few(const GemmI8& a, hipStream_t st) {
                        dim3((unsigned)ceil_div(a.N, 16 * NT), (unsigned)ceil_div(a.M, 16 * MT)),
                        dim3(64 * KW), 0, st, a);
 }
-template <int TYPE, bool BEST, int WR, int WT, int KW, int RT, int CT, int S>
-void launch_tile(const GemmI8& a, hipStream_t st) {
+template <int TYPE, bool BEST, int WR, int WT, int KW, int RT, int CT, int S, bool HALVES = false>
+void launch_tile(GemmI8 a, hipStream_t st) {
     // (a number of workgroups that is shared out among the XCDs evenly: the last have no tile)
-    const int64_t nt = ceil_div(a.N, 32 * RT * WR), mt = ceil_div(a.M, 32 * CT * WT);
-    hipLaunchKernelGGL((gemm_i8_tile_kernel<TYPE, BEST, WR, WT, KW, RT, CT, S>),
-                       dim3((unsigned)(ceil_div(nt * mt, 8) * 8)), dim3(64 * WR * WT * KW), 0, st, a);
+    const int64_t tiles = ceil_div(a.N, 32 * RT * WR) * ceil_div(a.M, 32 * CT * WT);
+    int64_t wgs = ceil_div(tiles, 8) * 8;
+    a.full = (int)wgs;
+    if (HALVES && tiles > 256 && tiles % 256 > 0 && tiles % 256 <= 128) {
+        a.full = (int)(tiles / 256 * 256);
+        wgs = a.full + 2 * (tiles % 256);
+    }
+    hipLaunchKernelGGL((gemm_i8_tile_kernel<TYPE, BEST, WR, WT, KW, RT, CT, S, HALVES>),
+                       dim3((unsigned)wgs), dim3(64 * WR * WT * KW), 0, st, a);
 }
 template <int TYPE, bool BEST>
 void launch_shape(GemmShape shape, const GemmI8& a, hipStream_t st) {
@@ -590,7 +626,7 @@ void launch_shape(GemmShape shape, const GemmI8& a, hipStream_t st) {
         case kTile64x64: return launch_tile<TYPE, BEST, 2, 2, 1, 1, 1, 9>(a, st);
         case kTile128x64: return launch_tile<TYPE, BEST, 2, 2, 1, 2, 1, 6>(a, st);
         case kTile128x128: return launch_tile<TYPE, BEST, 4, 2, 1, 1, 2, 4>(a, st);
-        case kTile256x128: return launch_tile<TYPE, BEST, 4, 2, 1, 2, 2, 3>(a, st);
+        case kTile256x128: return launch_tile<TYPE, BEST, 4, 2, 1, 2, 2, 3, !BEST>(a, st);
         case kTile256x256: return launch_tile<TYPE, BEST, 2, 4, 1, 4, 2, 4>(a, st);
     }
 }
@@ -635,7 +671,7 @@ TENZO_HIP_API int tenzo_hip_gemm_i8(const int8_t* codes, int64_t codes_stride,
     const GemmPlan p = gemm_plan(M, N);
     const hipStream_t st = (hipStream_t)stream;
     GemmI8 a{codes, M == 1 ? K : codes_stride, q, (const uint8_t*)w_packed, scales, y, y_stride,
-             out_idx ? (float2*)ws : nullptr, N, (int)M, (int)(K / 16), p.parts, dtype};
+             out_idx ? (float2*)ws : nullptr, N, (int)M, (int)(K / 16), p.parts, dtype, 0};
     if (dtype == 0)
         out_idx ? launch_shape<0, true>(p.shape, a, st) : launch_shape<0, false>(p.shape, a, st);
     else if (dtype == 1)

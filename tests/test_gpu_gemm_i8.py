@@ -59,6 +59,21 @@ def test_gemm_of_every_shape(torch_dev, ops, M, N, K):
         np.testing.assert_array_equal(idx.cpu().numpy(), plain.first_best(want))
 
 
+@pytest.mark.parametrize("M,N,K", [(1100, 14701, 48), (1100, 14800, 176), (2000, 9985, 32)])
+def test_tiles_in_halves(torch_dev, ops, M, N, K):
+    """Tiles of 256 x 128 past a multiple of 256, which come as halves (the last half of the first
+    case has no channel), against the call with the largest values, whose tiles stay whole."""
+    torch = torch_dev
+    tiles = -(-N // 256) * -(-M // 128)
+    assert tiles > 512 and 0 < tiles % 256 <= 128
+    args, want = make(torch, ops, M, N, K, seed=N)
+    for kind in (torch.float32, torch.bfloat16):
+        y = torch.full((M + 1, N), 3.0, dtype=kind, device="cuda")
+        ops.gemm_i8(*args, out=y[:M])
+        assert torch.equal(y[:M].cpu(), torch.from_numpy(want).to(kind)) and (y[M] == 3).all()
+        assert torch.equal(y[:M], ops.gemm_i8(*args, dtype=kind, want_idx=True)[0])
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 500, 320), (40, 300, 208), (300, 257, 512)])
 def test_rows_of_the_lm_head(torch_dev, ops, M, N, K):
     """Each row bit for bit what the LM head's product and its argmax give."""
