@@ -297,8 +297,8 @@ TENZO_HIP_API int tenzo_hip_tree_plan(const int32_t* parents, const int32_t* ctx
  * tree and the nodes j whose bit is set in its row of mask (mask_words words, up
  * to 1024, mask_stride words apart, 8-byte aligned; any bits, its own too; nodes
  * behind the last word are not seen). Accuracy as there but in calls that give 128
- * rows to a workgroup (over 40 rows times heads a kv head and sequence, a table of
- * over 1024 tokens, and enough of them): a query's element is held to 2^-24 of the
+ * rows to a workgroup (over 40 rows times heads a kv head and sequence, and
+ * enough of them or a wide table): a query's element is held to 2^-24 of the
  * largest of its group of 32 dims, in fp16 calls to 2^-19; weights to 2^-22, in
  * fp16 calls rounded once to fp16 (2^-11, as outputs are; below 2^-33 of a row's
  * largest they are lost). */

@@ -1154,6 +1154,25 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
 
 #include "attention_kv4_tree.h"
 
+// Many trees: a workgroup to a (row tile, kv head) with all of its tokens. 32 trees of up to 64 nodes
+// after up to 500 tokens, 32 / 8 heads, fp16: 30 us.
+template <bool HALF>
+__global__ void __launch_bounds__(256, 2) kv4_attn_tree_kernel(Kv4Attn a, Kv4Seqs sq) {
+    __shared__ Kv4TreeSmem sm;
+    const int unit = blockIdx.x / sq.Hkv;
+    Segment g;
+    g.h = blockIdx.x - unit * sq.Hkv;
+    if (!find_unit(sq, unit, a.G, kRowsRT, g.seq, g.tile)) return;
+    g.n = sq.rows(g.seq, g.first);
+    g.c = sq.length(g.seq);
+    g.t0 = 0;
+    g.len = g.c;
+    g.whole = true;
+    g.rec = 0;
+    g.split = 0;
+    kv4_tree_segment<HALF>(a, sq, g, sm);
+}
+
 // Several sequences of a few rows: all their steps in a row (sequence by sequence, unit by unit)
 // and an equal share of them to each of as many workgroups as the GPU holds at once, so that
 // lengths, which only the device knows, need not be alike. A share holds the end of a unit that
@@ -1374,6 +1393,22 @@ Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, int
     const int64_t per = cu ? ceil_div(T * G, B) : G;  // rows of an average sequence
     p.rows = per <= 4 ? 4 : 16;
     const int64_t ctx = (int64_t)table_width * kKv4Page;
+    // Many trees after short contexts: 128 rows a workgroup and a workgroup for all of their tokens,
+    // with no records. us, the plan below | this, 32 / 8 heads: fp16, 16 x up to 64 nodes after 200
+    // (207 times 128 rows) 27 | 17, 8 x 64 after 500 (102) 22 | 23, 32 x 64 after 500 (370) 58 | 30,
+    // after 1000 82 | 44, after 2000 75 | 71; fp32 16 x 64 after 200 28 | 27, 32 x 64 after 500 60 |
+    // 49, after 1000 84 | 68, after 2000 99 | 101, 64 x 64 after 2000 (780) 187 | 177, after 4000
+    // 243 | 287.
+    const double tiles = (double)T * G * Hkv / kRowsRT;
+    if (kind != kNoTree && per > 44 &&
+        ((ctx <= 1024 && tiles > (kind == kTreeHalf ? 110 : 360)) ||
+         (ctx <= 2048 && tiles > (kind == kTreeHalf ? 360 : 600)))) {
+        p.rows = kRowsRT;
+        p.rw = 1;
+        p.splits = 1;
+        p.wgs = (T * G / kRowsRT + B) * Hkv;
+        return p;
+    }
     // Trees, by rows x heads x tokens: 128 rows a workgroup and the steps dealt evenly cost 20 us
     // before their first step (queries split into parts, the records of 512 shares), then half to
     // two thirds of the time of 16 rows a workgroup. us, 16 rows | 128, B x up to n nodes after up to
@@ -1406,9 +1441,8 @@ Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, int
     // 5 heads, 16 rows | 32 | 128: a prompt of 100 tokens 7.5 | 8.9 | 21, one of 1000 38 | 34 | 44,
     // 32 of up to 128 44 | 32 | 21; 128 tokens after 4000 33 | 37 | 38, 200 after 7800 63 | 66 |
     // 56, 512 after 8000 160 | 200 | 102.
-    const double units128 = (double)T * G * Hkv / kRowsRT;
     p.rw = 1;
-    if (kind == kNoTree && per > 64 && (units128 > 320 || units128 * ctx > 3500 * kTile))
+    if (kind == kNoTree && per > 64 && (tiles > 320 || tiles * ctx > 3500 * kTile))
         p.rw = 8;
     else if (per > 16 && T * G / 16 * Hkv > 512 && ctx <= 1024)
         p.rw = 2;
@@ -1470,7 +1504,11 @@ int launch_kv4_even(const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
 template <bool HALF, bool TREE>
 int launch_kv4_plan(const Kv4Plan& p, const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
     if constexpr (TREE)
-        if (p.rows == kRowsRT) return launch_kv4_even<kRowsRT, HALF, true>(a, s, st);
+        if (p.rows == kRowsRT) {
+            if (p.even) return launch_kv4_even<kRowsRT, HALF, true>(a, s, st);
+            hipLaunchKernelGGL(kv4_attn_tree_kernel<HALF>, dim3(a.wgs), dim3(256), 0, st, a, s);
+            return launch_status("kv4_attn_tree_kernel");
+        }
     if (p.even)
         return p.rows == 4 ? launch_kv4_even<4, HALF, TREE>(a, s, st)
                            : launch_kv4_even<16, HALF, TREE>(a, s, st);

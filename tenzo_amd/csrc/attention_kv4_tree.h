@@ -158,7 +158,7 @@ __device__ __forceinline__ void kv4_tree_segment(const Kv4Attn& a, const Kv4Seqs
     bool gone = stage_pages(0);
     // Loads of the step at t: a wave has its page's codes and scales. Steps past the end load the last
     // page again, in place of a page that the pool does not hold another one is read, and masked.
-    const bool any = sq.n_blocks > 0;
+    const bool any = sq.n_blocks > 0 && t1 > t0;
     const uint32_t ring0 = lds_addr(&sm.ring[0]);
     int w0 = t0;  // the first token of the page numbers in LDS
     auto load = [&](int page, int slot) {

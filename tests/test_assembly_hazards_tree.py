@@ -79,7 +79,7 @@ def test_assembly_of_the_kernels(tmp_path):
                    capture_output=True)
     with open(out) as f:
         found = kernels(f.read())
-    assert len(found) == 2  # fp32 and fp16
+    assert len(found) == 4  # fp32 and fp16, steps dealt evenly and a workgroup for all
     for name, lines in found.items():
         assert not wrong(lines), (name, wrong(lines)[:3])
         assert sum(bool(CONVERT.match(c)) for c, _ in lines) >= 8, name

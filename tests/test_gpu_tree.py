@@ -98,7 +98,7 @@ class Trees(Setup):
         want = np.zeros((self.T, self.Hq, D)) if start is None else start.astype(np.float64)
         # queries and weights are held to 22 bits or more in fp32 calls (2^-21 for the two), in
         # fp16 calls of 128 rows weights to 11 (half a step: 2^-11), elsewhere every bit
-        half = self.dtype == np.float16 and self.kernel() == "128 even"
+        half = self.dtype == np.float16 and self.kernel().startswith("128")
         want, tol = plain.attention(self.q, self.mask, self.pools, self.tables, self.ctx,
                                     self.layer, self.cu, want, 2.0 ** -21,
                                     2.0 ** -11 if half else 2.0 ** -21)
@@ -268,6 +268,23 @@ def test_attention_joins(torch_dev, ops, seqs, Hkv, shares, dtype):
     assert s.kernel() == "128 even" and s.T * Hq > 1024
     assert 512 // ((s.T * Hq // Hkv // 128 + len(seqs)) * Hkv) == shares
     s.check(s.run(ops))
+
+
+@pytest.mark.parametrize("dtype,count,way", [(np.float16, 60, "tree"), (np.float16, 60, "bits"),
+                                             (np.float32, 190, "bits"), (np.float32, 190, "odd")])
+def test_attention_of_many_trees(torch_dev, ops, dtype, count, way):
+    """128 rows a workgroup, a workgroup for all tokens: padding slots, trees without nodes, nodes in
+    front of the cache, absent pages, rows behind the last sequence."""
+    rng = np.random.default_rng(count)
+    seqs = [(int(rng.integers(30, 65)), int(rng.integers(64, 330))) for _ in range(count)]
+    seqs[:8] = [(50, 0), (0, 7), (70, 60), (1, 1), (64, 64), (33, -3), (65, 320), (2, 17)]
+    s = Trees(seqs, 8, 2 if count < 100 else 1, way, dtype=dtype, tail=3, layers=1)
+    s.tables[4, 1], s.tables[9, 0], s.tables[10] = -1, s.nb, -7
+    s.dev(torch_dev)
+    print("many trees", dtype.__name__, count, way, s.kernel(), flush=True)
+    assert s.kernel() == "128"
+    out = torch_dev.full((s.T, 8, D), 7.0, dtype=s.d["q"].dtype, device="cuda")
+    s.check(s.run(ops, out), np.full((s.T, 8, D), 7.0))
 
 
 @BOTH

@@ -9,6 +9,10 @@ def plan(T, B, Hq, Hkv, width, cu, half):
     """(kernel, splits, bytes of workspace), as kv4_plan.plan has them."""
     G, ctx = Hq // Hkv, width * PAGE
     per = _up(T * G, B) if cu else G
+    tiles = T * Hq / 128
+    if per > 44 and (ctx <= 1024 and tiles > (110 if half else 360) or
+                     ctx <= 2048 and tiles > (360 if half else 600)):
+        return "128", 1, 0
     if per > (40 if half else 56) and ctx > 1024 and T * Hq * ctx > (14e6 if half else 22e6):
         most = (T * G // 128 + B) * Hkv * (_up(ctx, TILE) + 4)
         return "128 even", 1, min(_up(most, 4), 512) * 2 * 128 * RECORD
