@@ -287,6 +287,22 @@ def test_attention_of_many_trees(torch_dev, ops, dtype, count, way):
     s.check(s.run(ops, out), np.full((s.T, 8, D), 7.0))
 
 
+@pytest.mark.parametrize("seqs,Hq,kernel,width", [
+    ([(1 + i % 2, 200 + 40 * i) for i in range(70)], 2, "4 even", None),
+    ([(6, 300 + 30 * i) for i in range(65)], 8, "16 even", None),
+    ([(6, 300 + 30 * i) for i in range(64)], 8, "16 even", None),
+    ([(16 + i % 5, 30 + 7 * i) for i in range(70)], 8, "128 even", WIDE)])
+def test_attention_of_over_64_trees(torch_dev, ops, seqs, Hq, kernel, width):
+    """Steps dealt evenly over more sequences than a wave has lanes, some of them padding."""
+    seqs = list(seqs)
+    seqs[3], seqs[20], seqs[-1] = (5, 0), (0, 9), (9, 4)
+    s = Trees(seqs, Hq, 2, "tree", width=width, tail=2, layers=1).dev(torch_dev)
+    print("trees", len(seqs), s.kernel(), flush=True)
+    assert s.kernel() == kernel
+    out = torch_dev.full((s.T, Hq, D), 7.0, dtype=s.d["q"].dtype, device="cuda")
+    s.check(s.run(ops, out), np.full((s.T, Hq, D), 7.0))
+
+
 @BOTH
 def test_attention_queries_that_are_not_finite(torch_dev, ops, width):
     """A row with an infinity or NaN in its query is NaN where it sees a token, and no other row is
