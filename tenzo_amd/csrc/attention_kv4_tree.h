@@ -24,8 +24,8 @@
 // in two parts, 22 bits (2^-40). Their sum comes from the products too, from the same rounded
 // weights against ones.
 //
-// 16 trees of up to 64 nodes after up to 4036 tokens (32 / 8 heads, fp16): 59 us, with the join 69
-// (fp32 rows 89); 2 of up to 60 after up to 31941 (16 / 2): 45, 53 (65). A step takes two workgroups
+// 16 trees of up to 64 nodes after up to 4036 tokens (32 / 8 heads, fp16): 58 us, with the join 69
+// (fp32 rows 88); 2 of up to 60 after up to 31941 (16 / 2): 43, 52 (64). A step takes two workgroups
 // a CU 2.1 us, of which a SIMD's two waves spend 0.9 on products and as much on exponentials and
 // other vector work, little of it side by side. One workgroup alone takes 1.5, eight waves of 16
 // rows 2.2, and fragments of values read into two buffers 2.1.
