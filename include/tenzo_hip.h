@@ -299,9 +299,8 @@ TENZO_HIP_API int tenzo_hip_tree_plan(const int32_t* parents, const int32_t* ctx
  * behind the last word are not seen). Accuracy as there but in calls that give 128
  * rows to a workgroup (over 40 rows times heads a kv head and sequence, and
  * enough of them or a wide table): a query's element is held to 2^-24 of the
- * largest of its group of 32 dims, in fp16 calls to 2^-19; weights to 2^-22, in
- * fp16 calls rounded once to fp16 (2^-11, as outputs are; below 2^-33 of a row's
- * largest they are lost). */
+ * largest of its group of 32 dims, weights to 2^-22 (below 2^-37 of a row's largest
+ * they are lost). */
 TENZO_HIP_API size_t tenzo_hip_attn_tree_kv4_ws_bytes(int64_t T, int B, int Hq, int Hkv,
                                                       int table_width, int has_cu, int dtype);
 TENZO_HIP_API int tenzo_hip_attn_tree_kv4(const void* q, int dtype, int64_t q_stride,

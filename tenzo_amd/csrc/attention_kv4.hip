@@ -277,8 +277,9 @@ __device__ __forceinline__ int scan_work(const Kv4Attn& a, const Kv4Seqs& sq, in
 }
 
 // The same where there are 64 sequences at most: a lane has one, and a wave finds what it wants of
-// them by itself, without LDS and barriers (kernel and join together, 48 tokens at up to 8190, 32 / 8
-// heads, fp16: 59.8 -> 58.2 us; 2 trees of up to 60 nodes after 32000 53.4 -> 52.0).
+// them by itself, without LDS and barriers (kernel and join together, us without | with, in turn: 48
+// tokens at up to 8190, 32 / 8 heads, fp16, 58.7 | 57.7; 16 sequences of up to 7 after up to 4093, 16 / 2,
+// 25.0 | 23.7; 2 trees of up to 60 nodes after 32000 58.9 | 57.8).
 constexpr int kLaneSeqs = 64;
 template <int ROWS>
 struct LaneWork {
@@ -1190,7 +1191,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_rows_kernel(Kv4Attn a, Kv4Seq
 #include "attention_kv4_tree.h"
 
 // Many trees: a workgroup to a (row tile, kv head) with all of its tokens. 32 trees of up to 64 nodes
-// after up to 500 tokens, 32 / 8 heads, fp16: 30 us.
+// after up to 436 tokens, 32 / 8 heads, fp16: 35 us.
 template <bool HALF>
 __global__ void __launch_bounds__(256, 2) kv4_attn_tree_kernel(Kv4Attn a, Kv4Seqs sq) {
     __shared__ Kv4TreeSmem sm;
@@ -1458,10 +1459,10 @@ Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, int
     const int64_t ctx = (int64_t)table_width * kKv4Page;
     // Many trees after short contexts: 128 rows a workgroup and a workgroup for all of their tokens,
     // with no records. us, the plan below | this, 32 / 8 heads: fp16, 16 x up to 64 nodes after 200
-    // (207 times 128 rows) 27 | 17, 8 x 64 after 500 (102) 22 | 23, 32 x 64 after 500 (370) 58 | 30,
-    // after 1000 82 | 44, after 2000 75 | 71; fp32 16 x 64 after 200 28 | 27, 32 x 64 after 500 60 |
-    // 49, after 1000 84 | 68, after 2000 99 | 101, 64 x 64 after 2000 (780) 187 | 177, after 4000
-    // 243 | 287.
+    // (207 times 128 rows) 30 | 22, 8 x 64 after 500 (102) 24 | 29, 14 x 64 after 500 39 | 30, 32 x 64
+    // after 500 (370) 59 | 37, after 1000 68 | 58, after 2000 90 | 92; fp32 16 x 64 after 200 28 | 27, 32
+    // x 64 after 500 60 | 49, after 1000 84 | 68, after 2000 99 | 101, 64 x 64 after 2000 (780) 187 |
+    // 177, after 4000 243 | 287. (Between the two in fp16, 10 x 64 after 450 23 | 29.)
     const double tiles = (double)T * G * Hkv / kRowsRT;
     if (kind != kNoTree && per > 44 &&
         ((ctx <= 1024 && tiles > (kind == kTreeHalf ? 110 : 360)) ||
@@ -1475,12 +1476,12 @@ Kv4Plan kv4_plan(int64_t T, int B, int G, int Hkv, int table_width, bool cu, int
     // Trees, by rows x heads x tokens: 128 rows a workgroup and the steps dealt evenly cost 20 us
     // before their first step (queries split into parts, the records of 512 shares), then half to
     // two thirds of the time of 16 rows a workgroup. us, 16 rows | 128, B x up to n nodes after up to
-    // that many tokens: fp16, 16 / 2 heads, 1 x 26 after 16000 (7M) 26 | 28, 8 x 32 after 4000 (14M)
-    // 35 | 36, 32 / 8 heads, 4 x 64 after 2000 (14M) 38 | 35, 8 x 64 after 2000 (26M) 48 | 38, 16 x
-    // 64 after 4000 (134M) 126 | 69; fp32, the same but the first, 35 | 41, 38 | 43, 47 | 46, 127 |
-    // 85, and 1 x 64 after 16000 (33M) 66 | 54. A sequence of few rows leaves most of 128 unused:
-    // of 37 rows (19M) fp16 39 | 44, of 47 (48M) 81 | 62, fp32 of 47 (30M) 56 | 59, of 60 (62M) 91 |
-    // 80.
+    // that many tokens: fp16, 16 / 2 heads, 1 x 26 after 16000 (7M) 24 | 29, 8 x 32 after 4000 (14M)
+    // 33 | 37, 32 / 8 heads, 1 x 64 after 8000 (16M) 37 | 40, 8 x 64 after 2000 (26M) 54 | 45, 16 x
+    // 64 after 4000 (134M) 127 | 85; fp32 8 x 32 after 4000 35 | 41, 4 x 64 after 2000 (14M) 38 | 43, 8 x
+    // 64 after 2000 47 | 46, 16 x 64 after 4000 127 | 85, and 1 x 64 after 16000 (33M) 66 | 54. A
+    // sequence of few rows leaves most of 128 unused: fp16 of 37 rows 45 | 45 (19M) and 77 | 64 (38M), of
+    // 47 (48M) 88 | 66, fp32 of 47 (30M) 56 | 59, of 60 (62M) 91 | 80.
     const double pairs = (double)T * G * Hkv * ctx;
     if ((kind == kTreeHalf && per > 40 && pairs > 14e6 && ctx > 1024) ||
         (kind == kTreeFloat && per > 56 && pairs > 22e6 && ctx > 1024)) {
@@ -1553,8 +1554,8 @@ int launch_kv4_even(const Kv4Attn& a, const Kv4Seqs& s, hipStream_t st) {
     const int rc = launch_status("kv4_attn_even_kernel");
     if (rc) return rc;
     // Few rows, or many records of each: a head to a workgroup, its records to 8 groups of lanes.
-    // Shares of a unit in trees' calls, and us with 8 groups | one: 34 39 | 49, 19 34 | 43, 13 74 |
-    // 72, 8 44 | 40, 6 49 | 40.
+    // Shares of a unit in trees' calls, and us with 8 groups | one: 64 39 | 70, 32 62 | 70, 21 76 |
+    // 81, 18 59 | 60, 14 38 | 39, 13 58 | 61, 8 57 | 51, 6 49 | 44.
     const int64_t units = ((int64_t)a.T * a.G / ROWS + s.B) * s.Hkv;
     if ((int64_t)a.T * a.Hq <= kWideJoin || (ROWS == kRowsRT && a.wgs > 16 * units))
         hipLaunchKernelGGL((kv4_join_even_kernel<ROWS, HALF, true>), dim3(a.T, a.Hq), dim3(256), 0,

@@ -6,9 +6,10 @@
 // of 32 dims and its scale byte the group's, just what v_mfma_scale_f32_16x16x128_f8f6f4 takes, so
 // keys go from memory to the products as they are, 128 dims at once. Queries are split into parts
 // of 6 bits (E2M3) with a scale for each 32 dims of a row and each part: with 2^E <= the largest
-// element, a part in units of 2^(E - 1 - 5 p) leaves at most 2^(E - 4 - 5 p) of any. Four parts of an
-// fp16 query leave 2^-19 of the largest of its 32 dims, five of an fp32 one 2^-24; the products cost
-// half of (fp32: 5/8 of) what they do with fp16 operands in two parts.
+// element, a part in units of 2^(E - 1 - 5 p) leaves at most 2^(E - 4 - 5 p) of any. Five parts leave
+// 2^-24 of the largest of a query's 32 dims; the products cost 5/8 of what they do with fp16 operands in
+// two parts. (fp16 queries take five too: beside a dim 100 times as large as the others, four would
+// leave 2^-19 of it, 2^-12 of the others, less than their own 11 bits.)
 //
 // Codes and scales are loaded straight into a ring in LDS, kAhead steps before they are used (a step
 // takes little longer than its codes' way from memory: with one step ahead, in registers, each took
@@ -18,17 +19,21 @@
 //
 // A row's scores come out of the products as logarithms of its weights: queries carry 1/sqrt(128)
 // and log2 e, and the sums begin at kBits less the row's maximum so far. Only where a score goes
-// beyond what the weights' type holds (fp16 calls: 2^7 above the maximum; fp32 calls: at all) are
-// maximum, weights and sums moved. In fp16 calls weights are rounded to fp16 once (2^-11 of a weight
-// at most, as outputs are; those below 2^-33 of the largest are lost), in fp32 calls held
-// in two parts, 22 bits (2^-40). Their sum comes from the products too, from the same rounded
-// weights against ones.
+// beyond what the weights' type holds (fp16 calls: 2^3 above the maximum; fp32 calls: at all) are
+// maximum, weights and sums moved. Weights are held in two parts of fp16, 22 bits, whatever the call's
+// type, so that a tree is answered as exactly here as in the kernels of fewer rows (what is below
+// fp16's numbers is lost: 2^-37 of a row's largest weight in fp16 calls, 2^-40 in fp32 ones). Their sum
+// comes from the products too, from the same parts against ones.
 //
-// 16 trees of up to 64 nodes after up to 4036 tokens (32 / 8 heads, fp16): 58 us, with the join 69
-// (fp32 rows 88); 2 of up to 60 after up to 31941 (16 / 2): 43, 52 (64). A step takes two workgroups
-// a CU 2.1 us, of which a SIMD's two waves spend 0.9 on products and as much on exponentials and
-// other vector work, little of it side by side. One workgroup alone takes 1.5, eight waves of 16
-// rows 2.2, and fragments of values read into two buffers 2.1.
+// With one part of weights and four of queries fp16 calls take 16 to 20% less, at 1.27 times the error
+// of their outputs' rounding (2.64e-4 against 2.08e-4): a tree's answer would depend on what else is in
+// the batch. us, one and four | two and five: 16 trees of up to 64 nodes after up to 4036 tokens, 32 / 8
+// heads, fp16, with the join 67 | 84; 2 of up to 60 after up to 31941, 16 / 2, 51.5 | 61.6.
+//
+// Without the join 76 and 55 us (fp32 rows take as long). A step takes two workgroups a CU 2.5 us, of
+// which a SIMD's two waves spend 1.5 on products and 0.9 on exponentials and other vector work, little of
+// it side by side. (With one part of weights, where it was 2.1: one workgroup alone 1.5, eight waves of
+// 16 rows 2.2, fragments of values read into two buffers 2.1.)
 #pragma once
 
 constexpr int kHardScale = 252;  // scale bytes above it count as 0
@@ -113,9 +118,9 @@ __device__ __forceinline__ void lds_barrier() {
 template <bool HALF>
 __device__ __forceinline__ void kv4_tree_segment(const Kv4Attn& a, const Kv4Seqs& sq,
                                                  const Segment& g, Kv4TreeSmem& sm) {
-    constexpr int QP = HALF ? 4 : 5, PP = HALF ? 1 : 2;  // parts of queries and of weights
+    constexpr int QP = 5, PP = 2;  // parts of queries and of weights
     constexpr float kUnit = kQkScale * kLog2e;
-    constexpr float kBits = HALF ? 8.0f : 15.0f, kMost = 15.0f;  // log2 of the weights: usual, most
+    constexpr float kBits = HALF ? 12.0f : 15.0f, kMost = 15.0f;  // log2 of the weights: usual, most
     const int n = g.n, c = g.c, h = g.h, first = g.first, t0 = g.t0;
     const int row0 = g.tile * kRowsRT, t1 = min(t0 + g.len, c);
     int tid = threadIdx.x;
@@ -328,7 +333,7 @@ __device__ __forceinline__ void kv4_tree_segment(const Kv4Attn& a, const Kv4Seqs
                                                     s[ct][tt]);
             };
             // (the small parts first)
-            if constexpr (QP > 4) part(std::integral_constant<int, QP - 1>{});
+            part(std::integral_constant<int, 4>{});
             part(std::integral_constant<int, 3>{});
             part(std::integral_constant<int, 2>{});
             load(page, before);
@@ -391,8 +396,7 @@ __device__ __forceinline__ void kv4_tree_segment(const Kv4Attn& a, const Kv4Seqs
                         const float p1 = __builtin_amdgcn_exp2f(w[(e & 3) + 1]);
                         const uint32_t hi = pack16(p0, p1);
                         pf[ct][0].w[e >> 1] = hi;
-                        if (PP > 1)
-                            pf[ct][PP - 1].w[e >> 1] = pack16(rest_lo(p0, hi), rest_hi(p1, hi));
+                        pf[ct][1].w[e >> 1] = pack16(rest_lo(p0, hi), rest_hi(p1, hi));
                     }
 #pragma unroll
                 for (int p = 0; p < PP; ++p)
