@@ -33,6 +33,20 @@ def _ptr(t: torch.Tensor | None):
     return t.data_ptr()  # (the declared argument types convert it)
 
 
+def _f32(t: torch.Tensor, name: str, n: int | None = None) -> int:
+    """The address of fp32 values, n of them: what kernels read as such (gemm_i8, rope and the
+    attention over a cache in 4 bits give other types too)."""
+    if t.dtype is not torch.float32:
+        raise ValueError(f"{name}: {t.dtype}, not {torch.float32}")
+    if n is not None and t.numel() != n:
+        raise ValueError(f"{name}: {tuple(t.shape)}, not {n} values")
+    return _ptr(t)
+
+
+def _norm(w: torch.Tensor | None, K: int):
+    return None if w is None else _f32(w, "norm_w", K)
+
+
 # The small calls' kernels take 5 to 10 us, so their Python side shows: no Stream object, pointer
 # object or view where a number or the tensor itself will do. Per call, us, with them | without:
 # gemv_q4_0 10.3 | 7.3, attn_int8_decode 14.6 | 11.4, rmsnorm_quant31 + bitlinear_tl1 22.2 | 16.5.
@@ -85,8 +99,8 @@ def rmsnorm_quant31(x: torch.Tensor, norm_w: torch.Tensor | None = None, eps: fl
     norm = bool(do_norm) if do_norm is not None else norm_w is not None
     y = torch.empty_like(x2) if (want_y and norm) else None
     _lib.check(_lib.load().tenzo_hip_rmsnorm_quant31(
-        _ptr(x2), _ptr(norm_w), int(norm), eps, M, K, _ptr(codes), _ptr(q), _ptr(y), _stream()),
-        "rmsnorm_quant31")
+        _f32(x2, "x"), _norm(norm_w, K), int(norm), eps, M, K, _ptr(codes), _ptr(q), _ptr(y),
+        _stream()), "rmsnorm_quant31")
     return codes, q, y
 
 
@@ -153,15 +167,15 @@ def bitlinear_tl1_f32(x: torch.Tensor, w_packed: torch.Tensor, w_scale: float, N
     M = x2.shape[0]
     y = torch.empty((M, N), dtype=torch.float32, device=x.device)
     _lib.check(_lib.load().tenzo_hip_bitlinear_tl1_f32(
-        _ptr(x2), _ptr(w_packed), w_scale, M, N, K, _ptr(y), _stream()), "bitlinear_tl1_f32")
+        _f32(x2, "x"), _ptr(w_packed), w_scale, M, N, K, _ptr(y), _stream()), "bitlinear_tl1_f32")
     return y
 
 
 def rmsnorm(x: torch.Tensor, w: torch.Tensor | None, eps: float = 1e-5) -> torch.Tensor:
     """executeRMSNorm(in, w, out, dim, eps)."""
     y = torch.empty_like(x)
-    _lib.check(_lib.load().tenzo_hip_rmsnorm(_ptr(x), _ptr(w), _ptr(y), x.numel(), eps,
-                                             _stream()), "rmsnorm")
+    _lib.check(_lib.load().tenzo_hip_rmsnorm(_f32(x, "x"), _norm(w, x.numel()), _ptr(y), x.numel(),
+                                             eps, _stream()), "rmsnorm")
     return y
 
 
@@ -188,9 +202,9 @@ def attn_int8_decode(q, k_new, v_new, kc, vc, ks, vs, rope_cs, pos: int, want_ro
     q_rot = torch.empty_like(out) if want_rot else None
     k_rot = torch.empty((B, Hkv * D), dtype=torch.float32, device=q.device) if want_rot else None
     _lib.check(_lib.load().tenzo_hip_attn_int8_decode(
-        _ptr(q), _ptr(k_new), _ptr(v_new), _ptr(kc), _ptr(vc), _ptr(ks), _ptr(vs), _ptr(rope_cs),
-        B, Hq, Hkv, max_seq, pos, _ptr(out), _ptr(q_rot), _ptr(k_rot), _stream()),
-        "attn_int8_decode")
+        _f32(q, "q"), _f32(k_new, "k_new"), _f32(v_new, "v_new"), _ptr(kc), _ptr(vc), _ptr(ks),
+        _ptr(vs), _f32(rope_cs, "rope_cs"), B, Hq, Hkv, max_seq, pos, _ptr(out), _ptr(q_rot),
+        _ptr(k_rot), _stream()), "attn_int8_decode")
     return (out, q_rot, k_rot) if want_rot else out
 
 
@@ -212,9 +226,9 @@ def attn_tern_decode(mode, q, k_new, v_new, kb, vb, ks, vs, rope_cs, pos: int, w
     q_rot = torch.empty_like(out) if want_rot else None
     k_rot = torch.empty((B, Hkv * D), dtype=torch.float32, device=q.device) if want_rot else None
     _lib.check(_lib.load().tenzo_hip_attn_tern_decode(
-        int(mode), _ptr(q), _ptr(k_new), _ptr(v_new), _ptr(kb), _ptr(vb), _ptr(ks), _ptr(vs),
-        _ptr(rope_cs), B, Hq, Hkv, max_seq, pos, _ptr(out), _ptr(q_rot), _ptr(k_rot), _stream()),
-        "attn_tern_decode")
+        int(mode), _f32(q, "q"), _f32(k_new, "k_new"), _f32(v_new, "v_new"), _ptr(kb), _ptr(vb),
+        _ptr(ks), _ptr(vs), _f32(rope_cs, "rope_cs"), B, Hq, Hkv, max_seq, pos, _ptr(out),
+        _ptr(q_rot), _ptr(k_rot), _stream()), "attn_tern_decode")
     return (out, q_rot, k_rot) if want_rot else out
 
 
@@ -230,9 +244,9 @@ def attn_paged_int8_decode(q, k_new, v_new, pk, pv, pks, pvs, block_table, layer
     Hq = q.numel() // D
     out = torch.empty((1, Hq * D), dtype=torch.float32, device=q.device)
     _lib.check(_lib.load().tenzo_hip_attn_paged_int8_decode(
-        _ptr(q), _ptr(k_new), _ptr(v_new), _ptr(pk), _ptr(pv), _ptr(pks), _ptr(pvs),
-        _ptr(block_table), n_layers, layer, _ptr(rope_cs), Hq, Hkv, pos, _ptr(out), _stream()),
-        "attn_paged_int8_decode")
+        _f32(q, "q"), _f32(k_new, "k_new"), _f32(v_new, "v_new"), _ptr(pk), _ptr(pv), _ptr(pks),
+        _ptr(pvs), _ptr(block_table), n_layers, layer, _f32(rope_cs, "rope_cs"), Hq, Hkv, pos,
+        _ptr(out), _stream()), "attn_paged_int8_decode")
     return out
 
 
@@ -699,22 +713,22 @@ def i8_rows_repack(w: torch.Tensor, V: int, H: int) -> torch.Tensor:
 
 def lm_head_i8(x, norm_w, w_packed, scales, V: int, H: int, eps: float = 1e-5):
     logits = torch.empty(V, dtype=torch.float32, device=x.device)
-    _lib.check(_lib.load().tenzo_hip_lm_head_i8(_ptr(x), _ptr(norm_w), eps, _ptr(w_packed),
-                                                _ptr(scales), _ptr(logits), V, H, _stream()),
-               "lm_head_i8")
+    _lib.check(_lib.load().tenzo_hip_lm_head_i8(_f32(x, "x", H), _norm(norm_w, H), eps,
+                                                _ptr(w_packed), _f32(scales, "scales"),
+                                                _ptr(logits), V, H, _stream()), "lm_head_i8")
     return logits
 
 
 def actquant127(x: torch.Tensor, norm_w: torch.Tensor | None = None, eps: float = 1e-5):
     """compute_logits' activation quantization of each row of x ([M][K] or
-    [K]), after rms_norm_raw when norm_w is given. Returns (codes int8 [M][K],
-    actq int32 [M][2])."""
+    [K], fp32), after rms_norm_raw when norm_w ([K], fp32) is given. Returns
+    (codes int8 [M][K], actq int32 [M][2])."""
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     M, K = x2.shape
     codes = torch.empty((M, K), dtype=torch.int8, device=x.device)
     q = torch.empty((M, 2), dtype=torch.int32, device=x.device)
     _lib.check(_lib.load().tenzo_hip_rmsnorm_quant127(
-        _ptr(x2), _ptr(norm_w), int(norm_w is not None), eps, M, K, _ptr(codes), _ptr(q),
+        _f32(x2, "x"), _norm(norm_w, K), int(norm_w is not None), eps, M, K, _ptr(codes), _ptr(q),
         _stream()), "rmsnorm_quant127")
     return codes, q
 
@@ -724,8 +738,8 @@ def lm_head_i8_codes_into(codes, q, w_packed, scales, V: int, H: int, logits,
     """The LM-head GEMV on precomputed codes into caller-owned logits (and the
     fused greedy argmax into idx when given)."""
     _lib.check(_lib.load().tenzo_hip_lm_head_i8_codes(
-        _ptr(codes), _ptr(q), _ptr(w_packed), _ptr(scales), _ptr(logits), V, H, _ptr(idx),
-        _stream()), "lm_head_i8_codes")
+        _ptr(codes), _ptr(q), _ptr(w_packed), _f32(scales, "scales"), _f32(logits, "logits"), V, H,
+        _ptr(idx), _stream()), "lm_head_i8_codes")
     return logits
 
 
@@ -737,10 +751,10 @@ def _gemm_i8_ws(*args: int) -> int:
 def gemm_i8(codes, q, w_packed, scales, N: int, K: int, dtype=torch.float32,
             want_idx: bool = False, out=None):
     """The product of 8-bit integers with a scale for each token and each channel: codes [M][K]
-    int8 and q [M][2] of actquant127 (rows of codes any multiple of 16 apart), w_packed of
-    i8_rows_repack, scales [N] fp32. Returns y [M][N] of dtype (fp32, fp16 or bf16; or into out,
-    whose type it then has), each value float(sum) * (token's scale * channel's), the sums exact;
-    with want_idx (y, idx [M] int32), each row's first column of the largest value (in fp32;
+    int8 and q [M][2] of actquant127, which takes fp32 (rows of codes any multiple of 16 apart),
+    w_packed of i8_rows_repack, scales [N] fp32. Returns y [M][N] of dtype (fp32, fp16 or bf16; or
+    into out, whose type it then has), each value float(sum) * (token's scale * channel's), the sums
+    exact; with want_idx (y, idx [M] int32), each row's first column of the largest value (in fp32;
     NaN counts as -inf). lm_head_i8_codes_into for M rows, with its values bit for bit."""
     dev = _dev()
     if codes.dim() != 2 or codes.shape[1] != K or q.shape != (codes.shape[0], 2):
@@ -779,8 +793,8 @@ def gemm_i8(codes, q, w_packed, scales, N: int, K: int, dtype=torch.float32,
 
 def argmax(logits: torch.Tensor) -> torch.Tensor:
     out = torch.empty(1, dtype=torch.int32, device=logits.device)
-    _lib.check(_lib.load().tenzo_hip_argmax(_ptr(logits), logits.numel(), _ptr(out), _stream()),
-               "argmax")
+    _lib.check(_lib.load().tenzo_hip_argmax(_f32(logits, "logits"), logits.numel(), _ptr(out),
+                                            _stream()), "argmax")
     return out
 
 
@@ -789,8 +803,8 @@ def sample_top_k_top_p(logits: torch.Tensor, top_k: int, top_p: float, temperatu
     """sample_top_k_top_p's sampling branch on device logits with the draw r."""
     out = torch.empty(1, dtype=torch.int32, device=logits.device)
     _lib.check(_lib.load().tenzo_hip_sample_top_k_top_p(
-        _ptr(logits), logits.numel(), int(top_k), float(top_p), float(temperature), float(r),
-        _ptr(out), _stream()), "sample_top_k_top_p")
+        _f32(logits, "logits"), logits.numel(), int(top_k), float(top_p), float(temperature),
+        float(r), _ptr(out), _stream()), "sample_top_k_top_p")
     return int(out.item())
 
 
