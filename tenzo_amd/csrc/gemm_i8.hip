@@ -63,12 +63,13 @@ struct Out<1> {
 template <>
 struct Out<2> : Out<1> {};
 
-// The larger value, of equal ones the lower column; NaN counts as -inf.
+// The larger value, of equal ones the lower column; NaN counts as -inf. (Without a branch: of ||, &&
+// and if, the compiler lost the assignment for equal values where v and n are of an array of 16 - the
+// body of the branch was empty -, so that the higher of two equal columns could be the answer.)
 __device__ __forceinline__ void take_best(float& v, int& n, float ov, int on) {
-    if (ov > v || (ov == v && on < n)) {
-        v = ov;
-        n = on;
-    }
+    const bool take = (ov > v) | ((ov == v) & (on < n));
+    v = take ? ov : v;
+    n = take ? on : n;
 }
 
 // A token of 2 D from either half of a wave's rows of 16 lanes: lanes with bit 4 keep the upper D.
