@@ -355,7 +355,8 @@ TENZO_HIP_API int tenzo_hip_rope(const void* x, int dtype, int64_t x_stride,
  * are; 1 divided by factor; 2 theta times factor^(rot_dim / (rot_dim - 2)); 3 by
  * parts (YaRN, Peng et al. 2023): divided by factor below `slow` turns within the
  * trained positions, kept above `fast`, in between a blend linear in the turns,
- * with *mscale = 0.1 ln(factor) + 1 (1 otherwise). */
+ * with *mscale = 0.1 ln(factor) + 1 (1 otherwise). A model tuned with a blend that
+ * is linear in i instead has other frequencies there: give tenzo_hip_rope those. */
 TENZO_HIP_API int tenzo_hip_rope_freqs(int rot_dim, double theta, int scaling, double factor,
                                        double trained, double fast, double slow,
                                        double* freqs_host, float* mscale);

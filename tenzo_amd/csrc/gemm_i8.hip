@@ -119,7 +119,7 @@ __device__ __forceinline__ void best_halve(float (&v)[N], int (&n)[N], bool up) 
 // 128 bytes of a row, belongs to one wave's turn). The codes of the 16 MT tokens come the same way,
 // out of the L2. At the end the waves' sums meet in LDS. 1 x 2560 x 6912: 5.7 us, 24 x 2560 x 6912:
 // 8.4, where the weights take 3.5: a launch, 7 dependent rounds of loads, and the meeting;
-// 26 x 128256 x 2560: 64 to 67 us, 5.1 TB/s, bound by the weights.
+// 26 x 128256 x 2560: 64 to 66 us, 5.1 TB/s, bound by the weights.
 constexpr uint32_t kNone = 0x80000000u;  // an offset past every resource
 constexpr int kNt = 2;                   // a load that leaves nothing in the caches
 template <int MT, int NT, int KW>
@@ -237,8 +237,10 @@ __global__ void __launch_bounds__(64 * KW) gemm_i8_few_kernel(GemmI8 a) {
 // with the 16 lanes that LDS serves together in different banks. The codes are the first operand,
 // so that a register of the result holds 32 neighbouring channels of a token in 32 lanes.
 // Each half of a step's fragments (32 k) is read while the half before it is multiplied.
-// 4001 x 6912 x 2560, fp16: 78 us, 1.8 POP/s, bound by the matrix units and the clock that their
-// power leaves (zeros run faster); 300 x 128256 x 2560, fp16: 148 us.
+// 4001 x 6912 x 2560, fp16: 78 us, 1.8 POP/s. The matrix units are busy in 46% of the cycles (58% of
+// those in which a CU has a tile: 864 of them leave CUs without one a fifth of the time), at the 1.87 GHz
+// that the power of random data leaves: zeros take the same cycles at 2.4 GHz, 64 us. 300 x 128256 x
+// 2560, fp16, with the largest: 159 us.
 template <int WR, int WT, int KW, int RT, int CT, int S>
 struct GemmTile {
     static constexpr int W = WR * WT * KW, BN = 32 * RT * WR, BM = 32 * CT * WT;
@@ -561,7 +563,9 @@ struct GemmPlan {
 //     1 x 128256 x 2560     66    53    52    55    53 |    74    63     62      64      64      83
 //    32 x 128256 x 2560    177   163   123    91    65 |    87    74     69      79      71      89
 //   300 x 128256 x 2560                           680 |   486   243    195     182     148     197
-// (Over 180 sizes this rule takes 1% longer than the fastest shape of each.)
+// (Over 180 sizes this rule takes 1% longer than the fastest shape of each. From 33 to some 600 tokens
+// the fastest takes 2 to 4 times what its bytes do: a workgroup a CU walks the whole of K, one barrier
+// for each 64, two products of a wave between them; of the tiles only the smallest shares K.)
 // (channels and tokens of a workgroup, channels of a part)
 constexpr int kShapes[][3] = {{16, 16, 16},   {16, 16, 16},   {32, 16, 32},    {32, 32, 32},
                               {64, 32, 64},   {64, 32, 32},   {64, 64, 32},    {128, 64, 64},

@@ -108,7 +108,8 @@ constexpr int kMoveRows = 16, kMoveHeads = 8;
 // time, all read before one is written: a row's new slot is never above its old one, so slots that
 // are still to be read lie behind those that are written. 64 trees of up to 64 nodes, 30 layers of 5
 // heads: 8.6 us, the walk's chain of loads (a target, then 64 parents and tokens, for each node of the
-// path); one tree of 26, 3.4.
+// path), and rows that go by way of scratch memory between load and store (80 bytes a thread, int8
+// pools 144: the compiler does not hold `v` and `to` in registers); one tree of 26, 3.4.
 template <int PIECES>  // of 16 bytes, of a row's codes
 __global__ void __launch_bounds__(256) tree_accept_kernel(TreeAccept a, Kv4Seqs sq) {
     __shared__ int path[kMostNodes];

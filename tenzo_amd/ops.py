@@ -598,7 +598,8 @@ def rope_freqs(rot_dim: int, theta: float = 10000.0, scaling: str | None = None,
     on the CPU, mscale). scaling, for contexts `factor` times as long as the `trained` positions:
     "linear" divides them by factor, "base" raises theta instead, "parts" (YaRN) divides those of
     fewer than `slow` turns within the trained positions, keeps those of more than `fast`, blends
-    in between, and has an mscale of 0.1 ln(factor) + 1."""
+    in between, linearly in the turns, and has an mscale of 0.1 ln(factor) + 1. (A model tuned with a
+    blend that is linear in the pair's number has other frequencies there: give rope those.)"""
     f = torch.empty(max(rot_dim // 2, 1), dtype=torch.float64)
     m = ctypes.c_float()
     if scaling not in ROPE_SCALINGS:

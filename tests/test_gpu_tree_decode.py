@@ -3,8 +3,8 @@ small model of random weights in 8 bits. A step plans its trees, and in each lay
 quantizes, projects to q | k | v, turns q and k to the nodes' positions, appends to the paged cache
 in 4 bits, attends to context and ancestors and projects back; then the LM head gives the model's
 token after each node and the trees' accepted paths stay in the cache. The tokens have to be those
-of decoding one by one, whatever was drafted, and the cache's rows bit for bit theirs; then the same
-steps run from a captured graph."""
+of decoding one by one, whatever was drafted, and the cache's rows theirs but for codes that another
+order of sums moves by a step; then the same steps run from a captured graph."""
 import numpy as np
 import pytest
 
