@@ -33,18 +33,17 @@ def _ptr(t: torch.Tensor | None):
     return t.data_ptr()  # (the declared argument types convert it)
 
 
-def _f32(t: torch.Tensor, name: str, n: int | None = None) -> int:
-    """The address of fp32 values, n of them: what kernels read as such (gemm_i8, rope and the
-    attention over a cache in 4 bits give other types too)."""
-    if t.dtype is not torch.float32:
-        raise ValueError(f"{name}: {t.dtype}, not {torch.float32}")
-    if n is not None and t.numel() != n:
-        raise ValueError(f"{name}: {tuple(t.shape)}, not {n} values")
-    return _ptr(t)
-
-
-def _norm(w: torch.Tensor | None, K: int):
-    return None if w is None else _f32(w, "norm_w", K)
+# What kernels read as fp32 is looked at, since other entry points give other types too (gemm_i8,
+# rope, the attention over a cache in 4 bits): one condition in a call, and the message from here. 0.1
+# us of a call, 0.2 where there are four tensors to look at.
+def _not_f32(n=None, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.dtype is not torch.float32:
+            raise ValueError(f"{name}: {t.dtype}, not {torch.float32}")
+    for name, t in tensors.items():
+        if t is not None and n is not None and name in ("x", "norm_w") and t.shape[-1] != n:
+            raise ValueError(f"{name}: {tuple(t.shape)}, not {n} values")
+    raise ValueError(f"not fp32 of {n} values: {tensors}")
 
 
 # The small calls' kernels take 5 to 10 us, so their Python side shows: no Stream object, pointer
@@ -94,12 +93,15 @@ def rmsnorm_quant31(x: torch.Tensor, norm_w: torch.Tensor | None = None, eps: fl
     [M][2] viewed as {inv_scale(float bits), code_sum}, y or None)."""
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     M, K = x2.shape
+    if x2.dtype is not _F32 or norm_w is not None and (norm_w.dtype is not _F32 or
+                                                       norm_w.numel() != K):
+        _not_f32(K, x=x2, norm_w=norm_w)
     codes = torch.empty((M, padded(K)), dtype=torch.int8, device=x.device)
     q = torch.empty((M, 2), dtype=torch.int32, device=x.device)
     norm = bool(do_norm) if do_norm is not None else norm_w is not None
     y = torch.empty_like(x2) if (want_y and norm) else None
     _lib.check(_lib.load().tenzo_hip_rmsnorm_quant31(
-        _f32(x2, "x"), _norm(norm_w, K), int(norm), eps, M, K, _ptr(codes), _ptr(q), _ptr(y),
+        _ptr(x2), _ptr(norm_w), int(norm), eps, M, K, _ptr(codes), _ptr(q), _ptr(y),
         _stream()), "rmsnorm_quant31")
     return codes, q, y
 
@@ -163,19 +165,24 @@ def bitlinear_tl1_batch(codes: torch.Tensor, q: torch.Tensor, w_packed: torch.Te
 def bitlinear_tl1_f32(x: torch.Tensor, w_packed: torch.Tensor, w_scale: float, N: int,
                       K: int) -> torch.Tensor:
     """executeBitLinearTL1(act, w, out, M, K, N, scale) on device tensors."""
+    if x.dtype is not _F32:
+        _not_f32(x=x)
     x2 = _rows(x, K)
     M = x2.shape[0]
     y = torch.empty((M, N), dtype=torch.float32, device=x.device)
     _lib.check(_lib.load().tenzo_hip_bitlinear_tl1_f32(
-        _f32(x2, "x"), _ptr(w_packed), w_scale, M, N, K, _ptr(y), _stream()), "bitlinear_tl1_f32")
+        _ptr(x2), _ptr(w_packed), w_scale, M, N, K, _ptr(y), _stream()), "bitlinear_tl1_f32")
     return y
 
 
 def rmsnorm(x: torch.Tensor, w: torch.Tensor | None, eps: float = 1e-5) -> torch.Tensor:
     """executeRMSNorm(in, w, out, dim, eps)."""
+    n = x.numel()
+    if x.dtype is not _F32 or w is not None and (w.dtype is not _F32 or w.numel() != n):
+        _not_f32(n, x=x.reshape(-1), norm_w=w)
     y = torch.empty_like(x)
-    _lib.check(_lib.load().tenzo_hip_rmsnorm(_f32(x, "x"), _norm(w, x.numel()), _ptr(y), x.numel(),
-                                             eps, _stream()), "rmsnorm")
+    _lib.check(_lib.load().tenzo_hip_rmsnorm(_ptr(x), _ptr(w), _ptr(y), n, eps, _stream()),
+               "rmsnorm")
     return y
 
 
@@ -196,14 +203,16 @@ def attn_int8_decode(q, k_new, v_new, kc, vc, ks, vs, rope_cs, pos: int, want_ro
     int8 and ks/vs [B][Hkv][max_seq] fp16 (updated in place at pos);
     rope_cs [128] fp32 on the device. Returns out [B][Hq*128] (and rotated
     q, k when want_rot)."""
+    if not (q.dtype is k_new.dtype is v_new.dtype is rope_cs.dtype is _F32):
+        _not_f32(q=q, k_new=k_new, v_new=v_new, rope_cs=rope_cs)
     B, Hkv, max_seq, D = kc.shape
     Hq = q.numel() // (B * D)
     out = torch.empty((B, Hq * D), dtype=torch.float32, device=q.device)
     q_rot = torch.empty_like(out) if want_rot else None
     k_rot = torch.empty((B, Hkv * D), dtype=torch.float32, device=q.device) if want_rot else None
     _lib.check(_lib.load().tenzo_hip_attn_int8_decode(
-        _f32(q, "q"), _f32(k_new, "k_new"), _f32(v_new, "v_new"), _ptr(kc), _ptr(vc), _ptr(ks),
-        _ptr(vs), _f32(rope_cs, "rope_cs"), B, Hq, Hkv, max_seq, pos, _ptr(out), _ptr(q_rot),
+        _ptr(q), _ptr(k_new), _ptr(v_new), _ptr(kc), _ptr(vc), _ptr(ks),
+        _ptr(vs), _ptr(rope_cs), B, Hq, Hkv, max_seq, pos, _ptr(out), _ptr(q_rot),
         _ptr(k_rot), _stream()), "attn_int8_decode")
     return (out, q_rot, k_rot) if want_rot else out
 
@@ -217,6 +226,8 @@ def attn_tern_decode(mode, q, k_new, v_new, kb, vb, ks, vs, rope_cs, pos: int, w
 
     kb/vb [B][Hkv][max_seq][32] uint8 rows and ks/vs [B][Hkv][max_seq] fp32
     (updated in place at pos); the rest as attn_int8_decode."""
+    if not (q.dtype is k_new.dtype is v_new.dtype is rope_cs.dtype is _F32):
+        _not_f32(q=q, k_new=k_new, v_new=v_new, rope_cs=rope_cs)
     mode = KV_TERN_MODES.get(mode, mode)
     B, Hkv, max_seq, R = kb.shape
     assert R == 32 and kb.dtype == torch.uint8 and ks.dtype == torch.float32
@@ -226,8 +237,8 @@ def attn_tern_decode(mode, q, k_new, v_new, kb, vb, ks, vs, rope_cs, pos: int, w
     q_rot = torch.empty_like(out) if want_rot else None
     k_rot = torch.empty((B, Hkv * D), dtype=torch.float32, device=q.device) if want_rot else None
     _lib.check(_lib.load().tenzo_hip_attn_tern_decode(
-        int(mode), _f32(q, "q"), _f32(k_new, "k_new"), _f32(v_new, "v_new"), _ptr(kb), _ptr(vb),
-        _ptr(ks), _ptr(vs), _f32(rope_cs, "rope_cs"), B, Hq, Hkv, max_seq, pos, _ptr(out),
+        int(mode), _ptr(q), _ptr(k_new), _ptr(v_new), _ptr(kb), _ptr(vb),
+        _ptr(ks), _ptr(vs), _ptr(rope_cs), B, Hq, Hkv, max_seq, pos, _ptr(out),
         _ptr(q_rot), _ptr(k_rot), _stream()), "attn_tern_decode")
     return (out, q_rot, k_rot) if want_rot else out
 
@@ -238,14 +249,16 @@ def attn_paged_int8_decode(q, k_new, v_new, pk, pv, pks, pvs, block_table, layer
 
     pk/pv [blocks][n_layers][Hkv][16][128] int8 and pks/pvs [blocks][n_layers][Hkv][16]
     fp32 (updated in place at pos); block_table int32 covering position pos."""
+    if not (q.dtype is k_new.dtype is v_new.dtype is rope_cs.dtype is _F32):
+        _not_f32(q=q, k_new=k_new, v_new=v_new, rope_cs=rope_cs)
     nb, n_layers, Hkv, page, D = pk.shape
     assert page == 16 and pk.dtype == torch.int8 and pks.dtype == torch.float32
     assert block_table.dtype == torch.int32 and block_table.numel() * 16 > pos
     Hq = q.numel() // D
     out = torch.empty((1, Hq * D), dtype=torch.float32, device=q.device)
     _lib.check(_lib.load().tenzo_hip_attn_paged_int8_decode(
-        _f32(q, "q"), _f32(k_new, "k_new"), _f32(v_new, "v_new"), _ptr(pk), _ptr(pv), _ptr(pks),
-        _ptr(pvs), _ptr(block_table), n_layers, layer, _f32(rope_cs, "rope_cs"), Hq, Hkv, pos,
+        _ptr(q), _ptr(k_new), _ptr(v_new), _ptr(pk), _ptr(pv), _ptr(pks),
+        _ptr(pvs), _ptr(block_table), n_layers, layer, _ptr(rope_cs), Hq, Hkv, pos,
         _ptr(out), _stream()), "attn_paged_int8_decode")
     return out
 
@@ -598,8 +611,8 @@ def rope_freqs(rot_dim: int, theta: float = 10000.0, scaling: str | None = None,
     on the CPU, mscale). scaling, for contexts `factor` times as long as the `trained` positions:
     "linear" divides them by factor, "base" raises theta instead, "parts" (YaRN) divides those of
     fewer than `slow` turns within the trained positions, keeps those of more than `fast`, blends
-    in between, linearly in the turns, and has an mscale of 0.1 ln(factor) + 1. (A model tuned with a
-    blend that is linear in the pair's number has other frequencies there: give rope those.)"""
+    in between, linearly in the turns, and has an mscale of 0.1 ln(factor) + 1. (A model tuned with
+    a blend that is linear in the pair's number has other frequencies there: give rope those.)"""
     f = torch.empty(max(rot_dim // 2, 1), dtype=torch.float64)
     m = ctypes.c_float()
     if scaling not in ROPE_SCALINGS:
@@ -713,9 +726,12 @@ def i8_rows_repack(w: torch.Tensor, V: int, H: int) -> torch.Tensor:
 
 
 def lm_head_i8(x, norm_w, w_packed, scales, V: int, H: int, eps: float = 1e-5):
+    if x.dtype is not _F32 or scales.dtype is not _F32 or x.numel() != H or norm_w is not None and (
+            norm_w.dtype is not _F32 or norm_w.numel() != H):
+        _not_f32(H, x=x, norm_w=norm_w, scales=scales)
     logits = torch.empty(V, dtype=torch.float32, device=x.device)
-    _lib.check(_lib.load().tenzo_hip_lm_head_i8(_f32(x, "x", H), _norm(norm_w, H), eps,
-                                                _ptr(w_packed), _f32(scales, "scales"),
+    _lib.check(_lib.load().tenzo_hip_lm_head_i8(_ptr(x), _ptr(norm_w), eps,
+                                                _ptr(w_packed), _ptr(scales),
                                                 _ptr(logits), V, H, _stream()), "lm_head_i8")
     return logits
 
@@ -726,10 +742,13 @@ def actquant127(x: torch.Tensor, norm_w: torch.Tensor | None = None, eps: float 
     (codes int8 [M][K], actq int32 [M][2])."""
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     M, K = x2.shape
+    if x2.dtype is not _F32 or norm_w is not None and (norm_w.dtype is not _F32 or
+                                                       norm_w.numel() != K):
+        _not_f32(K, x=x2, norm_w=norm_w)
     codes = torch.empty((M, K), dtype=torch.int8, device=x.device)
     q = torch.empty((M, 2), dtype=torch.int32, device=x.device)
     _lib.check(_lib.load().tenzo_hip_rmsnorm_quant127(
-        _f32(x2, "x"), _norm(norm_w, K), int(norm_w is not None), eps, M, K, _ptr(codes), _ptr(q),
+        _ptr(x2), _ptr(norm_w), int(norm_w is not None), eps, M, K, _ptr(codes), _ptr(q),
         _stream()), "rmsnorm_quant127")
     return codes, q
 
@@ -738,8 +757,10 @@ def lm_head_i8_codes_into(codes, q, w_packed, scales, V: int, H: int, logits,
                           idx=None):
     """The LM-head GEMV on precomputed codes into caller-owned logits (and the
     fused greedy argmax into idx when given)."""
+    if not (scales.dtype is logits.dtype is _F32):
+        _not_f32(scales=scales, logits=logits)
     _lib.check(_lib.load().tenzo_hip_lm_head_i8_codes(
-        _ptr(codes), _ptr(q), _ptr(w_packed), _f32(scales, "scales"), _f32(logits, "logits"), V, H,
+        _ptr(codes), _ptr(q), _ptr(w_packed), _ptr(scales), _ptr(logits), V, H,
         _ptr(idx), _stream()), "lm_head_i8_codes")
     return logits
 
@@ -793,8 +814,10 @@ def gemm_i8(codes, q, w_packed, scales, N: int, K: int, dtype=torch.float32,
 
 
 def argmax(logits: torch.Tensor) -> torch.Tensor:
+    if logits.dtype is not _F32:
+        _not_f32(logits=logits)
     out = torch.empty(1, dtype=torch.int32, device=logits.device)
-    _lib.check(_lib.load().tenzo_hip_argmax(_f32(logits, "logits"), logits.numel(), _ptr(out),
+    _lib.check(_lib.load().tenzo_hip_argmax(_ptr(logits), logits.numel(), _ptr(out),
                                             _stream()), "argmax")
     return out
 
@@ -802,9 +825,11 @@ def argmax(logits: torch.Tensor) -> torch.Tensor:
 def sample_top_k_top_p(logits: torch.Tensor, top_k: int, top_p: float, temperature: float,
                        r: float) -> int:
     """sample_top_k_top_p's sampling branch on device logits with the draw r."""
+    if logits.dtype is not _F32:
+        _not_f32(logits=logits)
     out = torch.empty(1, dtype=torch.int32, device=logits.device)
     _lib.check(_lib.load().tenzo_hip_sample_top_k_top_p(
-        _f32(logits, "logits"), logits.numel(), int(top_k), float(top_p), float(temperature),
+        _ptr(logits), logits.numel(), int(top_k), float(top_p), float(temperature),
         float(r), _ptr(out), _stream()), "sample_top_k_top_p")
     return int(out.item())
 
