@@ -33,7 +33,8 @@
 // Without the join 76 and 55 us (fp32 rows take as long). A step takes two workgroups a CU 2.5 us, of
 // which a SIMD's two waves spend 1.5 on products and 0.9 on exponentials and other vector work, little of
 // it side by side. (With one part of weights, where it was 2.1: one workgroup alone 1.5, eight waves of
-// 16 rows 2.2, fragments of values read into two buffers 2.1.)
+// 16 rows 2.2, fragments of values read into two buffers 2.1.) All 256 registers are taken; 11 more
+// (2 or 3 where a workgroup has all tokens) wait in scratch memory for the steps with masks and the end.
 #pragma once
 
 constexpr int kHardScale = 252;  // scale bytes above it count as 0
